@@ -1,0 +1,134 @@
+"""libtgattn.so without a GPU: its exports, the structures that the binding packs, refusals,
+spills, and the frequencies of rotary positions."""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import os
+import re
+import subprocess
+
+import numpy as np
+import pytest
+import torch
+
+from tilegen_amd import attention as at
+from tilegen_amd import build, runtime
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+HEADER = os.path.join(ROOT, "include", "tilegen_attention.h")
+PACKED = {"tg_rope": at._ROPE, "tg_paged_append": at._APPEND, "tg_prefix_attention": at._ATTENTION}
+
+
+def test_exports_what_the_header_declares():
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    declared = set(re.findall(r"\b(\w+)\(const tg_\w+\*", text))
+    assert declared == {"launch_rope", "launch_paged_append", "launch_prefix_attention",
+                        "prefix_attention_workspace"}
+    out = subprocess.run(["nm", "-D", "--defined-only",
+                          os.path.join(runtime.lib_dir(), "libtgattn.so")],
+                         capture_output=True, text=True, check=True).stdout
+    exported = {line.split()[-1] for line in out.splitlines() if " T " in line}
+    assert declared <= exported
+    assert all(s in declared or s.startswith("_") for s in exported), exported
+
+
+def test_packed_fields_follow_the_header():
+    """The header's field types in order, as struct codes."""
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    for name, packed in PACKED.items():
+        body = re.search(r"typedef struct \{([^}]*)\} %s;" % name, text).group(1)
+        codes = ""
+        for line in body.split(";"):    # no field list mixes pointers and numbers
+            if line.strip():
+                kind = "P" if "*" in line else "d" if "double" in line else "q"
+                codes += kind * len(line.split(","))
+        flat = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([Pqd])", packed.format))
+        assert codes == flat, name
+        assert packed.size == 8 * len(codes)
+
+
+def test_refusals_without_a_device():
+    """Refused on the host, before any HIP call."""
+    L = at._lib()
+
+    def message(rc, code):
+        assert rc == code
+        return runtime.last_error()
+
+    assert "null" in message(L.launch_rope(None, None), -1)
+    rope = dict(x=0, y=0, positions=0, frequency=0, dtype=0, tokens=4, heads=2, dim=64,
+                rotary=64, layout=0, xt=128, xh=64, yt=128, yh=64, magnitude=1.0, sign=1)
+    for change, word in [(dict(), "null"), (dict(dtype=3), "dtype"), (dict(dim=0), "dim"),
+                         (dict(dim=1025), "dim"), (dict(rotary=66), "rotary"),
+                         (dict(rotary=7), "rotary"), (dict(layout=2), "layout"),
+                         (dict(tokens=-1), "negative"), (dict(sign=0), "sign")]:
+        args = at._ROPE.pack(*{**rope, **change}.values())
+        assert word in message(L.launch_rope(args, None), -1)
+    assert "tokens" in message(L.launch_rope(at._ROPE.pack(*{**rope, "tokens": 1 << 40}.values()),
+                                             None), -2)
+    assert L.launch_rope(at._ROPE.pack(*{**rope, "tokens": 0}.values()), None) == 0
+    names = [f for f in ("query kc vc prefix indptr indices lengths ends out lse workspace bytes "
+                         "dtype tokens sequences heads kv_heads dim pages page n_prefix "
+                         "prefix_length n_indices max_query max_length").split()]
+    base = dict.fromkeys(names, 0)
+    base.update(tokens=2, sequences=2, heads=4, kv_heads=2, dim=64, pages=9, page=16, n_prefix=2,
+                prefix_length=32, n_indices=4, max_query=1, max_length=20)
+    base.update({"s%d" % i: 64 for i in range(10)}, scale=0.125)
+
+    def attend(**change):
+        return at._ATTENTION.pack(*{**base, **change}.values())
+
+    need = L.prefix_attention_workspace(attend())
+    assert need > 0 and "null" in message(L.launch_prefix_attention(attend(), None), -1)
+    every = {n: 4096 for n in names[:10]}
+    assert "workspace" in message(L.launch_prefix_attention(
+        attend(**every, workspace=4096, bytes=need - 1), None), -1)
+    assert "aligned" in message(L.launch_prefix_attention(
+        attend(**every, workspace=4100, bytes=need), None), -1)
+    for change, code in [(dict(dtype=2), -1), (dict(dim=12), -1), (dict(dim=264), -1),
+                         (dict(kv_heads=3), -1), (dict(kv_heads=0), -1), (dict(page=0), -1),
+                         (dict(scale=0.0), -1), (dict(scale=math.nan), -1),
+                         (dict(prefix_length=33), -1), (dict(tokens=3), -1),
+                         (dict(max_length=1 << 40), -2), (dict(sequences=-1), -1),
+                         (dict(tokens=1 << 25, sequences=1 << 25), -2)]:
+        assert L.prefix_attention_workspace(attend(**change)) < 0, change
+        assert L.launch_prefix_attention(attend(**change), None) == code, change
+    assert L.prefix_attention_workspace(attend(tokens=0, sequences=0)) == 0
+    assert L.launch_prefix_attention(attend(tokens=0, sequences=0), None) == 0
+
+
+def test_operands_on_the_host_are_refused():
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    n = torch.zeros(2, dtype=torch.int64)
+    f = torch.zeros(32, dtype=torch.float64)
+    cache = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError):
+        at.rope(x, n, f)
+    with pytest.raises(ValueError):
+        at.paged_append(x, x, cache, cache, n, n, n, f)
+    with pytest.raises(ValueError):
+        at.prefix_attention(x, cache, cache, n, 0, n, n, n, max_length=1)
+
+
+def test_rope_frequencies():
+    """Against the formulas; kept, divided and ramped pairs."""
+    n = 64
+    plain = np.array([10000.0 ** (-i / n) for i in range(0, n, 2)])
+    f, m = at.rope_frequencies(n, device="cpu")
+    assert f.dtype == torch.float64 and m == 1.0
+    np.testing.assert_allclose(f.numpy(), plain, rtol=1e-15)
+    f, m = at.rope_frequencies(n, scaling="linear", factor=8, device="cpu")
+    np.testing.assert_allclose(f.numpy(), plain / 8, rtol=1e-15)
+    f, m = at.rope_frequencies(n, scaling="ntk", factor=8, device="cpu")
+    np.testing.assert_allclose(f.numpy()[[0, -1]], plain[[0, -1]] / [1, 8], rtol=1e-12)
+    f, m = at.rope_frequencies(n, scaling="yarn", factor=8, trained=4096, device="cpu")
+    turns = 4096 * plain / (2 * np.pi)
+    assert (f.numpy()[turns >= 32] == plain[turns >= 32]).all() and (turns >= 32).any()
+    np.testing.assert_allclose(f.numpy()[turns <= 1], plain[turns <= 1] / 8, rtol=1e-15)
+    assert (np.diff(f.numpy()) < 0).all() and m == pytest.approx(0.1 * math.log(8) + 1)
+    for bad in (dict(rotary=3), dict(rotary=4, scaling="x"), dict(rotary=4, factor=0.5),
+                dict(rotary=4, scaling="yarn")):
+        with pytest.raises(ValueError):
+            at.rope_frequencies(device="cpu", **bad)

@@ -1,0 +1,634 @@
+"""Rotary positions, the append to a paged cache and attention behind a shared prefix
+(tilegen_amd.attention) against the formulas in 64 bits.
+
+Tolerances come from the arithmetic.  u is the unit roundoff of the operands' type (2^-8
+bfloat16, 2^-11 float16, 2^-24 float32): a value rounded to it once is off by u of itself.
+
+rope: a value is a cos - b sin in 32 bits, rounded once.  The angle's fraction of a turn is
+exact to 2^-25 of itself, so the cosine and sine to about 2 pi 2^-26 + 2^-24; with the two
+products and the sum: |error| <= u |y| + 2^-21 (|a| + |b|) magnitude.
+
+attention: probabilities (up to 2^8 times the largest one's, see narrow.h) are rounded to the
+operands' type (relative u, and half the smallest float16, 2^-25, where they are below its
+normal range), the result once more; scores are off by at most dim 2^-23 scale sum |q k|, in the
+numerator and in the denominator; sums of n terms by n 2^-24 of the sum of magnitudes."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from tilegen_amd import attention as at
+
+pytestmark = pytest.mark.gpu
+
+U = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(seed)
+    return g
+
+
+def _normal(g, *shape, dtype):
+    return torch.randn(*shape, generator=g, device="cuda", dtype=torch.float32).to(dtype)
+
+
+# --------------------------------------------------------------------------- #
+# rope
+# --------------------------------------------------------------------------- #
+def _turned(x, positions, frequency, layout, magnitude=1.0, sign=1):
+    """The formula in 64 bits, on the CPU."""
+    y = x.detach().cpu().double().clone()
+    f = frequency.cpu().double().numpy()
+    p = positions.cpu().numpy().astype(np.float64)
+    angle = torch.from_numpy(sign * p[:, None] * f)
+    c, s = magnitude * torch.cos(angle)[:, None], magnitude * torch.sin(angle)[:, None]
+    n = f.size
+    first = slice(0, n) if layout == "half" else slice(0, 2 * n, 2)
+    second = slice(n, 2 * n) if layout == "half" else slice(1, 2 * n, 2)
+    a, b = y[..., first].clone(), y[..., second].clone()
+    y[..., first], y[..., second] = a * c - b * s, b * c + a * s
+    size = y.abs()
+    size[..., first] = size[..., second] = (a.abs() + b.abs()) * magnitude
+    return y, size
+
+
+def _check_turned(got, x, positions, frequency, layout, magnitude=1.0, sign=1):
+    want, size = _turned(x, positions, frequency, layout, magnitude, sign)
+    off = (got.cpu().double() - want).abs()
+    tiny = 2.0 ** -25 if got.dtype == F16 else 0.0
+    bound = U[got.dtype] * want.abs() + 2.0 ** -21 * size + tiny
+    bound *= 1 + 2.0 ** -6
+    assert (off <= bound).all(), float((off - bound).max())
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("tokens,heads,dim,rotary", [
+    (1, 1, 2, 2), (3, 2, 7, 4), (5, 3, 64, 64), (4, 5, 80, 38), (2, 40, 128, 128), (9, 1, 96, 0),
+    (1, 7, 256, 62), (4099, 2, 96, 64), (3, 1, 1024, 1024), (70, 3, 17, 16), (4, 300, 24, 24)])
+def test_rope(hip_ready, layout, dtype, tokens, heads, dim, rotary):
+    g = _gen(tokens + dim)
+    x = _normal(g, tokens, heads, dim, dtype=dtype)
+    positions = torch.randint(-1000, 10 ** 7, (tokens,), generator=g, device="cuda")
+    frequency, magnitude = at.rope_frequencies(rotary, scaling="yarn", factor=8, trained=2048)
+    keep = x.clone()
+    y = at.rope(x, positions, frequency, layout=layout, magnitude=magnitude)
+    _check_turned(y, x, positions, frequency, layout, magnitude)
+    d = at.rope_backward(x, positions, frequency, layout=layout, magnitude=magnitude)
+    _check_turned(d, x, positions, frequency, layout, magnitude, sign=-1)
+    assert torch.equal(x, keep)
+    assert at.rope(x, positions, frequency, layout=layout, magnitude=magnitude, out=x) is x
+    assert torch.equal(x, y)    # in place: the same bits
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_on_views(hip_ready, layout):
+    """Heads of a packed projection, odd offsets, transposed tokens and heads."""
+    g = _gen(1)
+    frequency, _ = at.rope_frequencies(48)
+    packed = _normal(g, 11, 9, 65, dtype=BF16)
+    positions = torch.arange(11, device="cuda") * 12345
+    out = torch.zeros(9, 11, 77, device="cuda", dtype=BF16)
+    x, y = packed[:, 2:7, 1:65], out[1:6, :, 5:69].transpose(0, 1)
+    assert at.rope(x, positions, frequency, layout=layout, out=y) is y
+    _check_turned(y, x, positions, frequency, layout)
+    y.zero_()
+    assert not out.any()        # nothing beside the view was written
+    wide = x[:, :1].expand(11, 4, 64)
+    _check_turned(at.rope(wide, positions, frequency, layout=layout), wide, positions, frequency,
+                  layout)
+    before = packed.clone()
+    at.rope(x, positions, frequency, layout=layout, out=x)
+    before[:, 2:7, 1:65] = x
+    assert torch.equal(packed, before)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_rope_gradient(hip_ready, layout):
+    """The gradient through autograd is the transposed map, and matches differences of the
+    formula (linear in x: exact but for rounding)."""
+    g = _gen(2)
+    frequency, magnitude = at.rope_frequencies(24, scaling="yarn", factor=4, trained=512)
+    positions = torch.tensor([0, 1, 77, 100000, 5], device="cuda")
+    x = _normal(g, 5, 3, 30, dtype=F32).requires_grad_()
+    w = _normal(g, 5, 3, 30, dtype=F32)
+    y = at.rope(x, positions, frequency, layout=layout, magnitude=magnitude)
+    (y * w).sum().backward()
+    _check_turned(x.grad, w, positions, frequency, layout, magnitude, sign=-1)
+    for t, h, i in ((0, 0, 0), (2, 1, 13), (3, 2, 23), (4, 0, 29), (3, 0, 12)):
+        plus, minus = x.detach().clone(), x.detach().clone()
+        plus[t, h, i] += 0.5
+        minus[t, h, i] -= 0.5
+        difference = sum(s * float((_turned(v, positions, frequency, layout, magnitude)[0]
+                                    * w.cpu().double()).sum())
+                         for s, v in ((1, plus), (-1, minus)))
+        # the two steps are exact to 2^-23 of x, the gradient to the bound above
+        assert abs(float(x.grad[t, h, i]) - difference) <= 2.0 ** -18 * magnitude
+    x.grad = None
+    at.rope(x, positions, frequency, layout=layout).sum().backward()   # a broadcast gradient
+    _check_turned(x.grad, torch.ones_like(w), positions, frequency, layout, sign=-1)
+
+
+# --------------------------------------------------------------------------- #
+# a batch with its cache
+# --------------------------------------------------------------------------- #
+class Batch:
+    """Random pages for a prefix and for each sequence, one page to spare on odd ones; cache
+    slots that no token has hold NaN."""
+
+    def __init__(self, dtype, heads, kv_heads, dim, page, prefix, lengths, counts, seed=0,
+                 spare=True):
+        g = self.g = _gen(seed)
+        self.dtype, self.heads, self.kv_heads, self.dim = dtype, heads, kv_heads, dim
+        self.page, self.prefix_length = page, prefix
+        self.lengths_host, self.counts = list(lengths), list(counts)
+        owned = [-(-max(0, n) // page) + (i % 2 if spare else 0) for i, n in enumerate(lengths)]
+        shared = -(-prefix // page)
+        self.pages = shared + sum(owned) + 2
+        order = torch.randperm(self.pages, generator=g, device="cuda")
+        self.prefix = order[:shared].contiguous()
+        self.indices = order[shared:shared + sum(owned)].contiguous()
+        self.indptr = self._ends(owned)
+        self.lengths = torch.tensor(self.lengths_host, dtype=torch.int64, device="cuda")
+        self.ends = self._ends(self.counts)
+        self.ends_host = [0] + np.cumsum(self.counts).tolist()
+        shape = (self.pages, page, kv_heads, dim)
+        self.kc = torch.full(shape, math.nan, device="cuda", dtype=dtype)
+        self.vc = torch.full(shape, math.nan, device="cuda", dtype=dtype)
+        tokens = sum(self.counts)
+        self.query = _normal(g, tokens, heads, dim, dtype=dtype)
+        self.key = _normal(g, tokens, kv_heads, dim, dtype=dtype)
+        self.value = _normal(g, tokens, kv_heads, dim, dtype=dtype)
+
+    @staticmethod
+    def _ends(n):
+        return torch.tensor([0] + list(np.cumsum(n)), dtype=torch.int64, device="cuda")
+
+    def places(self, b=None):
+        """(page, slot) of the prefix's keys, or of sequence b's."""
+        if b is None:
+            pages, n = self.prefix, self.prefix_length
+        else:
+            pages = self.indices[int(self.indptr[b]):int(self.indptr[b + 1])]
+            n = min(max(0, self.lengths_host[b]), pages.numel() * self.page)
+        at_ = torch.arange(n, device="cuda")
+        return pages[at_ // self.page], at_ % self.page
+
+    def fill(self):
+        for b in [None] + list(range(len(self.counts))):
+            page, slot = self.places(b)
+            for c in (self.kc, self.vc):
+                c[page, slot] = _normal(self.g, page.numel(), self.kv_heads, self.dim,
+                                        dtype=self.dtype)
+        return self
+
+    def attend(self, **more):
+        args = dict(query_indptr=self.ends, max_query=max(self.counts + [1]),
+                    max_length=max(self.lengths_host + [1]), return_lse=True)
+        if all(n == 1 for n in self.counts):
+            args["query_indptr"] = None
+        args.update(more)
+        return at.prefix_attention(self.query, self.kc, self.vc, self.prefix,
+                                   self.prefix_length, self.indptr, self.indices, self.lengths,
+                                   **args)
+
+    def want(self, scale=None):
+        """(out, lse, bound of |out|'s error, bound of lse's), 64 bits, on the CPU."""
+        scale = self.dim ** -0.5 if scale is None else scale
+        G = self.heads // self.kv_heads
+        T = sum(self.counts)
+        u = U[self.dtype]
+        out = torch.zeros(T, self.heads, self.dim, dtype=torch.float64)
+        lse = torch.full((T, self.heads), -math.inf, dtype=torch.float64)
+        eo, el = torch.zeros_like(out), torch.zeros_like(lse)
+        kp, vp = (c[self.places()].cpu().double() for c in (self.kc, self.vc))
+        q = self.query.cpu().double()
+        for b, n in enumerate(self.counts):
+            ko, vo = (c[self.places(b)].cpu().double() for c in (self.kc, self.vc))
+            for j in range(n):
+                t = self.ends_host[b] + j
+                see = min(max(0, self.lengths_host[b] - n + j + 1), ko.shape[0])
+                k, v = torch.cat([kp, ko[:see]]), torch.cat([vp, vo[:see]])
+                if not len(k):
+                    continue
+                for h in range(self.heads):
+                    kh, vh = k[:, h // G], v[:, h // G]
+                    s = scale * (kh @ q[t, h])
+                    es = self.dim * 2.0 ** -23 * scale * float((kh.abs() @ q[t, h].abs()).max())
+                    p = torch.softmax(s, 0)
+                    size = p @ vh.abs()
+                    out[t, h], lse[t, h] = p @ vh, torch.logsumexp(s, 0)
+                    el[t, h] = es + 2.0 ** -22 * (len(k) ** 0.5 + 4 + abs(float(lse[t, h])))
+                    eo[t, h] = (u * (size + out[t, h].abs()) + (2 * es + 2.0 ** -22 * len(k) ** 0.5)
+                                * size)
+                    if self.dtype == F16:
+                        eo[t, h] += 2.0 ** -25 * (vh.abs().sum(0) + 1)
+        return out, lse, eo * (1 + 2.0 ** -6), el
+
+    def check(self, got, scale=None):
+        out, lse, eo, el = self.want(scale)
+        o, e = got[0].cpu().double(), got[1].cpu().double()
+        assert torch.isfinite(o).all()
+        assert ((o - out).abs() <= eo).all(), float(((o - out).abs() / (eo + 1e-30)).max())
+        empty = lse == -math.inf
+        assert torch.equal(e == -math.inf, empty) and not o[empty].any()
+        assert ((e - lse)[~empty].abs() <= el[~empty]).all(), float(
+            ((e - lse).abs() / el)[~empty].max())
+
+
+ATTENTION = [
+    # heads, kv_heads, dim, page, prefix, lengths, counts
+    (1, 1, 8, 1, 1, [1], [1]),
+    (1, 1, 64, 16, 0, [1], [1]),
+    (4, 1, 40, 7, 33, [5, 0, 64], [1, 1, 1]),
+    (8, 2, 64, 16, 500, [60, 1, 17, 33], [1, 1, 1, 1]),
+    (6, 2, 80, 24, 31, [100, 24, 25], [1, 1, 1]),
+    (16, 1, 96, 24, 129, [40, 7, 90], [7, 1, 3]),
+    (5, 5, 72, 3, 64, [12, 30], [2, 9]),
+    (20, 1, 128, 16, 1000, [300, 2], [1, 2]),
+    (8, 8, 128, 32, 0, [200, 31, 0, 129], [1, 1, 1, 1]),
+    (3, 1, 136, 5, 77, [20, 41], [5, 0]),
+    (4, 2, 192, 16, 65, [70, 3], [33, 3]),
+    (2, 1, 256, 64, 700, [90, 200, 1], [17, 40, 1]),
+    (32, 8, 128, 16, 2100, [40] * 9, [1] * 9),
+    (16, 4, 128, 64, 600, [190, 77], [150, 70]),
+    (12, 4, 64, 16, 300, [64, 200, 33, 1], [64, 130, 20, 1]),
+    (8, 1, 64, 1, 40, [9, 4], [4, 4]),
+    # fewer tokens than new ones: the first see the prefix alone, or nothing
+    (4, 2, 64, 16, 20, [2, 0], [5, 3]),
+    (4, 2, 64, 16, 0, [2, 0], [5, 3]),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,prefix,lengths,counts", ATTENTION)
+def test_prefix_attention(hip_ready, dtype, heads, kv_heads, dim, page, prefix, lengths, counts):
+    b = Batch(dtype, heads, kv_heads, dim, page, prefix, lengths, counts, seed=dim).fill()
+    got = b.attend()
+    b.check(got)
+    # launch bounds below the truth are slower, not wrong; a run repeats bit for bit
+    b.check(b.attend(max_query=1, max_length=1))
+    again = b.attend()
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_hidden_keys_hold_anything(hip_ready, dtype):
+    """Infinities and NaN in keys and values that a row does not see, among them those of later
+    tokens of its own sequence, change nothing; those that it sees do."""
+    b = Batch(dtype, 4, 2, 64, 16, 40, [35, 9, 50], [6, 3, 20], seed=3).fill()
+    page, slot = b.places(0)
+    b.kc[page[-1], slot[-1]] = math.inf         # seen by the sequence's last token alone
+    b.vc[page[-1], slot[-1]] = math.nan
+    page, slot = b.places(2)
+    b.vc[page[-8], slot[-8], 0, 3] = -math.inf  # by its last eight, one element, one kv head
+    got, lse = b.attend()
+    clean = Batch(dtype, 4, 2, 64, 16, 40, [35, 9, 50], [6, 3, 20], seed=3).fill()
+    out, lse_want, eo, el = clean.want()
+    tainted = torch.zeros(out.shape, dtype=torch.bool)
+    tainted[5] = True
+    tainted[21:, :2, 3] = True
+    got = got.cpu().double()
+    assert ((got - out).abs() <= eo)[~tainted].all()
+    assert torch.isnan(got[5]).all()
+    assert (got[21:, :2, 3] == -math.inf).all()
+    rows = torch.arange(29) != 5
+    assert ((lse.cpu().double() - lse_want).abs() <= el)[rows].all()
+
+
+def test_scores_at_the_ends_of_the_range(hip_ready):
+    """Keys of -inf leave rows with no weight (0 and -inf, as a row without keys), the lowest
+    finite values do not; scores that climb through the whole range keep their softmax."""
+    b = Batch(BF16, 2, 1, 64, 16, 96, [40], [1], seed=4).fill()
+    b.query.fill_(1.0)
+    b.kc[b.places()] = -math.inf
+    b.kc[b.places(0)] = -math.inf
+    out, lse = b.attend()
+    assert not out.any() and (lse == -math.inf).all()
+    page, slot = b.places(0)
+    lowest = torch.finfo(BF16).min
+    b.kc[page[7], slot[7]] = 0.0
+    b.kc[page[7], slot[7], :, 0] = lowest       # one key with a finite score, far below all
+    out, lse = b.attend()
+    assert torch.equal(out[0], b.vc[page[7], slot[7], 0].expand(2, 64))
+    climb = Batch(F16, 3, 1, 64, 16, 700, [300], [1], seed=5).fill()
+    climb.query.fill_(1.0)
+    for place, lo, hi in ((climb.places(), -60.0, 20.0), (climb.places(0), 20.0, 90.0)):
+        n = place[0].numel()
+        climb.kc[place] = torch.linspace(lo, hi, n, device="cuda").to(F16)[:, None, None]
+    climb.check(climb.attend())
+    falling = Batch(BF16, 3, 1, 64, 16, 700, [300], [1], seed=6).fill()
+    falling.query.fill_(1.0)
+    page, slot = falling.places()
+    falling.kc[page, slot] = torch.linspace(90, -60, 700, device="cuda").to(BF16)[:, None, None]
+    falling.check(falling.attend())
+
+
+def test_pages_and_rows_that_point_nowhere(hip_ready):
+    """Pages outside the cache count as hidden, row pointers outside the list as its ends; a
+    length past a sequence's pages as their end; negative lengths as none."""
+    b = Batch(BF16, 4, 2, 64, 16, 64, [64, 64, 20, 7], [1, 1, 1, 1], seed=7, spare=False).fill()
+    b.prefix[1] = b.pages + 5
+    b.indices[1], b.indices[6] = -1, 2 ** 40
+    kc, vc = b.kc, b.vc
+    got, lse = b.attend()
+    # the same without those keys: all that is left stands on a prefix or a sequence of its own
+    for i, n in enumerate([64, 64, 20, 7]):
+        pages = torch.cat([b.prefix, b.indices[int(b.indptr[i]):int(b.indptr[i + 1])]]).cpu()
+        keys = torch.arange(64 + n)
+        page = pages[keys // 16]
+        fine = (page >= 0) & (page < b.pages)
+        k, v = (c.cpu()[page[fine], (keys % 16)[fine]].double() for c in (kc, vc))
+        for h in range(4):
+            s = k[:, h // 2] @ b.query[i, h].cpu().double() / 8
+            o = torch.softmax(s, 0) @ v[:, h // 2]
+            # the largest value is under 2^3: u of sums and results, twice
+            assert (got[i, h].cpu().double() - o).abs().max() <= 2.0 ** -5
+            assert abs(float(lse[i, h]) - float(torch.logsumexp(s, 0))) <= 2.0 ** -16
+    c = Batch(BF16, 4, 2, 64, 16, 0, [64, 64], [1, 1], seed=8, spare=False).fill()
+    c.lengths[0] = 1000         # 64 keys listed
+    full = c.attend(max_length=1000)
+    c.check(full)
+    c.lengths[1] = -5
+    out, lse = c.attend()
+    assert torch.equal(out[0], full[0][0]) and not out[1].any() and (lse[1] == -math.inf).all()
+    c.lengths[1] = 64
+    c.indptr[2] = 10 ** 12
+    assert torch.equal(c.attend()[0], full[0])
+    c.indptr[1] = -3            # sequence 0 has no pages, sequence 1 all of them
+    out, lse = c.attend()
+    assert not out[0].any() and (lse[0] == -math.inf).all() and torch.isfinite(out[1]).all()
+
+
+def test_strides_and_given_outputs(hip_ready):
+    """Caches as [pages, kv_heads, page, dim] and as halves of one array, queries of a packed
+    projection at odd offsets, an output with gaps."""
+    b = Batch(F16, 6, 2, 72, 16, 50, [40, 9], [2, 1], seed=9).fill()
+    want = b.attend()
+    b.check(want)
+    both = torch.zeros(b.pages, 2, b.kv_heads, 16, 74, device="cuda", dtype=F16)
+    k, v = both[:, 0, :, :, 1:73].transpose(1, 2), both[:, 1, :, :, 2:74].transpose(1, 2)
+    k.copy_(b.kc), v.copy_(b.vc)
+    packed = torch.zeros(3, 9, 73, device="cuda", dtype=F16)
+    packed[:, 1:7, 1:] = b.query
+    room = torch.zeros(3, 8, 80, device="cuda", dtype=F16)
+    out = room[:, 1:7, 3:75]
+    b.kc, b.vc, b.query = k, v, packed[:, 1:7, 1:]
+    got = b.attend(out=out)
+    assert got[0] is out and torch.equal(out, want[0]) and torch.equal(got[1], want[1])
+    out.zero_()
+    assert not room.any()
+    b.check(b.attend(scale=0.5), scale=0.5)
+
+
+def test_offsets_past_32_bits(hip_ready):
+    """Pages whose elements lie past 2^31, and 2^32 bytes, of the cache."""
+    pages, page, dim = 70000, 64, 256
+    kc = torch.empty(pages, page, 2, dim, device="cuda", dtype=BF16)      # 2.3 G elements
+    vc = torch.empty(pages, page, 2, dim, device="cuda", dtype=BF16)
+    b = Batch(BF16, 4, 2, dim, page, 100, [90, 3], [3, 2], seed=10)
+    b.prefix += pages - b.pages
+    b.indices += pages - b.pages
+    b.kc, b.vc, b.pages = kc, vc, pages
+    b.fill()
+    frequency, _ = at.rope_frequencies(dim)
+    at.paged_append(b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency,
+                    query_indptr=b.ends, offset=100)
+    for i in range(2):
+        at_, n = b.places(i), b.counts[i]
+        rows = slice(b.ends_host[i], b.ends_host[i + 1])
+        position = 100 + torch.arange(b.lengths_host[i] - n, b.lengths_host[i])
+        _check_turned(kc[at_][-n:], b.key[rows], position, frequency, "half")
+        assert torch.equal(vc[at_][-n:], b.value[rows])
+    b.check(b.attend())
+
+
+# --------------------------------------------------------------------------- #
+# append
+# --------------------------------------------------------------------------- #
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+@pytest.mark.parametrize("heads,kv_heads,dim,rotary,page,lengths,counts", [
+    (1, 1, 64, 64, 16, [1], [1]),
+    (0, 2, 128, 128, 16, [5, 33, 16], [1, 1, 1]),
+    (12, 4, 80, 38, 7, [30, 8, 50, 9], [30, 1, 0, 9]),
+    (3, 1, 17, 16, 1, [4, 9], [3, 2]),
+    (8, 8, 64, 0, 24, [200, 77], [150, 3]),
+    (4, 1, 256, 62, 64, [4200], [4200]),
+    (2, 2, 96, 96, 16, [3] * 150, [2] * 150),
+])
+def test_paged_append(hip_ready, layout, dtype, heads, kv_heads, dim, rotary, page, lengths,
+                      counts):
+    b = Batch(dtype, max(heads, 1), kv_heads, dim, page, 0, lengths, counts, seed=dim + page)
+    frequency, magnitude = at.rope_frequencies(rotary, scaling="linear", factor=2)
+    offset = 4097
+    kc, vc = b.kc.clone(), b.vc.clone()
+    query = at.paged_append(
+        b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency if rotary else None,
+        query=b.query if heads else None,
+        query_indptr=None if set(counts) == {1} else b.ends, offset=offset, layout=layout)
+    assert (query is None) == (heads == 0)
+    for i, n in enumerate(counts):
+        rows = slice(b.ends_host[i], b.ends_host[i + 1])
+        where = tuple(x[lengths[i] - n:] for x in b.places(i))
+        position = offset + torch.arange(lengths[i] - n, lengths[i])
+        _check_turned(kc[where], b.key[rows], position, frequency, layout)
+        assert torch.equal(vc[where], b.value[rows])
+        if heads:
+            _check_turned(query[rows], b.query[rows], position, frequency, layout)
+        kc[where] = math.nan
+        vc[where] = math.nan
+    assert torch.isnan(kc).all() and torch.isnan(vc).all()      # nothing else was written
+
+
+def test_paged_append_leaves_out_what_has_no_place(hip_ready):
+    b = Batch(BF16, 2, 1, 64, 16, 0, [40, 20, 17], [3, 18, 2], seed=11, spare=False)
+    frequency, _ = at.rope_frequencies(64)
+    b.lengths[1] = 50           # two pages hold 32: positions 32 .. 49 have none
+    b.indices[0] = -1           # not in use by the new tokens of sequence 0
+    b.indices[2] = b.pages      # positions 37 .. 39 of sequence 0
+    b.ends[3] = 22              # the last token belongs to no sequence
+    kc, vc = b.kc.clone(), b.vc.clone()
+    query = at.paged_append(b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency,
+                            query=b.query, query_indptr=b.ends)
+    written = ~torch.isnan(kc).flatten(1).any(1)
+    slots = (~torch.isnan(kc).any(-1).any(-1)).sum()
+    assert int(slots) == 1 and int(written.sum()) == 0       # sequence 2's one token
+    page = b.indices[int(b.indptr[2]) + 1]
+    assert torch.equal(vc[page, 0, 0], b.value[21, 0])
+    assert not query[22].any() and query[:22].any(-1).all()
+    out, lse = at.prefix_attention(b.query, kc, vc, b.prefix, 0, b.indptr, b.indices, b.lengths,
+                                   query_indptr=b.ends, max_query=18, max_length=50,
+                                   return_lse=True)
+    assert not out[22].any() and (lse[22] == -math.inf).all()
+
+
+# --------------------------------------------------------------------------- #
+# streams, graphs, refusals
+# --------------------------------------------------------------------------- #
+def _step(b, frequency):
+    q = at.paged_append(b.key, b.value, b.kc, b.vc, b.indptr, b.indices, b.lengths, frequency,
+                        query=b.query, query_indptr=b.ends, offset=b.prefix_length)
+    return at.prefix_attention(q, b.kc, b.vc, b.prefix, b.prefix_length, b.indptr, b.indices,
+                               b.lengths, query_indptr=b.ends, max_query=2, max_length=80)
+
+
+def test_other_streams(hip_ready):
+    """Two streams at work at once, each with a batch of its own."""
+    frequency, _ = at.rope_frequencies(64)
+    batches = [Batch(BF16, 8, 2, 64, 16, 3000, [70, 33], [2, 1], seed=s).fill() for s in (1, 2)]
+    want = [_step(b, frequency) for b in batches]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in batches]
+    got = [[], []]
+    for _ in range(20):
+        for s, b, to in zip(streams, batches, got):
+            with torch.cuda.stream(s):
+                to.append(_step(b, frequency))
+    torch.cuda.synchronize()
+    for w, outs in zip(want, got):
+        assert all(torch.equal(w, o) for o in outs)
+
+
+def test_in_a_graph(hip_ready):
+    """A captured step replayed with longer sequences each time, eager work between."""
+    frequency, _ = at.rope_frequencies(64)
+    b = Batch(BF16, 8, 2, 64, 16, 100, [80, 80], [2, 1], seed=12).fill()
+    eager = Batch(BF16, 8, 2, 64, 16, 100, [80, 80], [2, 1], seed=12).fill()
+    b.lengths -= 60
+    eager.lengths -= 60
+    _step(b, frequency)
+    _step(eager, frequency)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = _step(b, frequency)
+    for i in range(5):
+        b.lengths += 9
+        eager.lengths += 9
+        b.query.normal_(generator=_gen(i))
+        eager.query.copy_(b.query)
+        graph.replay()
+        want = _step(eager, frequency)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+    assert torch.equal(b.kc.nan_to_num(), eager.kc.nan_to_num())
+
+
+def test_nothing_to_do(hip_ready):
+    frequency, _ = at.rope_frequencies(64)
+    empty = torch.empty(0, 4, 64, device="cuda", dtype=BF16)
+    none = torch.empty(0, device="cuda", dtype=torch.int64)
+    assert at.rope(empty, none, frequency).shape == (0, 4, 64)
+    cache = torch.zeros(2, 16, 4, 64, device="cuda", dtype=BF16)
+    ends = torch.zeros(1, device="cuda", dtype=torch.int64)
+    q = at.paged_append(empty, empty, cache, cache.clone(), ends, none, none, frequency,
+                        query=empty)
+    assert q.shape == (0, 4, 64)
+    out, lse = at.prefix_attention(empty, cache, cache, none, 0, ends, none, none, max_length=1,
+                                   return_lse=True)
+    assert out.shape == (0, 4, 64) and lse.shape == (0, 4)
+    # a cache without pages: no row sees a key
+    b = Batch(BF16, 4, 2, 64, 16, 0, [5, 5], [1, 1])
+    b.kc, b.vc = b.kc[:0], b.vc[:0]
+    out, lse = b.attend()
+    assert not out.any() and (lse == -math.inf).all()
+
+
+def test_refusals(hip_ready):
+    frequency, _ = at.rope_frequencies(64)
+    x = torch.zeros(4, 2, 64, device="cuda", dtype=BF16)
+    pos = torch.arange(4, device="cuda")
+    for args, more in [
+            ((x.cpu(), pos, frequency), {}), ((x.double(), pos, frequency), {}),
+            ((x[0], pos, frequency), {}), ((x, pos[:3], frequency), {}),
+            ((x, pos.int(), frequency), {}), ((x, pos, frequency.float()), {}),
+            ((x, pos.cpu(), frequency), {}), ((x, pos, frequency), dict(layout="both")),
+            ((x[..., :32], pos, frequency), {}),                # rotary past the head
+            ((x.transpose(1, 2), pos, frequency[:1]), {}),      # heads not contiguous
+            ((x, pos, frequency), dict(out=x[:3])), ((x, pos, frequency), dict(out=x.float())),
+            ((x, pos, frequency), dict(out=x[:, :1].expand(4, 2, 64))),
+            ((x[:, :, :62], pos, frequency[:8]), dict(out=x[:, :, 2:])),    # overlaps
+            ((torch.zeros(1, 1, 1025, device="cuda"), pos[:1], frequency), {}),
+            ((x.float().requires_grad_(), pos, frequency), dict(out=x.float()))]:
+        with pytest.raises(ValueError):
+            at.rope(*args, **more)
+    b = Batch(BF16, 4, 2, 64, 16, 32, [20, 9], [1, 1]).fill()
+
+    def append(**change):
+        a = dict(key=b.key, value=b.value, key_cache=b.kc, value_cache=b.vc, indptr=b.indptr,
+                 indices=b.indices, lengths=b.lengths, frequency=frequency, query=b.query)
+        a.update(change)
+        return at.paged_append(**a)
+
+    def attend(**change):
+        a = dict(query=b.query, key_cache=b.kc, value_cache=b.vc, prefix=b.prefix,
+                 prefix_length=32, indptr=b.indptr, indices=b.indices, lengths=b.lengths,
+                 max_length=20)
+        a.update(change)
+        return at.prefix_attention(**a)
+
+    append(), attend()
+    for change in [dict(key=b.key[:1]), dict(value=b.value.half()), dict(value_cache=b.vc[:1]),
+                   dict(key_cache=b.kc[..., :32]), dict(indptr=b.indptr[:2]),
+                   dict(lengths=b.lengths[:1]), dict(lengths=b.lengths.int()),
+                   dict(indices=b.indices.float()), dict(query=b.query[:1]),
+                   dict(query_out=b.query[:1]), dict(query=None, query_out=b.query),
+                   dict(query_indptr=b.indptr[:2]), dict(layout="neither"),
+                   dict(key_cache=b.kc[:1].expand(b.kc.shape)),
+                   dict(frequency=torch.zeros(40, device="cuda", dtype=torch.float64))]:
+        with pytest.raises(ValueError):
+            append(**change)
+    for change in [dict(query=b.query.float()), dict(query=b.query[..., :32]),
+                   dict(query=b.query[:, :3]), dict(key_cache=b.kc.half()),
+                   dict(value_cache=b.vc[:, :8]), dict(prefix=b.prefix[:1]),
+                   dict(prefix_length=33), dict(prefix_length=-1), dict(max_length=-1),
+                   dict(scale=0.0), dict(scale=-1.0), dict(scale=math.nan),
+                   dict(scale=math.inf), dict(indptr=b.indptr[1:]), dict(lengths=b.lengths[:1]),
+                   dict(out=b.query[:1]), dict(out=b.query[:, :1].expand(2, 4, 64)),
+                   dict(query_indptr=b.indptr.int()), dict(max_length=2 ** 40),
+                   dict(query=torch.zeros(2, 4, 12, device="cuda", dtype=BF16),
+                        key_cache=b.kc[..., :12], value_cache=b.vc[..., :12]),
+                   dict(query=torch.zeros(2, 4, 264, device="cuda", dtype=BF16),
+                        key_cache=torch.zeros(9, 16, 2, 264, device="cuda", dtype=BF16),
+                        value_cache=torch.zeros(9, 16, 2, 264, device="cuda", dtype=BF16))]:
+        with pytest.raises(ValueError):
+            attend(**change)
+    append(), attend()
+
+
+def test_the_sparse_kernels_give_the_same(hip_ready):
+    """The same attention through this package's own SDDMM and SpMM, in 64 bits: the page
+    table as a CSR pattern over cache slots, one row a token."""
+    import scipy.sparse as sp
+
+    from tilegen_amd.schedules import TUNED
+    from tilegen_amd.variant import Variant
+    b = Batch(BF16, 1, 1, 64, 16, 90, [50, 3, 0, 16], [1, 1, 1, 1], seed=13).fill()
+    out, _ = b.attend()
+    rows, cols = [], []
+    for i in range(4):
+        for page, slot in (b.places(), b.places(i)):
+            cols.append((page * 16 + slot).cpu().numpy())
+            rows.append(np.full(page.numel(), i))
+    rows, cols = np.concatenate(rows), np.concatenate(cols)
+    A = sp.csr_matrix((np.full(rows.size, 1 / 8), (rows, cols)), shape=(4, b.pages * 16))
+    A.sort_indices()
+    K, V = (np.nan_to_num(c.cpu().double().numpy()).reshape(-1, 64) for c in (b.kc, b.vc))
+    Q = b.query[:, 0].cpu().double().numpy()
+    S = Variant("sddmm", TUNED["c5"]).run(A, U=Q, V=K)
+    P = A.copy()
+    for i in range(4):
+        s = S[A.indptr[i]:A.indptr[i + 1]]
+        e = np.exp(s - s.max())
+        P.data[A.indptr[i]:A.indptr[i + 1]] = e / e.sum()
+    want = Variant("spmm", TUNED["c4"]).run(P, B=V)
+    bound = b.want()[2][:, 0].numpy()
+    assert (np.abs(out[:, 0].cpu().double().numpy() - want) <= bound).all()

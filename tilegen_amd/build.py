@@ -4,7 +4,8 @@
    C++ compiler against the ROCm HIP runtime and hipRTC;
 2. ``libtg_vendor.so``, the rocSPARSE comparison (when rocSPARSE is installed),
    ``tilegen_bench``, the native host harness (TGM1 matrix + variant library),
-   and ``libtgna.so`` (hipcc), the SpMV entry point that allocates nothing;
+   ``libtgna.so`` (hipcc), the SpMV entry point that allocates nothing, and
+   ``libtgattn.so`` (hipcc), attention over a paged cache;
 3. the test oracle (``oracle/Makefile``: the C restatement, and the
    reference's own ref.cpp where its sources are present);
 4. the hipRTC code objects and C launchers of every named schedule
@@ -20,6 +21,7 @@ import shutil
 import subprocess
 import sys
 import time
+from concurrent.futures import ThreadPoolExecutor
 from typing import List, Optional
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -137,6 +139,50 @@ def noalloc_code_object(out: str) -> str:
     return out
 
 
+def attention_sources() -> List[str]:
+    src = os.path.join(PKG, "csrc", "attention")
+    return [os.path.join(src, f) for f in sorted(os.listdir(src)) if f.endswith(".hip")]
+
+
+def _attention_compile(source: str) -> List[str]:
+    """hipcc and the compile flags of one of libtgattn.so's sources."""
+    from .verify import hip_arch
+    return [os.path.join(ROCM, "bin", "hipcc"), "--offload-arch=%s" % hip_arch(), "-O3",
+            "-std=c++17", "-fPIC", "-fvisibility=hidden",
+            "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+            "-I", os.path.join(REPO, "include"), "-c", source]
+
+
+def build_attention() -> str:
+    """libtgattn.so: attention over a paged cache (include/tilegen_attention.h), hipcc for
+    gfx950, its sources side by side."""
+    lib_dir = os.path.join(PKG, "_lib")
+    obj_dir = os.path.join(REPO, "build", "attention")
+    os.makedirs(obj_dir, exist_ok=True)
+    out = os.path.join(lib_dir, "libtgattn.so")
+    tmp = out + ".tmp%d" % os.getpid()
+
+    def one(source: str) -> str:
+        obj = os.path.join(obj_dir, os.path.basename(source)[:-len(".hip")] + ".o")
+        _run(_attention_compile(source) + ["-o", obj])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objects = list(pool.map(one, attention_sources()))
+    _run([os.path.join(ROCM, "bin", "hipcc"), "-shared", "-o", tmp] + objects +
+         ["-L", lib_dir, "-ltgrt", "-Wl,-rpath," + lib_dir])
+    os.replace(tmp, out)
+    return out
+
+
+def attention_code_object(source: str, out: str) -> str:
+    """The device code object alone of one of libtgattn.so's sources, for checks of its
+    kernels' registers and spills."""
+    _run(_attention_compile(source) + ["--offload-device-only", "--no-gpu-bundle-output",
+                                       "-o", out])
+    return out
+
+
 def build_oracle(force: bool = False) -> None:
     _run(["make", "-s"] + (["-B"] if force else []) + ["-C", os.path.join(REPO, "oracle")])
 
@@ -208,6 +254,9 @@ def build_all(verbose: bool = True, force: bool = False) -> None:
     build_noalloc()
     if verbose:
         print("[build] no-alloc SpMV library (%.1fs)" % (time.time() - t0))
+    build_attention()
+    if verbose:
+        print("[build] attention library (%.1fs)" % (time.time() - t0))
     build_oracle(force)
     if force:
         from .verify import cache_dir

@@ -1,0 +1,3 @@
+#include "narrow.h"
+
+template hipError_t tg::launch_narrow<128>(const Attention&, int64_t, int, bool, hipStream_t);

@@ -1,0 +1,240 @@
+// launch_prefix_attention: how a call is split into parts, and the kernel that joins them.
+#include "prefix_attention.h"
+
+namespace tg {
+namespace {
+
+// Joins the parts of each row: M = max m_s, then sum 2^(m_s - M) O_s over sum 2^(m_s - M) l_s.
+// One wave has one row; lanes hold four elements of the head each, and where a head takes 16 or
+// 32 lanes the rest read other parts at the same time (LANES: lanes of one part).
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void join_parts(Attention a) {
+  const int lane = threadIdx.x & 63;
+  const i64 rows = static_cast<i64>(a.tokens) * a.heads;
+  const i64 row = static_cast<i64>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (row >= rows) return;
+  const int t = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<i64>(t) * a.heads);
+  const int b = a.ends ? sequence_of(a.ends, a.sequences, t) : t;
+  int parts = a.prefix_splits;
+  bool owned = b < a.sequences;
+  if (owned && a.own_splits) {
+    const Sequence s = sequence(a, b);
+    parts += own_parts(a, seen(s, t - s.first));
+  }
+  if (!owned) parts = 0;
+  float top = -INFINITY;
+  for (int s = lane; s < parts; s += 64) top = fmaxf(top, a.part_ml[s * rows + row].x);
+  for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
+  const int d = (lane % LANES) * 4;
+  float total = 0.f;
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (d < a.dim) {
+    for (int s = lane / LANES; s < parts; s += 64 / LANES) {
+      const float2 ml = a.part_ml[s * rows + row];
+      if (ml.x == -INFINITY) continue;
+      const float f = exp2f(ml.x - top);
+      const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + row) * a.dim + d);
+      total += ml.y * f;
+      sum[0] += v.x * f;
+      sum[1] += v.y * f;
+      sum[2] += v.z * f;
+      sum[3] += v.w * f;
+    }
+  }
+  for (int x = LANES; x < 64; x <<= 1) {
+    total += __shfl_xor(total, x);
+    for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor(sum[i], x);
+  }
+  if (lane < LANES && d < a.dim) {
+    T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + d;
+    const float f = total == 0.f ? 0.f : 1.f / total;
+    for (int i = 0; i < 4; ++i) out[i] = static_cast<T>(total == 0.f ? 0.f : sum[i] * f);
+  }
+  if (lane == 0 && a.lse) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+}
+
+int compute_units() {
+  static thread_local int cus[64] = {};
+  int device = 0;
+  if (hipGetDevice(&device) != hipSuccess || device < 0 || device >= 64) return 256;
+  if (!cus[device]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, device) != hipSuccess ||
+        n < 1)
+      n = 256;
+    cus[device] = n;
+  }
+  return cus[device];
+}
+
+struct Plan {
+  Attention a;
+  int prefix_nt, own_nt;
+  int64_t bytes;
+};
+
+int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
+
+int check(const tg_prefix_attention* r) {
+  const char* what = "launch_prefix_attention";
+  if (!r) return refuse(-1, what, "null arguments", 0);
+  if (r->dtype != TG_BF16 && r->dtype != TG_F16)
+    return refuse(-1, what, "dtype must be bfloat16 or float16", r->dtype);
+  if (r->dim < 8 || r->dim > 256 || r->dim % 8)
+    return refuse(-1, what, "dim must be a multiple of 8 up to 256", r->dim);
+  if (r->tokens < 0 || r->sequences < 0 || r->pages < 0 || r->n_prefix < 0 || r->n_indices < 0 ||
+      r->prefix_length < 0 || r->max_query < 0 || r->max_length < 0)
+    return refuse(-1, what, "negative size", 0);
+  if (r->kv_heads < 1 || r->heads < r->kv_heads || r->heads % r->kv_heads)
+    return refuse(-1, what, "heads must be a multiple of kv_heads", r->heads);
+  if (r->page < 1 || r->page > INT32_MAX)
+    return refuse(-1, what, "page must be 1 to 2^31 - 1", r->page);
+  if (!(r->scale > 0) || !(r->scale < 1e30))
+    return refuse(-1, what, "scale must be positive and finite", 0);
+  if (r->n_prefix < (r->prefix_length + r->page - 1) / r->page)
+    return refuse(-1, what, "prefix_length is past the prefix's pages", r->prefix_length);
+  if (r->prefix_length > INT32_MAX / 2 || r->max_length > INT32_MAX / 2)
+    return refuse(-2, what, "more than 2^30 keys", r->prefix_length);
+  if (r->tokens > 0x1000000 || r->sequences > 0x1000000 ||
+      r->tokens * r->heads > 0x4000000 || r->heads > 0x10000)
+    return refuse(-2, what, "more than 2^26 rows or 2^24 sequences", r->tokens);
+  if (!r->query_indptr && r->tokens > r->sequences)
+    return refuse(-1, what, "more tokens than sequences without query_indptr", r->tokens);
+  return 0;
+}
+
+int plan(const tg_prefix_attention* r, Plan* p) {
+  if (const int rc = check(r)) return rc;
+  Attention& a = p->a;
+  a = Attention{};
+  a.q = r->query;
+  a.k = r->key_cache;
+  a.v = r->value_cache;
+  a.prefix = r->prefix;
+  a.indptr = r->indptr;
+  a.indices = r->indices;
+  a.lengths = r->lengths;
+  a.ends = r->query_indptr;
+  a.out = r->out;
+  a.lse = r->lse;
+  a.q_token = r->query_token;
+  a.q_head = r->query_head;
+  a.o_token = r->out_token;
+  a.o_head = r->out_head;
+  a.kc_page = r->kc_page;
+  a.kc_slot = r->kc_slot;
+  a.kc_head = r->kc_head;
+  a.vc_page = r->vc_page;
+  a.vc_slot = r->vc_slot;
+  a.vc_head = r->vc_head;
+  a.pages = r->pages;
+  a.n_indices = r->n_indices;
+  a.tokens = static_cast<int>(r->tokens);
+  // without query_indptr sequence b is token b: those past the tokens have none
+  a.sequences = static_cast<int>(r->query_indptr ? r->sequences : r->tokens);
+  a.heads = static_cast<int>(r->heads);
+  a.kv_heads = static_cast<int>(r->kv_heads);
+  a.group = a.heads / a.kv_heads;
+  a.dim = static_cast<int>(r->dim);
+  a.page = static_cast<int>(r->page);
+  a.prefix_length = r->pages ? static_cast<int>(r->prefix_length) : 0;
+  a.scale = static_cast<float>(r->scale * 1.4426950408889634);
+  a.by_group = Div(a.group);
+  a.by_page = Div(a.page);
+  p->bytes = 0;
+  if (a.tokens == 0) return 0;
+  const int64_t want = 2 * compute_units();
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
+  p->prefix_nt = rows <= 16 ? 1 : 2;
+  a.prefix_tiles = static_cast<int>((rows + 16 * p->prefix_nt - 1) / (16 * p->prefix_nt));
+  if (a.prefix_length) {
+    const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
+    const int64_t most = (a.prefix_length + 255) / 256;
+    int64_t splits = (want + units - 1) / units;
+    splits = splits < most ? splits : most;
+    a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
+    a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
+  }
+  const int64_t max_query = r->query_indptr ? (r->max_query > 0 ? r->max_query : 1) : 1;
+  const int64_t own_rows = max_query * a.group;
+  p->own_nt = own_rows <= 16 ? 1 : 2;
+  if (a.pages && a.n_indices && a.sequences) {
+    int64_t tiles = (own_rows + 16 * p->own_nt - 1) / (16 * p->own_nt);
+    tiles = tiles < 4096 ? tiles : 4096;
+    a.own_tiles = static_cast<int>(tiles);
+    const int64_t length = r->max_length > 0 ? r->max_length : 1;
+    const int64_t units = tiles * a.kv_heads * a.sequences;
+    const int64_t most = (length + 255) / 256;
+    int64_t splits = (want + units - 1) / units;
+    splits = splits < most ? splits : most;
+    a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
+    a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
+  }
+  a.slots = a.prefix_splits + a.own_splits;
+  const i64 all = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;
+  const i64 first = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 8) * a.prefix_tiles;
+  if (all > 0xFFFFFF || first > 0xFFFFFF)
+    return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups", all > first ? all : first);
+  p->bytes = static_cast<int64_t>(a.slots) * a.tokens * a.heads * (a.dim + 2) * 4;
+  return 0;
+}
+
+hipError_t launch_parts(const Attention& a, int64_t dtype, int nt, bool prefix, hipStream_t s) {
+  if (a.dim <= 64) return launch_narrow<64>(a, dtype, nt, prefix, s);
+  if (a.dim <= 96) return launch_narrow<96>(a, dtype, nt, prefix, s);
+  if (a.dim <= 128) return launch_narrow<128>(a, dtype, nt, prefix, s);
+  return launch_narrow<256>(a, dtype, nt, prefix, s);
+}
+
+template <typename T>
+const void* join_of(int dim) {
+  if (dim <= 64) return reinterpret_cast<const void*>(&join_parts<T, 16>);
+  if (dim <= 128) return reinterpret_cast<const void*>(&join_parts<T, 32>);
+  return reinterpret_cast<const void*>(&join_parts<T, 64>);
+}
+
+}  // namespace
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" __attribute__((visibility("default"))) int64_t prefix_attention_workspace(
+    const tg_prefix_attention* r) {
+  Plan p;
+  if (const int rc = plan(r, &p)) return rc < 0 ? rc : -1;
+  return p.bytes;
+}
+
+extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
+    const tg_prefix_attention* r, void* stream) {
+  const char* what = "launch_prefix_attention";
+  Plan p;
+  if (const int rc = plan(r, &p)) return rc;
+  Attention& a = p.a;
+  if (a.tokens == 0) return 0;
+  if (!r->query || !r->out || !r->indptr || !r->lengths || (r->n_indices && !r->indices) ||
+      (r->prefix_length && !r->prefix) || (r->pages && (!r->key_cache || !r->value_cache)))
+    return refuse(-1, what, "null array", r->tokens);
+  if (r->workspace_bytes < p.bytes || (p.bytes && !r->workspace))
+    return refuse(-1, what, "the workspace is too small; bytes needed", p.bytes);
+  if (reinterpret_cast<uintptr_t>(r->workspace) % 16)
+    return refuse(-1, what, "the workspace is not 16-byte aligned", 0);
+  a.part = static_cast<float*>(r->workspace);
+  a.part_ml = reinterpret_cast<float2*>(a.part + static_cast<int64_t>(a.slots) * a.tokens *
+                                                     a.heads * a.dim);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (a.prefix_splits) {
+    const hipError_t e = launch_parts(a, r->dtype, p.prefix_nt, true, s);
+    if (e != hipSuccess) return hip_failed(e, what);
+  }
+  if (a.own_splits) {
+    const hipError_t e = launch_parts(a, r->dtype, p.own_nt, false, s);
+    if (e != hipSuccess) return hip_failed(e, what);
+  }
+  const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+  void* args[] = {&a};
+  const hipError_t e = hipLaunchKernel(
+      r->dtype == TG_F16 ? join_of<_Float16>(a.dim) : join_of<__bf16>(a.dim),
+      dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), args, 0, s);
+  return e == hipSuccess ? 0 : hip_failed(e, what);
+}
