@@ -13,88 +13,9 @@
 // is the same.  So most tiles need neither the exchange between lanes nor the rescaling.
 #pragma once
 
-#include "prefix_attention.h"
+#include "parts.h"
 
 namespace tg {
-
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-typedef short s16x8 __attribute__((ext_vector_type(8)));
-
-template <typename T>
-struct Matrix;
-
-template <>
-struct Matrix<__bf16> {
-  typedef __bf16 x8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mul16(s16x8 a, s16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(x8, a),
-                                                   __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  }
-  static constexpr short kExponent = 0x7F80;
-};
-
-template <>
-struct Matrix<_Float16> {
-  typedef _Float16 x8 __attribute__((ext_vector_type(8)));
-  static __device__ __forceinline__ f32x4 mul16(s16x8 a, s16x8 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(x8, a),
-                                                  __builtin_bit_cast(x8, b), c, 0, 0, 0);
-  }
-  static constexpr short kExponent = 0x7C00;
-};
-
-// A value of the other half of the wave, and of the other half of each half, beside one's own:
-// the pair holds both, in either order.
-struct Both {
-  float a, b;
-};
-__device__ __forceinline__ Both halves(float v) {
-  const unsigned x = __builtin_bit_cast(unsigned, v);
-  const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-  const unsigned a = r[0], b = r[1];
-  return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
-}
-__device__ __forceinline__ Both quarters(float v) {
-  const unsigned x = __builtin_bit_cast(unsigned, v);
-  const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-  const unsigned a = r[0], b = r[1];
-  return {__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
-}
-
-// The larger, and the sum, of a value over the four lanes that hold one row.
-__device__ __forceinline__ float row_max(float v) {
-  const Both h = halves(v);
-  const Both q = quarters(fmaxf(h.a, h.b));
-  return fmaxf(q.a, q.b);
-}
-__device__ __forceinline__ float row_sum(float v) {
-  const Both h = halves(v);
-  const Both q = quarters(h.a + h.b);
-  return q.a + q.b;
-}
-
-constexpr int kWaves = 4;
-constexpr float kSlack = 8.f;   // log2 of how far scores may pass the running maximum
-// Scores times scale less the maximum is one fused operation, exact in the product where the
-// maximum has been rounded.  Past this the rounding, 2^-24 of it, is no longer small against
-// one, and the product is rounded too.
-constexpr float kHuge = 16777216.f;
-__device__ __forceinline__ float apart(float s, float scale, float base) {
-#pragma clang fp contract(off)
-  const float x = s * scale;
-  return x - base;
-}
-
-// Rows and keys of one workgroup's part.
-struct Part {
-  const int64_t* list;  // pages
-  int k0, k1;           // keys, k0 < k1, all of them on the list
-  int row0, rows;       // its first row and the end of all rows (row = token * group + head)
-  int token0;
-  int before, step;     // the row of token j sees min(k1, before + step j) keys
-  int slot;
-};
 
 template <int DP, int NT>
 struct NarrowLds {
@@ -278,14 +199,12 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
       l[nt] += sum;
     }
     __builtin_amdgcn_wave_barrier();
-    typedef __attribute__((address_space(3))) s16x4 Lds4;
-    char* from = values + (4 * quad + (col >> 2)) * L::kRow + (col & 3) * 8;
+    const char* from = values + (4 * quad + (col >> 2)) * L::kRow + (col & 3) * 8;
     if (!strange) {
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(from + 32 * d));
-        const s16x4 hi =
-            __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(from + 32 * d + 16 * L::kRow));
+        const s16x4 lo = transposed(from + 32 * d);
+        const s16x4 hi = transposed(from + 32 * d + 16 * L::kRow);
         const s16x8 vt = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) o[nt][d] = M::mul16(vt, prob[nt], o[nt][d]);
@@ -298,9 +217,8 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
         const int mine = key < 16 ? key - 4 * quad : key - 16 - 4 * quad;
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(from + 32 * d));
-          const s16x4 hi =
-              __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds4*)(from + 32 * d + 16 * L::kRow));
+          const s16x4 lo = transposed(from + 32 * d);
+          const s16x4 hi = transposed(from + 32 * d + 16 * L::kRow);
           s16x8 vt = s16x8(0);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {

@@ -70,9 +70,11 @@ __device__ __forceinline__ int own_parts(const Attention& a, int keys) {
   return n < a.own_splits ? n : a.own_splits;
 }
 
-// Enqueues the parts of the prefix (or of the own pages) for one padded head size.
+// Enqueue the parts of the prefix (or of the own pages) for one padded head size.
 template <int DP>
 hipError_t launch_narrow(const Attention& a, int64_t dtype, int nt, bool prefix,
                          hipStream_t stream);
+template <int DP>
+hipError_t launch_wide(const Attention& a, int64_t dtype, bool prefix, hipStream_t stream);
 
 }  // namespace tg

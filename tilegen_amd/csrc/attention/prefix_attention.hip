@@ -75,6 +75,10 @@ struct Plan {
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
+// 16-row tiles of a narrow wave for that many query rows to the same keys, or 0: wide.
+int rows_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 0; }
+int tile_rows(int nt) { return nt ? 16 * nt : 128; }
+
 int check(const tg_prefix_attention* r) {
   const char* what = "launch_prefix_attention";
   if (!r) return refuse(-1, what, "null arguments", 0);
@@ -145,21 +149,22 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   if (a.tokens == 0) return 0;
   const int64_t want = 2 * compute_units();
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
-  p->prefix_nt = rows <= 16 ? 1 : 2;
-  a.prefix_tiles = static_cast<int>((rows + 16 * p->prefix_nt - 1) / (16 * p->prefix_nt));
+  p->prefix_nt = rows_tiles(rows);
+  const int prefix_rows = tile_rows(p->prefix_nt);
+  a.prefix_tiles = static_cast<int>((rows + prefix_rows - 1) / prefix_rows);
   if (a.prefix_length) {
     const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
     const int64_t most = (a.prefix_length + 255) / 256;
-    int64_t splits = (want + units - 1) / units;
-    splits = splits < most ? splits : most;
+    int64_t splits = want / units;
+    splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
     a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
   }
   const int64_t max_query = r->query_indptr ? (r->max_query > 0 ? r->max_query : 1) : 1;
   const int64_t own_rows = max_query * a.group;
-  p->own_nt = own_rows <= 16 ? 1 : 2;
+  p->own_nt = rows_tiles(own_rows);
   if (a.pages && a.n_indices && a.sequences) {
-    int64_t tiles = (own_rows + 16 * p->own_nt - 1) / (16 * p->own_nt);
+    int64_t tiles = (own_rows + tile_rows(p->own_nt) - 1) / tile_rows(p->own_nt);
     tiles = tiles < 4096 ? tiles : 4096;
     a.own_tiles = static_cast<int>(tiles);
     const int64_t length = r->max_length > 0 ? r->max_length : 1;
@@ -179,11 +184,16 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   return 0;
 }
 
+template <int DP>
 hipError_t launch_parts(const Attention& a, int64_t dtype, int nt, bool prefix, hipStream_t s) {
-  if (a.dim <= 64) return launch_narrow<64>(a, dtype, nt, prefix, s);
-  if (a.dim <= 96) return launch_narrow<96>(a, dtype, nt, prefix, s);
-  if (a.dim <= 128) return launch_narrow<128>(a, dtype, nt, prefix, s);
-  return launch_narrow<256>(a, dtype, nt, prefix, s);
+  return nt ? launch_narrow<DP>(a, dtype, nt, prefix, s) : launch_wide<DP>(a, dtype, prefix, s);
+}
+
+hipError_t launch_parts(const Attention& a, int64_t dtype, int nt, bool prefix, hipStream_t s) {
+  if (a.dim <= 64) return launch_parts<64>(a, dtype, nt, prefix, s);
+  if (a.dim <= 96) return launch_parts<96>(a, dtype, nt, prefix, s);
+  if (a.dim <= 128) return launch_parts<128>(a, dtype, nt, prefix, s);
+  return launch_parts<256>(a, dtype, nt, prefix, s);
 }
 
 template <typename T>
