@@ -19,19 +19,35 @@ namespace tg {
 template <int DP>
 struct Wide {
   static constexpr int kRows = 128, kKeys = 64;
-  static constexpr int kSlots = DP == 96 ? 16 : DP / 8;     // 16-byte chunks of a row, padded
-  static constexpr int kLoads = kKeys * kSlots / 256;       // of each thread, keys and values
-  static constexpr int kPass = 256 / kSlots;                // rows that one load of all covers
-  // LDS rows.  Keys are read 16 bytes of 8 rows at a time: 16 bytes more than a power of two
-  // spread them over all banks.  Values are read as 64 bytes of 4 rows: 64 bytes more.
-  static constexpr int kKeyRow = DP * 2 + 16;
-  static constexpr int kValueRow = DP == 96 ? 192 : DP * 2 + 64;
-  static constexpr int kBuffer = kKeys * (kKeyRow + kValueRow);
+  static constexpr int kPitch = DP == 64 ? 128 : DP == 256 ? 512 : 256;   // bytes of an LDS row
+  static constexpr int kChunks = kPitch / 16;
+  static constexpr int kLoads = kKeys * kChunks / 256;    // of each thread, keys and values
+  static constexpr int kPass = 256 / kChunks;             // rows that one load of all covers
+  static constexpr int kTile = kKeys * kPitch;
+  static constexpr int kBuffer = 2 * kTile;               // keys, then values
   static constexpr int kPerCu = DP == 256 ? 1 : 2;
+
+  // Loads go straight to LDS, 16 bytes a lane side by side, so rows cannot be padded; instead a
+  // row's chunks change places, and a lane fetches the chunk that belongs to its place.  Keys
+  // are read as one chunk of 8 rows at a time, values as 4 chunks of 4 rows: with these
+  // either is spread over all 64 banks.
+  static __device__ __forceinline__ int key_place(int row) {
+    return kPitch == 128 ? row >> 1 & 7 : row & 15;
+  }
+  static __device__ __forceinline__ int value_place(int row) {
+    return kPitch == 128 ? (row >> 1 & 1) << 2 : (row & 3) << 2;
+  }
 };
 
-// Addresses of a tile's rows.  EVEN: pages hold whole groups of 16 keys, so that a wave's rows of
-// one load stand on one page: its number and offset are uniform.
+// 16 bytes of every active lane to LDS at `to` + 16 * lane, without a register between.
+__device__ __forceinline__ void load_to_lds(const void* from, char* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) unsigned*)from,
+      (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
+}
+
+// EVEN: pages hold whole groups of 16 keys, so that a wave's rows of one load stand on one page
+// and its number is uniform.
 template <typename T, int DP, bool EVEN, bool OWN>
 __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int kv_head,
                                           char* lds) {
@@ -39,7 +55,8 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   using M = Matrix<T>;
   using C = Chunk<T>;
   constexpr int KS = DP / 16, DT = DP / 32;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
 
   // queries: the B operand, elements 16 s + 8 half .. of row col
@@ -61,72 +78,67 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   }
   const int all = min(p.before + p.step * static_cast<int>(a.by_group(p.row0)), p.k1);
 
-  // this thread's chunk of rows first + kPass i of a tile
-  const int chunk = tid % W::kSlots, first = tid / W::kSlots;
-  const bool mine = chunk * 8 < a.dim;
-  const T* kc = static_cast<const T*>(a.k) + kv_head * a.kc_head + chunk * 8;
-  const T* vc = static_cast<const T*>(a.v) + kv_head * a.vc_head + chunk * 8;
+  // this thread's place in rows first + kPass i of a tile, and the chunks that belong there
+  const int place = tid % W::kChunks, first = tid / W::kChunks;
+  const T* kc = static_cast<const T*>(a.k) + kv_head * a.kc_head;
+  const T* vc = static_cast<const T*>(a.v) + kv_head * a.vc_head;
   const int tiles = (p.k1 - p.k0 + W::kKeys - 1) / W::kKeys;
 
-  i64 pg[W::kLoads];
-  int slot[W::kLoads];
-  unsigned long long gone;      // keys of the tile in the registers that have no page
-  auto find = [&](int tile) {
+  // The pages of a tile's keys, lane = key: asked for two tiles ahead and before the tile's own
+  // loads, since loads return in order.  Keys past the end stand for the last one (hidden).
+  auto pages_of = [&](int tile) {
+    return p.list[a.by_page(min(p.k0 + tile * W::kKeys + lane, p.k1 - 1))];
+  };
+  unsigned key_at[2], value_at[2];    // EVEN: bytes from a group's first row to this lane's place
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = first + W::kPass * i;
+    key_at[i] = (r & 15) * static_cast<unsigned>(a.kc_slot) * 2 + (place ^ W::key_place(r)) * 16;
+    value_at[i] =
+        (r & 15) * static_cast<unsigned>(a.vc_slot) * 2 + (place ^ W::value_place(r)) * 16;
+  }
+  auto load = [&](int tile, i64 pages) {
+    char* to = lds + (tile & 1) * W::kBuffer + wave * 1024;
     const int key0 = p.k0 + tile * W::kKeys;
+    const bool tail = key0 + W::kKeys > p.k1;
 #pragma unroll
     for (int i = 0; i < W::kLoads; ++i) {
+      const int r = first + W::kPass * i;
+      const int kd = (place ^ W::key_place(r)) * 8, vd = (place ^ W::value_place(r)) * 8;
+      i64 page;
+      const char *ka, *va;
       if (EVEN) {
-        const int group = __builtin_amdgcn_readfirstlane((first + W::kPass * i) & ~15);
+        const int group = __builtin_amdgcn_readfirstlane(r & ~15);
+        page = static_cast<i64>(
+            static_cast<uint64_t>(
+                static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(pages >> 32), group)))
+                << 32 |
+            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(pages), group)));
         const int key = min(key0 + group, (p.k1 - 1) & ~15);
-        const int nth = a.by_page(key);
-        slot[i] = key - nth * a.page + min((first + W::kPass * i) & 15, p.k1 - 1 - key);
-        pg[i] = p.list[nth];
+        const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
+        unsigned kat = key_at[i & 1], vat = value_at[i & 1];
+        if (tail) {
+          const unsigned in = min(r & 15, p.k1 - 1 - key);
+          kat = in * static_cast<unsigned>(a.kc_slot) * 2 + kd * 2;
+          vat = in * static_cast<unsigned>(a.vc_slot) * 2 + vd * 2;
+        }
+        ka = reinterpret_cast<const char*>(kc + page * a.kc_page + slot * a.kc_slot) + kat;
+        va = reinterpret_cast<const char*>(vc + page * a.vc_page + slot * a.vc_slot) + vat;
       } else {
-        const int key = min(key0 + first + W::kPass * i, p.k1 - 1);
-        const int nth = a.by_page(key);
-        slot[i] = key - nth * a.page;
-        pg[i] = p.list[nth];
+        page = __shfl(pages, r);
+        const int key = min(key0 + r, p.k1 - 1);
+        const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
+        ka = reinterpret_cast<const char*>(kc + page * a.kc_page + slot * a.kc_slot + kd);
+        va = reinterpret_cast<const char*>(vc + page * a.vc_page + slot * a.vc_slot + vd);
+      }
+      if (page >= 0 && page < a.pages) {
+        if (kd < a.dim) load_to_lds(ka, to + 4096 * i);
+        if (vd < a.dim) load_to_lds(va, to + W::kTile + 4096 * i);
+      } else {    // no page: hidden below, and zero, since 0 times a NaN would be NaN
+        *reinterpret_cast<s16x8*>(to + 4096 * i + 16 * lane) = s16x8(0);
+        *reinterpret_cast<s16x8*>(to + W::kTile + 4096 * i + 16 * lane) = s16x8(0);
       }
     }
-  };
-  s16x8 k[W::kLoads], v[W::kLoads];
-  auto load = [&]() {
-    unsigned bad = 0;
-#pragma unroll
-    for (int i = 0; i < W::kLoads; ++i) {
-      i64 page = pg[i];
-      if (page < 0 || page >= a.pages) {
-        page = 0;
-        bad |= 1u << i;
-      }
-      if (mine) {
-        k[i] = __builtin_bit_cast(s16x8, C::load(kc + page * a.kc_page + slot[i] * a.kc_slot));
-        v[i] = __builtin_bit_cast(s16x8, C::load(vc + page * a.vc_page + slot[i] * a.vc_slot));
-      }
-    }
-    return bad;
-  };
-  auto store = [&](int buffer, unsigned bad) {
-    char* to = lds + buffer * W::kBuffer;
-    if (bad) {
-#pragma unroll
-      for (int i = 0; i < W::kLoads; ++i)
-        if (bad >> i & 1) v[i] = s16x8(0);
-    }
-    if (mine) {
-#pragma unroll
-      for (int i = 0; i < W::kLoads; ++i) {
-        const int r = first + W::kPass * i;
-        *reinterpret_cast<s16x8*>(to + r * W::kKeyRow + chunk * 16) = k[i];
-        *reinterpret_cast<s16x8*>(to + W::kKeys * W::kKeyRow + r * W::kValueRow + chunk * 16) = v[i];
-      }
-    }
-  };
-  // which keys of a tile have no page: lane = key
-  auto lost = [&](int tile) {
-    const int key = min(p.k0 + tile * W::kKeys + lane, p.k1 - 1);
-    const i64 page = p.list[a.by_page(key)];
-    return __ballot(page < 0 || page >= a.pages);
   };
 
   f32x16 o[DT];
@@ -136,31 +148,27 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   bool huge = false;
 
   // elements past the head: zero keys, once (their queries are zero, and must not meet a NaN)
-  if (!mine && chunk * 8 < DP) {
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
+  for (int i = 0; i < W::kLoads; ++i)
+    if ((place ^ W::key_place(first + W::kPass * i)) * 8 >= a.dim)
 #pragma unroll
-      for (int i = 0; i < W::kLoads; ++i)
-        *reinterpret_cast<s16x8*>(lds + b * W::kBuffer + (first + W::kPass * i) * W::kKeyRow +
-                                  chunk * 16) = s16x8(0);
-  }
-  find(0);
-  unsigned bad = load();
-  find(1);
-  store(0, bad);
-  gone = lost(0);
+      for (int b = 0; b < 2; ++b)
+        *reinterpret_cast<s16x8*>(lds + b * W::kBuffer + 4096 * i + 16 * tid) = s16x8(0);
+  i64 pages = pages_of(0), next = pages_of(1);
+  load(0, pages);
   __syncthreads();
 
   for (int tile = 0; tile < tiles; ++tile) {
     const int key0 = p.k0 + tile * W::kKeys;
     const char* keys = lds + (tile & 1) * W::kBuffer;
-    const char* values = keys + W::kKeys * W::kKeyRow;
+    const char* values = keys + W::kTile;
     const bool more = tile + 1 < tiles;
-    const unsigned long long without = gone;
+    // keys that have no page
+    const unsigned long long without = __ballot(pages < 0 || pages >= a.pages);
+    pages = next;
     if (more) {
-      bad = load();
-      find(tile + 2);
-      gone = lost(tile + 1);
+      next = pages_of(tile + 2);
+      load(tile + 1, pages);
     }
     f32x16 s[2];
 #pragma unroll
@@ -168,8 +176,8 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
       s[t] = f32x16(0.f);
 #pragma unroll
       for (int e = 0; e < KS; ++e) {
-        const s16x8 ka = *reinterpret_cast<const s16x8*>(keys + (32 * t + col) * W::kKeyRow +
-                                                         32 * e + 16 * half);
+        const s16x8 ka = *reinterpret_cast<const s16x8*>(
+            keys + (32 * t + col) * W::kPitch + ((2 * e + half) ^ W::key_place(col)) * 16);
         s[t] = M::mul32(ka, q[e], s[t]);
       }
     }
@@ -224,11 +232,11 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     l += sum;
 
     // V^T, an A operand: lanes name rows 4 half + i/4 of 16 keys and columns 16 (lane/16 % 2) ..
-    const char* from = values + (4 * half + (lane & 15) / 4) * W::kValueRow +
-                       32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+    const int vrow = 4 * half + (lane & 15) / 4;
     auto value = [&](int step, int d) {
-      const char* at = from + 16 * step * W::kValueRow + 64 * d;
-      const s16x4 lo = transposed(at), hi = transposed(at + 8 * W::kValueRow);
+      const int chunk = (4 * d + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ W::value_place(vrow);
+      const char* at = values + (16 * step + vrow) * W::kPitch + chunk * 16 + 8 * (lane & 1);
+      const s16x4 lo = transposed(at), hi = transposed(at + 8 * W::kPitch);
       return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
     };
     bool strange = false;
@@ -239,7 +247,8 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
         for (int d = 0; d < DT; ++d) {
           const s16x8 vt = value(step, d);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) strange |= (vt[i] & M::kExponent) == M::kExponent;
+          for (int i = 0; i < 8; ++i)   // (nothing was stored past the head)
+            strange |= 32 * d + col < a.dim && (vt[i] & M::kExponent) == M::kExponent;
         }
       strange = __any(strange);
     }
@@ -251,25 +260,23 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     } else {
       // an infinity or NaN among the values of a tile that not all rows see: key by key, added
       // to the rows that see it alone (0 times either would be NaN in the others)
-#pragma unroll
-      for (int step = 0; step < 4; ++step)
 #pragma unroll 1
-        for (int key = 0; key < 16; ++key) {
-          const int i = (key / 8) * 4 + key % 4;
-          const bool holds = key % 8 / 4 == half;
+      for (int key = 0; key < W::kKeys; ++key) {
+        const int step = key / 16, i = key % 16 / 8 * 4 + key % 4;
+        const bool holds = key % 8 / 4 == half;
+        const s16x8 pr = step == 0 ? prob[0] : step == 1 ? prob[1] : step == 2 ? prob[2] : prob[3];
 #pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            const s16x8 vt = value(step, d);
-            s16x8 one = s16x8(0);
+        for (int d = 0; d < DT; ++d) {
+          const s16x8 vt = value(step, d);
+          s16x8 one = s16x8(0);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (holds && e == i) one[e] = vt[e];
-            const f32x16 part = M::mul32(one, prob[step], f32x16(0.f));
-            if (key0 + 16 * step + key < see) o[d] += part;
-          }
+          for (int e = 0; e < 8; ++e)
+            if (holds && e == i) one[e] = vt[e];
+          const f32x16 part = M::mul32(one, pr, f32x16(0.f));
+          if (key0 + key < see) o[d] += part;
         }
+      }
     }
-    if (more) store((tile + 1) & 1, bad);
     __syncthreads();
   }
 
@@ -358,7 +365,8 @@ hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
 
 template <int DP>
 hipError_t launch_wide(const Attention& a, int64_t dtype, bool prefix, hipStream_t stream) {
-  const bool even = a.page % 16 == 0;
+  const bool even = a.page % 16 == 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24) &&
+                    a.vc_slot >= 0 && a.vc_slot < (1 << 24);
   if (dtype == TG_F16)
     return even ? launch_wide_as<DP, _Float16, true>(a, prefix, stream)
                 : launch_wide_as<DP, _Float16, false>(a, prefix, stream);
