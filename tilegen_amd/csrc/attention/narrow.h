@@ -282,15 +282,11 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
   }
 }
 
-// Prefix: workgroups go over (key range, kv head) in eighths, one for each XCD, and within one
-// over the row tiles, so that the tiles that read the same keys share an L2.
 template <typename T, int DP, bool FULL, int NT>
 __global__ __launch_bounds__(64 * kWaves) void narrow_prefix(Attention a) {
   __shared__ __align__(16) char lds[NarrowLds<DP, NT>::kBytes];
-  const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
-  const int tile = i % a.prefix_tiles, unit = i / a.prefix_tiles * 8 + x;
-  if (unit >= a.kv_heads * a.prefix_splits) return;
-  const int split = unit / a.kv_heads;
+  int tile, kv_head, split;
+  if (!prefix_place(a, &tile, &kv_head, &split)) return;
   Part p;
   p.list = a.prefix;
   p.k0 = split * a.prefix_chunk;
@@ -301,7 +297,7 @@ __global__ __launch_bounds__(64 * kWaves) void narrow_prefix(Attention a) {
   p.before = a.prefix_length;
   p.step = 0;
   p.slot = split;
-  narrow_part<T, DP, FULL, NT>(a, p, unit - split * a.kv_heads, lds);
+  narrow_part<T, DP, FULL, NT>(a, p, kv_head, lds);
 }
 
 template <typename T, int DP, bool FULL, int NT>
@@ -338,7 +334,7 @@ hipError_t launch_narrow_as(const Attention& a, bool prefix, hipStream_t stream)
   i64 grid;
   const void* f;
   if (prefix) {
-    grid = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;
+    grid = prefix_grid(a);
     f = reinterpret_cast<const void*>(&narrow_prefix<T, DP, FULL, NT>);
   } else {
     grid = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;

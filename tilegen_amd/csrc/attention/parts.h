@@ -94,6 +94,25 @@ struct Part {
   int slot;
 };
 
+// The prefix's workgroups: those that read the same keys (the row tiles of a kv head and a key
+// range) follow one another, and every XCD takes an eighth of all in that order (workgroup i
+// goes to XCD i % 8), so that they share an L2 and all XCDs have as much to do.
+__host__ __device__ inline i64 prefix_count(const Attention& a) {
+  return static_cast<i64>(a.prefix_tiles) * a.kv_heads * a.prefix_splits;
+}
+inline i64 prefix_grid(const Attention& a) { return (prefix_count(a) + 7) / 8 * 8; }
+__device__ __forceinline__ bool prefix_place(const Attention& a, int* tile, int* kv_head,
+                                             int* split) {
+  const int n = static_cast<int>(prefix_count(a));
+  const int i = static_cast<int>(blockIdx.x & 7) * ((n + 7) / 8) + (blockIdx.x >> 3);
+  if (static_cast<int>(blockIdx.x >> 3) >= (n + 7) / 8 || i >= n) return false;
+  const int unit = i / a.prefix_tiles;
+  *tile = i - unit * a.prefix_tiles;
+  *split = unit / a.kv_heads;
+  *kv_head = unit - *split * a.kv_heads;
+  return true;
+}
+
 // The four keys of V^T that the transposing LDS read gives a lane: 16 lanes name 4 rows of 16
 // values (8 bytes each) and lane i of them receives column i of the four rows.
 __device__ __forceinline__ s16x4 transposed(const char* at) {

@@ -25,6 +25,7 @@ struct Attention {
   int prefix_splits, prefix_chunk, prefix_tiles;
   int own_splits, own_chunk, own_tiles;
   int slots;
+  int even;           // the wide kernel's scalar addresses hold (wide.h)
 };
 
 // The new tokens of sequence b and the keys of its own pages.

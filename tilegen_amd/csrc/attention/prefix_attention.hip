@@ -145,6 +145,10 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   a.scale = static_cast<float>(r->scale * 1.4426950408889634);
   a.by_group = Div(a.group);
   a.by_page = Div(a.page);
+  // pages of whole groups of 16 keys, keys and values with the same strides, and a group's rows
+  // within 32 bits of its first
+  a.even = a.page % 16 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
+           a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
   p->bytes = 0;
   if (a.tokens == 0) return 0;
   const int64_t want = 2 * compute_units();

@@ -12,6 +12,8 @@
 // many vector cycles as its products take matrix cycles: two workgroups a CU overlap them.
 #pragma once
 
+#include <type_traits>
+
 #include "parts.h"
 
 namespace tg {
@@ -46,9 +48,7 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* to) {
       (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
 }
 
-// EVEN: pages hold whole groups of 16 keys, so that a wave's rows of one load stand on one page
-// and its number is uniform.
-template <typename T, int DP, bool EVEN, bool OWN>
+template <typename T, int DP, bool OWN>
 __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int kv_head,
                                           char* lds) {
   using W = Wide<DP>;
@@ -84,62 +84,74 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   const T* vc = static_cast<const T*>(a.v) + kv_head * a.vc_head;
   const int tiles = (p.k1 - p.k0 + W::kKeys - 1) / W::kKeys;
 
-  // The pages of a tile's keys, lane = key: asked for two tiles ahead and before the tile's own
-  // loads, since loads return in order.  Keys past the end stand for the last one (hidden).
-  auto pages_of = [&](int tile) {
-    return p.list[a.by_page(min(p.k0 + tile * W::kKeys + lane, p.k1 - 1))];
+  // Where a tile's keys are, lane = key: bytes from the head's first key (values have the same
+  // strides where `even`), or negative where a key has no page.  Pages are asked for a tile
+  // before they are needed and before that tile's loads, since loads return in order.  Keys past the
+  // end stand for the last one (hidden).
+  auto key_of_lane = [&](int tile) { return min(p.k0 + tile * W::kKeys + lane, p.k1 - 1); };
+  auto pages_of = [&](int tile) { return p.list[a.by_page(key_of_lane(tile))]; };
+  auto offsets_of = [&](int tile, i64 page) -> i64 {
+    const int key = key_of_lane(tile);
+    const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
+    if (page < 0 || page >= a.pages) return -1;
+    return a.even ? (page * a.kc_page + slot * a.kc_slot) * 2
+                  : page << 32 | static_cast<unsigned>(slot);
   };
-  unsigned key_at[2], value_at[2];    // EVEN: bytes from a group's first row to this lane's place
+  // Where pages hold whole groups of 16 keys (`even`) a wave's rows of one load stand on one
+  // page: the group's offset is uniform, and `in_group` bytes lead to this lane's row.
+  unsigned in_group[2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = first + W::kPass * i;
-    key_at[i] = (r & 15) * static_cast<unsigned>(a.kc_slot) * 2 + (place ^ W::key_place(r)) * 16;
-    value_at[i] =
-        (r & 15) * static_cast<unsigned>(a.vc_slot) * 2 + (place ^ W::value_place(r)) * 16;
-  }
-  auto load = [&](int tile, i64 pages) {
-    char* to = lds + (tile & 1) * W::kBuffer + wave * 1024;
-    const int key0 = p.k0 + tile * W::kKeys;
-    const bool tail = key0 + W::kKeys > p.k1;
+  for (int i = 0; i < 2; ++i)
+    in_group[i] = ((first + W::kPass * i) & 15) * static_cast<unsigned>(a.kc_slot) * 2;
+  // one tile's keys or values
+  auto load = [&](auto which, int tile, i64 offsets) {
+    constexpr bool kKeys = decltype(which)::value;
+    char* to = lds + (tile & 1) * W::kBuffer + (kKeys ? 0 : W::kTile) + wave * 1024;
+    const T* cache = kKeys ? kc : vc;
+    auto chunk = [&](int row) {
+      return place ^ (kKeys ? W::key_place(row) : W::value_place(row));
+    };
+    if (a.even && p.k0 + (tile + 1) * W::kKeys <= p.k1 && !__any(offsets < 0)) {
+      const char* at[W::kLoads];
 #pragma unroll
-    for (int i = 0; i < W::kLoads; ++i) {
-      const int r = first + W::kPass * i;
-      const int kd = (place ^ W::key_place(r)) * 8, vd = (place ^ W::value_place(r)) * 8;
-      i64 page;
-      const char *ka, *va;
-      if (EVEN) {
-        const int group = __builtin_amdgcn_readfirstlane(r & ~15);
-        page = static_cast<i64>(
-            static_cast<uint64_t>(
-                static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(pages >> 32), group)))
-                << 32 |
-            static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(pages), group)));
-        const int key = min(key0 + group, (p.k1 - 1) & ~15);
-        const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
-        unsigned kat = key_at[i & 1], vat = value_at[i & 1];
-        if (tail) {
-          const unsigned in = min(r & 15, p.k1 - 1 - key);
-          kat = in * static_cast<unsigned>(a.kc_slot) * 2 + kd * 2;
-          vat = in * static_cast<unsigned>(a.vc_slot) * 2 + vd * 2;
-        }
-        ka = reinterpret_cast<const char*>(kc + page * a.kc_page + slot * a.kc_slot) + kat;
-        va = reinterpret_cast<const char*>(vc + page * a.vc_page + slot * a.vc_slot) + vat;
-      } else {
-        page = __shfl(pages, r);
-        const int key = min(key0 + r, p.k1 - 1);
-        const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
-        ka = reinterpret_cast<const char*>(kc + page * a.kc_page + slot * a.kc_slot + kd);
-        va = reinterpret_cast<const char*>(vc + page * a.vc_page + slot * a.vc_slot + vd);
+      for (int i = 0; i < W::kLoads; ++i) {
+        const int group = __builtin_amdgcn_readfirstlane((first + W::kPass * i) & ~15);
+        const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(offsets), group);
+        const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(offsets >> 32), group);
+        at[i] = reinterpret_cast<const char*>(cache) + (static_cast<uint64_t>(hi) << 32 | lo);
       }
-      if (page >= 0 && page < a.pages) {
-        if (kd < a.dim) load_to_lds(ka, to + 4096 * i);
-        if (vd < a.dim) load_to_lds(va, to + W::kTile + 4096 * i);
+      if constexpr (W::kPass >= 16) {     // the same chunk of all rows
+        if (chunk(first) * 8 < a.dim)
+#pragma unroll
+          for (int i = 0; i < W::kLoads; ++i)
+            load_to_lds(at[i] + (in_group[0] + chunk(first) * 16), to + 4096 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < W::kLoads; ++i) {
+          const int c = chunk(first + W::kPass * i);
+          if (c * 8 < a.dim) load_to_lds(at[i] + (in_group[i & 1] + c * 16), to + 4096 * i);
+        }
+      }
+      return;
+    }
+    const i64 page_stride = kKeys ? a.kc_page : a.vc_page;
+    const i64 slot_stride = kKeys ? a.kc_slot : a.vc_slot;
+#pragma unroll 1
+    for (int i = 0; i < W::kLoads; ++i) {
+      const int r = first + W::kPass * i, d = chunk(r) * 8;
+      const i64 at = __shfl(offsets, r);
+      if (at >= 0) {
+        const T* from = a.even ? cache + at / 2
+                               : cache + (at >> 32) * page_stride +
+                                     static_cast<i64>(static_cast<unsigned>(at)) * slot_stride;
+        if (d < a.dim) load_to_lds(from + d, to + 4096 * i);
       } else {    // no page: hidden below, and zero, since 0 times a NaN would be NaN
         *reinterpret_cast<s16x8*>(to + 4096 * i + 16 * lane) = s16x8(0);
-        *reinterpret_cast<s16x8*>(to + W::kTile + 4096 * i + 16 * lane) = s16x8(0);
       }
     }
   };
+  const std::integral_constant<bool, true> keys_of{};
+  const std::integral_constant<bool, false> values_of{};
 
   f32x16 o[DT];
 #pragma unroll
@@ -154,112 +166,191 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
 #pragma unroll
       for (int b = 0; b < 2; ++b)
         *reinterpret_cast<s16x8*>(lds + b * W::kBuffer + 4096 * i + 16 * tid) = s16x8(0);
-  i64 pages = pages_of(0), next = pages_of(1);
-  load(0, pages);
-  __syncthreads();
 
-  for (int tile = 0; tile < tiles; ++tile) {
-    const int key0 = p.k0 + tile * W::kKeys;
-    const char* keys = lds + (tile & 1) * W::kBuffer;
-    const char* values = keys + W::kTile;
-    const bool more = tile + 1 < tiles;
-    // keys that have no page
-    const unsigned long long without = __ballot(pages < 0 || pages >= a.pages);
-    pages = next;
-    if (more) {
-      next = pages_of(tile + 2);
-      load(tile + 1, pages);
-    }
-    f32x16 s[2];
+  // scores of the keys at `keys`
+  auto score = [&](const char* keys, f32x16* s) {
+    s[0] = f32x16(0.f);
+    s[1] = f32x16(0.f);
+#pragma unroll
+    for (int e = 0; e < KS; ++e)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const s16x8 k = *reinterpret_cast<const s16x8*>(
+            keys + (32 * t + col) * W::kPitch + ((2 * e + half) ^ W::key_place(col)) * 16);
+        s[t] = M::mul32(k, q[e], s[t]);
+      }
+  };
+  // -inf where a row sees fewer keys, and for keys without a page (a bit each); this lane's
+  // keys are 32 t + 8 (i / 4) + i % 4 from its first
+  auto hide = [&](f32x16* s, int left, unsigned long long without) {
+    left -= 4 * half;
+    without >>= 4 * half;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      s[t] = f32x16(0.f);
+      const unsigned word = static_cast<unsigned>(without >> (32 * t));
 #pragma unroll
-      for (int e = 0; e < KS; ++e) {
-        const s16x8 ka = *reinterpret_cast<const s16x8*>(
-            keys + (32 * t + col) * W::kPitch + ((2 * e + half) ^ W::key_place(col)) * 16);
-        s[t] = M::mul32(ka, q[e], s[t]);
+      for (int i = 0; i < 16; ++i) {
+        const int at = 8 * (i / 4) + i % 4;
+        if (32 * t + at >= left || (word >> at & 1)) s[t][i] = -INFINITY;
       }
     }
-    const bool partial = without != 0 || key0 + W::kKeys > all;
-    if (partial) {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 32 * t + 8 * (i / 4) + 4 * half + i % 4;
-          if (key0 + at >= see || (without >> at & 1)) s[t][i] = -INFINITY;
-        }
-    }
+  };
+  auto largest = [&](const f32x16* s) {
     float top = s[0][0];
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int i = 0; i < 16; ++i) top = fmaxf(top, s[t][i]);
+    return top;
+  };
+  // lets the running maximum follow where a row's scores have left it far behind
+  auto follow = [&](float top) {
     top *= a.scale;
     if (__any(top > m + kSlack)) {
       const Both both = halves(top);
-      const float now = fmaxf(fmaxf(both.a, both.b), m);
-      const float f = m == -INFINITY ? 0.f : exp2f(m - now);
-      m = now;
-      huge |= __any(fabsf(now) > kHuge && now != -INFINITY);
+      const float to = fmaxf(fmaxf(both.a, both.b), m);
+      const float f = m == -INFINITY ? 0.f : exp2f(m - to);
+      m = to;
+      huge |= __any(fabsf(to) > kHuge && to != -INFINITY);
       l *= f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) o[d] *= f;
     }
-    const float base = m == -INFINITY ? 0.f : m;
-    s16x8 prob[4];
+  };
+  // probabilities of 32 keys: the B operands of two products
+  auto weigh = [&](const f32x16& s, float scale, float base, s16x8* prob) {
     float sum = 0.f;
-    if (!huge) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[t][i], a.scale, -base));
-          sum += e;
-          prob[2 * t + i / 8][i % 8] = __builtin_bit_cast(short, static_cast<T>(e));
-        }
-    } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float e = __builtin_amdgcn_exp2f(apart(s[t][i], a.scale, base));
-          sum += e;
-          prob[2 * t + i / 8][i % 8] = __builtin_bit_cast(short, static_cast<T>(e));
-        }
+    for (int i = 0; i < 16; ++i) {
+      const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i], scale, -base));
+      sum += e;
+      prob[i / 8][i % 8] = __builtin_bit_cast(short, static_cast<T>(e));
     }
-    l += sum;
+    return sum;
+  };
+  // V^T, an A operand: lanes name rows 4 half + i/4 of 16 keys and columns 16 (lane/16 % 2) ..
+  const int vrow = 4 * half + (lane & 15) / 4;
+  auto value = [&](const char* values, int step, int d) {
+    const int c = (4 * d + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ W::value_place(vrow);
+    const char* at = values + (16 * step + vrow) * W::kPitch + c * 16 + 8 * (lane & 1);
+    const s16x4 lo = transposed(at), hi = transposed(at + 8 * W::kPitch);
+    return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  };
+  // (scale, base) for weigh; past kHuge the products are rounded before
+  auto bases = [&](f32x16* s, float* scale, float* base) {
+    *base = m == -INFINITY ? 0.f : m;
+    *scale = a.scale;
+    if (huge) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[t][i] = apart(s[t][i], a.scale, *base);
+      *base = 0.f;
+      *scale = 1.f;
+    }
+  };
 
-    // V^T, an A operand: lanes name rows 4 half + i/4 of 16 keys and columns 16 (lane/16 % 2) ..
-    const int vrow = 4 * half + (lane & 15) / 4;
-    auto value = [&](int step, int d) {
-      const int chunk = (4 * d + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ W::value_place(vrow);
-      const char* at = values + (16 * step + vrow) * W::kPitch + chunk * 16 + 8 * (lane & 1);
-      const s16x4 lo = transposed(at), hi = transposed(at + 8 * W::kPitch);
-      return s16x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+  // Tiles that all rows see whole.  A tile's scores are taken while the tile before it is weighed:
+  // its keys are loaded two tiles ahead, its values one.
+  const int whole = (all - p.k0) / W::kKeys > 0 ? (all - p.k0) / W::kKeys : 0;
+  if (whole) {
+    i64 now_at = offsets_of(0, pages_of(0)), next_at = offsets_of(1, pages_of(1));
+    i64 third = pages_of(2);
+    float top;
+    load(keys_of, 0, now_at);
+    load(values_of, 0, now_at);
+    if (whole > 1) load(keys_of, 1, next_at);
+    __syncthreads();
+    f32x16 s0[2], s1[2];
+    score(lds, s0);
+    if (const unsigned long long without = __ballot(now_at < 0)) hide(s0, W::kKeys, without);
+    top = largest(s0);
+    __syncthreads();    // tile 2's keys take the place of tile 0's
+
+    // with `now` the tile's scores and `top` a lane's largest: adds it, and leaves the next
+    // one's scores in `then`
+    auto add = [&](int tile, f32x16* now, f32x16* then) {
+      const char* keys = lds + ((tile + 1) & 1) * W::kBuffer;
+      const char* values = lds + (tile & 1) * W::kBuffer + W::kTile;
+      const unsigned long long without = __ballot(next_at < 0);
+      if (tile + 1 < whole) {
+        const i64 fourth = pages_of(tile + 3);
+        const i64 at = offsets_of(tile + 2, third);
+        load(values_of, tile + 1, next_at);
+        if (tile + 2 < whole) load(keys_of, tile + 2, at);
+        next_at = at;
+        third = fourth;
+      }
+      follow(top);
+      float scale, base;
+      bases(now, &scale, &base);
+      // Products and vector instructions side by side: the first half's exponentials under the
+      // next tile's scores, the second's under the first half's values, the next
+      // largest under the rest.
+      s16x8 prob[4];
+      score(keys, then);
+      l += weigh(now[0], scale, base, prob);
+      l += weigh(now[1], scale, base, prob + 2);
+#pragma unroll
+      for (int step = 0; step < 4; ++step)
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+          o[d] = M::mul32(value(values, step, d), prob[step], o[d]);
+      top = largest(then);
+      asm volatile("" : "+v"(top), "+v"(l));    // here, not where they are used
+      if (without) {
+        hide(then, W::kKeys, without);
+        top = largest(then);
+      }
+      __syncthreads();
     };
+    for (int tile = 0; tile < whole; tile += 2) {
+      add(tile, s0, s1);
+      if (tile + 1 < whole) add(tile + 1, s1, s0);
+    }
+  }
+
+  // Tiles that end inside, or that some rows see in part: one after the other.
+#pragma unroll 1
+  for (int tile = whole; tile < tiles; ++tile) {
+    const i64 at = offsets_of(tile, pages_of(tile));
+    load(keys_of, tile, at);
+    load(values_of, tile, at);
+    __syncthreads();
+    const char* keys = lds + (tile & 1) * W::kBuffer;
+    const char* values = keys + W::kTile;
+    const int left = see - (p.k0 + tile * W::kKeys);
+    f32x16 s[2];
+    score(keys, s);
+    hide(s, left, __ballot(at < 0));
+    follow(largest(s));
+    float scale, base;
+    bases(s, &scale, &base);
+    s16x8 prob[4];
+    l += weigh(s[0], scale, base, prob);
+    l += weigh(s[1], scale, base, prob + 2);
     bool strange = false;
-    if (OWN && partial) {
+    if (OWN) {
 #pragma unroll 1
       for (int step = 0; step < 4; ++step)
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const s16x8 vt = value(step, d);
+          const s16x8 vt = value(values, step, d);
 #pragma unroll
           for (int i = 0; i < 8; ++i)   // (nothing was stored past the head)
             strange |= 32 * d + col < a.dim && (vt[i] & M::kExponent) == M::kExponent;
         }
       strange = __any(strange);
     }
-    if (!OWN || !strange) {
+    if (!strange) {
 #pragma unroll
       for (int step = 0; step < 4; ++step)
 #pragma unroll
-        for (int d = 0; d < DT; ++d) o[d] = M::mul32(value(step, d), prob[step], o[d]);
+        for (int d = 0; d < DT; ++d)
+          o[d] = M::mul32(value(values, step, d), prob[step], o[d]);
     } else {
-      // an infinity or NaN among the values of a tile that not all rows see: key by key, added
-      // to the rows that see it alone (0 times either would be NaN in the others)
+      // an infinity or NaN among values that not all rows see: key by key, added to the rows
+      // that see it alone (0 times either would be NaN in the others)
 #pragma unroll 1
       for (int key = 0; key < W::kKeys; ++key) {
         const int step = key / 16, i = key % 16 / 8 * 4 + key % 4;
@@ -267,13 +358,13 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
         const s16x8 pr = step == 0 ? prob[0] : step == 1 ? prob[1] : step == 2 ? prob[2] : prob[3];
 #pragma unroll
         for (int d = 0; d < DT; ++d) {
-          const s16x8 vt = value(step, d);
+          const s16x8 vt = value(values, step, d);
           s16x8 one = s16x8(0);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (holds && e == i) one[e] = vt[e];
           const f32x16 part = M::mul32(one, pr, f32x16(0.f));
-          if (key0 + key < see) o[d] += part;
+          if (key < left) o[d] += part;
         }
       }
     }
@@ -298,13 +389,11 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   }
 }
 
-template <typename T, int DP, bool EVEN>
+template <typename T, int DP>
 __global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_prefix(Attention a) {
   __shared__ __align__(16) char lds[2 * Wide<DP>::kBuffer];
-  const int x = blockIdx.x & 7, i = blockIdx.x >> 3;
-  const int tile = i % a.prefix_tiles, unit = i / a.prefix_tiles * 8 + x;
-  if (unit >= a.kv_heads * a.prefix_splits) return;
-  const int split = unit / a.kv_heads;
+  int tile, kv_head, split;
+  if (!prefix_place(a, &tile, &kv_head, &split)) return;
   Part p;
   p.list = a.prefix;
   p.k0 = split * a.prefix_chunk;
@@ -315,10 +404,10 @@ __global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_prefix(Attention a
   p.before = a.prefix_length;
   p.step = 0;
   p.slot = split;
-  wide_part<T, DP, EVEN, false>(a, p, unit - split * a.kv_heads, lds);
+  wide_part<T, DP, false>(a, p, kv_head, lds);
 }
 
-template <typename T, int DP, bool EVEN>
+template <typename T, int DP>
 __global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_own(Attention a) {
   __shared__ __align__(16) char lds[2 * Wide<DP>::kBuffer];
   int i = blockIdx.x;
@@ -342,21 +431,21 @@ __global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_own(Attention a) {
     p.k1 = seen(s, a.by_group(last));
     if (split + 1 < a.own_splits) p.k1 = min(p.k1, p.k0 + a.own_chunk);
     if (p.k0 >= p.k1) continue;
-    wide_part<T, DP, EVEN, true>(a, p, head, lds);
+    wide_part<T, DP, true>(a, p, head, lds);
     __syncthreads();
   }
 }
 
-template <int DP, typename T, bool EVEN>
+template <int DP, typename T>
 hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
   i64 grid;
   const void* f;
   if (prefix) {
-    grid = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 7) / 8 * 8 * a.prefix_tiles;
-    f = reinterpret_cast<const void*>(&wide_prefix<T, DP, EVEN>);
+    grid = prefix_grid(a);
+    f = reinterpret_cast<const void*>(&wide_prefix<T, DP>);
   } else {
     grid = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;
-    f = reinterpret_cast<const void*>(&wide_own<T, DP, EVEN>);
+    f = reinterpret_cast<const void*>(&wide_own<T, DP>);
   }
   Attention copy = a;
   void* args[] = {&copy};
@@ -365,13 +454,8 @@ hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
 
 template <int DP>
 hipError_t launch_wide(const Attention& a, int64_t dtype, bool prefix, hipStream_t stream) {
-  const bool even = a.page % 16 == 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24) &&
-                    a.vc_slot >= 0 && a.vc_slot < (1 << 24);
-  if (dtype == TG_F16)
-    return even ? launch_wide_as<DP, _Float16, true>(a, prefix, stream)
-                : launch_wide_as<DP, _Float16, false>(a, prefix, stream);
-  return even ? launch_wide_as<DP, __bf16, true>(a, prefix, stream)
-              : launch_wide_as<DP, __bf16, false>(a, prefix, stream);
+  return dtype == TG_F16 ? launch_wide_as<DP, _Float16>(a, prefix, stream)
+                         : launch_wide_as<DP, __bf16>(a, prefix, stream);
 }
 
 }  // namespace tg
