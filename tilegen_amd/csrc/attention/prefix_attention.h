@@ -76,6 +76,7 @@ template <int DP>
 hipError_t launch_narrow(const Attention& a, int64_t dtype, int nt, bool prefix,
                          hipStream_t stream);
 template <int DP>
-hipError_t launch_wide(const Attention& a, int64_t dtype, bool prefix, hipStream_t stream);
+hipError_t launch_wide(const Attention& a, int64_t dtype, int rows, bool prefix,
+                       hipStream_t stream);
 
 }  // namespace tg

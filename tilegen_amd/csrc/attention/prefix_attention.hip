@@ -69,15 +69,16 @@ int compute_units() {
 
 struct Plan {
   Attention a;
-  int prefix_nt, own_nt;
+  int prefix_rows, own_rows;    // of one workgroup: narrow 16 and 32, wide 128 and 256
   int64_t bytes;
 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
-// 16-row tiles of a narrow wave for that many query rows to the same keys, or 0: wide.
-int rows_tiles(int64_t rows) { return rows <= 16 ? 1 : rows <= 64 ? 2 : 0; }
-int tile_rows(int nt) { return nt ? 16 * nt : 128; }
+// Rows of one workgroup where that many query rows read the same keys.
+int rows_of(int64_t rows, int dim) {
+  return rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 || dim > 128 ? 128 : 256;
+}
 
 int check(const tg_prefix_attention* r) {
   const char* what = "launch_prefix_attention";
@@ -153,22 +154,21 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   if (a.tokens == 0) return 0;
   const int64_t want = 2 * compute_units();
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
-  p->prefix_nt = rows_tiles(rows);
-  const int prefix_rows = tile_rows(p->prefix_nt);
-  a.prefix_tiles = static_cast<int>((rows + prefix_rows - 1) / prefix_rows);
+  p->prefix_rows = rows_of(rows, a.dim);
+  a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
   if (a.prefix_length) {
     const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
     const int64_t most = (a.prefix_length + 255) / 256;
-    int64_t splits = want / units;
+    int64_t splits = (p->prefix_rows == 256 ? want / 2 : want) / units;
     splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
     a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
   }
   const int64_t max_query = r->query_indptr ? (r->max_query > 0 ? r->max_query : 1) : 1;
   const int64_t own_rows = max_query * a.group;
-  p->own_nt = rows_tiles(own_rows);
+  p->own_rows = rows_of(own_rows, a.dim);
   if (a.pages && a.n_indices && a.sequences) {
-    int64_t tiles = (own_rows + tile_rows(p->own_nt) - 1) / tile_rows(p->own_nt);
+    int64_t tiles = (own_rows + p->own_rows - 1) / p->own_rows;
     tiles = tiles < 4096 ? tiles : 4096;
     a.own_tiles = static_cast<int>(tiles);
     const int64_t length = r->max_length > 0 ? r->max_length : 1;
@@ -189,15 +189,16 @@ int plan(const tg_prefix_attention* r, Plan* p) {
 }
 
 template <int DP>
-hipError_t launch_parts(const Attention& a, int64_t dtype, int nt, bool prefix, hipStream_t s) {
-  return nt ? launch_narrow<DP>(a, dtype, nt, prefix, s) : launch_wide<DP>(a, dtype, prefix, s);
+hipError_t launch_parts(const Attention& a, int64_t dtype, int rows, bool prefix, hipStream_t s) {
+  return rows < 128 ? launch_narrow<DP>(a, dtype, rows / 16, prefix, s)
+                    : launch_wide<DP>(a, dtype, rows, prefix, s);
 }
 
-hipError_t launch_parts(const Attention& a, int64_t dtype, int nt, bool prefix, hipStream_t s) {
-  if (a.dim <= 64) return launch_parts<64>(a, dtype, nt, prefix, s);
-  if (a.dim <= 96) return launch_parts<96>(a, dtype, nt, prefix, s);
-  if (a.dim <= 128) return launch_parts<128>(a, dtype, nt, prefix, s);
-  return launch_parts<256>(a, dtype, nt, prefix, s);
+hipError_t launch_parts(const Attention& a, int64_t dtype, int rows, bool prefix, hipStream_t s) {
+  if (a.dim <= 64) return launch_parts<64>(a, dtype, rows, prefix, s);
+  if (a.dim <= 96) return launch_parts<96>(a, dtype, rows, prefix, s);
+  if (a.dim <= 128) return launch_parts<128>(a, dtype, rows, prefix, s);
+  return launch_parts<256>(a, dtype, rows, prefix, s);
 }
 
 template <typename T>
@@ -238,11 +239,11 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
                                                      a.heads * a.dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (a.prefix_splits) {
-    const hipError_t e = launch_parts(a, r->dtype, p.prefix_nt, true, s);
+    const hipError_t e = launch_parts(a, r->dtype, p.prefix_rows, true, s);
     if (e != hipSuccess) return hip_failed(e, what);
   }
   if (a.own_splits) {
-    const hipError_t e = launch_parts(a, r->dtype, p.own_nt, false, s);
+    const hipError_t e = launch_parts(a, r->dtype, p.own_rows, false, s);
     if (e != hipSuccess) return hip_failed(e, what);
   }
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;

@@ -18,16 +18,19 @@
 
 namespace tg {
 
-template <int DP>
+// NW: waves of a workgroup.
+template <int DP, int NW>
 struct Wide {
-  static constexpr int kRows = 128, kKeys = 64;
+  static constexpr int kRows = 32 * NW, kKeys = 64;
   static constexpr int kPitch = DP == 64 ? 128 : DP == 256 ? 512 : 256;   // bytes of an LDS row
   static constexpr int kChunks = kPitch / 16;
-  static constexpr int kLoads = kKeys * kChunks / 256;    // of each thread, keys and values
-  static constexpr int kPass = 256 / kChunks;             // rows that one load of all covers
+  static constexpr int kThreads = 64 * NW;
+  static constexpr int kLoads = kKeys * kChunks / kThreads;   // of each thread, keys and values
+  static constexpr int kPass = kThreads / kChunks;            // rows that one load of all covers
+  static constexpr int kSpan = kThreads * 16;                 // and their bytes
   static constexpr int kTile = kKeys * kPitch;
   static constexpr int kBuffer = 2 * kTile;               // keys, then values
-  static constexpr int kPerCu = DP == 256 ? 1 : 2;
+  static constexpr int kPerCu = DP == 256 || NW == 8 ? 1 : 2;
 
   // Loads go straight to LDS, 16 bytes a lane side by side, so rows cannot be padded; instead a
   // row's chunks change places, and a lane fetches the chunk that belongs to its place.  Keys
@@ -48,10 +51,50 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* to) {
       (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
 }
 
-template <typename T, int DP, bool OWN>
+// The order of a whole tile's instructions: after each product the vector instructions that fit
+// beside it (32 cycles: one exponential takes 16, others 4) and the LDS reads of a later one.
+template <int KS, int DT>
+__device__ __forceinline__ void side_by_side() {
+  constexpr int kMatrix = 0x008, kVector = 0x002, kExp = 0x400, kRead = 0x100;
+  constexpr int kAhead = 4, kScores = 2 * KS, kValues = 4 * DT;
+  __builtin_amdgcn_sched_group_barrier(kRead, kAhead, 0);
+#pragma unroll
+  for (int i = 0; i < kScores / 2 - kAhead / 2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kVector, 24 / KS, 0);
+    __builtin_amdgcn_sched_group_barrier(kExp, 8 / KS, 0);
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kVector, 32 / KS, 0);
+    __builtin_amdgcn_sched_group_barrier(kExp, 8 / KS, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(kVector, 32 / KS, 0);
+    __builtin_amdgcn_sched_group_barrier(kExp, 8 / KS, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kValues / 2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(kVector, 20 / DT, 0);
+    __builtin_amdgcn_sched_group_barrier(kExp, 8 / DT, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < kValues / 2; ++i) {
+    __builtin_amdgcn_sched_group_barrier(kMatrix, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(kRead, 2, 0);
+    __builtin_amdgcn_sched_group_barrier(kVector, 12 / DT, 0);
+  }
+}
+
+template <typename T, int DP, int NW, bool OWN>
 __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int kv_head,
                                           char* lds) {
-  using W = Wide<DP>;
+  using W = Wide<DP, NW>;
   using M = Matrix<T>;
   using C = Chunk<T>;
   constexpr int KS = DP / 16, DT = DP / 32;
@@ -124,12 +167,12 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
         if (chunk(first) * 8 < a.dim)
 #pragma unroll
           for (int i = 0; i < W::kLoads; ++i)
-            load_to_lds(at[i] + (in_group[0] + chunk(first) * 16), to + 4096 * i);
+            load_to_lds(at[i] + (in_group[0] + chunk(first) * 16), to + W::kSpan * i);
       } else {
 #pragma unroll
         for (int i = 0; i < W::kLoads; ++i) {
           const int c = chunk(first + W::kPass * i);
-          if (c * 8 < a.dim) load_to_lds(at[i] + (in_group[i & 1] + c * 16), to + 4096 * i);
+          if (c * 8 < a.dim) load_to_lds(at[i] + (in_group[i & 1] + c * 16), to + W::kSpan * i);
         }
       }
       return;
@@ -144,9 +187,9 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
         const T* from = a.even ? cache + at / 2
                                : cache + (at >> 32) * page_stride +
                                      static_cast<i64>(static_cast<unsigned>(at)) * slot_stride;
-        if (d < a.dim) load_to_lds(from + d, to + 4096 * i);
+        if (d < a.dim) load_to_lds(from + d, to + W::kSpan * i);
       } else {    // no page: hidden below, and zero, since 0 times a NaN would be NaN
-        *reinterpret_cast<s16x8*>(to + 4096 * i + 16 * lane) = s16x8(0);
+        *reinterpret_cast<s16x8*>(to + W::kSpan * i + 16 * lane) = s16x8(0);
       }
     }
   };
@@ -165,7 +208,7 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     if ((place ^ W::key_place(first + W::kPass * i)) * 8 >= a.dim)
 #pragma unroll
       for (int b = 0; b < 2; ++b)
-        *reinterpret_cast<s16x8*>(lds + b * W::kBuffer + 4096 * i + 16 * tid) = s16x8(0);
+        *reinterpret_cast<s16x8*>(lds + b * W::kBuffer + W::kSpan * i + 16 * tid) = s16x8(0);
 
   // scores of the keys at `keys`
   auto score = [&](const char* keys, f32x16* s) {
@@ -298,6 +341,7 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
           o[d] = M::mul32(value(values, step, d), prob[step], o[d]);
       top = largest(then);
       asm volatile("" : "+v"(top), "+v"(l));    // here, not where they are used
+      side_by_side<KS, DT>();
       if (without) {
         hide(then, W::kKeys, without);
         top = largest(then);
@@ -389,27 +433,27 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   }
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_prefix(Attention a) {
-  __shared__ __align__(16) char lds[2 * Wide<DP>::kBuffer];
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_prefix(Attention a) {
+  __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
   int tile, kv_head, split;
   if (!prefix_place(a, &tile, &kv_head, &split)) return;
   Part p;
   p.list = a.prefix;
   p.k0 = split * a.prefix_chunk;
   p.k1 = min(p.k0 + a.prefix_chunk, a.prefix_length);
-  p.row0 = tile * Wide<DP>::kRows;
+  p.row0 = tile * Wide<DP, NW>::kRows;
   p.rows = a.tokens * a.group;
   p.token0 = 0;
   p.before = a.prefix_length;
   p.step = 0;
   p.slot = split;
-  wide_part<T, DP, false>(a, p, kv_head, lds);
+  wide_part<T, DP, NW, false>(a, p, kv_head, lds);
 }
 
-template <typename T, int DP>
-__global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_own(Attention a) {
-  __shared__ __align__(16) char lds[2 * Wide<DP>::kBuffer];
+template <typename T, int DP, int NW>
+__global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_own(Attention a) {
+  __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
   int i = blockIdx.x;
   const int head = i % a.kv_heads;
   i /= a.kv_heads;
@@ -425,37 +469,45 @@ __global__ __launch_bounds__(256, Wide<DP>::kPerCu) void wide_own(Attention a) {
   p.step = 1;
   p.slot = a.prefix_splits + split;
   p.k0 = split * a.own_chunk;
-  for (int tile = first; tile * Wide<DP>::kRows < p.rows; tile += a.own_tiles) {
-    p.row0 = tile * Wide<DP>::kRows;
-    const int last = min(p.row0 + Wide<DP>::kRows, p.rows) - 1;
+  for (int tile = first; tile * Wide<DP, NW>::kRows < p.rows; tile += a.own_tiles) {
+    p.row0 = tile * Wide<DP, NW>::kRows;
+    const int last = min(p.row0 + Wide<DP, NW>::kRows, p.rows) - 1;
     p.k1 = seen(s, a.by_group(last));
     if (split + 1 < a.own_splits) p.k1 = min(p.k1, p.k0 + a.own_chunk);
     if (p.k0 >= p.k1) continue;
-    wide_part<T, DP, true>(a, p, head, lds);
+    wide_part<T, DP, NW, true>(a, p, head, lds);
     __syncthreads();
   }
 }
 
-template <int DP, typename T>
+template <int DP, typename T, int NW>
 hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
   i64 grid;
   const void* f;
   if (prefix) {
     grid = prefix_grid(a);
-    f = reinterpret_cast<const void*>(&wide_prefix<T, DP>);
+    f = reinterpret_cast<const void*>(&wide_prefix<T, DP, NW>);
   } else {
     grid = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;
-    f = reinterpret_cast<const void*>(&wide_own<T, DP>);
+    f = reinterpret_cast<const void*>(&wide_own<T, DP, NW>);
   }
   Attention copy = a;
   void* args[] = {&copy};
-  return hipLaunchKernel(f, dim3(static_cast<unsigned>(grid)), dim3(256), args, 0, stream);
+  return hipLaunchKernel(f, dim3(static_cast<unsigned>(grid)), dim3(64 * NW), args, 0, stream);
+}
+
+template <int DP, typename T>
+hipError_t launch_wide_rows(const Attention& a, int rows, bool prefix, hipStream_t stream) {
+  if constexpr (DP <= 128)
+    if (rows == 256) return launch_wide_as<DP, T, 8>(a, prefix, stream);
+  return launch_wide_as<DP, T, 4>(a, prefix, stream);
 }
 
 template <int DP>
-hipError_t launch_wide(const Attention& a, int64_t dtype, bool prefix, hipStream_t stream) {
-  return dtype == TG_F16 ? launch_wide_as<DP, _Float16>(a, prefix, stream)
-                         : launch_wide_as<DP, __bf16>(a, prefix, stream);
+hipError_t launch_wide(const Attention& a, int64_t dtype, int rows, bool prefix,
+                       hipStream_t stream) {
+  return dtype == TG_F16 ? launch_wide_rows<DP, _Float16>(a, rows, prefix, stream)
+                         : launch_wide_rows<DP, __bf16>(a, rows, prefix, stream);
 }
 
 }  // namespace tg

@@ -1,3 +1,3 @@
 #include "wide.h"
 
-template hipError_t tg::launch_wide<64>(const Attention&, int64_t, bool, hipStream_t);
+template hipError_t tg::launch_wide<64>(const Attention&, int64_t, int, bool, hipStream_t);
