@@ -136,9 +136,9 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   auto offsets_of = [&](int tile, i64 page) -> i64 {
     const int key = key_of_lane(tile);
     const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
-    if (page < 0 || page >= a.pages) return -1;
-    return a.even ? (page * a.kc_page + slot * a.kc_slot) * 2
-                  : page << 32 | static_cast<unsigned>(slot);
+    const i64 at = a.even ? (page * a.kc_page + slot * a.kc_slot) * 2
+                          : page << 32 | static_cast<unsigned>(slot);
+    return page < 0 || page >= a.pages ? -1 : at;
   };
   // Where pages hold whole groups of 16 keys (`even`) a wave's rows of one load stand on one
   // page: the group's offset is uniform, and `in_group` bytes lead to this lane's row.
@@ -298,7 +298,7 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   const int whole = (all - p.k0) / W::kKeys > 0 ? (all - p.k0) / W::kKeys : 0;
   if (whole) {
     i64 now_at = offsets_of(0, pages_of(0)), next_at = offsets_of(1, pages_of(1));
-    i64 third = pages_of(2);
+    i64 page0 = pages_of(2), page1;
     float top;
     load(keys_of, 0, now_at);
     load(values_of, 0, now_at);
@@ -311,19 +311,17 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     __syncthreads();    // tile 2's keys take the place of tile 0's
 
     // with `now` the tile's scores and `top` a lane's largest: adds it, and leaves the next
-    // one's scores in `then`
-    auto add = [&](int tile, f32x16* now, f32x16* then) {
+    // one's scores in `then`.  `page`: of tile + 2; page_then: of the one after, still on its
+    // way (a copy of it would wait for it and for the loads behind it)
+    auto add = [&](int tile, f32x16* now, f32x16* then, const i64& page, i64& page_then) {
       const char* keys = lds + ((tile + 1) & 1) * W::kBuffer;
       const char* values = lds + (tile & 1) * W::kBuffer + W::kTile;
       const unsigned long long without = __ballot(next_at < 0);
-      if (tile + 1 < whole) {
-        const i64 fourth = pages_of(tile + 3);
-        const i64 at = offsets_of(tile + 2, third);
-        load(values_of, tile + 1, next_at);
-        if (tile + 2 < whole) load(keys_of, tile + 2, at);
-        next_at = at;
-        third = fourth;
-      }
+      const i64 at = offsets_of(tile + 2, page);
+      page_then = pages_of(tile + 3);
+      if (tile + 1 < whole) load(values_of, tile + 1, next_at);
+      if (tile + 2 < whole) load(keys_of, tile + 2, at);
+      next_at = at;
       follow(top);
       float scale, base;
       bases(now, &scale, &base);
@@ -348,9 +346,11 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
       }
       __syncthreads();
     };
-    for (int tile = 0; tile < whole; tile += 2) {
-      add(tile, s0, s1);
-      if (tile + 1 < whole) add(tile + 1, s1, s0);
+    for (int tile = 0;;) {
+      add(tile, s0, s1, page0, page1);
+      if (++tile == whole) break;
+      add(tile, s1, s0, page1, page0);
+      if (++tile == whole) break;
     }
   }
 
