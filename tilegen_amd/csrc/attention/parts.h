@@ -72,7 +72,6 @@ __device__ __forceinline__ float row_sum(float v) {
   return q.a + q.b;
 }
 
-constexpr int kWaves = 4;
 constexpr float kSlack = 8.f;   // log2 of how far scores may pass the running maximum
 // Scores times scale less the maximum is one fused operation, exact in the product where the
 // maximum has been rounded.  Past this the rounding, 2^-24 of it, is no longer small against
@@ -94,6 +93,41 @@ struct Part {
   int slot;
 };
 
+// 16 bytes of every active lane to LDS at `to` + 16 * lane, without a register between.
+__device__ __forceinline__ void load_to_lds(const void* from, char* to) {
+  __builtin_amdgcn_global_load_lds(
+      (const __attribute__((address_space(1))) unsigned*)from,
+      (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
+}
+
+// The same, from a uniform address and 32-bit offsets or from any address, written out: the
+// compiler knows nothing of it and inserts no wait, so that a wave can read one tile from LDS
+// while another is on its way.  (It returns no register; the waits are the caller's, wait_loads.)
+__device__ __forceinline__ unsigned lds_address(char* to) {
+  return static_cast<unsigned>(
+      reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) char*)to));
+}
+__device__ __forceinline__ void fetch_to_lds(const char* from, unsigned offset, char* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                   lds_address(to)),
+               "v"(offset), "s"(from)
+               : "memory", "m0");
+}
+__device__ __forceinline__ void fetch_to_lds(const void* from, char* to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                   lds_address(to)),
+               "v"(from)
+               : "memory", "m0");
+}
+
+// Waits until at most N of this wave's loads are on their way (they return in order), or until
+// its LDS reads are done; neither lets the compiler move memory accesses past it.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // The prefix's workgroups: those that read the same keys (the row tiles of a kv head and a key
 // range) follow one another, and every XCD takes an eighth of all in that order (workgroup i
 // goes to XCD i % 8), so that they share an L2 and all XCDs have as much to do.
@@ -111,6 +145,25 @@ __device__ __forceinline__ bool prefix_place(const Attention& a, int* tile, int*
   *split = unit / a.kv_heads;
   *kv_head = unit - *split * a.kv_heads;
   return true;
+}
+
+// The own pages' workgroups: a sequence's row tile and key range go to an XCD in turn, all kv
+// heads of it to the same one.  (A head to each XCD would have every XCD read 256 bytes of each
+// key's 2 KB, say, which stand in few channels of its L2.)
+inline i64 own_grid(const Attention& a) {
+  const i64 units = static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences;
+  return (units + 7) / 8 * 8 * a.kv_heads;
+}
+__device__ __forceinline__ bool own_place(const Attention& a, int* tile, int* split, int* kv_head,
+                                          int* b) {
+  const int i = blockIdx.x >> 3, group = i / a.kv_heads;
+  int unit = group * 8 + (blockIdx.x & 7);
+  *kv_head = i - group * a.kv_heads;
+  *split = unit % a.own_splits;
+  unit /= a.own_splits;
+  *tile = unit % a.own_tiles;
+  *b = unit / a.own_tiles;
+  return *b < a.sequences;
 }
 
 // The four keys of V^T that the transposing LDS read gives a lane: 16 lanes name 4 rows of 16

@@ -146,10 +146,11 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   a.scale = static_cast<float>(r->scale * 1.4426950408889634);
   a.by_group = Div(a.group);
   a.by_page = Div(a.page);
-  // pages of whole groups of 16 keys, keys and values with the same strides, and a group's rows
-  // within 32 bits of its first
-  a.even = a.page % 16 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
-           a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
+  // pages of whole groups of 16 (8) keys, keys and values with the same strides, and a group's
+  // rows within 32 bits of its first
+  a.eights = a.page % 8 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
+             a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
+  a.even = a.eights && a.page % 16 == 0;
   p->bytes = 0;
   if (a.tokens == 0) return 0;
   const int64_t want = 2 * compute_units();
@@ -180,7 +181,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
   }
   a.slots = a.prefix_splits + a.own_splits;
-  const i64 all = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;
+  const i64 all = (static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences + 8) * a.kv_heads;
   const i64 first = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 8) * a.prefix_tiles;
   if (all > 0xFFFFFF || first > 0xFFFFFF)
     return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups", all > first ? all : first);

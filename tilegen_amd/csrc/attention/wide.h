@@ -44,13 +44,6 @@ struct Wide {
   }
 };
 
-// 16 bytes of every active lane to LDS at `to` + 16 * lane, without a register between.
-__device__ __forceinline__ void load_to_lds(const void* from, char* to) {
-  __builtin_amdgcn_global_load_lds(
-      (const __attribute__((address_space(1))) unsigned*)from,
-      (__attribute__((address_space(3))) unsigned*)to, 16, 0, 0);
-}
-
 // The order of a whole tile's instructions: after each product the vector instructions that fit
 // beside it (32 cycles: one exponential takes 16, others 4) and the LDS reads of a later one.
 template <int KS, int DT>
@@ -454,13 +447,9 @@ __global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_prefix(A
 template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_own(Attention a) {
   __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
-  int i = blockIdx.x;
-  const int head = i % a.kv_heads;
-  i /= a.kv_heads;
-  const int split = i % a.own_splits;
-  i /= a.own_splits;
-  const int first = i % a.own_tiles;
-  const Sequence s = sequence(a, i / a.own_tiles);
+  int first, split, head, b;
+  if (!own_place(a, &first, &split, &head, &b)) return;
+  const Sequence s = sequence(a, b);
   Part p;
   p.list = s.list;
   p.rows = s.count * a.group;
@@ -488,7 +477,7 @@ hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
     grid = prefix_grid(a);
     f = reinterpret_cast<const void*>(&wide_prefix<T, DP, NW>);
   } else {
-    grid = static_cast<i64>(a.kv_heads) * a.own_splits * a.own_tiles * a.sequences;
+    grid = own_grid(a);
     f = reinterpret_cast<const void*>(&wide_own<T, DP, NW>);
   }
   Attention copy = a;
