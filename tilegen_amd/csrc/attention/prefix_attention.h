@@ -25,7 +25,8 @@ struct Attention {
   int prefix_splits, prefix_chunk, prefix_tiles;
   int own_splits, own_chunk, own_tiles;
   int slots;
-  int even, eights;   // the scalar addresses of wide.h and of narrow.h hold
+  int even;           // the wide kernel's scalar addresses hold (wide.h)
+  int sorted;         // own parts go from the longest sequence to the shortest (parts.h)
 };
 
 // The new tokens of sequence b and the keys of its own pages.

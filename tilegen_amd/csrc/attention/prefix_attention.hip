@@ -5,49 +5,84 @@ namespace tg {
 namespace {
 
 // Joins the parts of each row: M = max m_s, then sum 2^(m_s - M) O_s over sum 2^(m_s - M) l_s.
-// One wave has one row; lanes hold four elements of the head each, and where a head takes 16 or
-// 32 lanes the rest read other parts at the same time (LANES: lanes of one part).
-template <typename T, int LANES>
+// A lane holds four elements of the head; where a head takes 16 or 32 lanes the others read
+// other parts at the same time (LANES: lanes of one part), and WAVES waves share a row where it
+// has many.  Memory bounds it, so the weights come first and the parts' loads wait for nothing.
+template <typename T, int LANES, int WAVES>
 __global__ __launch_bounds__(256) void join_parts(Attention a) {
-  const int lane = threadIdx.x & 63;
+  constexpr int kAtOnce = WAVES * 64 / LANES;     // parts
+  __shared__ float4 s_sum[WAVES == 1 ? 1 : 256];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const i64 rows = static_cast<i64>(a.tokens) * a.heads;
-  const i64 row = static_cast<i64>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const i64 row = static_cast<i64>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? wave : 0);
   if (row >= rows) return;
   const int t = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<i64>(t) * a.heads);
   const int b = a.ends ? sequence_of(a.ends, a.sequences, t) : t;
-  int parts = a.prefix_splits;
-  bool owned = b < a.sequences;
-  if (owned && a.own_splits) {
+  int parts = b < a.sequences ? a.prefix_splits : 0;
+  if (b < a.sequences && a.own_splits) {
     const Sequence s = sequence(a, b);
     parts += own_parts(a, seen(s, t - s.first));
   }
-  if (!owned) parts = 0;
+  const float2* ml = a.part_ml + row;
   float top = -INFINITY;
-  for (int s = lane; s < parts; s += 64) top = fmaxf(top, a.part_ml[s * rows + row].x);
+  for (int s = lane; s < parts; s += 64) top = fmaxf(top, ml[s * rows].x);
+#pragma unroll
   for (int x = 32; x; x >>= 1) top = fmaxf(top, __shfl_xor(top, x));
-  const int d = (lane % LANES) * 4;
+  const float base = top == -INFINITY ? 0.f : top;
   float total = 0.f;
+  for (int s = lane; s < parts; s += 64) {
+    const float2 v = ml[s * rows];
+    total += v.y * exp2f(v.x - base);
+  }
+#pragma unroll
+  for (int x = 32; x; x >>= 1) total += __shfl_xor(total, x);
+  const int d = (lane % LANES) * 4;
+  const int first = WAVES == 1 ? lane / LANES : threadIdx.x / LANES;
   float sum[4] = {0.f, 0.f, 0.f, 0.f};
   if (d < a.dim) {
-    for (int s = lane / LANES; s < parts; s += 64 / LANES) {
-      const float2 ml = a.part_ml[s * rows + row];
-      if (ml.x == -INFINITY) continue;
-      const float f = exp2f(ml.x - top);
-      const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + row) * a.dim + d);
-      total += ml.y * f;
-      sum[0] += v.x * f;
-      sum[1] += v.y * f;
-      sum[2] += v.z * f;
-      sum[3] += v.w * f;
+    const float* from = a.part + row * a.dim + d;
+    const i64 stride = rows * a.dim;
+    for (int s0 = first; s0 < parts; s0 += 4 * kAtOnce) {
+      float f[4];
+      float4 v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int s = s0 + i * kAtOnce;
+        f[i] = 0.f;
+        v[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (s < parts) {
+          f[i] = exp2f(ml[s * rows].x - base);
+          v[i] = *reinterpret_cast<const float4*>(from + s * stride);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sum[0] += v[i].x * f[i];
+        sum[1] += v[i].y * f[i];
+        sum[2] += v[i].z * f[i];
+        sum[3] += v[i].w * f[i];
+      }
     }
   }
-  for (int x = LANES; x < 64; x <<= 1) {
-    total += __shfl_xor(total, x);
+  for (int x = LANES; x < 64; x <<= 1)
     for (int i = 0; i < 4; ++i) sum[i] += __shfl_xor(sum[i], x);
+  if (WAVES > 1) {
+    s_sum[threadIdx.x] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) {
+      const float4 v = s_sum[64 * w + lane];
+      sum[0] += v.x;
+      sum[1] += v.y;
+      sum[2] += v.z;
+      sum[3] += v.w;
+    }
   }
   if (lane < LANES && d < a.dim) {
     T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head + d;
     const float f = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
     for (int i = 0; i < 4; ++i) out[i] = static_cast<T>(total == 0.f ? 0.f : sum[i] * f);
   }
   if (lane == 0 && a.lse) a.lse[row] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
@@ -146,14 +181,13 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   a.scale = static_cast<float>(r->scale * 1.4426950408889634);
   a.by_group = Div(a.group);
   a.by_page = Div(a.page);
-  // pages of whole groups of 16 (8) keys, keys and values with the same strides, and a group's
-  // rows within 32 bits of its first
-  a.eights = a.page % 8 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
-             a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
-  a.even = a.eights && a.page % 16 == 0;
+  // pages of whole groups of 16 keys, keys and values with the same strides, and a group's rows
+  // within 32 bits of its first
+  a.even = a.page % 16 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
+           a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
   p->bytes = 0;
   if (a.tokens == 0) return 0;
-  const int64_t want = 2 * compute_units();
+  const int64_t cus = compute_units(), want = 2 * cus;
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
   p->prefix_rows = rows_of(rows, a.dim);
   a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
@@ -178,10 +212,11 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     int64_t splits = (want + units - 1) / units;
     splits = splits < most ? splits : most;
     a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
+    a.sorted = units > want && a.sequences <= 256;
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
   }
   a.slots = a.prefix_splits + a.own_splits;
-  const i64 all = (static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences + 8) * a.kv_heads;
+  const i64 all = static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences * a.kv_heads;
   const i64 first = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 8) * a.prefix_tiles;
   if (all > 0xFFFFFF || first > 0xFFFFFF)
     return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups", all > first ? all : first);
@@ -202,11 +237,16 @@ hipError_t launch_parts(const Attention& a, int64_t dtype, int rows, bool prefix
   return launch_parts<256>(a, dtype, rows, prefix, s);
 }
 
-template <typename T>
+template <typename T, int WAVES>
 const void* join_of(int dim) {
-  if (dim <= 64) return reinterpret_cast<const void*>(&join_parts<T, 16>);
-  if (dim <= 128) return reinterpret_cast<const void*>(&join_parts<T, 32>);
-  return reinterpret_cast<const void*>(&join_parts<T, 64>);
+  if (dim <= 64) return reinterpret_cast<const void*>(&join_parts<T, 16, WAVES>);
+  if (dim <= 128) return reinterpret_cast<const void*>(&join_parts<T, 32, WAVES>);
+  return reinterpret_cast<const void*>(&join_parts<T, 64, WAVES>);
+}
+
+template <typename T>
+const void* join_of(int dim, bool shared) {
+  return shared ? join_of<T, 4>(dim) : join_of<T, 1>(dim);
 }
 
 }  // namespace
@@ -248,9 +288,10 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
     if (e != hipSuccess) return hip_failed(e, what);
   }
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
+  const bool shared = a.slots > 16;
   void* args[] = {&a};
   const hipError_t e = hipLaunchKernel(
-      r->dtype == TG_F16 ? join_of<_Float16>(a.dim) : join_of<__bf16>(a.dim),
-      dim3(static_cast<unsigned>((rows + 3) / 4)), dim3(256), args, 0, s);
+      r->dtype == TG_F16 ? join_of<_Float16>(a.dim, shared) : join_of<__bf16>(a.dim, shared),
+      dim3(static_cast<unsigned>(shared ? rows : (rows + 3) / 4)), dim3(256), args, 0, s);
   return e == hipSuccess ? 0 : hip_failed(e, what);
 }

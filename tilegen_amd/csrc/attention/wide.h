@@ -448,7 +448,7 @@ template <typename T, int DP, int NW>
 __global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_own(Attention a) {
   __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
   int first, split, head, b;
-  if (!own_place(a, &first, &split, &head, &b)) return;
+  own_place<64 * NW>(a, &first, &split, &head, &b);
   const Sequence s = sequence(a, b);
   Part p;
   p.list = s.list;
