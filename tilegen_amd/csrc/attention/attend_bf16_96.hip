@@ -1,0 +1,3 @@
+#include "attend.h"
+
+template hipError_t tg::launch_parts<__bf16, 96>(const Attention&, int, int, hipStream_t);

@@ -1,0 +1,3 @@
+#include "attend.h"
+
+template hipError_t tg::launch_parts<_Float16, 128>(const Attention&, int, int, hipStream_t);

@@ -83,6 +83,8 @@ __device__ __forceinline__ float apart(float s, float scale, float base) {
   return x - base;
 }
 
+constexpr int kWaves = 4;       // of a workgroup
+
 // Rows and keys of one workgroup's part.
 struct Part {
   const int64_t* list;  // pages
@@ -101,19 +103,15 @@ __device__ __forceinline__ void load_to_lds(const void* from, char* to) {
 }
 
 // The prefix's workgroups: those that read the same keys (the row tiles of a kv head and a key
-// range) follow one another, and every XCD takes an eighth of all in that order (workgroup i
-// goes to XCD i % 8), so that they share an L2 and all XCDs have as much to do.
-__host__ __device__ inline i64 prefix_count(const Attention& a) {
-  return static_cast<i64>(a.prefix_tiles) * a.kv_heads * a.prefix_splits;
-}
-inline i64 prefix_grid(const Attention& a) { return (prefix_count(a) + 7) / 8 * 8; }
-__device__ __forceinline__ bool prefix_place(const Attention& a, int* tile, int* kv_head,
-                                             int* split) {
-  const int n = static_cast<int>(prefix_count(a));
-  const int i = static_cast<int>(blockIdx.x & 7) * ((n + 7) / 8) + (blockIdx.x >> 3);
-  if (static_cast<int>(blockIdx.x >> 3) >= (n + 7) / 8 || i >= n) return false;
-  const int unit = i / a.prefix_tiles;
-  *tile = i - unit * a.prefix_tiles;
+// range) follow one another, and every XCD takes an eighth of all in that order, so that they
+// share an L2 and all XCDs have as much to do.  `i` counts the workgroups of one XCD.
+__device__ __forceinline__ bool prefix_place(const Attention& a, int xcd, int i, int* tile,
+                                             int* kv_head, int* split) {
+  const int n = a.prefix_tiles * a.kv_heads * a.prefix_splits, each = (n + 7) / 8;
+  const int at = xcd * each + i;
+  if (i >= each || at >= n) return false;
+  const int unit = at / a.prefix_tiles;
+  *tile = at - unit * a.prefix_tiles;
   *split = unit / a.kv_heads;
   *kv_head = unit - *split * a.kv_heads;
   return true;
@@ -121,23 +119,21 @@ __device__ __forceinline__ bool prefix_place(const Attention& a, int* tile, int*
 
 // The own pages' workgroups: the kv heads of a sequence's row tile and key range side by side.
 // (All heads of it on one XCD instead measured 5% slower.)
-inline i64 own_grid(const Attention& a) {
-  return static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences * a.kv_heads;
-}
+//
 // With `sorted`, at most as many sequences as a workgroup has threads stand in the order of their
 // lengths, the longest first: long parts that start last would leave most of the chip idle
 // behind them.  Each thread ranks one sequence.
-template <int THREADS>
-__device__ __forceinline__ void own_place(const Attention& a, int* tile, int* split, int* kv_head,
-                                          int* b) {
-  int unit = blockIdx.x / a.kv_heads;
-  *kv_head = blockIdx.x - unit * a.kv_heads;
+__device__ __forceinline__ bool own_place(const Attention& a, int i, int* tile, int* split,
+                                          int* kv_head, int* b) {
+  int unit = i / a.kv_heads;
+  *kv_head = i - unit * a.kv_heads;
   *split = unit % a.own_splits;
   unit /= a.own_splits;
   *tile = unit % a.own_tiles;
   *b = unit / a.own_tiles;
+  if (*b >= a.sequences) return false;
   if (a.sorted) {
-    __shared__ __align__(16) int lengths[THREADS];
+    __shared__ __align__(16) int lengths[64 * kWaves];
     __shared__ int found;
     const int tid = threadIdx.x;
     const int64_t length = tid < a.sequences ? a.lengths[tid] : -1;
@@ -157,6 +153,7 @@ __device__ __forceinline__ void own_place(const Attention& a, int* tile, int* sp
     __syncthreads();
     *b = __builtin_amdgcn_readfirstlane(found);
   }
+  return true;
 }
 
 // The four keys of V^T that the transposing LDS read gives a lane: 16 lanes name 4 rows of 16

@@ -25,6 +25,7 @@ struct Attention {
   int prefix_splits, prefix_chunk, prefix_tiles;
   int own_splits, own_chunk, own_tiles;
   int slots;
+  int prefix_eights, own_eights;    // workgroups, in eights
   int even;           // the wide kernel's scalar addresses hold (wide.h)
   int sorted;         // own parts go from the longest sequence to the shortest (parts.h)
 };
@@ -72,12 +73,8 @@ __device__ __forceinline__ int own_parts(const Attention& a, int keys) {
   return n < a.own_splits ? n : a.own_splits;
 }
 
-// Enqueue the parts of the prefix (or of the own pages) for one padded head size.
-template <int DP>
-hipError_t launch_narrow(const Attention& a, int64_t dtype, int nt, bool prefix,
-                         hipStream_t stream);
-template <int DP>
-hipError_t launch_wide(const Attention& a, int64_t dtype, int rows, bool prefix,
-                       hipStream_t stream);
+// Enqueues the parts for one type and padded head size.
+template <typename T, int DP>
+hipError_t launch_parts(const Attention& a, int prefix_rows, int own_rows, hipStream_t stream);
 
 }  // namespace tg

@@ -104,16 +104,11 @@ int compute_units() {
 
 struct Plan {
   Attention a;
-  int prefix_rows, own_rows;    // of one workgroup: narrow 16 and 32, wide 128 and 256
+  int prefix_rows, own_rows;    // of one workgroup: narrow 16, wide 128
   int64_t bytes;
 };
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
-
-// Rows of one workgroup where that many query rows read the same keys.
-int rows_of(int64_t rows, int dim) {
-  return rows <= 16 ? 16 : rows <= 64 ? 32 : rows <= 128 || dim > 128 ? 128 : 256;
-}
 
 int check(const tg_prefix_attention* r) {
   const char* what = "launch_prefix_attention";
@@ -187,54 +182,67 @@ int plan(const tg_prefix_attention* r, Plan* p) {
            a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
   p->bytes = 0;
   if (a.tokens == 0) return 0;
-  const int64_t cus = compute_units(), want = 2 * cus;
+  const int64_t cus = compute_units();
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
-  p->prefix_rows = rows_of(rows, a.dim);
-  a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
-  if (a.prefix_length) {
-    const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
-    const int64_t most = (a.prefix_length + 255) / 256;
-    int64_t splits = (p->prefix_rows == 256 ? want / 2 : want) / units;
-    splits = splits < 1 ? 1 : splits < most ? splits : most;
-    a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
-    a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
-  }
   const int64_t max_query = r->query_indptr ? (r->max_query > 0 ? r->max_query : 1) : 1;
-  const int64_t own_rows = max_query * a.group;
-  p->own_rows = rows_of(own_rows, a.dim);
+  p->prefix_rows = rows <= 16 ? 16 : 128;
+  p->own_rows = max_query * a.group <= 16 ? 16 : p->prefix_rows;
+  // workgroups that the chip holds at once
+  const int64_t room = a.dim > 128 ? cus : 2 * cus;
+  int64_t own = 0, own_keys = 0;    // workgroups, and keys that they read between them (half of the bound)
   if (a.pages && a.n_indices && a.sequences) {
-    int64_t tiles = (own_rows + p->own_rows - 1) / p->own_rows;
+    int64_t tiles = (max_query * a.group + p->own_rows - 1) / p->own_rows;
     tiles = tiles < 4096 ? tiles : 4096;
     a.own_tiles = static_cast<int>(tiles);
     const int64_t length = r->max_length > 0 ? r->max_length : 1;
     const int64_t units = tiles * a.kv_heads * a.sequences;
     const int64_t most = (length + 255) / 256;
-    int64_t splits = (want + units - 1) / units;
-    splits = splits < most ? splits : most;
+    int64_t splits = room / 2 / units;
+    splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
-    a.sorted = units > want && a.sequences <= 256;
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
+    a.sorted = units > room && a.sequences <= 256;
+    own = units * a.own_splits;
+    own_keys = units * length / 2;
+  }
+  a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
+  int64_t prefix = 0;
+  if (a.prefix_length) {
+    const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
+    const int64_t most = (a.prefix_length + 255) / 256;
+    // The prefix's parts are alike and run once, so they get what room the own pages leave.  Few
+    // of those (under an eighth of the work) run behind: 8 sequences on 131072 shared keys 112 us
+    // against 122 on three quarters.  Where all fit, they do; where they do not (128 sequences
+    // of up to 2048 keys, 32768 shared), parts that take turns beside the prefix's load while
+    // those multiply: 253 us on three quarters, 278 on all, 277 on half.
+    const int64_t keys = units * a.prefix_length;
+    int64_t left = room;
+    if (own_keys * 8 > own_keys + keys) {
+      left = own <= room / 2 ? room - own : room - room * 5 / 8 * own_keys / (own_keys + keys);
+      left = left < room / 2 ? room / 2 : left;
+    }
+    int64_t splits = left / units;
+    splits = splits < 1 ? 1 : splits < most ? splits : most;
+    a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
+    a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
+    prefix = units * a.prefix_splits;
   }
   a.slots = a.prefix_splits + a.own_splits;
-  const i64 all = static_cast<i64>(a.own_splits) * a.own_tiles * a.sequences * a.kv_heads;
-  const i64 first = (static_cast<i64>(a.kv_heads) * a.prefix_splits + 8) * a.prefix_tiles;
-  if (all > 0xFFFFFF || first > 0xFFFFFF)
-    return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups", all > first ? all : first);
+  if (own > 0xFFFFFF || prefix > 0xFFFFFF)
+    return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups",
+                  own > prefix ? own : prefix);
+  a.prefix_eights = static_cast<int>((prefix + 7) / 8);
+  a.own_eights = static_cast<int>((own + 7) / 8);
   p->bytes = static_cast<int64_t>(a.slots) * a.tokens * a.heads * (a.dim + 2) * 4;
   return 0;
 }
 
-template <int DP>
-hipError_t launch_parts(const Attention& a, int64_t dtype, int rows, bool prefix, hipStream_t s) {
-  return rows < 128 ? launch_narrow<DP>(a, dtype, rows / 16, prefix, s)
-                    : launch_wide<DP>(a, dtype, rows, prefix, s);
-}
-
-hipError_t launch_parts(const Attention& a, int64_t dtype, int rows, bool prefix, hipStream_t s) {
-  if (a.dim <= 64) return launch_parts<64>(a, dtype, rows, prefix, s);
-  if (a.dim <= 96) return launch_parts<96>(a, dtype, rows, prefix, s);
-  if (a.dim <= 128) return launch_parts<128>(a, dtype, rows, prefix, s);
-  return launch_parts<256>(a, dtype, rows, prefix, s);
+template <typename T>
+hipError_t launch_parts(const Plan& p, hipStream_t s) {
+  if (p.a.dim <= 64) return launch_parts<T, 64>(p.a, p.prefix_rows, p.own_rows, s);
+  if (p.a.dim <= 96) return launch_parts<T, 96>(p.a, p.prefix_rows, p.own_rows, s);
+  if (p.a.dim <= 128) return launch_parts<T, 128>(p.a, p.prefix_rows, p.own_rows, s);
+  return launch_parts<T, 256>(p.a, p.prefix_rows, p.own_rows, s);
 }
 
 template <typename T, int WAVES>
@@ -279,12 +287,9 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
   a.part_ml = reinterpret_cast<float2*>(a.part + static_cast<int64_t>(a.slots) * a.tokens *
                                                      a.heads * a.dim);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (a.prefix_splits) {
-    const hipError_t e = launch_parts(a, r->dtype, p.prefix_rows, true, s);
-    if (e != hipSuccess) return hip_failed(e, what);
-  }
-  if (a.own_splits) {
-    const hipError_t e = launch_parts(a, r->dtype, p.own_rows, false, s);
+  if (a.slots) {
+    const hipError_t e = r->dtype == TG_F16 ? launch_parts<_Float16>(p, s)
+                                            : launch_parts<__bf16>(p, s);
     if (e != hipSuccess) return hip_failed(e, what);
   }
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;

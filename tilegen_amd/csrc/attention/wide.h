@@ -18,19 +18,17 @@
 
 namespace tg {
 
-// NW: waves of a workgroup.
-template <int DP, int NW>
+template <int DP>
 struct Wide {
-  static constexpr int kRows = 32 * NW, kKeys = 64;
+  static constexpr int kRows = 32 * kWaves, kKeys = 64;
   static constexpr int kPitch = DP == 64 ? 128 : DP == 256 ? 512 : 256;   // bytes of an LDS row
   static constexpr int kChunks = kPitch / 16;
-  static constexpr int kThreads = 64 * NW;
+  static constexpr int kThreads = 64 * kWaves;
   static constexpr int kLoads = kKeys * kChunks / kThreads;   // of each thread, keys and values
   static constexpr int kPass = kThreads / kChunks;            // rows that one load of all covers
   static constexpr int kSpan = kThreads * 16;                 // and their bytes
   static constexpr int kTile = kKeys * kPitch;
   static constexpr int kBuffer = 2 * kTile;               // keys, then values
-  static constexpr int kPerCu = DP == 256 || NW == 8 ? 1 : 2;
 
   // Loads go straight to LDS, 16 bytes a lane side by side, so rows cannot be padded; instead a
   // row's chunks change places, and a lane fetches the chunk that belongs to its place.  Keys
@@ -84,10 +82,10 @@ __device__ __forceinline__ void side_by_side() {
   }
 }
 
-template <typename T, int DP, int NW, bool OWN>
+template <typename T, int DP, bool OWN>
 __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int kv_head,
                                           char* lds) {
-  using W = Wide<DP, NW>;
+  using W = Wide<DP>;
   using M = Matrix<T>;
   using C = Chunk<T>;
   constexpr int KS = DP / 16, DT = DP / 32;
@@ -424,79 +422,6 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
               f32x4{o[d][4 * b], o[d][4 * b + 1], o[d][4 * b + 2], o[d][4 * b + 3]};
     if (half == 0) a.part_ml[at] = make_float2(m, l);
   }
-}
-
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_prefix(Attention a) {
-  __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
-  int tile, kv_head, split;
-  if (!prefix_place(a, &tile, &kv_head, &split)) return;
-  Part p;
-  p.list = a.prefix;
-  p.k0 = split * a.prefix_chunk;
-  p.k1 = min(p.k0 + a.prefix_chunk, a.prefix_length);
-  p.row0 = tile * Wide<DP, NW>::kRows;
-  p.rows = a.tokens * a.group;
-  p.token0 = 0;
-  p.before = a.prefix_length;
-  p.step = 0;
-  p.slot = split;
-  wide_part<T, DP, NW, false>(a, p, kv_head, lds);
-}
-
-template <typename T, int DP, int NW>
-__global__ __launch_bounds__(64 * NW, (Wide<DP, NW>::kPerCu)) void wide_own(Attention a) {
-  __shared__ __align__(16) char lds[2 * Wide<DP, NW>::kBuffer];
-  int first, split, head, b;
-  own_place<64 * NW>(a, &first, &split, &head, &b);
-  const Sequence s = sequence(a, b);
-  Part p;
-  p.list = s.list;
-  p.rows = s.count * a.group;
-  p.token0 = s.first;
-  p.before = s.before + 1;
-  p.step = 1;
-  p.slot = a.prefix_splits + split;
-  p.k0 = split * a.own_chunk;
-  for (int tile = first; tile * Wide<DP, NW>::kRows < p.rows; tile += a.own_tiles) {
-    p.row0 = tile * Wide<DP, NW>::kRows;
-    const int last = min(p.row0 + Wide<DP, NW>::kRows, p.rows) - 1;
-    p.k1 = seen(s, a.by_group(last));
-    if (split + 1 < a.own_splits) p.k1 = min(p.k1, p.k0 + a.own_chunk);
-    if (p.k0 >= p.k1) continue;
-    wide_part<T, DP, NW, true>(a, p, head, lds);
-    __syncthreads();
-  }
-}
-
-template <int DP, typename T, int NW>
-hipError_t launch_wide_as(const Attention& a, bool prefix, hipStream_t stream) {
-  i64 grid;
-  const void* f;
-  if (prefix) {
-    grid = prefix_grid(a);
-    f = reinterpret_cast<const void*>(&wide_prefix<T, DP, NW>);
-  } else {
-    grid = own_grid(a);
-    f = reinterpret_cast<const void*>(&wide_own<T, DP, NW>);
-  }
-  Attention copy = a;
-  void* args[] = {&copy};
-  return hipLaunchKernel(f, dim3(static_cast<unsigned>(grid)), dim3(64 * NW), args, 0, stream);
-}
-
-template <int DP, typename T>
-hipError_t launch_wide_rows(const Attention& a, int rows, bool prefix, hipStream_t stream) {
-  if constexpr (DP <= 128)
-    if (rows == 256) return launch_wide_as<DP, T, 8>(a, prefix, stream);
-  return launch_wide_as<DP, T, 4>(a, prefix, stream);
-}
-
-template <int DP>
-hipError_t launch_wide(const Attention& a, int64_t dtype, int rows, bool prefix,
-                       hipStream_t stream) {
-  return dtype == TG_F16 ? launch_wide_rows<DP, _Float16>(a, rows, prefix, stream)
-                         : launch_wide_rows<DP, __bf16>(a, rows, prefix, stream);
 }
 
 }  // namespace tg
