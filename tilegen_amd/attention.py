@@ -68,42 +68,55 @@ def _lib():
 # --------------------------------------------------------------------------- #
 # checks
 # --------------------------------------------------------------------------- #
-def _heads(name: str, t: torch.Tensor, device: torch.device, dtype: torch.dtype, dims: int,
+# The checks are most of what a small call costs the host, so each asks the common case in one
+# condition and works out what is wrong only when it fails.
+def _heads(name: str, t: torch.Tensor, device: int, dtype: torch.dtype, dims: int,
            write: bool = False):
     """(shape, strides) of an operand whose last axis is a head."""
-    if t.device != device or t.dtype != dtype:
-        raise ValueError("%s is %s on %s, expected %s on %s" % (name, t.dtype, t.device, dtype,
-                                                                device))
     shape, strides = t.shape, t.stride()
-    if len(shape) != dims:
-        raise ValueError("%s has %d axes, expected %d" % (name, len(shape), dims))
-    if strides[-1] != 1 and shape[-1] > 1:
-        raise ValueError("%s: the elements of a head are not contiguous (strides %s)"
-                         % (name, strides))
+    if not (t.get_device() == device and t.dtype is dtype and len(shape) == dims
+            and (strides[-1] == 1 or shape[-1] <= 1)):
+        _refuse_heads(name, t, device, dtype, dims)
     if write and 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
         raise ValueError("%s is written, but its elements share memory (strides %s)"
                          % (name, strides))
     return shape, strides
 
 
-def _list(name: str, t: torch.Tensor, device: torch.device, n: Optional[int] = None,
+def _refuse_heads(name, t, device, dtype, dims):
+    if t.get_device() != device or t.dtype != dtype:
+        raise ValueError("%s is %s on %s, expected %s on device %d" % (name, t.dtype, t.device,
+                                                                       dtype, device))
+    if t.dim() != dims:
+        raise ValueError("%s has %d axes, expected %d" % (name, t.dim(), dims))
+    raise ValueError("%s: the elements of a head are not contiguous (strides %s)"
+                     % (name, t.stride()))
+
+
+def _list(name: str, t: torch.Tensor, device: int, n: Optional[int] = None,
           dtype: torch.dtype = torch.int64) -> int:
     """The address of a one-dimensional contiguous array (of n entries)."""
-    if t.device != device or t.dtype != dtype or t.dim() != 1 or not t.is_contiguous():
-        raise ValueError("%s is %s %s on %s, expected a contiguous list of %s on %s" % (
+    if not (t.get_device() == device and t.dtype is dtype and t.dim() == 1
+            and t.is_contiguous()):
+        raise ValueError("%s is %s %s on %s, expected a contiguous list of %s on device %d" % (
             name, t.dtype, tuple(t.shape), t.device, dtype, device))
     if n is not None and t.shape[0] != n:
         raise ValueError("%s has %d entries, expected %d" % (name, t.shape[0], n))
     return t.data_ptr()
 
 
-def _operand(name: str, t: torch.Tensor, dtypes) -> Tuple[torch.device, torch.dtype]:
+def _operand(name: str, t: torch.Tensor, dtypes) -> Tuple[int, torch.dtype]:
+    """(device, type) that a call goes by."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s is not a tensor on a HIP device" % name)
     if t.dtype not in dtypes:
         raise ValueError("%s is %s, expected one of %s" % (name, t.dtype,
                                                            ", ".join(map(str, dtypes))))
-    return t.device, t.dtype
+    return t.get_device(), t.dtype
+
+
+def _like(x: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _layout(layout: str) -> int:
@@ -112,12 +125,17 @@ def _layout(layout: str) -> int:
     return _LAYOUTS[layout]
 
 
-def _call(entry, packed: bytes, device: torch.device, what: str) -> None:
-    if device.index == torch.cuda.current_device():
-        rc = entry(packed, torch.cuda.current_stream().cuda_stream)
+# torch's current stream as a handle, without the object that current_stream() builds (2.7 us)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda device: torch.cuda.current_stream(device).cuda_stream)
+
+
+def _call(entry, packed: bytes, device: int, what: str) -> None:
+    if device == torch.cuda.current_device():
+        rc = entry(packed, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = entry(packed, torch.cuda.current_stream().cuda_stream)
+            rc = entry(packed, _raw_stream(device))
     if rc:
         _raise(rc, what)
 
@@ -188,7 +206,7 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     device, dtype = _operand("x", x, _DTYPES)
     shape, xs = _heads("x", x, device, dtype, 3)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = _like(x)
     elif out is not x:
         _apart("out", out, "x", x)
     oshape, ys = _heads("out", out, device, dtype, 3, write=True)
@@ -302,7 +320,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
         if qshape[0] != tokens or qshape[2] != dim:
             raise ValueError("query is %s, key %s" % (tuple(qshape), tuple(shape)))
         if query_out is None:
-            query_out = torch.empty(qshape, dtype=dtype, device=device)
+            query_out = _like(query)
         elif query_out is not query:
             _apart("query_out", query_out, "query", query)
         oshape, os_ = _heads("query_out", query_out, device, dtype, 3, write=True)
@@ -362,11 +380,11 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     (p_indptr, p_indices, p_lengths, p_ends), sequences = _table(
         indptr, indices, lengths, query_indptr, tokens, device)
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=device)
+        out = _like(query)
     oshape, os_ = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))
-    lse = torch.empty(shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    lse = query.new_empty(shape[:2], dtype=torch.float32) if return_lse else None
     fields = [query.data_ptr(), key_cache.data_ptr(), value_cache.data_ptr(),
               _list("prefix", prefix, device), p_indptr, p_indices, p_lengths, p_ends,
               out.data_ptr(), lse.data_ptr() if return_lse else 0, 0, 0, _DTYPES[dtype], tokens,
@@ -378,7 +396,7 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     n = L.prefix_attention_workspace(_ATTENTION.pack(*fields))
     if n < 0:
         _raise(n, "prefix_attention")
-    workspace = torch.empty(n, dtype=torch.uint8, device=device)
+    workspace = query.new_empty(n, dtype=torch.uint8)
     fields[10], fields[11] = workspace.data_ptr(), n
     _call(L.launch_prefix_attention, _ATTENTION.pack(*fields), device, "prefix_attention")
     return (out, lse) if return_lse else out
