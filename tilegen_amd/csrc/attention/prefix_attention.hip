@@ -196,7 +196,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     a.own_tiles = static_cast<int>(tiles);
     const int64_t length = r->max_length > 0 ? r->max_length : 1;
     const int64_t units = tiles * a.kv_heads * a.sequences;
-    const int64_t most = (length + 255) / 256;
+    const int64_t most = (length + 127) / 128;
     int64_t splits = room / 2 / units;
     splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
@@ -209,19 +209,17 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   int64_t prefix = 0;
   if (a.prefix_length) {
     const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
-    const int64_t most = (a.prefix_length + 255) / 256;
-    // The prefix's parts are alike and run once, so they get what room the own pages leave.  Few
-    // of those (under an eighth of the work) run behind: 8 sequences on 131072 shared keys 112 us
-    // against 122 on three quarters.  Where all fit, they do; where they do not (128 sequences
-    // of up to 2048 keys, 32768 shared), parts that take turns beside the prefix's load while
-    // those multiply: 253 us on three quarters, 278 on all, 277 on half.
+    const int64_t most = (a.prefix_length + 127) / 128;
+    // The prefix's parts are alike and start first, so they get the room that their share of the
+    // keys to read asks for, and the own pages' take turns in the rest: their loads run beside the
+    // prefix's products.  64 sequences of up to 4096 keys, 16384 shared: 184 us with a quarter of
+    // the room, 227 with three; 128 of up to 2048, 32768 shared: 257 us with five eighths, 253
+    // with six, 278 with all, 470 with two.  Own pages that are under an eighth of the work run
+    // behind: 8 sequences on 131072 shared keys 112 us, 122 where they were given a quarter.
     const int64_t keys = units * a.prefix_length;
-    int64_t left = room;
-    if (own_keys * 8 > own_keys + keys) {
-      left = own <= room / 2 ? room - own : room - room * 5 / 8 * own_keys / (own_keys + keys);
-      left = left < room / 2 ? room / 2 : left;
-    }
-    int64_t splits = left / units;
+    const int64_t left =
+        own_keys * 8 > own_keys + keys ? room - room * own_keys / (own_keys + keys) : room;
+    int64_t splits = left == room ? room / units : (left + units / 2) / units;
     splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
     a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
