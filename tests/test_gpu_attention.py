@@ -261,6 +261,15 @@ ATTENTION = [
     (16, 4, 128, 64, 600, [190, 77], [150, 70]),
     (12, 4, 64, 16, 300, [64, 200, 33, 1], [64, 130, 20, 1]),
     (8, 1, 64, 1, 40, [9, 4], [4, 4]),
+    # wide over many tiles: pages of 8-key groups, of neither 8 nor 16, heads of all sizes
+    (16, 1, 96, 24, 1501, [40, 7, 90], [7, 1, 3]),
+    (9, 1, 64, 7, 1100, [600, 31], [9, 4]),
+    (40, 2, 128, 20, 1300, [1, 140], [1, 1]),
+    (24, 1, 256, 16, 1217, [700, 80], [1, 3]),
+    (17, 1, 200, 8, 900, [33], [1]),
+    # more workgroups than the chip holds: the longest sequences first, and more than are ranked
+    (8, 8, 64, 16, 40, [(37 * i) % 90 for i in range(80)], [1] * 80),
+    (2, 2, 40, 16, 0, [(11 * i) % 50 for i in range(300)], [1] * 300),
     # fewer tokens than new ones: the first see the prefix alone, or nothing
     (4, 2, 64, 16, 20, [2, 0], [5, 3]),
     (4, 2, 64, 16, 0, [2, 0], [5, 3]),
@@ -277,6 +286,52 @@ def test_prefix_attention(hip_ready, dtype, heads, kv_heads, dim, page, prefix, 
     b.check(b.attend(max_query=1, max_length=1))
     again = b.attend()
     assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_hidden_keys_of_few_rows(hip_ready, dtype):
+    """As below, where a sequence's new tokens fill less than one narrow tile."""
+    b = Batch(dtype, 2, 1, 96, 24, 70, [33, 64], [4, 8], seed=14).fill()
+    clean = b.want()
+    page, slot = b.places(0)
+    b.vc[page[-1], slot[-1]] = math.inf
+    b.kc[page[-2], slot[-2]] = math.nan         # seen by tokens 2 and 3
+    page, slot = b.places(1)
+    b.vc[page[-4], slot[-4], 0, 95] = math.nan  # seen by the last four
+    got, lse = (x.cpu().double() for x in b.attend())
+    fine = torch.ones(12, 2, 96, dtype=torch.bool)
+    fine[2:4] = False
+    fine[8:, :, 95] = False
+    assert ((got - clean[0]).abs() <= clean[2])[fine].all()
+    assert torch.isnan(got[~fine]).all()
+    rows = torch.tensor([i not in (2, 3) for i in range(12)])
+    assert ((lse - clean[1]).abs() <= clean[3])[rows].all()
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (40, 1, 128, 8),
+                                                     (20, 1, 96, 7), (17, 1, 256, 24)])
+def test_lost_pages_inside_a_long_prefix(hip_ready, heads, kv_heads, dim, page):
+    """Pages of the prefix that do not exist count as hidden, wherever their tiles stand, and what
+    the first page of the cache holds does not matter."""
+    b = Batch(BF16, heads, kv_heads, dim, page, 1200, [30, 9], [1, 1], seed=dim).fill()
+    n = -(-1200 // page)
+    lost = [0, 3, n // 2, n // 2 + 1, n - 2]
+    whole = b.prefix.clone()
+    b.prefix[lost] = torch.tensor([-1, b.pages, 2 ** 40, -2 ** 40, b.pages + 1], device="cuda")
+    used = bool((whole == 0).any() or (b.indices == 0).any())
+    if not used:
+        b.kc[0], b.vc[0] = math.nan, math.inf
+    got = b.attend()
+    # the same keys as a prefix without those pages
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[lost] = False
+    short = Batch(BF16, heads, kv_heads, dim, page, 1200, [30, 9], [1, 1], seed=dim)
+    short.kc, short.vc, short.query = b.kc, b.vc, b.query
+    short.indptr, short.indices = b.indptr, b.indices
+    short.prefix = whole[keep.cuda()].contiguous()
+    short.prefix_length = 1200 - page * len(lost)
+    short.check(got)
+    short.check(short.attend())
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
@@ -388,12 +443,13 @@ def test_strides_and_given_outputs(hip_ready):
     b.check(b.attend(scale=0.5), scale=0.5)
 
 
-def test_offsets_past_32_bits(hip_ready):
+@pytest.mark.parametrize("heads", [4, 16])     # narrow and wide
+def test_offsets_past_32_bits(hip_ready, heads):
     """Pages whose elements lie past 2^31, and 2^32 bytes, of the cache."""
     pages, page, dim = 70000, 64, 256
     kc = torch.empty(pages, page, 2, dim, device="cuda", dtype=BF16)      # 2.3 G elements
     vc = torch.empty(pages, page, 2, dim, device="cuda", dtype=BF16)
-    b = Batch(BF16, 4, 2, dim, page, 100, [90, 3], [3, 2], seed=10)
+    b = Batch(BF16, heads, 2, dim, page, 100, [90, 3], [3, 2], seed=10)
     b.prefix += pages - b.pages
     b.indices += pages - b.pages
     b.kc, b.vc, b.pages = kc, vc, pages

@@ -175,14 +175,6 @@ def build_attention() -> str:
     return out
 
 
-def attention_code_object(source: str, out: str) -> str:
-    """The device code object alone of one of libtgattn.so's sources, for checks of its
-    kernels' registers and spills."""
-    _run(_attention_compile(source) + ["--offload-device-only", "--no-gpu-bundle-output",
-                                       "-o", out])
-    return out
-
-
 def build_oracle(force: bool = False) -> None:
     _run(["make", "-s"] + (["-B"] if force else []) + ["-C", os.path.join(REPO, "oracle")])
 

@@ -139,6 +139,7 @@ int check(const tg_prefix_attention* r) {
 }
 
 int plan(const tg_prefix_attention* r, Plan* p) {
+  const char* what = "launch_prefix_attention";
   if (const int rc = check(r)) return rc;
   Attention& a = p->a;
   a = Attention{};
@@ -176,9 +177,9 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   a.scale = static_cast<float>(r->scale * 1.4426950408889634);
   a.by_group = Div(a.group);
   a.by_page = Div(a.page);
-  // pages of whole groups of 16 keys, keys and values with the same strides, and a group's rows
+  // pages of whole groups of 8 keys, keys and values with the same strides, and a group's rows
   // within 32 bits of its first
-  a.even = a.page % 16 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
+  a.even = a.page % 8 == 0 && a.kc_page == a.vc_page && a.kc_slot == a.vc_slot &&
            a.kc_page >= 0 && a.kc_slot >= 0 && a.kc_slot < (1 << 24);
   p->bytes = 0;
   if (a.tokens == 0) return 0;
@@ -203,6 +204,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
     a.sorted = units > room && a.sequences <= 256;
     own = units * a.own_splits;
+    if (own > 0xFFFFFF) return refuse(-2, what, "more than 2^24 workgroups", own);
     own_keys = units * length / 2;
   }
   a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
@@ -226,9 +228,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     prefix = units * a.prefix_splits;
   }
   a.slots = a.prefix_splits + a.own_splits;
-  if (own > 0xFFFFFF || prefix > 0xFFFFFF)
-    return refuse(-2, "launch_prefix_attention", "more than 2^24 workgroups",
-                  own > prefix ? own : prefix);
+  if (prefix > 0xFFFFFF) return refuse(-2, what, "more than 2^24 workgroups", prefix);
   a.prefix_eights = static_cast<int>((prefix + 7) / 8);
   a.own_eights = static_cast<int>((own + 7) / 8);
   p->bytes = static_cast<int64_t>(a.slots) * a.tokens * a.heads * (a.dim + 2) * 4;

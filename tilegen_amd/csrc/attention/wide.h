@@ -118,25 +118,39 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   const T* vc = static_cast<const T*>(a.v) + kv_head * a.vc_head;
   const int tiles = (p.k1 - p.k0 + W::kKeys - 1) / W::kKeys;
 
-  // Where a tile's keys are, lane = key: bytes from the head's first key (values have the same
-  // strides where `even`), or negative where a key has no page.  Pages are asked for a tile
-  // before they are needed and before that tile's loads, since loads return in order.  Keys past the
-  // end stand for the last one (hidden).
-  auto key_of_lane = [&](int tile) { return min(p.k0 + tile * W::kKeys + lane, p.k1 - 1); };
+  // Where keys are: bytes from the head's first key, or negative where a key has no page.  Where
+  // pages hold whole groups of 8 keys (`even`) a lane knows where one group starts, 64 lanes 8 tiles
+  // of them; a wave's rows of one load stand in one group, so that the address is uniform.
+  // Elsewhere a lane knows one key of one tile.  Pages are asked for a tile before they are needed
+  // and before that tile's loads, since loads return in order.  Keys past the end stand for the
+  // last one (hidden).
+  auto key_of_lane = [&](int tile) {
+    return min(a.even ? p.k0 + (tile >> 3) * 8 * W::kKeys + 8 * lane
+                      : p.k0 + tile * W::kKeys + lane,
+               p.k1 - 1);
+  };
   auto pages_of = [&](int tile) { return p.list[a.by_page(key_of_lane(tile))]; };
   auto offsets_of = [&](int tile, i64 page) -> i64 {
-    const int key = key_of_lane(tile);
+    const int key = key_of_lane(tile) & (a.even ? ~7 : ~0);
     const int slot = key - static_cast<int>(a.by_page(key)) * a.page;
     const i64 at = a.even ? (page * a.kc_page + slot * a.kc_slot) * 2
                           : page << 32 | static_cast<unsigned>(slot);
     return page < 0 || page >= a.pages ? -1 : at;
   };
-  // Where pages hold whole groups of 16 keys (`even`) a wave's rows of one load stand on one
-  // page: the group's offset is uniform, and `in_group` bytes lead to this lane's row.
-  unsigned in_group[2];
+  // a bit for each key of a tile that has no page
+  auto lost = [&](int tile, i64 offsets) -> unsigned long long {
+    unsigned long long none = __ballot(offsets < 0);
+    if (!a.even || none == 0) return none;
+    none = none >> (tile % 8 * 8) & 0xFF;
+    unsigned long long keys = 0;
+    for (int i = 0; i < 8; ++i)
+      if (none >> i & 1) keys |= 0xFFull << (8 * i);
+    return keys;
+  };
+  unsigned in_group[2];     // bytes from a group's first row to this lane's
 #pragma unroll
   for (int i = 0; i < 2; ++i)
-    in_group[i] = ((first + W::kPass * i) & 15) * static_cast<unsigned>(a.kc_slot) * 2;
+    in_group[i] = ((first + W::kPass * i) & 7) * static_cast<unsigned>(a.kc_slot) * 2;
   // one tile's keys or values
   auto load = [&](auto which, int tile, i64 offsets) {
     constexpr bool kKeys = decltype(which)::value;
@@ -145,16 +159,18 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     auto chunk = [&](int row) {
       return place ^ (kKeys ? W::key_place(row) : W::value_place(row));
     };
-    if (a.even && p.k0 + (tile + 1) * W::kKeys <= p.k1 && !__any(offsets < 0)) {
+    const int key0 = p.k0 + tile * W::kKeys;
+    if (a.even && key0 + W::kKeys <= p.k1 && !__any(offsets < 0)) {
       const char* at[W::kLoads];
 #pragma unroll
       for (int i = 0; i < W::kLoads; ++i) {
-        const int group = __builtin_amdgcn_readfirstlane((first + W::kPass * i) & ~15);
+        const int group =
+            tile % 8 * 8 + __builtin_amdgcn_readfirstlane((first + W::kPass * i) >> 3);
         const unsigned lo = __builtin_amdgcn_readlane(static_cast<int>(offsets), group);
         const unsigned hi = __builtin_amdgcn_readlane(static_cast<int>(offsets >> 32), group);
         at[i] = reinterpret_cast<const char*>(cache) + (static_cast<uint64_t>(hi) << 32 | lo);
       }
-      if constexpr (W::kPass >= 16) {     // the same chunk of all rows
+      if constexpr (W::kPass >= 16) {     // the same chunk, and place in a group, of all rows
         if (chunk(first) * 8 < a.dim)
 #pragma unroll
           for (int i = 0; i < W::kLoads; ++i)
@@ -173,9 +189,10 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
 #pragma unroll 1
     for (int i = 0; i < W::kLoads; ++i) {
       const int r = first + W::kPass * i, d = chunk(r) * 8;
-      const i64 at = __shfl(offsets, r);
+      const int key = min(key0 + r, p.k1 - 1);
+      const i64 at = __shfl(offsets, a.even ? tile % 8 * 8 + ((key - key0) >> 3) : r);
       if (at >= 0) {
-        const T* from = a.even ? cache + at / 2
+        const T* from = a.even ? cache + at / 2 + (key & 7) * slot_stride
                                : cache + (at >> 32) * page_stride +
                                      static_cast<i64>(static_cast<unsigned>(at)) * slot_stride;
         if (d < a.dim) load_to_lds(from + d, to + W::kSpan * i);
@@ -288,16 +305,17 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   // its keys are loaded two tiles ahead, its values one.
   const int whole = (all - p.k0) / W::kKeys > 0 ? (all - p.k0) / W::kKeys : 0;
   if (whole) {
-    i64 now_at = offsets_of(0, pages_of(0)), next_at = offsets_of(1, pages_of(1));
+    const i64 at0 = offsets_of(0, pages_of(0));
+    i64 where = a.even ? at0 : offsets_of(1, pages_of(1));    // of the next tile's keys
     i64 page0 = pages_of(2), page1;
     float top;
-    load(keys_of, 0, now_at);
-    load(values_of, 0, now_at);
-    if (whole > 1) load(keys_of, 1, next_at);
+    load(keys_of, 0, at0);
+    load(values_of, 0, at0);
+    if (whole > 1) load(keys_of, 1, where);
     __syncthreads();
     f32x16 s0[2], s1[2];
     score(lds, s0);
-    if (const unsigned long long without = __ballot(now_at < 0)) hide(s0, W::kKeys, without);
+    if (const unsigned long long without = lost(0, at0)) hide(s0, W::kKeys, without);
     top = largest(s0);
     __syncthreads();    // tile 2's keys take the place of tile 0's
 
@@ -307,12 +325,12 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     auto add = [&](int tile, f32x16* now, f32x16* then, const i64& page, i64& page_then) {
       const char* keys = lds + ((tile + 1) & 1) * W::kBuffer;
       const char* values = lds + (tile & 1) * W::kBuffer + W::kTile;
-      const unsigned long long without = __ballot(next_at < 0);
-      const i64 at = offsets_of(tile + 2, page);
+      const unsigned long long without = lost(tile + 1, where);
+      const i64 here = where;
+      if (!a.even || (tile + 2) % 8 == 0) where = offsets_of(tile + 2, page);
       page_then = pages_of(tile + 3);
-      if (tile + 1 < whole) load(values_of, tile + 1, next_at);
-      if (tile + 2 < whole) load(keys_of, tile + 2, at);
-      next_at = at;
+      if (tile + 1 < whole) load(values_of, tile + 1, here);
+      if (tile + 2 < whole) load(keys_of, tile + 2, where);
       follow(top);
       float scale, base;
       bases(now, &scale, &base);
@@ -357,7 +375,7 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
     const int left = see - (p.k0 + tile * W::kKeys);
     f32x16 s[2];
     score(keys, s);
-    hide(s, left, __ballot(at < 0));
+    hide(s, left, lost(tile, at));
     follow(largest(s));
     float scale, base;
     bases(s, &scale, &base);
