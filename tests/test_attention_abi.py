@@ -73,14 +73,15 @@ def test_refusals_without_a_device():
                          "dtype tokens sequences heads kv_heads dim pages page n_prefix "
                          "prefix_length n_indices max_query max_length").split()]
     base = dict.fromkeys(names, 0)
-    base.update(tokens=2, sequences=2, heads=4, kv_heads=2, dim=64, pages=9, page=16, n_prefix=2,
-                prefix_length=32, n_indices=4, max_query=1, max_length=20)
+    base.update(tokens=2, sequences=2, heads=4, kv_heads=2, dim=64, pages=999, page=16,
+                n_prefix=200, prefix_length=3200, n_indices=4, max_query=1, max_length=20)
     base.update({"s%d" % i: 64 for i in range(10)}, scale=0.125)
 
     def attend(**change):
         return at._ATTENTION.pack(*{**base, **change}.values())
 
     need = L.prefix_attention_workspace(attend())
+    assert L.prefix_attention_workspace(attend(prefix_length=32)) == 0   # one launch, no parts
     assert need > 0 and "null" in message(L.launch_prefix_attention(attend(), None), -1)
     every = {n: 4096 for n in names[:10]}
     assert "workspace" in message(L.launch_prefix_attention(
@@ -90,7 +91,7 @@ def test_refusals_without_a_device():
     for change, code in [(dict(dtype=2), -1), (dict(dim=12), -1), (dict(dim=264), -1),
                          (dict(kv_heads=3), -1), (dict(kv_heads=0), -1), (dict(page=0), -1),
                          (dict(scale=0.0), -1), (dict(scale=math.nan), -1),
-                         (dict(prefix_length=33), -1), (dict(tokens=3), -1),
+                         (dict(prefix_length=3201), -1), (dict(tokens=3), -1),
                          (dict(max_length=1 << 40), -2), (dict(sequences=-1), -1),
                          (dict(tokens=1 << 25, sequences=1 << 25), -2)]:
         assert L.prefix_attention_workspace(attend(**change)) < 0, change

@@ -396,7 +396,8 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     n = L.prefix_attention_workspace(_ATTENTION.pack(*fields))
     if n < 0:
         _raise(n, "prefix_attention")
-    workspace = query.new_empty(n, dtype=torch.uint8)
-    fields[10], fields[11] = workspace.data_ptr(), n
+    if n:
+        workspace = query.new_empty(n, dtype=torch.uint8)
+        fields[10], fields[11] = workspace.data_ptr(), n
     _call(L.launch_prefix_attention, _ATTENTION.pack(*fields), device, "prefix_attention")
     return (out, lse) if return_lse else out

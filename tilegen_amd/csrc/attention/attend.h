@@ -25,7 +25,7 @@ struct Attend {
 template <typename T, int DP, int ROWS, bool OWN>
 __device__ __forceinline__ void part(const Attention& a, const Part& p, int kv_head, char* lds) {
   if constexpr (ROWS == 16)
-    narrow_part<T, DP>(a, p, kv_head, lds);
+    narrow_part<T, DP, false>(a, p, kv_head, lds);
   else
     wide_part<T, DP, OWN>(a, p, kv_head, lds);
 }
@@ -81,6 +81,58 @@ hipError_t launch(const Attention& a, hipStream_t stream) {
   void* args[] = {&copy};
   return hipLaunchKernel(reinterpret_cast<const void*>(&attend<T, DP, PREFIX, OWN>),
                          dim3(static_cast<unsigned>(a.prefix_eights + a.own_eights) * 8),
+                         dim3(64 * kWaves), args, 0, stream);
+}
+
+// A small call in one launch: a workgroup takes all keys of a sequence's rows for one kv head,
+// the prefix's among them, and writes their results.  The last kv_heads workgroups write those of
+// tokens that belong to no sequence.
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * kWaves, (DP == 256 ? 1 : 2)) void attend_whole(Attention a) {
+  __shared__ __align__(16) char lds[Narrow<DP>::kBytes];
+  const int b = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - b * a.kv_heads;
+  auto nothing = [&](int from, int to) {    // rows that see no key
+    for (int row = from + threadIdx.x / 64; row < to; row += kWaves) {
+      const int t = a.by_group(row), h = kv_head * a.group + row - t * a.group;
+      T* out = static_cast<T*>(a.out) + t * a.o_token + h * a.o_head;
+      for (int d = threadIdx.x & 63; d < a.dim; d += 64) out[d] = T(0);
+      if (a.lse && threadIdx.x % 64 == 0) a.lse[static_cast<i64>(t) * a.heads + h] = -INFINITY;
+    }
+  };
+  if (b >= a.sequences) {
+    i64 end = a.ends ? a.ends[a.sequences] : a.tokens;
+    end = end < 0 ? 0 : end > a.tokens ? a.tokens : end;
+    nothing(static_cast<int>(end) * a.group, a.tokens * a.group);
+    return;
+  }
+  const Sequence s = sequence(a, b);
+  Part p;
+  p.list = a.prefix;
+  p.own_list = s.list;
+  p.own_from = a.prefix_length;
+  p.k0 = 0;
+  p.rows = s.count * a.group;
+  p.token0 = s.first;
+  p.before = a.prefix_length + s.before + 1;
+  p.step = 1;
+  for (p.row0 = 0; p.row0 < p.rows; p.row0 += 16) {
+    const int last = min(p.row0 + 16, p.rows) - 1;
+    p.k1 = a.prefix_length + (a.own_tiles ? seen(s, a.by_group(last)) : 0);
+    if (p.k1 == 0) {
+      nothing(s.first * a.group + p.row0, s.first * a.group + last + 1);
+      continue;
+    }
+    narrow_part<T, DP, true>(a, p, kv_head, lds);
+    __syncthreads();
+  }
+}
+
+template <typename T, int DP>
+hipError_t launch_whole(const Attention& a, hipStream_t stream) {
+  Attention copy = a;
+  void* args[] = {&copy};
+  return hipLaunchKernel(reinterpret_cast<const void*>(&attend_whole<T, DP>),
+                         dim3(static_cast<unsigned>((a.sequences + 1) * a.kv_heads)),
                          dim3(64 * kWaves), args, 0, stream);
 }
 

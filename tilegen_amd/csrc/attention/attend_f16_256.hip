@@ -1,3 +1,4 @@
 #include "attend.h"
 
 template hipError_t tg::launch_parts<_Float16, 256>(const Attention&, int, int, hipStream_t);
+template hipError_t tg::launch_whole<_Float16, 256>(const Attention&, hipStream_t);

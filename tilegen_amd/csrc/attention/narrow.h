@@ -28,7 +28,8 @@ struct Narrow {
   static constexpr int kBytes = (kValues > kSums ? kValues : kSums) + kTops;
 };
 
-template <typename T, int DP>
+// BOTH: the prefix's keys and a sequence's own, and the rows' results instead of a part's sums.
+template <typename T, int DP, bool BOTH>
 __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, int kv_head,
                                             char* lds) {
   using W = Narrow<DP>;
@@ -55,9 +56,11 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
       if (live && d < a.dim) q[s] = __builtin_bit_cast(s16x8, C::load(at + d));
     }
     see = live ? min(p.before + p.step * j, p.k1) : 0;
+    if (BOTH && live) see = max(see, p.own_from);
   }
   // every live row sees the keys below `all`
-  const int all = min(p.before + p.step * static_cast<int>(a.by_group(p.row0)), p.k1);
+  int all = min(p.before + p.step * static_cast<int>(a.by_group(p.row0)), p.k1);
+  if (BOTH) all = max(all, p.own_from);
 
   f32x4 o[DT];
   float m = -INFINITY, l = 0.f;
@@ -78,9 +81,11 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int key = min(p.k0 + 32 * tile + 16 * t + col, p.k1 - 1);
-      const int nth = a.by_page(key);
-      slot[t] = key - nth * a.page;
-      pg[t] = p.list[nth];
+      const bool own = BOTH && key >= p.own_from;
+      const int in = own ? key - p.own_from : key;
+      const int nth = a.by_page(in);
+      slot[t] = in - nth * a.page;
+      pg[t] = (own ? p.own_list : p.list)[nth];
     }
   };
   s16x8 k[2][KS], v[2][KS];
@@ -248,15 +253,23 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
     }
     const int j = a.by_group(row), h = kv_head * a.group + row - j * a.group;
     const i64 at = static_cast<i64>(p.token0 + j) * a.heads + h;
-    const i64 rows = static_cast<i64>(a.tokens) * a.heads;
-    *reinterpret_cast<f32x4*>(a.part + (p.slot * rows + at) * a.dim + d) = sum;
-    if (d == 0) {
+    if (BOTH || d == 0) {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float2 ml = tops[w * 16 + r];
         total += ml.x == -INFINITY ? 0.f : ml.y * exp2f(ml.x - top);
       }
-      a.part_ml[p.slot * rows + at] = make_float2(top, total);
+    }
+    if (BOTH) {
+      T* out = static_cast<T*>(a.out) + (p.token0 + j) * a.o_token + h * a.o_head + d;
+      const float f = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[e] = static_cast<T>(total == 0.f ? 0.f : sum[e] * f);
+      if (d == 0 && a.lse) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * kLn2;
+    } else {
+      const i64 rows = static_cast<i64>(a.tokens) * a.heads;
+      *reinterpret_cast<f32x4*>(a.part + (p.slot * rows + at) * a.dim + d) = sum;
+      if (d == 0) a.part_ml[p.slot * rows + at] = make_float2(top, total);
     }
   }
 }

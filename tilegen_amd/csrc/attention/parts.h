@@ -93,6 +93,10 @@ struct Part {
   int token0;
   int before, step;     // the row of token j sees min(k1, before + step j) keys
   int slot;
+  // of narrow parts that take the prefix and a sequence's own pages (`list`: the prefix's) in one:
+  // keys from own_from on stand on own_list, and every row sees those before
+  const int64_t* own_list;
+  int own_from;
 };
 
 // 16 bytes of every active lane to LDS at `to` + 16 * lane, without a register between.

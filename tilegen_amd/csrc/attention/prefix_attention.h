@@ -73,8 +73,10 @@ __device__ __forceinline__ int own_parts(const Attention& a, int keys) {
   return n < a.own_splits ? n : a.own_splits;
 }
 
-// Enqueues the parts for one type and padded head size.
+// Enqueue the parts, or the whole of a small call, for one type and padded head size.
 template <typename T, int DP>
 hipError_t launch_parts(const Attention& a, int prefix_rows, int own_rows, hipStream_t stream);
+template <typename T, int DP>
+hipError_t launch_whole(const Attention& a, hipStream_t stream);
 
 }  // namespace tg
