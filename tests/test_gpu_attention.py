@@ -688,3 +688,43 @@ def test_the_sparse_kernels_give_the_same(hip_ready):
     want = Variant("spmm", TUNED["c4"]).run(P, B=V)
     bound = b.want()[2][:, 0].numpy()
     assert (np.abs(out[:, 0].cpu().double().numpy() - want) <= bound).all()
+
+
+def test_paged_decode(hip_ready):
+    """The decode loop of tilegen_amd.paged_decode against attention over its unrotated inputs in
+    64 bits.  The calls round rotated queries and keys to bfloat16: scores are off by 2 u scale
+    sum |q k| (rotated) more than in the tests above."""
+    from tilegen_amd import paged_decode
+    heads, kv_heads, dim, prompt = 4, 2, 64, 90
+    r = paged_decode.run(sequences=3, prompt=prompt, steps=20, heads=heads, kv_heads=kv_heads,
+                         dim=dim, page=16, start=9, seed=3, keep=True)
+    f, magnitude, counts, u = r["frequency"], r["magnitude"], r["counts"], U[BF16]
+
+    def turn(x, position):
+        return _turned(x, torch.tensor(position), f, "half", magnitude)[0]
+
+    keys = [turn(r["prompt"][0], list(range(prompt)))] * 3
+    values = [r["prompt"][1].cpu().double()] * 3
+    lengths = [0, 0, 0]
+    for call, (q, k, v, out) in enumerate(r["calls"]):
+        n = counts if call == 0 else [1, 1, 1]
+        row = 0
+        for b in range(3):
+            mine = slice(row, row + n[b])
+            at_ = [prompt + lengths[b] + j for j in range(n[b])]
+            keys[b] = torch.cat([keys[b], turn(k[mine], at_)])
+            values[b] = torch.cat([values[b], v[mine].cpu().double()])
+            qs = turn(q[mine], at_)
+            lengths[b] += n[b]
+            for j in range(n[b]):
+                see = prompt + lengths[b] - n[b] + j + 1
+                for h in range(heads):
+                    kh, vh = keys[b][:see, h // 2], values[b][:see, h // 2]
+                    p = torch.softmax(kh @ qs[j, h] / 8, 0)
+                    es = float((kh.abs() @ qs[j, h].abs()).max()) / 8 * (2 * u + dim * 2.0 ** -23)
+                    size = p @ vh.abs()
+                    bound = 2 * u * size + (math.exp(2 * es) - 1) * size
+                    off = (out[row + j, h].cpu().double() - p @ vh).abs()
+                    assert (off <= bound).all(), (call, b, j, h)
+            row += n[b]
+    assert len(r["calls"]) == 21 and lengths == [n + 20 for n in counts]
