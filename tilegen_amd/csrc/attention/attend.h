@@ -84,13 +84,14 @@ hipError_t launch(const Attention& a, hipStream_t stream) {
                          dim3(64 * kWaves), args, 0, stream);
 }
 
-// A small call in one launch: a workgroup takes all keys of a sequence's rows for one kv head,
-// the prefix's among them, and writes their results.  The last kv_heads workgroups write those of
-// tokens that belong to no sequence.
+// A small call in one launch: a workgroup takes all keys of 16 of a sequence's rows (own_tiles
+// such tiles, and in turns those past them) for one kv head, the prefix's among them, and writes
+// their results.  The last kv_heads workgroups write those of tokens that belong to no sequence.
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * kWaves, (DP == 256 ? 1 : 2)) void attend_whole(Attention a) {
   __shared__ __align__(16) char lds[Narrow<DP>::kBytes];
-  const int b = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - b * a.kv_heads;
+  const int unit = blockIdx.x / a.kv_heads, kv_head = blockIdx.x - unit * a.kv_heads;
+  const int b = unit / a.own_tiles, tile = unit - b * a.own_tiles;
   auto nothing = [&](int from, int to) {    // rows that see no key
     for (int row = from + threadIdx.x / 64; row < to; row += kWaves) {
       const int t = a.by_group(row), h = kv_head * a.group + row - t * a.group;
@@ -115,9 +116,9 @@ __global__ __launch_bounds__(64 * kWaves, (DP == 256 ? 1 : 2)) void attend_whole
   p.token0 = s.first;
   p.before = a.prefix_length + s.before + 1;
   p.step = 1;
-  for (p.row0 = 0; p.row0 < p.rows; p.row0 += 16) {
+  for (p.row0 = tile * 16; p.row0 < p.rows; p.row0 += a.own_tiles * 16) {
     const int last = min(p.row0 + 16, p.rows) - 1;
-    p.k1 = a.prefix_length + (a.own_tiles ? seen(s, a.by_group(last)) : 0);
+    p.k1 = a.prefix_length + (a.pages ? seen(s, a.by_group(last)) : 0);
     if (p.k1 == 0) {
       nothing(s.first * a.group + p.row0, s.first * a.group + last + 1);
       continue;
@@ -132,7 +133,7 @@ hipError_t launch_whole(const Attention& a, hipStream_t stream) {
   Attention copy = a;
   void* args[] = {&copy};
   return hipLaunchKernel(reinterpret_cast<const void*>(&attend_whole<T, DP>),
-                         dim3(static_cast<unsigned>((a.sequences + 1) * a.kv_heads)),
+                         dim3(static_cast<unsigned>((a.sequences * a.own_tiles + 1) * a.kv_heads)),
                          dim3(64 * kWaves), args, 0, stream);
 }
 

@@ -16,7 +16,8 @@ __global__ __launch_bounds__(256) void join_parts(Attention a) {
   const i64 rows = static_cast<i64>(a.tokens) * a.heads;
   const i64 row = static_cast<i64>(blockIdx.x) * (4 / WAVES) + (WAVES == 1 ? wave : 0);
   if (row >= rows) return;
-  const int t = static_cast<int>(row / a.heads), h = static_cast<int>(row - static_cast<i64>(t) * a.heads);
+  const int t = static_cast<int>(row / a.heads);
+  const int h = static_cast<int>(row - static_cast<i64>(t) * a.heads);
   const int b = a.ends ? sequence_of(a.ends, a.sequences, t) : t;
   int parts = b < a.sequences ? a.prefix_splits : 0;
   if (b < a.sequences && a.own_splits) {
@@ -129,12 +130,12 @@ int check(const tg_prefix_attention* r) {
     return refuse(-1, what, "page must be 1 to 2^31 - 1", r->page);
   if (!(r->scale > 0) || !(r->scale < 1e30))
     return refuse(-1, what, "scale must be positive and finite", 0);
-  if (r->n_prefix < (r->prefix_length + r->page - 1) / r->page)
-    return refuse(-1, what, "prefix_length is past the prefix's pages", r->prefix_length);
   if (r->prefix_length > INT32_MAX / 2 || r->max_length > INT32_MAX / 2)
     return refuse(-2, what, "more than 2^30 keys", r->prefix_length);
-  if (r->tokens > 0x1000000 || r->sequences > 0x1000000 ||
-      r->tokens * r->heads > 0x4000000 || r->heads > 0x10000)
+  if (r->n_prefix < (r->prefix_length + r->page - 1) / r->page)
+    return refuse(-1, what, "prefix_length is past the prefix's pages", r->prefix_length);
+  if (r->tokens > 0x1000000 || r->sequences > 0x1000000 || r->heads > 0x10000 ||
+      r->tokens * r->heads > 0x4000000)
     return refuse(-2, what, "more than 2^26 rows or 2^24 sequences", r->tokens);
   if (!r->query_indptr && r->tokens > r->sequences)
     return refuse(-1, what, "more tokens than sequences without query_indptr", r->tokens);
@@ -189,20 +190,56 @@ int plan(const tg_prefix_attention* r, Plan* p) {
   if (a.tokens == 0) return 0;
   const int64_t cus = compute_units();
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.group;
-  const int64_t max_query = r->query_indptr ? (r->max_query > 0 ? r->max_query : 1) : 1;
-  p->prefix_rows = rows <= 16 ? 16 : 128;
-  p->own_rows = max_query * a.group <= 16 ? 16 : p->prefix_rows;
+  const int64_t bound = r->max_query < a.tokens ? r->max_query : a.tokens;
+  const int64_t max_query = r->query_indptr && bound > 0 ? bound : 1;
+  const int64_t each = max_query * a.group;    // rows of a sequence's own pages, for one kv head
+  const int64_t length = r->max_length > 0 ? r->max_length : 1;
   // workgroups that the chip holds at once
   const int64_t room = a.dim > 128 ? cus : 2 * cus;
-  int64_t own = 0, own_keys = 0;    // workgroups, and keys that they read between them (half of the bound)
+  const int64_t heads = static_cast<int64_t>(a.sequences) * a.kv_heads;
+  const int64_t tiles16 = (each + 15) / 16;
+  // Few keys and no more workgroups than run at once: one launch that reads the prefix for each
+  // 16 rows.  A call in parts takes 14.5 us up to some thousand keys (two launches); a whole
+  // one 10.6 us with few, 10.8 with 360 keys of 64 elements and 15.1 with 660, 12.4 with 360 of
+  // 128 and 18.8 with 660.
+  if (heads && (a.prefix_length + r->max_length) * a.dim <= kWholeElements &&
+      heads * tiles16 <= room) {
+    a.own_tiles = static_cast<int>(tiles16);
+    p->whole = true;
+    return 0;
+  }
+  // A sequence's own pages: narrow workgroups read them again for every 16 rows, wide ones
+  // once for 128 but with long turns.  4 sequences of 8 to 16 rows run as fast either way; 24 rows
+  // of 3 sequences, 1500 keys: 14.5 us narrow, 20.5 wide; 28 of 24 (8 kv heads): 50 and 72; 64 of
+  // 64 (4 kv heads), 6000 keys: 290 and 183; 112 of 24, 900 keys: 25.9 and 27.9, 6000 keys: 54
+  // and 37.
+  p->own_rows = each <= 48 || (length <= 1024 && heads * tiles16 <= room) ? 16 : 128;
+  // And the prefix: narrow while that is half of a round of parts of 128 keys.  8 sequences of 32
+  // heads (8 kv heads), 2000 keys: 15.1 us narrow, 20.5 wide; 16 of 32 (4 kv heads), 2000 keys,
+  // twice that: 21.1 and 17.1.
+  const int64_t most_prefix = (a.prefix_length + 127) / 128;
+  p->prefix_rows =
+      rows <= 16 || (p->own_rows == 16 && (rows + 15) / 16 * a.kv_heads * most_prefix <= room / 2)
+          ? 16
+          : 128;
+  if (p->prefix_rows == 16) p->own_rows = 16;
+  // workgroups, and keys that they read between them: about half of the bound
+  int64_t own = 0, own_keys = 0;
   if (a.pages && a.n_indices && a.sequences) {
-    int64_t tiles = (max_query * a.group + p->own_rows - 1) / p->own_rows;
+    int64_t tiles = (each + p->own_rows - 1) / p->own_rows;
     tiles = tiles < 4096 ? tiles : 4096;
     a.own_tiles = static_cast<int>(tiles);
-    const int64_t length = r->max_length > 0 ? r->max_length : 1;
-    const int64_t units = tiles * a.kv_heads * a.sequences;
+    const int64_t units = tiles * heads;
     const int64_t most = (length + 127) / 128;
-    int64_t splits = room / 2 / units;
+    // Lengths differ, so a round of parts of the bound is half empty: wide ones take a whole round
+    // (24 sequences of 28 rows, 4000 keys: 110 us, 169 with half), narrow ones, whose loads
+    // share the memory, half of one.  Where all run at once the longest would end alone, so long
+    // ones are cut in any case: 48 sequences, 8 kv heads, 4000 keys: 111 us, 161 without.  More
+    // than run at once go in order of length instead, and cutting them costs: 128 sequences, 8 kv
+    // heads, 2048 keys: 138 us, 149 in three.
+    int64_t splits = (p->own_rows == 16 ? room / 2 : room) / units;
+    if (p->own_rows == 16 && units <= room && length > 1024 && splits < (length + 767) / 768)
+      splits = (length + 767) / 768;
     splits = splits < 1 ? 1 : splits < most ? splits : most;
     a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
@@ -211,21 +248,10 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     if (own > 0xFFFFFF) return refuse(-2, what, "more than 2^24 workgroups", own);
     own_keys = units * length / 2;
   }
-  // Few rows a sequence, few keys, and no more workgroups than run at once: one launch that reads the
-  // prefix for each sequence.  A call in parts takes 14.5 us up to some thousand keys (two
-  // launches); a whole one 10.6 us with few, 10.8 with 360 keys of 64 elements and 15.1 with 660,
-  // 12.4 with 360 of 128 and 18.8 with 660.
-  if (p->own_rows == 16 && a.sequences &&
-      (a.prefix_length + r->max_length) * a.dim <= kWholeElements &&
-      static_cast<int64_t>(a.sequences) * a.kv_heads <= room) {
-    p->whole = true;
-    return 0;
-  }
   a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
   int64_t prefix = 0;
   if (a.prefix_length) {
     const int64_t units = static_cast<int64_t>(a.prefix_tiles) * a.kv_heads;
-    const int64_t most = (a.prefix_length + 127) / 128;
     // The prefix's parts are alike and start first, so they get the room that their share of the
     // keys to read asks for, and the own pages' take turns in the rest: their loads run beside the
     // prefix's products.  64 sequences of up to 4096 keys, 16384 shared: 184 us with a quarter of
@@ -236,7 +262,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     const int64_t left =
         own_keys * 8 > own_keys + keys ? room - room * own_keys / (own_keys + keys) : room;
     int64_t splits = left == room ? room / units : (left + units / 2) / units;
-    splits = splits < 1 ? 1 : splits < most ? splits : most;
+    splits = splits < 1 ? 1 : splits < most_prefix ? splits : most_prefix;
     a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
     a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
     prefix = units * a.prefix_splits;
