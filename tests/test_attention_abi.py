@@ -133,3 +133,28 @@ def test_rope_frequencies():
                 dict(rotary=4, scaling="yarn")):
         with pytest.raises(ValueError):
             at.rope_frequencies(device="cpu", **bad)
+
+
+def test_sizes_at_the_ends_of_64_bits():
+    """Refused, or used as the bounds they are, without overflow on the way."""
+    L = at._lib()
+    names = ("query kc vc prefix indptr indices lengths ends out lse workspace bytes dtype tokens "
+             "sequences heads kv_heads dim pages page n_prefix prefix_length n_indices max_query "
+             "max_length").split()
+    base = dict.fromkeys(names, 0)
+    base.update(tokens=2, sequences=2, heads=4, kv_heads=2, dim=64, pages=999, page=16,
+                n_prefix=200, prefix_length=3200, n_indices=4, max_query=1, max_length=20)
+    base.update({"s%d" % i: 64 for i in range(10)}, scale=0.125)
+    most = (1 << 63) - 1
+
+    def workspace(**change):
+        return L.prefix_attention_workspace(at._ATTENTION.pack(*{**base, **change}.values()))
+
+    for change in (dict(prefix_length=most), dict(max_length=most), dict(pages=1 << 31),
+                   dict(heads=1 << 62, kv_heads=1 << 61), dict(heads=1 << 17),
+                   dict(sequences=most)):
+        assert workspace(**change) < 0, change
+    # a bound on new tokens above all tokens is all tokens
+    for tokens in (2, 40):
+        sizes = dict(tokens=tokens, ends=4096)
+        assert workspace(**sizes, max_query=most) == workspace(**sizes, max_query=tokens) > 0

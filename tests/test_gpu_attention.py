@@ -728,3 +728,156 @@ def test_paged_decode(hip_ready):
                     assert (off <= bound).all(), (call, b, j, h)
             row += n[b]
     assert len(r["calls"]) == 21 and lengths == [n + 20 for n in counts]
+
+
+# --------------------------------------------------------------------------- #
+# workgroups of 128 rows: bounds above what the batch has make small batches take them
+# --------------------------------------------------------------------------- #
+WIDE = dict(max_query=10 ** 6, max_length=1100)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,prefix,lengths,counts", [
+    # heads, kv_heads, dim, page, prefix, lengths, counts: 49 rows of a kv head or more
+    (16, 1, 40, 7, 33, [40, 7, 90, 0], [7, 1, 3, 0]),
+    (16, 4, 64, 16, 129, [300, 20, 64], [40, 9, 3]),
+    (7, 1, 64, 1, 70, [66, 130, 5], [3, 64, 5]),
+    (12, 4, 80, 24, 0, [200, 33, 1], [130, 20, 1]),
+    (50, 1, 96, 16, 500, [65, 0, 40], [1, 1, 1]),
+    (24, 2, 96, 3, 64, [140, 2], [9, 2]),
+    (16, 4, 128, 64, 600, [190, 77], [150, 70]),
+    (60, 1, 128, 16, 63, [63, 64, 129], [1, 1, 1]),
+    (25, 1, 128, 20, 1, [300, 2], [1, 2]),
+    (32, 1, 200, 8, 90, [33, 70], [1, 2]),
+    (20, 1, 256, 5, 65, [120, 31], [5, 4]),
+    (14, 2, 256, 64, 200, [90, 200, 1], [17, 40, 1]),
+    # fewer tokens than new ones, and no key at all
+    (32, 1, 64, 16, 20, [2, 0], [5, 3]),
+    (32, 1, 128, 16, 0, [2, 0], [5, 3]),
+])
+def test_wide(hip_ready, dtype, heads, kv_heads, dim, page, prefix, lengths, counts):
+    b = Batch(dtype, heads, kv_heads, dim, page, prefix, lengths, counts, seed=dim + 1).fill()
+    got = b.attend(**WIDE)
+    b.check(got)
+    b.check(b.attend(max_query=10 ** 6, max_length=30000))
+    again = b.attend(**WIDE)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("heads,kv_heads,dim,page,prefix,lengths,counts", [
+    (8, 2, 64, 16, 2000, [(13 * i) % 70 for i in range(40)], [1] * 40),
+    (6, 2, 96, 24, 1900, [(13 * i) % 70 for i in range(48)], [1] * 48),
+    (8, 8, 40, 7, 700, [30] * 20, [1 + i % 3 for i in range(20)]),
+    (8, 4, 256, 16, 1100, [(7 * i) % 40 for i in range(20)], [1] * 20),
+])
+def test_wide_prefix_and_narrow_own_pages(hip_ready, dtype, heads, kv_heads, dim, page, prefix,
+                                          lengths, counts):
+    b = Batch(dtype, heads, kv_heads, dim, page, prefix, lengths, counts, seed=dim + 2).fill()
+    b.check(b.attend())
+
+
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(100, 2, 64, 16), (40, 1, 128, 8),
+                                                     (52, 1, 96, 7), (50, 1, 256, 24)])
+def test_wide_with_lost_pages(hip_ready, heads, kv_heads, dim, page):
+    b = Batch(BF16, heads, kv_heads, dim, page, 700, [200, 9], [1, 1], seed=dim + 3,
+              spare=False).fill()
+    n = -(-700 // page)
+    lost, own = [0, 3, n // 2, n // 2 + 1, n - 2], 1
+    whole, mine = b.prefix.clone(), b.indices.clone()
+    b.prefix[lost] = torch.tensor([-1, b.pages, 2 ** 40, -2 ** 40, b.pages + 1], device="cuda")
+    b.indices[own] = -2 ** 33
+    if not bool((whole == 0).any() or (mine == 0).any()):
+        b.kc[0], b.vc[0] = math.nan, math.inf
+    got = b.attend(**WIDE)
+    keep = torch.ones(n, dtype=torch.bool)
+    keep[lost] = False
+    short = Batch(BF16, heads, kv_heads, dim, page, 700, [200 - page, 9], [1, 1], seed=0,
+                  spare=False)
+    short.kc, short.vc, short.query = b.kc, b.vc, b.query
+    short.indices = torch.cat([mine[:own], mine[own + 1:]])
+    short.prefix = whole[keep.cuda()].contiguous()
+    short.prefix_length = 700 - page * len(lost)
+    short.check(got)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim", [64, 96, 128, 256])
+def test_wide_with_hidden_keys_that_hold_anything(hip_ready, dtype, dim):
+    shape = (dtype, 4, 2, dim, 16, 40, [35, 9, 90], [6, 3, 60])
+    b = Batch(*shape, seed=3).fill()
+    page, slot = b.places(0)
+    b.kc[page[-1], slot[-1]] = math.inf         # seen by the sequence's last token alone
+    b.vc[page[-1], slot[-1]] = math.nan
+    page, slot = b.places(2)
+    b.vc[page[-8], slot[-8], 0, 3] = -math.inf  # by its last eight, one element, one kv head
+    got, lse = b.attend(**WIDE)
+    out, lse_want, eo, el = Batch(*shape, seed=3).fill().want()
+    tainted = torch.zeros(out.shape, dtype=torch.bool)
+    tainted[5] = True
+    tainted[61:, :2, 3] = True
+    got = got.cpu().double()
+    assert ((got - out).abs() <= eo)[~tainted].all()
+    assert torch.isnan(got[5]).all()
+    assert (got[61:, :2, 3] == -math.inf).all()
+    rows = torch.arange(69) != 5
+    assert ((lse.cpu().double() - lse_want).abs() <= el)[rows].all()
+
+
+def test_wide_at_the_ends_of_the_range(hip_ready):
+    b = Batch(BF16, 50, 1, 64, 16, 96, [40], [1], seed=4).fill()
+    b.query.fill_(1.0)
+    b.kc[b.places()] = -math.inf
+    b.kc[b.places(0)] = -math.inf
+    out, lse = b.attend(**WIDE)
+    assert not out.any() and (lse == -math.inf).all()
+    page, slot = b.places(0)
+    b.kc[page[7], slot[7]] = 0.0
+    b.kc[page[7], slot[7], :, 0] = torch.finfo(BF16).min    # one finite score, far below all
+    out, lse = b.attend(**WIDE)
+    assert torch.equal(out[0], b.vc[page[7], slot[7], 0].expand(50, 64))
+    for dtype, first, last in ((F16, -60.0, 90.0), (BF16, 90.0, -60.0)):
+        for dim in (64, 128):
+            c = Batch(dtype, 50, 1, dim, 16, 700, [300], [1], seed=5).fill()
+            c.query.fill_(1.0)
+            for place, lo, hi in ((c.places(), first, first + (last - first) / 2),
+                                  (c.places(0), first + (last - first) / 2, last)):
+                n = place[0].numel()
+                c.kc[place] = torch.linspace(lo, hi, n, device="cuda").to(dtype)[:, None, None]
+            c.check(c.attend(**WIDE))
+
+
+@pytest.mark.parametrize("page,dim", [(16, 72), (10, 72), (16, 128), (6, 256)])
+def test_wide_with_other_strides(hip_ready, page, dim):
+    """Caches that are halves of one array with heads before slots, at odd offsets."""
+    b = Batch(F16, 60, 2, dim, page, 150, [140, 9], [2, 1], seed=9).fill()
+    want = b.attend(**WIDE)
+    b.check(want)
+    both = torch.zeros(b.pages, 2, b.kv_heads, page, dim + 2, device="cuda", dtype=F16)
+    k = both[:, 0, :, :, 1:dim + 1].transpose(1, 2)
+    v = both[:, 1, :, :, 2:].transpose(1, 2)
+    k.copy_(b.kc), v.copy_(b.vc)
+    packed = torch.zeros(3, 63, dim + 1, device="cuda", dtype=F16)
+    packed[:, 1:61, 1:] = b.query
+    b.query = packed[:, 1:61, 1:]
+    kc, vc = b.kc, b.vc
+    for b.kc, b.vc in ((k, v), (kc, v), (k, vc)):      # alike strides, and not
+        got = b.attend(**WIDE)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_wide_past_32_bits(hip_ready):
+    """test_offsets_past_32_bits for workgroups of 128 rows, pages of 64 and of 60 keys."""
+    pages, dim = 70000, 256
+    pool = torch.empty(2, pages * 64 * 2 * dim, device="cuda", dtype=BF16)
+    for page in (64, 60):
+        kc, vc = (x[:pages * page * 2 * dim].view(pages, page, 2, dim) for x in pool)
+        b = Batch(BF16, 64, 2, dim, page, 100, [90, 3], [3, 2], seed=10)
+        b.prefix += pages - b.pages
+        b.indices += pages - b.pages
+        b.kc, b.vc, b.pages = kc, vc, pages
+        b.fill()
+        frequency, _ = at.rope_frequencies(dim)
+        at.paged_append(b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency,
+                        query_indptr=b.ends, offset=100)
+        b.check(b.attend(**WIDE))

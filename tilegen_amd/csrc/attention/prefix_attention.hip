@@ -7,7 +7,9 @@ namespace {
 // Joins the parts of each row: M = max m_s, then sum 2^(m_s - M) O_s over sum 2^(m_s - M) l_s.
 // A lane holds four elements of the head; where a head takes 16 or 32 lanes the others read
 // other parts at the same time (LANES: lanes of one part), and WAVES waves share a row where it
-// has many.  Memory bounds it, so the weights come first and the parts' loads wait for nothing.
+// has many.  Memory bounds it, so the weights come first and the parts' loads wait for nothing:
+// 16384 rows of 128 in 7 parts (38 MB by then in the caches) take 11.4 us, 1024 rows in some 17
+// take 6.0, most of it latency.
 template <typename T, int LANES, int WAVES>
 __global__ __launch_bounds__(256) void join_parts(Attention a) {
   constexpr int kAtOnce = WAVES * 64 / LANES;     // parts
@@ -132,6 +134,7 @@ int check(const tg_prefix_attention* r) {
     return refuse(-1, what, "scale must be positive and finite", 0);
   if (r->prefix_length > INT32_MAX / 2 || r->max_length > INT32_MAX / 2)
     return refuse(-2, what, "more than 2^30 keys", r->prefix_length);
+  if (r->pages > INT32_MAX) return refuse(-2, what, "more than 2^31 pages", r->pages);
   if (r->n_prefix < (r->prefix_length + r->page - 1) / r->page)
     return refuse(-1, what, "prefix_length is past the prefix's pages", r->prefix_length);
   if (r->tokens > 0x1000000 || r->sequences > 0x1000000 || r->heads > 0x10000 ||
