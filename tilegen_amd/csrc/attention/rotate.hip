@@ -3,7 +3,7 @@
 //
 // Memory bounds it: every value is read and written once, in 16-byte units, and the cosines and
 // sines are computed once a token for all its heads.  16384 tokens of 40 heads of 128 in
-// bfloat16 (336 MB) take 64.8 us, 5.2 TB/s; an append of 16384 tokens with their queries (403 MB)
+// bfloat16 (336 MB) take 59 us, 5.7 TB/s; an append of 16384 tokens with their queries (403 MB)
 // 79, 5.1 TB/s; a plain copy of 1 GiB reaches 4.8.  8 tokens take 3.0 us, an append of 32 with its
 // page lookups 4.2: the latency of the loads that follow from one another.
 #include "attention.h"
@@ -260,7 +260,12 @@ int enqueue(Rows a, int64_t dtype, int64_t layout, bool append, const char* what
   a.by_token = Div(a.per_token);
   a.by_page = Div(append ? a.page : 1);
   const bool whole = a.dim % n == 0 && (!halves || a.half % n == 0);
-  const int tokens = a.tokens >= 4096 ? kMostTokens : 1;
+  // Workgroups of one token fill the chip best while there are few tokens, and where a token's
+  // heads are work for all threads; else four share a workgroup's start.  16384 tokens of 40
+  // heads of 128: 59 us by one, 63 by four; of 4 heads: 13.2 and 7.7.  An append looks up its
+  // place first: 4096 tokens of 32 and 8 heads 19.1 and 17.9, 16384 77.7 and 79.1.
+  const int tokens =
+      a.tokens < 4096 || (!append && a.per_token >= kThreads) ? 1 : kMostTokens;
   const void* k = dtype == TG_F32   ? kernel_of<float>(layout, whole, append)
                   : dtype == TG_F16 ? kernel_of<_Float16>(layout, whole, append)
                                     : kernel_of<__bf16>(layout, whole, append);
