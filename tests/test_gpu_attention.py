@@ -881,3 +881,31 @@ def test_wide_past_32_bits(hip_ready):
         at.paged_append(b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency,
                         query_indptr=b.ends, offset=100)
         b.check(b.attend(**WIDE))
+
+
+def test_gradients_that_do_not_exist_are_refused(hip_ready):
+    frequency, _ = at.rope_frequencies(64)
+    b = Batch(BF16, 4, 2, 64, 16, 32, [20, 9], [1, 1], seed=12).fill()
+    query = b.query.clone().requires_grad_()
+    for call in (lambda: at.paged_append(b.key, b.value, b.kc, b.vc, b.indptr, b.indices, b.lengths,
+                                         frequency, query=query),
+                 lambda: at.prefix_attention(query, b.kc, b.vc, b.prefix, 32, b.indptr, b.indices,
+                                             b.lengths, max_length=20)):
+        with pytest.raises(ValueError, match="backward"):
+            call()
+        with torch.no_grad():
+            call()
+
+
+@pytest.mark.parametrize("prefix", [32, 900])      # in one launch, and in parts
+def test_attention_over_its_own_query(hip_ready, prefix):
+    """out may be the query, and may share no other memory with the operands."""
+    b = Batch(BF16, 4, 2, 64, 16, prefix, [40, 9], [30, 1], seed=13).fill()
+    want = b.attend()[0]
+    packed = torch.zeros(31, 6, 64, device="cuda", dtype=BF16)
+    packed[:, :4] = b.query
+    b.query = packed[:, :4]
+    for out in (packed[:, 1:5], b.kc.view(-1, 4, 64)[:31]):
+        with pytest.raises(ValueError, match="overlaps"):
+            b.attend(out=out)
+    assert torch.equal(b.attend(out=b.query)[0], want) and not packed[:, 4:].any()

@@ -11,6 +11,11 @@ Modules keep the reference's names and entry points:
     env               toolchain / GPU probe
     runtime           ctypes binding of libtgrt (include/tgrt.h)
 
+Attention over a paged cache with a CSR page table, on torch tensors (no counterpart in the
+reference):
+    attention         rotary positions, paged append, attention behind a shared prefix
+    paged_decode      a decode loop that runs the three together
+
 Around them (the reference's scripts/ and harness, rebuilt for this backend):
     variant           one compiled variant: launch, geometry, timing handles
     schedules         tuned schedule per BASELINE case, test schedules
@@ -20,7 +25,8 @@ Around them (the reference's scripts/ and harness, rebuilt for this backend):
     vendor            rocSPARSE SpMV timing beside the tuned kernel
     profiling         rocprofv3 summaries for profiles/
     cpu_tuned         CPU-tuned OpenMP schedules for the CPU baseline
-    build             in-tree native build (libtgrt, harness, oracle, kernel cache)
+    build             in-tree native build (libtgrt, harness, attention, oracle, kernel
+                      cache)
 """
 
 __version__ = "0.1.0"

@@ -10,7 +10,8 @@ batch shares are a list of their own and are read once for the batch.
 Operands are torch tensors on one HIP device, bfloat16 or float16 (``rope`` and
 ``paged_append`` float32 too); any strides whose heads are contiguous.  Kernels are enqueued on
 torch's current stream of that device and nothing waits for them.  Calls that the kernels
-cannot serve raise ``ValueError`` before anything is enqueued; HIP's own failures raise
+cannot serve raise ``ValueError`` before anything is enqueued, ones that autograd would have to
+follow among them (``rope`` alone has a backward pass); HIP's own failures raise
 ``TileGenHipError``.  The C ABI below is ``include/tilegen_attention.h`` (``libtgattn.so``); it
 allocates nothing, and may be captured into a graph like the calls here.
 
@@ -267,6 +268,15 @@ def rope_backward(grad: torch.Tensor, positions: torch.Tensor, frequency: torch.
 # --------------------------------------------------------------------------- #
 # the cache
 # --------------------------------------------------------------------------- #
+def _no_gradient(what: str, *operands: Optional[torch.Tensor]) -> None:
+    """Refuses what autograd would follow: its results would have no gradient, silently."""
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                raise ValueError("%s has no backward pass: call it under torch.no_grad(), or "
+                                 "with detached operands" % what)
+
+
 def _caches(key_cache, value_cache, device, dtype, write):
     kshape, ks = _heads("key_cache", key_cache, device, dtype, 4, write)
     vshape, vs = _heads("value_cache", value_cache, device, dtype, 4, write)
@@ -305,6 +315,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     query_indptr[-1] belong to no sequence (a batch padded for a graph): nothing is written for
     them and their queries come back zero."""
     device, dtype = _operand("key", key, _DTYPES)
+    _no_gradient("paged_append", key, value, query, key_cache, value_cache)
     shape, ks = _heads("key", key, device, dtype, 3)
     vshape, vs = _heads("value", value, device, dtype, 3)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, True)
@@ -372,6 +383,7 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     caches' type for the matrix instructions that weigh the values.  Results do not depend on
     the order in which workgroups run."""
     device, dtype = _operand("query", query, _CACHED)
+    _no_gradient("prefix_attention", query, key_cache, value_cache)
     shape, qs = _heads("query", query, device, dtype, 3)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, False)
     tokens, heads, dim = shape
@@ -381,6 +393,9 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
         indptr, indices, lengths, query_indptr, tokens, device)
     if out is None:
         out = _like(query)
+    else:
+        for name, t in (("query", query), ("key_cache", key_cache), ("value_cache", value_cache)):
+            _apart("out", out, name, t)
     oshape, os_ = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))
