@@ -12,9 +12,9 @@
 // many vector cycles as its products take matrix cycles.  So the next tile's scores are computed
 // while this one's probabilities are, instruction by instruction (side_by_side), and two
 // workgroups share a CU.  1024 rows of each of 8 kv heads of 128 on 32768 keys (137 GFLOP):
-// 187 us, 735 TFLOP/s; with matrix cores alone a product of 8192^3 reaches 1330.  64 rows a wave
-// (half the LDS reads, one wave a SIMD) took 1.8 times as long; eight waves a workgroup 158 us
-// for the prefix alone, but longer beside narrow parts in one launch.
+// 187 us, 735 TFLOP/s; a plain product of 8192^3 reaches 1330.  64 rows a wave (half the LDS
+// reads, one wave a SIMD) took 1.8 times as long; eight waves and 256 rows a workgroup as long
+// for the prefix and 8% longer beside own pages.
 #pragma once
 
 #include <type_traits>
