@@ -237,14 +237,16 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     // Lengths differ, so a round of parts of the bound is half empty: wide ones take a whole round
     // (24 sequences of 28 rows, 4000 keys: 110 us, 169 with half), narrow ones, whose loads
     // share the memory, half of one.  Where all run at once the longest would end alone, so long
-    // ones are cut in any case: 48 sequences, 8 kv heads, 4000 keys: 111 us, 161 without.  More
-    // than run at once go in order of length instead, and cutting them costs: 128 sequences, 8 kv
-    // heads, 2048 keys: 138 us, 149 in three.
+    // ones are cut in any case, into three parts or more: 48 sequences, 8 kv heads, 4000 keys: 111
+    // us, 161 without; 1800 keys: 60 and 80; but 1500 keys in two 62 to 85, 69 to 78 without.
+    // More than run at once go in order of length instead, and cutting them costs: 128
+    // sequences, 8 kv heads, 2048 keys: 138 us, 149 in three.
     int64_t splits = (p->own_rows == 16 ? room / 2 : room) / units;
-    if (p->own_rows == 16 && units <= room && length > 1024 && splits < (length + 767) / 768)
+    if (p->own_rows == 16 && units <= room && length > 1536 && splits < (length + 767) / 768)
       splits = (length + 767) / 768;
     splits = splits < 1 ? 1 : splits < most ? splits : most;
-    a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, 128));
+    const int64_t tile = p->own_rows == 16 ? 128 : 64;    // keys of a workgroup's turn
+    a.own_chunk = static_cast<int>(up((length + splits - 1) / splits, tile));
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
     a.sorted = units > room && a.sequences <= 256;
     own = units * a.own_splits;
@@ -267,6 +269,11 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     int64_t splits = left == room ? room / units : (left + units / 2) / units;
     splits = splits < 1 ? 1 : splits < most_prefix ? splits : most_prefix;
     a.prefix_chunk = static_cast<int>(up((a.prefix_length + splits - 1) / splits, 128));
+    // Parts of 128 keys, two tiles, while they are at most half a round, else at least four: 8
+    // sequences of 32 heads (8 kv heads) on 8192 keys 19.0 us, 25.4 in a whole round of the
+    // smallest parts; on 3000 keys 17.9 and 16.0.
+    if (p->prefix_rows > 16 && a.prefix_chunk < 256 && units * most_prefix > room / 2)
+      a.prefix_chunk = 256;
     a.prefix_splits = (a.prefix_length + a.prefix_chunk - 1) / a.prefix_chunk;
     prefix = units * a.prefix_splits;
   }
