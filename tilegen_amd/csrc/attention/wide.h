@@ -124,11 +124,11 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   const int tiles = (p.k1 - p.k0 + W::kKeys - 1) / W::kKeys;
 
   // Where keys are: bytes from the head's first key, or negative where a key has no page.  Where
-  // pages hold whole groups of 8 keys (`even`) a lane knows where one group starts, 64 lanes 8 tiles
-  // of them; a wave's rows of one load stand in one group, so that the address is uniform.
-  // Elsewhere a lane knows one key of one tile.  Pages are asked for a tile before they are needed
-  // and before that tile's loads, since loads return in order.  Keys past the end stand for the
-  // last one (hidden).
+  // pages hold whole groups of 8 keys (`even`) a lane knows where one group starts, 64 lanes 8
+  // tiles of them; a wave's rows of one load stand in one group, so that the address is uniform.
+  // Elsewhere a lane knows one key of one tile.  Pages are asked for a tile before they are
+  // needed and before that tile's loads, since loads return in order.  Keys past the end stand
+  // for the last one (hidden).
   auto key_of_lane = [&](int tile) {
     return min(a.even ? p.k0 + (tile >> 3) * 8 * W::kKeys + 8 * lane
                       : p.k0 + tile * W::kKeys + lane,
