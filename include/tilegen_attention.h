@@ -54,8 +54,9 @@ int launch_rope(const tg_rope* a, void* stream);
  * pages indices[indptr[b]:indptr[b+1]]: position p to slot p % page of the page numbered
  * p / page.  Keys are turned at offset + p first, and so are the same rows of `query` into
  * query_out (heads = 0: none).  rotary = 0: nothing is turned.  A token whose position falls
- * outside its sequence's pages, or whose page is outside the cache, is not written; one past
- * query_indptr[sequences] is not written and its query comes back zero. */
+ * outside its sequence's pages, or whose page is outside the cache, is not written; one before
+ * query_indptr[0] or past query_indptr[sequences] belongs to no sequence (slices of a larger
+ * batch's row pointers, or a padded batch): it is not written and its query comes back zero. */
 typedef struct {
   const void *key, *value, *query;
   void *key_cache, *value_cache, *query_out;
@@ -76,7 +77,8 @@ int launch_paged_append(const tg_paged_append* a, void* stream);
  * position: with n new tokens (as above), token j sees positions 0 .. lengths[b] - n + j.  Query
  * head h reads kv head h / (heads / kv_heads).  lse (may be NULL): the logarithm of each row's
  * sum of exponentials, [tokens, heads].  A row that sees no key, or whose scores are all -inf,
- * gives 0 and -inf.  A key whose page is outside the cache counts as hidden.
+ * gives 0 and -inf, and so does one of no sequence (as above).  A key whose page is outside the
+ * cache counts as hidden.
  *
  * max_query and max_length are the host's bounds on n and lengths[b]; they size the launch,
  * and larger values on the device are still right.  workspace holds

@@ -909,3 +909,45 @@ def test_attention_over_its_own_query(hip_ready, prefix):
         with pytest.raises(ValueError, match="overlaps"):
             b.attend(out=out)
     assert torch.equal(b.attend(out=b.query)[0], want) and not packed[:, 4:].any()
+
+
+# --------------------------------------------------------------------------- #
+# row pointers, numbers and memory that calls must not mix up
+# --------------------------------------------------------------------------- #
+def _bits(t):
+    return t.view(torch.int16)
+
+
+@pytest.mark.parametrize("first,last", [(1, 3), (1, 2), (2, 3)])
+@pytest.mark.parametrize("prefix", [32, 900])      # in one launch, and in parts
+def test_a_block_of_row_pointers(hip_ready, prefix, first, last):
+    """Sequences first .. last of a batch by slices of its row pointers: the tokens before and
+    after theirs belong to no sequence."""
+    lengths, counts = [40, 9, 33], [3, 1, 5]
+    b = Batch(BF16, 4, 2, 64, 16, prefix, lengths, counts, seed=15).fill()
+    out, lse, eo, el = b.want()
+    indptr, ends = b.indptr[first:last + 1], b.ends[first:last + 1]
+    rows = torch.zeros(9, dtype=torch.bool)
+    rows[b.ends_host[first]:b.ends_host[last]] = True
+    given = torch.full_like(b.query, math.nan)
+    spoil = torch.full((1 << 22,), math.nan, device="cuda")     # what fresh memory may hold
+    del spoil
+    got, got_lse = at.prefix_attention(
+        b.query, b.kc, b.vc, b.prefix, prefix, indptr, b.indices, b.lengths[first:last],
+        query_indptr=ends, max_query=5, max_length=40, out=given, return_lse=True)
+    got, got_lse = got.cpu().double(), got_lse.cpu().double()
+    assert ((got - out).abs() <= eo)[rows].all() and ((got_lse - lse).abs() <= el)[rows].all()
+    assert not got[~rows].any() and (got_lse[~rows] == -math.inf).all()
+    frequency, _ = at.rope_frequencies(64)
+    kc, vc = b.kc.clone(), b.vc.clone()
+    query = at.paged_append(b.key, b.value, kc, vc, indptr, b.indices, b.lengths[first:last],
+                            frequency, query=b.query, query_indptr=ends)
+    assert not query[~rows.cuda()].any() and query[rows.cuda()].any(-1).all()
+    for i in range(first, last):
+        new = tuple(x[lengths[i] - counts[i]:] for x in b.places(i))
+        mine = slice(b.ends_host[i], b.ends_host[i + 1])
+        assert torch.equal(vc[new], b.value[mine])
+        _check_turned(kc[new], b.key[mine],
+                      torch.arange(lengths[i] - counts[i], lengths[i]), frequency, "half")
+        kc[new], vc[new] = b.kc[new], b.vc[new]
+    assert torch.equal(_bits(kc), _bits(b.kc)) and torch.equal(_bits(vc), _bits(b.vc))

@@ -311,9 +311,10 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     ``lengths[b]`` counts the tokens of sequence b's own pages, the new ones included: its n new
     tokens, rows query_indptr[b] to query_indptr[b + 1] (one each where that is None), go to
     positions lengths[b] - n and on, and are turned at ``offset`` (the shared prefix's length)
-    more.  A token whose page is not on its list, or not in the cache, is left out.  Rows past
-    query_indptr[-1] belong to no sequence (a batch padded for a graph): nothing is written for
-    them and their queries come back zero."""
+    more.  A token whose page is not on its list, or not in the cache, is left out.  Rows before
+    query_indptr[0] (slices of a larger batch's row pointers) and from query_indptr[-1] on (a
+    batch padded for a graph) belong to no sequence: nothing is written for them and their
+    queries come back zero."""
     device, dtype = _operand("key", key, _DTYPES)
     _no_gradient("paged_append", key, value, query, key_cache, value_cache)
     shape, ks = _heads("key", key, device, dtype, 3)
@@ -374,8 +375,8 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     Query head h reads kv head h // (heads // kv_heads); dim is a multiple of 8 up to 256;
     ``scale`` is 1 / sqrt(dim) by default.  ``max_query`` and ``max_length`` bound the new tokens
     and the length of a sequence: they size the launch (larger ones on the device are still
-    right, only slower).  A row that sees no key (or scores of -inf alone) gives 0; what hidden
-    keys and values hold does not matter.  With ``return_lse`` also each row's logarithm of
+    right, only slower).  A row that sees no key (or scores of -inf alone), or belongs to no
+    sequence, gives 0; what hidden keys and values hold does not matter.  With ``return_lse`` also each row's logarithm of
     the sum of its exponentials, float32 [tokens, heads] (-inf for such a row), by which results
     over disjoint keys can be joined.
 

@@ -101,8 +101,10 @@ __global__ __launch_bounds__(64 * kWaves, (DP == 256 ? 1 : 2)) void attend_whole
     }
   };
   if (b >= a.sequences) {
-    i64 end = a.ends ? a.ends[a.sequences] : a.tokens;
-    end = end < 0 ? 0 : end > a.tokens ? a.tokens : end;
+    i64 begin = a.ends ? a.ends[0] : 0, end = a.ends ? a.ends[a.sequences] : a.tokens;
+    begin = begin < 0 ? 0 : begin > a.tokens ? a.tokens : begin;
+    end = end < begin ? begin : end > a.tokens ? a.tokens : end;
+    nothing(0, static_cast<int>(begin) * a.group);
     nothing(static_cast<int>(end) * a.group, a.tokens * a.group);
     return;
   }

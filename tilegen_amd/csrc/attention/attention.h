@@ -46,10 +46,12 @@ struct Div {
 };
 
 // The sequence of token t: how many of ends[1 .. sequences] are at most t (equal ends are
-// empty sequences).  A whole wave asks for one token; each round looks at 64 places.
+// empty sequences); `sequences`, which is none, for a token before ends[0] as for one past the
+// last.  A whole wave asks for one token; each round looks at 64 places.
 __device__ __forceinline__ int sequence_of(const int64_t* __restrict__ ends, int sequences,
                                            i64 t) {
   const int lane = threadIdx.x & 63;
+  const bool before = t < ends[0];
   int lo = 0, hi = sequences;  // the answer is in lo .. hi
   while (lo < hi) {
     const int step = (hi - lo + 63) / 64;
@@ -59,7 +61,7 @@ __device__ __forceinline__ int sequence_of(const int64_t* __restrict__ ends, int
     lo += n * step;
     hi = min(hi, lo + step - 1);
   }
-  return lo;
+  return before ? sequences : lo;
 }
 
 // Host side: one message format for refusals and HIP errors.
