@@ -56,7 +56,10 @@ int launch_rope(const tg_rope* a, void* stream);
  * query_out (heads = 0: none).  rotary = 0: nothing is turned.  A token whose position falls
  * outside its sequence's pages, or whose page is outside the cache, is not written; one before
  * query_indptr[0] or past query_indptr[sequences] belongs to no sequence (slices of a larger
- * batch's row pointers, or a padded batch): it is not written and its query comes back zero. */
+ * batch's row pointers, or a padded batch): it is not written and its query comes back zero.
+ * query_out may be query (the same strides); it may not overlap it otherwise, or key, value or a
+ * cache, and the caches may not overlap one another (they may be one where rotary is 0 and value
+ * is key).  Rows that stand in the caches may not be among the slots that are written. */
 typedef struct {
   const void *key, *value, *query;
   void *key_cache, *value_cache, *query_out;

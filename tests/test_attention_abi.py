@@ -158,3 +158,57 @@ def test_sizes_at_the_ends_of_64_bits():
     for tokens in (2, 40):
         sizes = dict(tokens=tokens, ends=4096)
         assert workspace(**sizes, max_query=most) == workspace(**sizes, max_query=tokens) > 0
+
+
+def _append_args(**change):
+    names = ("key value query kc vc out indptr indices lengths ends frequency dtype tokens sequences "
+             "heads kv_heads dim rotary layout pages page n_indices offset key_token key_head "
+             "value_token value_head query_token query_head out_token out_head kc_page kc_slot "
+             "kc_head vc_page vc_slot vc_head magnitude").split()
+    base = dict.fromkeys(names, 0)
+    base.update(dtype=0, tokens=5, sequences=5, heads=4, kv_heads=2, dim=64, rotary=64, pages=9,
+                page=16, n_indices=5, magnitude=1.0)
+    for token, head in (("key_token", "key_head"), ("value_token", "value_head"),
+                        ("query_token", "query_head"), ("out_token", "out_head")):
+        base.update({token: 512, head: 64})
+    for c in ("kc", "vc"):
+        base.update({c + "_page": 2048, c + "_slot": 128, c + "_head": 64})
+    base.update(key=1 << 20, value=2 << 20, query=3 << 20, out=4 << 20, kc=5 << 20, vc=6 << 20)
+    base.update(change)
+    return at._APPEND.pack(*base.values())
+
+
+def test_append_over_its_own_operands():
+    """Refused where what is written shares memory with what is read or written beside it, and
+    there alone: slices of one array may lie between one another.  (The row pointers are null, so
+    that calls without a fault end in that refusal and nothing is launched.)"""
+    L = at._lib()
+
+    def message(**change):
+        assert L.launch_paged_append(_append_args(**change), None) == -1
+        return runtime.last_error()
+
+    q, k, v = 3 << 20, (3 << 20) + 4 * 128, (3 << 20) + 6 * 128     # packed, 8 heads a token
+    packed = dict(query=q, key=k, value=v)
+    for fine in (dict(), packed, dict(packed, out=q), dict(out=3 << 20),
+                 dict(vc=(5 << 20) + 2048, kc_page=2048, vc_page=2048, page=8),
+                 # keys by slots, values by heads, in halves of a page
+                 dict(vc=(5 << 20) + 4096, kc_page=4096, vc_page=4096, vc_slot=64, vc_head=1024),
+                 dict(heads=0, query=0, out=0), dict(kc=5 << 20, vc=5 << 20, rotary=0, value=1 << 20),
+                 dict(key=(5 << 20) + 4096)):       # a key from the cache
+        assert "null" in message(**fine), fine
+    for change, out, other in [
+            (dict(out=q + 128), "query_out", "query"), (dict(packed, out=k - 2), "query_out", "query"),
+            (dict(packed, out=k), "query_out", "key"),
+            (dict(packed, heads=2, out=v), "query_out", "value"),
+            (dict(out=(1 << 20) + 2), "query_out", "key"), (dict(out=2 << 20), "query_out", "value"),
+            (dict(out=(1 << 20) + 4 * 1024 + 254), "query_out", "key"),
+            (dict(out=(5 << 20) + 9 * 4096 - 2), "query_out", "key_cache"),
+            (dict(out=6 << 20), "query_out", "value_cache"),
+            (dict(out=3 << 20, out_head=128), "query_out", "query"),
+            (dict(vc=5 << 20), "value_cache", "key_cache"),
+            (dict(vc=(5 << 20) + 4094, kc_page=4096, vc_page=4096), "value_cache", "key_cache"),
+            (dict(vc=5 << 20, rotary=0), "value_cache", "key_cache")]:
+        want = "%s overlaps %s" % (out, other)
+        assert message(**change).endswith(want), (change, runtime.last_error())
+    assert "null" in message(out=(1 << 20) + 4 * 1024 + 256)    # past the last key's second head

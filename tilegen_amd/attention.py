@@ -314,7 +314,8 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     more.  A token whose page is not on its list, or not in the cache, is left out.  Rows before
     query_indptr[0] (slices of a larger batch's row pointers) and from query_indptr[-1] on (a
     batch padded for a graph) belong to no sequence: nothing is written for them and their
-    queries come back zero."""
+    queries come back zero.  ``query_out`` may be ``query`` itself, and share no other memory
+    with the operands."""
     device, dtype = _operand("key", key, _DTYPES)
     _no_gradient("paged_append", key, value, query, key_cache, value_cache)
     shape, ks = _heads("key", key, device, dtype, 3)
@@ -333,8 +334,6 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
             raise ValueError("query is %s, key %s" % (tuple(qshape), tuple(shape)))
         if query_out is None:
             query_out = _like(query)
-        elif query_out is not query:
-            _apart("query_out", query_out, "query", query)
         oshape, os_ = _heads("query_out", query_out, device, dtype, 3, write=True)
         if oshape != qshape:
             raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(qshape)))

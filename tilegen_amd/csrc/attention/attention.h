@@ -78,4 +78,102 @@ inline int hip_failed(hipError_t e, const char* what) {
   return tg_fail(static_cast<int>(e), msg);
 }
 
+// An operand as a call describes it: `size` elements along each axis, `stride` elements apart.
+struct Operand {
+  const char* name;
+  const void* at;
+  int axes;
+  int64_t size[4], stride[4];
+};
+
+inline bool same(const Operand& x, const Operand& y) {
+  bool yes = x.at == y.at && x.axes == y.axes;
+  for (int i = 0; yes && i < x.axes; ++i)
+    yes = x.size[i] == y.size[i] && (x.size[i] <= 1 || x.stride[i] == y.stride[i]);
+  return yes;
+}
+
+// Whether two operands have a byte in common: whether the distance between them is a sum of steps
+// along their axes.  Steps of one length count together; from the longest on, each number of
+// them is tried that the shorter ones can make up for, which is two or three where one axis lies
+// inside the next, as in slices of one array.  Layouts that need many trials count as sharing.
+class Sharing {
+ public:
+  Sharing(const Operand& x, const Operand& y, int bytes) {
+    empty_ = !x.at || !y.at;
+    add(x, bytes, 1);
+    add(y, bytes, -1);
+    step(1, -(bytes - 1), bytes - 1);
+    for (int i = 1; i < n_; ++i)    // the longest first
+      for (int j = i; j && steps_[j].length > steps_[j - 1].length; --j) {
+        const Step other = steps_[j];
+        steps_[j] = steps_[j - 1];
+        steps_[j - 1] = other;
+      }
+    for (int i = n_; i--;) {
+      least_[i] = least_[i + 1] + steps_[i].length * steps_[i].least;
+      most_[i] = most_[i + 1] + steps_[i].length * steps_[i].most;
+    }
+    distance_ = static_cast<Wide>(reinterpret_cast<uintptr_t>(y.at)) -
+                static_cast<Wide>(reinterpret_cast<uintptr_t>(x.at));
+  }
+  bool operator()() {
+    return !empty_ && distance_ >= least_[0] && distance_ <= most_[0] && reach(0, distance_);
+  }
+
+ private:
+  using Wide = __int128;
+  struct Step {
+    Wide length, least, most;   // how often it may be taken
+  };
+  void step(Wide length, Wide least, Wide most) {
+    if (length == 0) return;
+    if (length < 0) {
+      const Wide from = -most;
+      length = -length;
+      most = -least;
+      least = from;
+    }
+    for (int i = 0; i < n_; ++i)
+      if (steps_[i].length == length) {
+        steps_[i].least += least;
+        steps_[i].most += most;
+        return;
+      }
+    steps_[n_++] = {length, least, most};
+  }
+  void add(const Operand& x, int bytes, int sign) {
+    for (int i = 0; i < x.axes; ++i) {
+      if (x.size[i] < 1) empty_ = true;
+      const Wide last = x.size[i] - 1;
+      step(static_cast<Wide>(x.stride[i]) * bytes, sign < 0 ? -last : 0, sign < 0 ? 0 : last);
+    }
+  }
+  static Wide down(Wide n, Wide d) { return n / d - (n % d < 0); }
+  bool reach(int i, Wide left) {
+    if (i == n_) return left == 0;
+    const Step& s = steps_[i];
+    Wide from = -down(most_[i + 1] - left, s.length), to = down(left - least_[i + 1], s.length);
+    if (from < s.least) from = s.least;
+    if (to > s.most) to = s.most;
+    for (Wide n = from; n <= to; ++n) {
+      if (++trials_ > 16384) return true;
+      if (reach(i + 1, left - n * s.length)) return true;
+    }
+    return false;
+  }
+  Step steps_[9];
+  Wide least_[10] = {}, most_[10] = {}, distance_;
+  int n_ = 0, trials_ = 0;
+  bool empty_;
+};
+
+// Refuses an output that shares memory with another operand.
+inline int apart(const char* what, const Operand& out, const Operand& x, int bytes) {
+  if (!Sharing(out, x, bytes)()) return 0;
+  char msg[256];
+  std::snprintf(msg, sizeof(msg), "%s: %s overlaps %s", what, out.name, x.name);
+  return tg_fail(-1, msg);
+}
+
 }  // namespace tg

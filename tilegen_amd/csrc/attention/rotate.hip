@@ -340,6 +340,31 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_append(const 
   if (!r->query_indptr && r->tokens > r->sequences)
     return refuse(-1, what, "more tokens than sequences without query_indptr", r->tokens);
   if (r->tokens == 0) return 0;
+  // What is written shares no memory with what else is written, or with the rows of new tokens.
+  // (Rows of new tokens may stand in the caches themselves: which slots are written is known on
+  // the device alone.)
+  const Operand key = {"key", r->key, 3, {r->tokens, r->kv_heads, r->dim},
+                       {r->key_token, r->key_head, 1}};
+  const Operand value = {"value", r->value, 3, {r->tokens, r->kv_heads, r->dim},
+                         {r->value_token, r->value_head, 1}};
+  const Operand query = {"query", r->query, 3, {r->tokens, r->heads, r->dim},
+                         {r->query_token, r->query_head, 1}};
+  const Operand out = {"query_out", r->query_out, 3, {r->tokens, r->heads, r->dim},
+                       {r->out_token, r->out_head, 1}};
+  const Operand kc = {"key_cache", r->key_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->kc_page, r->kc_slot, r->kc_head, 1}};
+  const Operand vc = {"value_cache", r->value_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->vc_page, r->vc_slot, r->vc_head, 1}};
+  const int bytes = r->dtype == TG_F32 ? 4 : 2;
+  if (r->heads) {
+    if (!same(out, query))
+      if (const int rc = apart(what, out, query, bytes)) return rc;
+    for (const Operand* x : {&key, &value, &kc, &vc})
+      if (const int rc = apart(what, out, *x, bytes)) return rc;
+  }
+  // one cache for both holds the same values twice where nothing is turned and value is key
+  if (!(r->rotary == 0 && same(key, value) && same(kc, vc)))
+    if (const int rc = apart(what, vc, kc, bytes)) return rc;
   if (!r->key || !r->value || !r->key_cache || !r->value_cache || !r->indptr || !r->lengths ||
       (r->n_indices && !r->indices) || (r->heads && (!r->query || !r->query_out)) ||
       (r->rotary && !r->frequency))
