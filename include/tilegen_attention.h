@@ -86,7 +86,8 @@ int launch_paged_append(const tg_paged_append* a, void* stream);
  * max_query and max_length are the host's bounds on n and lengths[b]; they size the launch,
  * and larger values on the device are still right.  workspace holds
  * prefix_attention_workspace(a) bytes, 16-byte aligned, until the kernels have run; calls
- * that overlap need one each. */
+ * that overlap need one each.  out may be query (the same strides); it may not overlap it
+ * otherwise, or a cache. */
 typedef struct {
   const void *query, *key_cache, *value_cache;
   const int64_t *prefix, *indptr, *indices, *lengths, *query_indptr;

@@ -951,3 +951,19 @@ def test_a_block_of_row_pointers(hip_ready, prefix, first, last):
                       torch.arange(lengths[i] - counts[i], lengths[i]), frequency, "half")
         kc[new], vc[new] = b.kc[new], b.vc[new]
     assert torch.equal(_bits(kc), _bits(b.kc)) and torch.equal(_bits(vc), _bits(b.vc))
+
+
+def test_slices_of_one_array(hip_ready):
+    """Outputs that lie between their operands without a byte in common."""
+    b = Batch(BF16, 4, 4, 64, 16, 32, [20, 9], [1, 1], seed=12).fill()
+    frequency, _ = at.rope_frequencies(64)
+    pos = torch.arange(2, device="cuda")
+    packed = torch.zeros(2, 13, 64, device="cuda", dtype=BF16)
+    packed[:, :4] = b.query
+    want = at.rope(b.query, pos, frequency)
+    at.rope(packed[:, :4], pos, frequency, out=packed[:, 4:8])
+    assert torch.equal(packed[:, 4:8], want)
+    want = b.attend()[0]
+    b.query = packed[:, :4]
+    b.attend(out=packed[:, 8:12])
+    assert torch.equal(packed[:, 8:12], want) and not packed[:, 12:].any()

@@ -147,22 +147,6 @@ def _raise(rc: int, what: str) -> None:
     _rt.check(rc, what)
 
 
-def _apart(name: str, out: torch.Tensor, source_name: str, x: torch.Tensor) -> None:
-    """out is x itself, or shares none of its memory's span."""
-    if out.data_ptr() == x.data_ptr() and out.stride() == x.stride():
-        return
-
-    def span(t):
-        size = t.element_size()
-        last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * size
-
-    if out.numel() and x.numel():
-        (a, b), (c, d) = span(out), span(x)
-        if a < d and c < b:
-            raise ValueError("%s overlaps %s without being it" % (name, source_name))
-
-
 # --------------------------------------------------------------------------- #
 # rotary positions
 # --------------------------------------------------------------------------- #
@@ -208,8 +192,6 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     shape, xs = _heads("x", x, device, dtype, 3)
     if out is None:
         out = _like(x)
-    elif out is not x:
-        _apart("out", out, "x", x)
     oshape, ys = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))
@@ -249,8 +231,9 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequency: torch.Tensor, *,
     A pair is elements (i, i + n) (layout "half") or (2 i, 2 i + 1) ("interleaved") of the
     first 2 n elements of each head, n = len(frequency); the others are copied.  Angles are
     taken in 64 bits, so positions may be as large as they come; the turn is made in 32 bits
-    and rounded once.  ``out`` may be x itself.  Heads may be those of a packed projection
-    (``qkv[:, :heads + kv_heads]``), queries and keys in one call.  Differentiable in x."""
+    and rounded once.  ``out`` may be x itself, and share no other memory with it.  Heads may be
+    those of a packed projection (``qkv[:, :heads + kv_heads]``), queries and keys in one call.
+    Differentiable in x."""
     if x.requires_grad and torch.is_grad_enabled():
         if out is not None:
             raise ValueError("out cannot be given where x needs a gradient")
@@ -377,7 +360,8 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     right, only slower).  A row that sees no key (or scores of -inf alone), or belongs to no
     sequence, gives 0; what hidden keys and values hold does not matter.  With ``return_lse`` also each row's logarithm of
     the sum of its exponentials, float32 [tokens, heads] (-inf for such a row), by which results
-    over disjoint keys can be joined.
+    over disjoint keys can be joined.  ``out`` may be the query, and share no other memory with
+    the operands.
 
     Scores, probabilities and sums are held in 32 bits; probabilities are rounded to the
     caches' type for the matrix instructions that weigh the values.  Results do not depend on
@@ -393,9 +377,6 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
         indptr, indices, lengths, query_indptr, tokens, device)
     if out is None:
         out = _like(query)
-    else:
-        for name, t in (("query", query), ("key_cache", key_cache), ("value_cache", value_cache)):
-            _apart("out", out, name, t)
     oshape, os_ = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))

@@ -339,6 +339,18 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
     return refuse(-1, what, "the workspace is too small; bytes needed", p.bytes);
   if (reinterpret_cast<uintptr_t>(r->workspace) % 16)
     return refuse(-1, what, "the workspace is not 16-byte aligned", 0);
+  const Operand query = {"query", r->query, 3, {r->tokens, r->heads, r->dim},
+                         {r->query_token, r->query_head, 1}};
+  const Operand out = {"out", r->out, 3, {r->tokens, r->heads, r->dim},
+                       {r->out_token, r->out_head, 1}};
+  const Operand kc = {"key_cache", r->key_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->kc_page, r->kc_slot, r->kc_head, 1}};
+  const Operand vc = {"value_cache", r->value_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->vc_page, r->vc_slot, r->vc_head, 1}};
+  if (!same(out, query))
+    if (const int rc = apart(what, out, query, 2)) return rc;
+  for (const Operand* x : {&kc, &vc})
+    if (const int rc = apart(what, out, *x, 2)) return rc;
   a.part = static_cast<float*>(r->workspace);
   a.part_ml = reinterpret_cast<float2*>(a.part + static_cast<int64_t>(a.slots) * a.tokens *
                                                      a.heads * a.dim);

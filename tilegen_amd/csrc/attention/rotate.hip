@@ -304,6 +304,10 @@ extern "C" __attribute__((visibility("default"))) int launch_rope(const tg_rope*
     return rc;
   if (r->sign != 1 && r->sign != -1) return refuse(-1, what, "sign must be 1 or -1", r->sign);
   if (r->tokens == 0 || r->heads == 0) return 0;
+  const Operand x = {"x", r->x, 3, {r->tokens, r->heads, r->dim}, {r->x_token, r->x_head, 1}};
+  const Operand y = {"out", r->y, 3, {r->tokens, r->heads, r->dim}, {r->y_token, r->y_head, 1}};
+  if (!same(y, x))
+    if (const int rc = apart(what, y, x, r->dtype == TG_F32 ? 4 : 2)) return rc;
   if (!r->x || !r->y || !r->positions || (r->rotary && !r->frequency))
     return refuse(-1, what, "null array", r->tokens);
   Rows a = {};
