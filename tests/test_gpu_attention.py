@@ -967,3 +967,21 @@ def test_slices_of_one_array(hip_ready):
     b.query = packed[:, :4]
     b.attend(out=packed[:, 8:12])
     assert torch.equal(packed[:, 8:12], want) and not packed[:, 12:].any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("dim,page", [(64, 16), (96, 16), (128, 7), (256, 24)])
+@pytest.mark.parametrize("wide", [False, True])
+def test_an_infinity_at_the_end_of_the_prefix(hip_ready, dtype, dim, page, wide):
+    """Places past the prefix's last key, in the tile that it ends in, have no part in the sums."""
+    for prefix in (100, 900):
+        b = Batch(dtype, 60 if wide else 2, 1, dim, page, prefix, [20, 9], [1, 1], seed=16).fill()
+        out, lse, eo, el = b.want()
+        pages, slots = b.places()
+        b.vc[pages[-1], slots[-1], 0, 3] = math.inf
+        b.vc[pages[-1], slots[-1], 0, 5] = -math.inf
+        got, got_lse = (x.cpu().double() for x in b.attend(
+            **dict(WIDE, query_indptr=b.ends) if wide else {}))
+        assert (got[:, :, 3] == math.inf).all() and (got[:, :, 5] == -math.inf).all()
+        got[:, :, [3, 5]] = out[:, :, [3, 5]]
+        assert ((got - out).abs() <= eo).all() and ((got_lse - lse).abs() <= el).all()

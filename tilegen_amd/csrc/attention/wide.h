@@ -127,8 +127,8 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   // pages hold whole groups of 8 keys (`even`) a lane knows where one group starts, 64 lanes 8
   // tiles of them; a wave's rows of one load stand in one group, so that the address is uniform.
   // Elsewhere a lane knows one key of one tile.  Pages are asked for a tile before they are
-  // needed and before that tile's loads, since loads return in order.  Keys past the end stand
-  // for the last one (hidden).
+  // needed and before that tile's loads, since loads return in order.  Lookups past the end
+  // are the last key's.
   auto key_of_lane = [&](int tile) {
     return min(a.even ? p.k0 + (tile >> 3) * 8 * W::kKeys + 8 * lane
                       : p.k0 + tile * W::kKeys + lane,
@@ -196,12 +196,13 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
       const int r = first + W::kPass * i, d = chunk(r) * 8;
       const int key = min(key0 + r, p.k1 - 1);
       const i64 at = __shfl(offsets, a.even ? tile % 8 * 8 + ((key - key0) >> 3) : r);
-      if (at >= 0) {
+      if (at >= 0 && key0 + r < p.k1) {
         const T* from = a.even ? cache + at / 2 + (key & 7) * slot_stride
                                : cache + (at >> 32) * page_stride +
                                      static_cast<i64>(static_cast<unsigned>(at)) * slot_stride;
         if (d < a.dim) load_to_lds(from + d, to + W::kSpan * i);
-      } else {    // no page: hidden below, and zero, since 0 times a NaN would be NaN
+      } else {    // no page, or past the end: hidden below, and zero, since 0 times an infinity
+                  // or a NaN would be NaN
         *reinterpret_cast<s16x8*>(to + W::kSpan * i + 16 * lane) = s16x8(0);
       }
     }
