@@ -985,3 +985,23 @@ def test_an_infinity_at_the_end_of_the_prefix(hip_ready, dtype, dim, page, wide)
         assert (got[:, :, 3] == math.inf).all() and (got[:, :, 5] == -math.inf).all()
         got[:, :, [3, 5]] = out[:, :, [3, 5]]
         assert ((got - out).abs() <= eo).all() and ((got_lse - lse).abs() <= el).all()
+
+
+@pytest.mark.parametrize("more", [{}, dict(max_length=1100, max_query=10 ** 6)])
+def test_scores_that_are_not_numbers(hip_ready, more):
+    """A NaN among a row's scores makes its result NaN, also where no other score is there to
+    give a maximum: to the row, to a wave, to a part."""
+    for heads in (2, 60):
+        # all of a row's keys; those of one wave's tile; in one launch, and in parts
+        for prefix, bad in ((0, 0), (96, 96), (900, 900), (900, 32), (128, 32)):
+            b = Batch(BF16, heads, 1, 64, 16, prefix, [1, 0], [1, 1], seed=17).fill()
+            page, slot = b.places()
+            b.kc[page[:bad], slot[:bad]] = math.nan
+            if bad == prefix:
+                b.kc[b.places(0)] = math.nan
+            out, lse = b.attend(**more)
+            assert torch.isnan(out[0]).all() and torch.isnan(lse[0]).all(), (heads, prefix, bad)
+            if bad:
+                assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
+            else:
+                assert not out[1].any() and (lse[1] == -math.inf).all()

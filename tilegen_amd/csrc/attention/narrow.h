@@ -264,7 +264,8 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         const float2 ml = tops[w * 16 + r];
-        total += ml.x == -INFINITY ? 0.f : ml.y * exp2f(ml.x - top);
+        // without a maximum the sum is 0, or NaN from scores that are
+        total += ml.x == -INFINITY ? ml.y : ml.y * exp2f(ml.x - top);
       }
     }
     if (BOTH) {
