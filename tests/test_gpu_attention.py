@@ -1005,3 +1005,25 @@ def test_scores_that_are_not_numbers(hip_ready, more):
                 assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
             else:
                 assert not out[1].any() and (lse[1] == -math.inf).all()
+
+
+@pytest.mark.parametrize("heads,first", [(2, 128), (50, 128), (50, 64)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_scores_that_climb_by_their_last_bit(hip_ready, dtype, heads, first):
+    """Past 2^27 neighbouring scores are 16 apart.  Probabilities are powers of two, which are
+    exact, and the results, under 1, rounded once (twice u for the sums' order)."""
+    b = Batch(dtype, heads, 1, 64, 16, 0, [640], [1], seed=18).fill()
+    page, slot = b.places(0)
+    b.query.zero_()
+    b.query[..., 0], b.query[..., 1] = 32768.0, 16.0
+    b.kc[page, slot] = 0.0
+    b.kc[page, slot, 0, 0] = 4096.0
+    b.kc[page[:first], slot[:first], 0, 1] = 1.0
+    b.kc[page[first:], slot[first:], 0, 1] = 2.0
+    out, lse = b.attend(scale=math.log(2.0), max_length=640 if heads < 50 else 30000,
+                        max_query=10 ** 6, query_indptr=b.ends)
+    weight = torch.ones(640, dtype=torch.float64)
+    weight[:first] = 2.0 ** -16
+    want = weight @ b.vc[page, slot, 0].cpu().double() / weight.sum()
+    off = (out[0].cpu().double() - want).abs()
+    assert (off <= 2.0 ** -7).all(), float(off.max())

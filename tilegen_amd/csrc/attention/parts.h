@@ -72,7 +72,10 @@ __device__ __forceinline__ float row_sum(float v) {
   return q.a + q.b;
 }
 
-constexpr float kSlack = 8.f;   // log2 of how far scores may pass the running maximum
+// log2 of how far scores may pass the running maximum.  Their difference is compared with it, which
+// is exact for neighbours: past 2^27, where they are 16 apart, maximum + kSlack would round up to
+// the next one and leave a probability of 2^16, more than float16 holds.
+constexpr float kSlack = 8.f;
 // Scores times scale less the maximum is one fused operation, exact in the product where the
 // maximum has been rounded.  Past this the rounding, 2^-24 of it, is no longer small against
 // one, and the product is rounded too.
