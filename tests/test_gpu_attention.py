@@ -1027,3 +1027,27 @@ def test_scores_that_climb_by_their_last_bit(hip_ready, dtype, heads, first):
     want = weight @ b.vc[page, slot, 0].cpu().double() / weight.sum()
     off = (out[0].cpu().double() - want).abs()
     assert (off <= 2.0 ** -7).all(), float(off.max())
+
+
+def test_many_small_probabilities(hip_ready):
+    """131071 keys 18 nats under one other, in one part for many rows: 0.2% of the weight.  Each
+    probability is off by at most 2^-25 of the 2^7 that the largest is (float16's smallest number
+    is 2^-24); 32-bit sums over 16 keys at a time, and the rounded result, by u."""
+    n, kv = 131072, 64
+    kc = torch.zeros(n // 64, 64, kv, 8, device="cuda", dtype=F16)
+    vc = torch.ones(n // 64, 64, kv, 8, device="cuda", dtype=F16)
+    kc[..., 0] = -18.0
+    kc[0, 0, :, 0] = vc[0, 0] = 0.0
+    q = torch.zeros(1024, kv, 8, device="cuda", dtype=F16)
+    q[..., 0] = 1.0
+    none = torch.zeros(0, dtype=torch.int64, device="cuda")
+    zero = torch.zeros(2, dtype=torch.int64, device="cuda")
+    small = (n - 1) * math.exp(-18)
+    want = small / (1 + small)
+    for tokens in (1024, 1):
+        ends = torch.tensor([0, tokens], device="cuda")
+        out = at.prefix_attention(q[:tokens], kc, vc, torch.arange(n // 64, device="cuda"), n, zero,
+                                  none, zero[:1], query_indptr=ends, max_query=tokens,
+                                  max_length=0, scale=1.0)
+        off = float((out.double() - want).abs().max())
+        assert off <= 2 * U[F16] * want + n * 2.0 ** -32, (tokens, off, want)

@@ -9,8 +9,8 @@
 // gives just that from values stored as they come.
 //
 // The running maximum of a row follows the scores only when they pass it by 2^8: until then
-// probabilities are up to 256 times too large, sums and products as well, and their quotient
-// is the same.  So most tiles need neither the exchange between lanes nor the rescaling.
+// probabilities are up to 256 times too large (in float16 another 128 times, base_of), sums and
+// products as well, and their quotient is the same.  So most tiles need neither the exchange between lanes nor the rescaling.
 //
 // Memory bounds it: 16 rows are half a matrix instruction's worth of work for the bytes read.
 // Keys go straight to registers (the A operand is 16 bytes of a key a lane), the next tile's
@@ -176,8 +176,8 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
     float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     top *= a.scale;
-    if (__any(top - m > kSlack)) {
-      const float now = fmaxf(row_max(top), m);
+    if (__any(top - m > kSlack + M::kLift)) {
+      const float now = fmaxf(base_of<T>(row_max(top)), m);
       const float f = m == -INFINITY ? 0.f : exp2f(m - now);
       m = now;
       huge |= __any(fabsf(now) > kHuge && now != -INFINITY);

@@ -26,6 +26,7 @@ struct Matrix<__bf16> {
                                                    __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static constexpr short kExponent = 0x7F80;
+  static constexpr float kLift = 0.f;
 };
 
 template <>
@@ -40,6 +41,7 @@ struct Matrix<_Float16> {
                                                   __builtin_bit_cast(x8, b), c, 0, 0, 0);
   }
   static constexpr short kExponent = 0x7C00;
+  static constexpr float kLift = 7.f;
 };
 
 // A value of the other half of the wave, and of the other half of each half, beside one's own:
@@ -84,6 +86,17 @@ __device__ __forceinline__ float apart(float s, float scale, float base) {
 #pragma clang fp contract(off)
   const float x = s * scale;
   return x - base;
+}
+
+// What a row's probabilities are taken against: its largest score, 2^kLift down, so that the
+// largest probability is 2^kLift, and 2^(kLift + kSlack) before the maximum follows, 2^15 in
+// float16.  The factor is in sums and products alike.  It keeps probabilities down to 2^-32 of the
+// largest apart from 0 where float16 by itself ends at 2^-25: on long prefixes what is below counts
+// (131071 keys 18 nats under one have 0.2% of the weight).  Past kHuge differences are whole and the
+// lift would be rounded.
+template <typename T>
+__device__ __forceinline__ float base_of(float top) {
+  return fabsf(top) > kHuge ? top : top - Matrix<T>::kLift;
 }
 
 constexpr int kWaves = 4;       // of a workgroup

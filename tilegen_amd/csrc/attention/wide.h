@@ -263,9 +263,9 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   // lets the running maximum follow where a row's scores have left it far behind
   auto follow = [&](float top) {
     top *= a.scale;
-    if (__any(top - m > kSlack)) {
+    if (__any(top - m > kSlack + M::kLift)) {
       const Both both = halves(top);
-      const float to = fmaxf(fmaxf(both.a, both.b), m);
+      const float to = fmaxf(base_of<T>(fmaxf(both.a, both.b)), m);
       const float f = m == -INFINITY ? 0.f : exp2f(m - to);
       m = to;
       huge |= __any(fabsf(to) > kHuge && to != -INFINITY);
