@@ -1051,3 +1051,40 @@ def test_many_small_probabilities(hip_ready):
                                   max_length=0, scale=1.0)
         off = float((out.double() - want).abs().max())
         assert off <= 2 * U[F16] * want + n * 2.0 ** -32, (tokens, off, want)
+
+
+def test_second_derivatives_of_rope(hip_ready):
+    """The gradient of a loss of the gradient.  Two turns after one another: the bound above
+    twice, the first's error turned with the rest; |a| + |b| stays under 2^4."""
+    g = _gen(21)
+    frequency, magnitude = at.rope_frequencies(24, scaling="yarn", factor=4, trained=512)
+    positions = torch.tensor([0, 1, 77, 100000, 5], device="cuda")
+    x = _normal(g, 5, 3, 30, dtype=F32).requires_grad_()
+    w = _normal(g, 5, 3, 30, dtype=F32)
+    y = at.rope(x, positions, frequency, magnitude=magnitude)
+    first, = torch.autograd.grad((y * y).sum() / 2, x, create_graph=True)
+    assert first.requires_grad
+    second, = torch.autograd.grad((first * w).sum(), x)
+    # d/dx w . R'(R x) = R' R w
+    there = _turned(w, positions, frequency, "half", magnitude)[0]
+    want = _turned(there, positions, frequency, "half", magnitude, -1)[0]
+    assert ((second.cpu().double() - want).abs() <= 2.0 ** -15 * magnitude ** 2).all()
+    grad = w.clone().requires_grad_()
+    back = at.rope_backward(grad, positions, frequency, magnitude=magnitude)
+    back.backward(x.detach())
+    _check_turned(grad.grad, x, positions, frequency, "half", magnitude)
+
+
+def test_tangents_of_rope(hip_ready):
+    """Forward mode: the tangent of the result is the map of x's."""
+    import torch.autograd.forward_ad as fw
+    g = _gen(22)
+    frequency, _ = at.rope_frequencies(16)
+    positions = torch.arange(4, device="cuda")
+    x, t = (_normal(g, 4, 2, 20, dtype=F32) for _ in range(2))
+    for turn, sign in ((at.rope, 1), (at.rope_backward, -1)):
+        with fw.dual_level():
+            y = fw.unpack_dual(turn(fw.make_dual(x, t), positions, frequency))
+            assert y.tangent is not None
+            _check_turned(y.primal, x, positions, frequency, "half", sign=sign)
+            _check_turned(y.tangent, t, positions, frequency, "half", sign=sign)

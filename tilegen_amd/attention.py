@@ -32,6 +32,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 from . import runtime as _rt
 
@@ -205,21 +206,48 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     return out
 
 
+def _followed(x: torch.Tensor) -> bool:
+    """Whether autograd follows x, backward or forward."""
+    return (x.requires_grad and torch.is_grad_enabled()) or (
+        _forward._current_level >= 0 and _forward.unpack_dual(x).tangent is not None)
+
+
 class _Rope(torch.autograd.Function):
+    """The map is linear in x: its derivative along a tangent is the same map, its gradient the
+    transposed one, and either is a call that autograd may follow again."""
+
     @staticmethod
-    def forward(ctx, x, positions, frequency, layout, magnitude):
+    def forward(ctx, x, positions, frequency, layout, magnitude, sign):
         ctx.save_for_backward(positions, frequency)
-        ctx.how = layout, magnitude
-        return _turn(x, positions, frequency, layout, magnitude, None, 1, "rope")
+        ctx.save_for_forward(positions, frequency)
+        ctx.how = layout, magnitude, sign
+        return _turn(x, positions, frequency, layout, magnitude, None, sign, "rope")
+
+    @staticmethod
+    def _again(ctx, x, flip):
+        if x is None:
+            return None
+        positions, frequency = ctx.saved_tensors
+        layout, magnitude, sign = ctx.how
+        if x.stride(-1) != 1:       # a broadcast gradient, of a sum for example
+            x = x.contiguous()
+        return _linear(x, positions, frequency, layout, magnitude, None, flip * sign, "rope")
 
     @staticmethod
     def backward(ctx, grad):
-        positions, frequency = ctx.saved_tensors
-        layout, magnitude = ctx.how
-        if grad.stride(-1) != 1:    # a broadcast gradient, of a sum for example
-            grad = grad.contiguous()
-        return rope_backward(grad, positions, frequency, layout=layout,
-                             magnitude=magnitude), None, None, None, None
+        return _Rope._again(ctx, grad, -1), None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, *_):
+        return _Rope._again(ctx, tangent, 1)
+
+
+def _linear(x, positions, frequency, layout, magnitude, out, sign, what):
+    if isinstance(x, torch.Tensor) and _followed(x):
+        if out is not None:
+            raise ValueError("out cannot be given where x needs a gradient")
+        return _Rope.apply(x, positions, frequency, layout, magnitude, sign)
+    return _turn(x, positions, frequency, layout, magnitude, out, sign, what)
 
 
 def rope(x: torch.Tensor, positions: torch.Tensor, frequency: torch.Tensor, *,
@@ -233,19 +261,16 @@ def rope(x: torch.Tensor, positions: torch.Tensor, frequency: torch.Tensor, *,
     taken in 64 bits, so positions may be as large as they come; the turn is made in 32 bits
     and rounded once.  ``out`` may be x itself, and share no other memory with it.  Heads may be
     those of a packed projection (``qkv[:, :heads + kv_heads]``), queries and keys in one call.
-    Differentiable in x."""
-    if x.requires_grad and torch.is_grad_enabled():
-        if out is not None:
-            raise ValueError("out cannot be given where x needs a gradient")
-        return _Rope.apply(x, positions, frequency, layout, magnitude)
-    return _turn(x, positions, frequency, layout, magnitude, out, 1, "rope")
+    Differentiable in x, as often as need be, backward and forward."""
+    return _linear(x, positions, frequency, layout, magnitude, out, 1, "rope")
 
 
 def rope_backward(grad: torch.Tensor, positions: torch.Tensor, frequency: torch.Tensor, *,
                   layout: str = "half", magnitude: float = 1.0,
                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """The gradient of ``rope`` by x: the transposed map, which turns the other way."""
-    return _turn(grad, positions, frequency, layout, magnitude, out, -1, "rope_backward")
+    """The gradient of ``rope`` by x: the transposed map, which turns the other way.
+    Differentiable in grad."""
+    return _linear(grad, positions, frequency, layout, magnitude, out, -1, "rope_backward")
 
 
 # --------------------------------------------------------------------------- #
