@@ -1088,3 +1088,44 @@ def test_tangents_of_rope(hip_ready):
             assert y.tangent is not None
             _check_turned(y.primal, x, positions, frequency, "half", sign=sign)
             _check_turned(y.tangent, t, positions, frequency, "half", sign=sign)
+
+
+def test_lost_derivatives(hip_ready):
+    """Operands whose derivatives a call would drop, outputs that have a history of their own, and
+    tangents of calls without derivatives are refused."""
+    import torch.autograd.forward_ad as fw
+    frequency, _ = at.rope_frequencies(64)
+    b = Batch(BF16, 4, 2, 64, 16, 32, [20, 9], [1, 1], seed=12).fill()
+    pos = torch.arange(2, device="cuda")
+    needs = frequency.clone().requires_grad_()
+    grad_out = torch.empty_like(b.query).requires_grad_()
+
+    def append(**change):
+        return at.paged_append(**dict(dict(
+            key=b.key, value=b.value, key_cache=b.kc, value_cache=b.vc, indptr=b.indptr,
+            indices=b.indices, lengths=b.lengths, frequency=frequency, query=b.query), **change))
+
+    def attend(**change):
+        return at.prefix_attention(**dict(dict(
+            query=b.query, key_cache=b.kc, value_cache=b.vc, prefix=b.prefix, prefix_length=32,
+            indptr=b.indptr, indices=b.indices, lengths=b.lengths, max_length=20), **change))
+
+    calls = [lambda: at.rope(b.query, pos, needs), lambda: at.rope_backward(b.query, pos, needs),
+             lambda: append(frequency=needs),
+             lambda: at.rope(b.query, pos, frequency, out=grad_out),
+             lambda: at.rope_backward(b.query, pos, frequency, out=grad_out),
+             lambda: at.rope_backward(b.query.clone().requires_grad_(), pos, frequency,
+                                      out=torch.empty_like(b.query)),
+             lambda: append(query_out=grad_out), lambda: attend(out=grad_out)]
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
+        with torch.no_grad():
+            call()
+    with fw.dual_level():
+        dual = fw.make_dual(b.query, b.query)
+        for call in (lambda: append(query=dual), lambda: attend(query=dual),
+                     lambda: at.rope(dual, pos, frequency, out=torch.empty_like(b.query))):
+            with pytest.raises(ValueError):
+                call()
+        append(), attend()      # a level without tangents among the operands

@@ -206,10 +206,28 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     return out
 
 
-def _followed(x: torch.Tensor) -> bool:
-    """Whether autograd follows x, backward or forward."""
-    return (x.requires_grad and torch.is_grad_enabled()) or (
-        _forward._current_level >= 0 and _forward.unpack_dual(x).tangent is not None)
+def _tangent(t) -> bool:
+    return _forward._current_level >= 0 and _forward.unpack_dual(t).tangent is not None
+
+
+def _followed(t: torch.Tensor) -> bool:
+    """Whether autograd follows t, backward or forward."""
+    return (t.requires_grad and torch.is_grad_enabled()) or _tangent(t)
+
+
+def _no_gradient(what: str, *operands: Optional[torch.Tensor]) -> None:
+    """Refuses what autograd would follow: its results would have no gradient, silently.  An output
+    that it follows would lose its own."""
+    lost = False
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                lost = True
+    if _forward._current_level >= 0:
+        lost = lost or any(_tangent(t) for t in operands if t is not None)
+    if lost:
+        raise ValueError("%s has no backward pass for these operands: call it under "
+                         "torch.no_grad(), or with detached operands" % what)
 
 
 class _Rope(torch.autograd.Function):
@@ -246,7 +264,9 @@ def _linear(x, positions, frequency, layout, magnitude, out, sign, what):
     if isinstance(x, torch.Tensor) and _followed(x):
         if out is not None:
             raise ValueError("out cannot be given where x needs a gradient")
+        _no_gradient(what, frequency)
         return _Rope.apply(x, positions, frequency, layout, magnitude, sign)
+    _no_gradient(what, frequency, out)
     return _turn(x, positions, frequency, layout, magnitude, out, sign, what)
 
 
@@ -276,15 +296,6 @@ def rope_backward(grad: torch.Tensor, positions: torch.Tensor, frequency: torch.
 # --------------------------------------------------------------------------- #
 # the cache
 # --------------------------------------------------------------------------- #
-def _no_gradient(what: str, *operands: Optional[torch.Tensor]) -> None:
-    """Refuses what autograd would follow: its results would have no gradient, silently."""
-    if torch.is_grad_enabled():
-        for t in operands:
-            if t is not None and t.requires_grad:
-                raise ValueError("%s has no backward pass: call it under torch.no_grad(), or "
-                                 "with detached operands" % what)
-
-
 def _caches(key_cache, value_cache, device, dtype, write):
     kshape, ks = _heads("key_cache", key_cache, device, dtype, 4, write)
     vshape, vs = _heads("value_cache", value_cache, device, dtype, 4, write)
@@ -325,7 +336,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     queries come back zero.  ``query_out`` may be ``query`` itself, and share no other memory
     with the operands."""
     device, dtype = _operand("key", key, _DTYPES)
-    _no_gradient("paged_append", key, value, query, key_cache, value_cache)
+    _no_gradient("paged_append", key, value, query, key_cache, value_cache, frequency, query_out)
     shape, ks = _heads("key", key, device, dtype, 3)
     vshape, vs = _heads("value", value, device, dtype, 3)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, True)
@@ -392,7 +403,7 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     caches' type for the matrix instructions that weigh the values.  Results do not depend on
     the order in which workgroups run."""
     device, dtype = _operand("query", query, _CACHED)
-    _no_gradient("prefix_attention", query, key_cache, value_cache)
+    _no_gradient("prefix_attention", query, key_cache, value_cache, out)
     shape, qs = _heads("query", query, device, dtype, 3)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, False)
     tokens, heads, dim = shape
