@@ -1129,3 +1129,35 @@ def test_lost_derivatives(hip_ready):
             with pytest.raises(ValueError):
                 call()
         append(), attend()      # a level without tangents among the operands
+
+
+def test_autograd_notices_what_is_written(hip_ready):
+    """Tensors that a backward pass has saved and a call has written since make it fail, as torch's
+    own writes do; inference tensors have no such count."""
+    frequency, _ = at.rope_frequencies(64)
+    pos = torch.arange(2, device="cuda")
+    w = torch.ones(64, device="cuda", dtype=BF16, requires_grad=True)
+    b = Batch(BF16, 4, 2, 64, 16, 32, [20, 9], [1, 1], seed=12).fill()
+
+    def append(**more):
+        at.paged_append(b.key, b.value, b.kc, b.vc, b.indptr, b.indices, b.lengths, frequency,
+                        query=b.query, **more)
+
+    other = torch.zeros_like(b.query)
+    for saved, call in ((b.query, lambda: at.rope(b.query, pos, frequency, out=b.query)),
+                        (other, lambda: at.rope_backward(b.query, pos, frequency, out=other)),
+                        (b.kc, append), (b.vc, append), (other, lambda: append(query_out=other)),
+                        (other, lambda: b.attend(out=other))):
+        loss = (saved * w).sum()
+        call()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            loss.backward()
+    loss = (b.query * w).sum()      # read alone
+    append(), b.attend(), at.rope(b.query, pos, frequency)
+    loss.backward()
+    with torch.inference_mode():
+        made = torch.zeros_like(b.query)
+    at.rope(b.query, pos, frequency, out=made)
+    with torch.inference_mode():
+        at.rope(b.query, pos, frequency, out=made)
+        append(query_out=made)

@@ -142,6 +142,10 @@ def _call(entry, packed: bytes, device: int, what: str) -> None:
         _raise(rc, what)
 
 
+# Tells autograd that the kernels write over tensors that it may have saved.
+_written = torch.autograd.graph.increment_version
+
+
 def _raise(rc: int, what: str) -> None:
     if rc < 0:  # an argument the library refused
         raise ValueError(_rt.last_error())
@@ -191,7 +195,8 @@ def rope_frequencies(rotary: int, base: float = 10000.0, scaling: Optional[str] 
 def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     device, dtype = _operand("x", x, _DTYPES)
     shape, xs = _heads("x", x, device, dtype, 3)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _like(x)
     oshape, ys = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
@@ -203,6 +208,8 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
         heads, dim, 2 * frequency.shape[0], _layout(layout), xs[0], xs[1], ys[0], ys[1],
         magnitude, sign)
     _call(_lib().launch_rope, packed, device, what)
+    if given:
+        _written(out)
     return out
 
 
@@ -347,12 +354,15 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     (p_indptr, p_indices, p_lengths, p_ends), sequences = _table(
         indptr, indices, lengths, query_indptr, tokens, device)
     heads, q, out, qs, os_ = 0, 0, 0, (0, 0), (0, 0)
+    written = (key_cache, value_cache)
     if query is not None:
         qshape, qs = _heads("query", query, device, dtype, 3)
         if qshape[0] != tokens or qshape[2] != dim:
             raise ValueError("query is %s, key %s" % (tuple(qshape), tuple(shape)))
         if query_out is None:
             query_out = _like(query)
+        else:
+            written += (query_out,)
         oshape, os_ = _heads("query_out", query_out, device, dtype, 3, write=True)
         if oshape != qshape:
             raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(qshape)))
@@ -370,6 +380,7 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
         offset, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2],
         vcs[0], vcs[1], vcs[2], magnitude)
     _call(_lib().launch_paged_append, packed, device, "paged_append")
+    _written(written)
     return query_out
 
 
@@ -411,7 +422,8 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
         raise ValueError("query is %s, the caches %s" % (tuple(shape), tuple(cache)))
     (p_indptr, p_indices, p_lengths, p_ends), sequences = _table(
         indptr, indices, lengths, query_indptr, tokens, device)
-    if out is None:
+    given = out is not None
+    if not given:
         out = _like(query)
     oshape, os_ = _heads("out", out, device, dtype, 3, write=True)
     if oshape != shape:
@@ -432,4 +444,6 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
         workspace = query.new_empty(n, dtype=torch.uint8)
         fields[10], fields[11] = workspace.data_ptr(), n
     _call(L.launch_prefix_attention, _ATTENTION.pack(*fields), device, "prefix_attention")
+    if given:
+        _written(out)
     return (out, lse) if return_lse else out
