@@ -1161,3 +1161,21 @@ def test_autograd_notices_what_is_written(hip_ready):
     with torch.inference_mode():
         at.rope(b.query, pos, frequency, out=made)
         append(query_out=made)
+
+
+def test_numbers_that_do_not_fit(hip_ready):
+    """Bounds, offsets and factors that no field of the C structures holds are refused as others
+    are."""
+    frequency, _ = at.rope_frequencies(64)
+    b = Batch(BF16, 4, 2, 64, 16, 32, [20, 9], [1, 1], seed=12).fill()
+    pos = torch.arange(2, device="cuda")
+    for more in (dict(max_length=2 ** 70), dict(max_query=-2 ** 70), dict(max_length=1.5),
+                 dict(scale="one")):
+        with pytest.raises(ValueError):
+            b.attend(**more)
+    for more in (dict(offset=2 ** 64), dict(offset=0.5), dict(magnitude="one")):
+        with pytest.raises(ValueError):
+            at.paged_append(b.key, b.value, b.kc, b.vc, b.indptr, b.indices, b.lengths, frequency,
+                            **more)
+    with pytest.raises(ValueError):
+        at.rope(b.query, pos, frequency, magnitude=None)

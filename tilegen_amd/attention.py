@@ -46,6 +46,15 @@ _ROPE = struct.Struct("4P10qdq")
 _APPEND = struct.Struct("11P26qd")
 _ATTENTION = struct.Struct("11P24qd")
 
+
+def _pack(layout: struct.Struct, *fields) -> bytes:
+    try:
+        return layout.pack(*fields)
+    except struct.error as e:
+        raise ValueError("a size, bound or offset that is no 64-bit whole number, or a factor that "
+                         "is no number: %s" % e) from None
+
+
 _LIB = None
 
 
@@ -202,8 +211,8 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))
     tokens, heads, dim = shape
-    packed = _ROPE.pack(
-        x.data_ptr(), out.data_ptr(), _list("positions", positions, device, tokens),
+    packed = _pack(
+        _ROPE, x.data_ptr(), out.data_ptr(), _list("positions", positions, device, tokens),
         _list("frequency", frequency, device, dtype=torch.float64), _DTYPES[dtype], tokens,
         heads, dim, 2 * frequency.shape[0], _layout(layout), xs[0], xs[1], ys[0], ys[1],
         magnitude, sign)
@@ -373,10 +382,10 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     if frequency is not None:
         p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
         rotary = 2 * frequency.shape[0]
-    packed = _APPEND.pack(
-        key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(), value_cache.data_ptr(), out,
-        p_indptr, p_indices, p_lengths, p_ends, p_frequency, _DTYPES[dtype], tokens, sequences,
-        heads, kv_heads, dim, rotary, _layout(layout), cache[0], cache[1], indices.shape[0],
+    packed = _pack(
+        _APPEND, key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(),
+        value_cache.data_ptr(), out, p_indptr, p_indices, p_lengths, p_ends, p_frequency,
+        _DTYPES[dtype], tokens, sequences, heads, kv_heads, dim, rotary, _layout(layout), cache[0], cache[1], indices.shape[0],
         offset, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2],
         vcs[0], vcs[1], vcs[2], magnitude)
     _call(_lib().launch_paged_append, packed, device, "paged_append")
@@ -437,13 +446,13 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
               os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2],
               dim ** -0.5 if scale is None else scale]
     L = _lib()
-    n = L.prefix_attention_workspace(_ATTENTION.pack(*fields))
+    n = L.prefix_attention_workspace(_pack(_ATTENTION, *fields))
     if n < 0:
         _raise(n, "prefix_attention")
     if n:
         workspace = query.new_empty(n, dtype=torch.uint8)
         fields[10], fields[11] = workspace.data_ptr(), n
-    _call(L.launch_prefix_attention, _ATTENTION.pack(*fields), device, "prefix_attention")
+    _call(L.launch_prefix_attention, _pack(_ATTENTION, *fields), device, "prefix_attention")
     if given:
         _written(out)
     return (out, lse) if return_lse else out
