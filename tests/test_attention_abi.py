@@ -212,3 +212,13 @@ def test_append_over_its_own_operands():
         want = "%s overlaps %s" % (out, other)
         assert message(**change).endswith(want), (change, runtime.last_error())
     assert "null" in message(out=(1 << 20) + 4 * 1024 + 256)    # past the last key's second head
+
+
+def test_more_sequences_than_the_search_can_count():
+    """The search for a token's sequence looks up to 64 steps past the last one, in 32 bits."""
+    L = at._lib()
+    for sequences in ((1 << 31) - 1, (1 << 31) - 64, (1 << 30) + 1):
+        assert L.launch_paged_append(_append_args(sequences=sequences, ends=4096), None) == -1
+        assert "sequences" in runtime.last_error()
+    assert L.launch_paged_append(_append_args(sequences=1 << 30, ends=4096), None) == -1
+    assert "null" in runtime.last_error()

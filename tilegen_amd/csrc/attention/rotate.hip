@@ -13,6 +13,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxDim = 1024;
+constexpr int kMaxSequences = 1 << 30;   // sequence_of's places stay within 32 bits
 constexpr int kMostTokens = 4;   // tokens of one workgroup
 
 struct Rows {
@@ -336,8 +337,8 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_append(const 
     return rc;
   if (r->kv_heads < 1 || r->kv_heads > 0x10000)
     return refuse(-1, what, "kv_heads must be 1 to 65536", r->kv_heads);
-  if (r->sequences < 0 || r->sequences > 0x7FFFFFFF)
-    return refuse(-1, what, "sequences must be 0 to 2^31 - 1", r->sequences);
+  if (r->sequences < 0 || r->sequences > kMaxSequences)
+    return refuse(-1, what, "sequences must be 0 to 2^30", r->sequences);
   if (r->page < 1 || r->page > 0x7FFFFFFF)
     return refuse(-1, what, "page must be 1 to 2^31 - 1", r->page);
   if (r->pages < 0 || r->n_indices < 0) return refuse(-1, what, "negative size", r->pages);
