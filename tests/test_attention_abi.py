@@ -222,3 +222,28 @@ def test_more_sequences_than_the_search_can_count():
         assert "sequences" in runtime.last_error()
     assert L.launch_paged_append(_append_args(sequences=1 << 30, ends=4096), None) == -1
     assert "null" in runtime.last_error()
+
+
+def test_launches_that_hip_would_refuse():
+    """A grid has under 2^32 threads: calls beyond are refused before anything is enqueued, in the
+    parts' launch (here 4096 row tiles of the prefix for each of 32 kv heads beside 2^24 - 32
+    workgroups of own pages) and in the joining's, four rows a workgroup."""
+    L = at._lib()
+    base = dict.fromkeys(("query kc vc prefix indptr indices lengths ends out lse workspace bytes "
+                          "dtype").split(), 0)
+    base.update(tokens=0, sequences=0, heads=32, kv_heads=32, dim=64, pages=999, page=16,
+                n_prefix=200, prefix_length=3200, n_indices=4, max_query=1, max_length=20)
+    base.update({"s%d" % i: 64 for i in range(10)}, scale=0.125)
+
+    def workspace(**change):
+        return L.prefix_attention_workspace(at._ATTENTION.pack(*{**base, **change}.values()))
+
+    many = (1 << 19) - 1
+    assert workspace(tokens=many, sequences=many) < 0
+    assert "workgroups" in runtime.last_error()
+    assert workspace(tokens=many, sequences=many, prefix_length=0) > 0
+    assert workspace(tokens=many - 4096, sequences=many - 4096) > 0
+    rows = dict(ends=4096, sequences=1, heads=16, kv_heads=1, max_query=1 << 22)
+    assert workspace(**rows, tokens=1 << 22) < 0
+    assert "rows" in runtime.last_error()
+    assert workspace(**rows, tokens=(1 << 22) - 1) > 0

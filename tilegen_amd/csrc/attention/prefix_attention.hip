@@ -113,6 +113,7 @@ struct Plan {
 };
 
 constexpr int64_t kWholeElements = 45056;
+constexpr int64_t kMostWorkgroups = 0xFFFFFF;   // of 256 threads: HIP launches under 2^32 threads
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
 
@@ -138,8 +139,8 @@ int check(const tg_prefix_attention* r) {
   if (r->n_prefix < (r->prefix_length + r->page - 1) / r->page)
     return refuse(-1, what, "prefix_length is past the prefix's pages", r->prefix_length);
   if (r->tokens > 0x1000000 || r->sequences > 0x1000000 || r->heads > 0x10000 ||
-      r->tokens * r->heads > 0x4000000)
-    return refuse(-2, what, "more than 2^26 rows or 2^24 sequences", r->tokens);
+      r->tokens * r->heads > 4 * kMostWorkgroups)    // join_parts: 4 rows each
+    return refuse(-2, what, "2^26 rows or more than 2^24 sequences", r->tokens);
   if (!r->query_indptr && r->tokens > r->sequences)
     return refuse(-1, what, "more tokens than sequences without query_indptr", r->tokens);
   return 0;
@@ -250,7 +251,7 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     a.own_splits = static_cast<int>((length + a.own_chunk - 1) / a.own_chunk);
     a.sorted = units > room && a.sequences <= 256;
     own = units * a.own_splits;
-    if (own > 0xFFFFFF) return refuse(-2, what, "more than 2^24 workgroups", own);
+    if (own > kMostWorkgroups) return refuse(-2, what, "2^24 workgroups or more", own);
     own_keys = units * length / 2;
   }
   a.prefix_tiles = static_cast<int>((rows + p->prefix_rows - 1) / p->prefix_rows);
@@ -278,7 +279,8 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     prefix = units * a.prefix_splits;
   }
   a.slots = a.prefix_splits + a.own_splits;
-  if (prefix > 0xFFFFFF) return refuse(-2, what, "more than 2^24 workgroups", prefix);
+  if ((prefix + 7) / 8 + (own + 7) / 8 > kMostWorkgroups / 8)
+    return refuse(-2, what, "2^24 workgroups or more", prefix + own);
   a.prefix_eights = static_cast<int>((prefix + 7) / 8);
   a.own_eights = static_cast<int>((own + 7) / 8);
   p->bytes = static_cast<int64_t>(a.slots) * a.tokens * a.heads * (a.dim + 2) * 4;
@@ -366,7 +368,7 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
     if (e != hipSuccess) return hip_failed(e, what);
   }
   const int64_t rows = static_cast<int64_t>(a.tokens) * a.heads;
-  const bool shared = a.slots > 16;
+  const bool shared = a.slots > 16 && rows <= kMostWorkgroups;
   void* args[] = {&a};
   const hipError_t e = hipLaunchKernel(
       r->dtype == TG_F16 ? join_of<_Float16>(a.dim, shared) : join_of<__bf16>(a.dim, shared),
