@@ -247,3 +247,10 @@ def test_launches_that_hip_would_refuse():
     assert workspace(**rows, tokens=1 << 22) < 0
     assert "rows" in runtime.last_error()
     assert workspace(**rows, tokens=(1 << 22) - 1) > 0
+
+
+def test_scales_that_are_0_in_32_bits():
+    L = at._lib()
+    base = [0] * 12 + [0, 2, 2, 4, 2, 64, 999, 16, 200, 3200, 4, 1, 20] + [64] * 10
+    for scale, fine in ((1e-46, False), (5e-324, False), (1e-44, True), (1.0, True)):
+        assert (L.prefix_attention_workspace(at._ATTENTION.pack(*base, scale)) > 0) == fine, scale

@@ -131,7 +131,8 @@ int check(const tg_prefix_attention* r) {
     return refuse(-1, what, "heads must be a multiple of kv_heads", r->heads);
   if (r->page < 1 || r->page > INT32_MAX)
     return refuse(-1, what, "page must be 1 to 2^31 - 1", r->page);
-  if (!(r->scale > 0) || !(r->scale < 1e30))
+  // (in 32 bits: 0 times the -inf of a hidden score would be NaN)
+  if (!(r->scale > 0) || !(r->scale < 1e30) || static_cast<float>(r->scale) == 0.f)
     return refuse(-1, what, "scale must be positive and finite", 0);
   if (r->prefix_length > INT32_MAX / 2 || r->max_length > INT32_MAX / 2)
     return refuse(-2, what, "more than 2^30 keys", r->prefix_length);
