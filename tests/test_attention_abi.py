@@ -254,3 +254,41 @@ def test_scales_that_are_0_in_32_bits():
     base = [0] * 12 + [0, 2, 2, 4, 2, 64, 999, 16, 200, 3200, 4, 1, 20] + [64] * 10
     for scale, fine in ((1e-46, False), (5e-324, False), (1e-44, True), (1.0, True)):
         assert (L.prefix_attention_workspace(at._ATTENTION.pack(*base, scale)) > 0) == fine, scale
+
+
+def test_plans_and_launches_go_by_the_operands_device(monkeypatch):
+    """The workspace's size and the launch are asked for with the operands' device current,
+    whichever was before (a stand-in library; host tensors count as device -1)."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.device
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def prefix_attention_workspace(self, packed):
+            seen.append(("workspace", current[0]))
+            return 64
+
+        def launch_prefix_attention(self, packed, stream):
+            seen.append(("launch", current[0], stream))
+            return 0
+
+    monkeypatch.setattr(at, "_lib", Library)
+    monkeypatch.setattr(at, "_operand", lambda name, t, dtypes: (t.get_device(), t.dtype))
+    monkeypatch.setattr(at, "_raw_stream", lambda device: 1000 + device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    q = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    cache = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16)
+    n = torch.zeros(3, dtype=torch.int64)
+    for current[0] in (0, -1):
+        seen.clear()
+        at.prefix_attention(q, cache, cache, n, 0, n, n, n[:2], max_length=1)
+        assert seen == [("workspace", -1), ("launch", -1, 999)]

@@ -141,12 +141,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
-def _call(entry, packed: bytes, device: int, what: str) -> None:
+def _on(device: int, entry, *args) -> int:
+    """A C entry with the operands' device current: it launches there, and plans for its units."""
     if device == torch.cuda.current_device():
-        rc = entry(packed, _raw_stream(device))
-    else:
-        with torch.cuda.device(device):
-            rc = entry(packed, _raw_stream(device))
+        return entry(*args)
+    with torch.cuda.device(device):
+        return entry(*args)
+
+
+def _call(entry, packed: bytes, device: int, what: str) -> None:
+    rc = _on(device, entry, packed, _raw_stream(device))
     if rc:
         _raise(rc, what)
 
@@ -446,7 +450,7 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
               os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2],
               dim ** -0.5 if scale is None else scale]
     L = _lib()
-    n = L.prefix_attention_workspace(_pack(_ATTENTION, *fields))
+    n = _on(device, L.prefix_attention_workspace, _pack(_ATTENTION, *fields))
     if n < 0:
         _raise(n, "prefix_attention")
     if n:
