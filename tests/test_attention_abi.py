@@ -292,3 +292,11 @@ def test_plans_and_launches_go_by_the_operands_device(monkeypatch):
         seen.clear()
         at.prefix_attention(q, cache, cache, n, 0, n, n, n[:2], max_length=1)
         assert seen == [("workspace", -1), ("launch", -1, 999)]
+
+
+def test_paged_decode_refuses_what_it_cannot_run():
+    """Before it asks for a device."""
+    from tilegen_amd import paged_decode
+    for sizes in (dict(sequences=0), dict(start=0), dict(prompt=-1), dict(steps=-1)):
+        with pytest.raises(ValueError, match=list(sizes)[0]):
+            paged_decode.run(**sizes)

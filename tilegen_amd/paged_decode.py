@@ -64,6 +64,10 @@ def run(sequences: int = 32, prompt: int = 8192, steps: int = 64, heads: int = 3
     """Decodes ``steps`` tokens for each sequence after first answers of 1 to ``start`` tokens;
     {"us_per_step"} and, with ``keep``, what went in and came out: the prompt's keys and values, the
     first answers' counts, and every call's (query, key, value, result), none rotated."""
+    for name, n, least in (("sequences", sequences, 1), ("start", start, 1), ("prompt", prompt, 0),
+                           ("steps", steps, 0)):
+        if n < least:
+            raise ValueError("%s is %d, expected at least %d" % (name, n, least))
     dtype = torch.bfloat16
     g = torch.Generator(device="cuda")
     g.manual_seed(seed)
