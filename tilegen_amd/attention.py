@@ -47,12 +47,9 @@ _APPEND = struct.Struct("11P26qd")
 _ATTENTION = struct.Struct("11P24qd")
 
 
-def _pack(layout: struct.Struct, *fields) -> bytes:
-    try:
-        return layout.pack(*fields)
-    except struct.error as e:
-        raise ValueError("a size, bound or offset that is no 64-bit whole number, or a factor that "
-                         "is no number: %s" % e) from None
+def _unfit(e: struct.error) -> ValueError:
+    return ValueError("a size, bound or offset that is no 64-bit whole number, or a factor that is "
+                      "no number: %s" % e)
 
 
 _LIB = None
@@ -215,11 +212,14 @@ def _turn(x, positions, frequency, layout, magnitude, out, sign, what):
     if oshape != shape:
         raise ValueError("out is %s, expected %s" % (tuple(oshape), tuple(shape)))
     tokens, heads, dim = shape
-    packed = _pack(
-        _ROPE, x.data_ptr(), out.data_ptr(), _list("positions", positions, device, tokens),
-        _list("frequency", frequency, device, dtype=torch.float64), _DTYPES[dtype], tokens,
-        heads, dim, 2 * frequency.shape[0], _layout(layout), xs[0], xs[1], ys[0], ys[1],
-        magnitude, sign)
+    try:
+        packed = _ROPE.pack(
+            x.data_ptr(), out.data_ptr(), _list("positions", positions, device, tokens),
+            _list("frequency", frequency, device, dtype=torch.float64), _DTYPES[dtype], tokens,
+            heads, dim, 2 * frequency.shape[0], _layout(layout), xs[0], xs[1], ys[0], ys[1],
+            magnitude, sign)
+    except struct.error as e:
+        raise _unfit(e) from None
     _call(_lib().launch_rope, packed, device, what)
     if given:
         _written(out)
@@ -281,12 +281,15 @@ class _Rope(torch.autograd.Function):
 
 
 def _linear(x, positions, frequency, layout, magnitude, out, sign, what):
-    if isinstance(x, torch.Tensor) and _followed(x):
-        if out is not None:
-            raise ValueError("out cannot be given where x needs a gradient")
-        _no_gradient(what, frequency)
-        return _Rope.apply(x, positions, frequency, layout, magnitude, sign)
-    _no_gradient(what, frequency, out)
+    forward = _forward._current_level >= 0
+    if getattr(x, "requires_grad", False) or forward:
+        if _followed(x):
+            if out is not None:
+                raise ValueError("out cannot be given where x needs a gradient")
+            _no_gradient(what, frequency)
+            return _Rope.apply(x, positions, frequency, layout, magnitude, sign)
+    if frequency.requires_grad or out is not None or forward:
+        _no_gradient(what, frequency, out)
     return _turn(x, positions, frequency, layout, magnitude, out, sign, what)
 
 
@@ -386,12 +389,15 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     if frequency is not None:
         p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
         rotary = 2 * frequency.shape[0]
-    packed = _pack(
-        _APPEND, key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(),
-        value_cache.data_ptr(), out, p_indptr, p_indices, p_lengths, p_ends, p_frequency,
-        _DTYPES[dtype], tokens, sequences, heads, kv_heads, dim, rotary, _layout(layout), cache[0], cache[1], indices.shape[0],
-        offset, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2],
-        vcs[0], vcs[1], vcs[2], magnitude)
+    try:
+        packed = _APPEND.pack(
+            key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(), value_cache.data_ptr(), out,
+            p_indptr, p_indices, p_lengths, p_ends, p_frequency, _DTYPES[dtype], tokens, sequences,
+            heads, kv_heads, dim, rotary, _layout(layout), cache[0], cache[1], indices.shape[0],
+            offset, ks[0], ks[1], vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1],
+            kcs[2], vcs[0], vcs[1], vcs[2], magnitude)
+    except struct.error as e:
+        raise _unfit(e) from None
     _call(_lib().launch_paged_append, packed, device, "paged_append")
     _written(written)
     return query_out
@@ -401,6 +407,19 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
 # attention
 # --------------------------------------------------------------------------- #
 _CACHED = (torch.bfloat16, torch.float16)
+
+
+def _attend(query, fields, packed: bytes, device: int) -> int:
+    """Plans and launches with the device current, the workspace from torch."""
+    L = _lib()
+    n = L.prefix_attention_workspace(packed)
+    if n < 0:
+        return n
+    if n:
+        workspace = query.new_empty(n, dtype=torch.uint8)
+        fields[10], fields[11] = workspace.data_ptr(), n
+        packed = _ATTENTION.pack(*fields)
+    return L.launch_prefix_attention(packed, _raw_stream(device))
 
 
 def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
@@ -418,9 +437,9 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     ``scale`` is 1 / sqrt(dim) by default.  ``max_query`` and ``max_length`` bound the new tokens
     and the length of a sequence: they size the launch (larger ones on the device are still
     right, only slower).  A row that sees no key (or scores of -inf alone), or belongs to no
-    sequence, gives 0; what hidden keys and values hold does not matter.  With ``return_lse`` also each row's logarithm of
-    the sum of its exponentials, float32 [tokens, heads] (-inf for such a row), by which results
-    over disjoint keys can be joined.  ``out`` may be the query, and share no other memory with
+    sequence, gives 0; what hidden keys and values hold does not matter.  With ``return_lse``
+    also each row's logarithm of the sum of its exponentials, float32 [tokens, heads] (-inf for
+    such a row), by which results over disjoint keys can be joined.  ``out`` may be the query, and share no other memory with
     the operands.
 
     Scores, probabilities and sums are held in 32 bits; probabilities are rounded to the
@@ -449,14 +468,13 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
               prefix_length, indices.shape[0], max_query, max_length, qs[0], qs[1], os_[0],
               os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2],
               dim ** -0.5 if scale is None else scale]
-    L = _lib()
-    n = _on(device, L.prefix_attention_workspace, _pack(_ATTENTION, *fields))
-    if n < 0:
-        _raise(n, "prefix_attention")
-    if n:
-        workspace = query.new_empty(n, dtype=torch.uint8)
-        fields[10], fields[11] = workspace.data_ptr(), n
-    _call(L.launch_prefix_attention, _pack(_ATTENTION, *fields), device, "prefix_attention")
+    try:
+        packed = _ATTENTION.pack(*fields)
+    except struct.error as e:
+        raise _unfit(e) from None
+    rc = _on(device, _attend, query, fields, packed, device)
+    if rc:
+        _raise(rc, "prefix_attention")
     if given:
         _written(out)
     return (out, lse) if return_lse else out

@@ -168,9 +168,25 @@ class Sharing {
   bool empty_;
 };
 
+// Whether the spans of their addresses meet, which mostly settles it (and costs the host little).
+inline bool meet(const Operand& x, const Operand& y, int bytes) {
+  auto reach = [&](const Operand& o, __int128* from, __int128* to) {
+    *from = *to = static_cast<__int128>(reinterpret_cast<uintptr_t>(o.at));
+    for (int i = 0; i < o.axes; ++i) {
+      const __int128 far = static_cast<__int128>(o.size[i] - 1) * o.stride[i] * bytes;
+      *(far < 0 ? from : to) += far;
+    }
+    *to += bytes;
+  };
+  __int128 x0, x1, y0, y1;
+  reach(x, &x0, &x1);
+  reach(y, &y0, &y1);
+  return x0 < y1 && y0 < x1;
+}
+
 // Refuses an output that shares memory with another operand.
 inline int apart(const char* what, const Operand& out, const Operand& x, int bytes) {
-  if (!Sharing(out, x, bytes)()) return 0;
+  if (!meet(out, x, bytes) || !Sharing(out, x, bytes)()) return 0;
   char msg[256];
   std::snprintf(msg, sizeof(msg), "%s: %s overlaps %s", what, out.name, x.name);
   return tg_fail(-1, msg);
