@@ -300,3 +300,38 @@ def test_paged_decode_refuses_what_it_cannot_run():
     for sizes in (dict(sequences=0), dict(start=0), dict(prompt=-1), dict(steps=-1)):
         with pytest.raises(ValueError, match=list(sizes)[0]):
             paged_decode.run(**sizes)
+
+
+# (head size, rows of a prefix workgroup, of an own pages' one): bytes of scratch a lane, vector
+# registers spilled.  The first reserves its bytes and touches none.
+SPILLS = {(64, 128, 16): (68, 0), (128, 128, 128): (184, 45), (256, 128, 128): (336, 111)}
+
+
+def test_kernels_that_spill(tmp_path):
+    """Kernels keep their values in registers, but for those listed, and those to that extent.
+    (Scalar registers go to lanes of vector registers, not to memory.)"""
+    readelf = "/opt/rocm/llvm/bin/llvm-readelf"
+    if not os.path.exists(readelf):
+        pytest.skip("llvm-readelf not available")
+    found, most = 0, {}
+    for co in build.attention_code_objects(str(tmp_path)):
+        notes = subprocess.run([readelf, "--notes", co], capture_output=True, text=True,
+                               check=True).stdout
+        for k in re.split(r"\n\s+- \.", notes):
+            name = re.search(r"\.name:\s+(\S+)", k)
+            if not name or ".vgpr_spill_count" not in k:
+                continue
+            used = tuple(int(re.search(r"\.%s:\s+(\d+)" % f, k).group(1))
+                         for f in ("private_segment_fixed_size", "vgpr_spill_count"))
+            sizes = re.search(r"6attend\w*?Li(\d+)ELi(\d+)ELi(\d+)E", name.group(1))
+            at_most = SPILLS.get(tuple(map(int, sizes.groups()))) if sizes else None
+            at_most = at_most or (0, 0)
+            assert used[0] <= at_most[0] and used[1] <= at_most[1], (name.group(1), used)
+            found += 1
+            if at_most != (0, 0):
+                key = tuple(map(int, sizes.groups()))
+                most[key] = max(most.get(key, (0, 0)), used)
+    # attend by prefix and own rows and attend_whole for 4 head sizes and 2 types; joins of 3 widths
+    # for 2 types, in one wave and four; rotations by type, layout, whole chunks, append
+    assert found == 4 * 8 + 12 + 24
+    assert most == SPILLS       # a list that is out of date says so

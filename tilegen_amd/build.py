@@ -175,6 +175,19 @@ def build_attention() -> str:
     return out
 
 
+def attention_code_objects(out_dir: str) -> List[str]:
+    """libtgattn's device code objects alone (the same sources and flags as the library, device
+    pass only), for checks of their kernels' registers and spills."""
+    def one(source: str) -> str:
+        out = os.path.join(out_dir, os.path.basename(source)[:-len(".hip")] + ".co")
+        _run(_attention_compile(source) +
+             ["--offload-device-only", "--no-gpu-bundle-output", "-o", out])
+        return out
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        return list(pool.map(one, attention_sources()))
+
+
 def build_oracle(force: bool = False) -> None:
     _run(["make", "-s"] + (["-B"] if force else []) + ["-C", os.path.join(REPO, "oracle")])
 
