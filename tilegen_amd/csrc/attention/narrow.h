@@ -176,7 +176,7 @@ __device__ __forceinline__ void narrow_part(const Attention& a, const Part& p, i
     float top = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])),
                       fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
     top *= a.scale;
-    if (__any(top - m > kSlack + M::kLift)) {
+    if (__any(passes<T>(top, m))) {
       const float now = fmaxf(base_of<T>(row_max(top)), m);
       const float f = m == -INFINITY ? 0.f : exp2f(m - now);
       m = now;

@@ -263,7 +263,7 @@ __device__ __forceinline__ void wide_part(const Attention& a, const Part& p, int
   // lets the running maximum follow where a row's scores have left it far behind
   auto follow = [&](float top) {
     top *= a.scale;
-    if (__any(top - m > kSlack + M::kLift)) {
+    if (__any(passes<T>(top, m))) {
       const Both both = halves(top);
       const float to = fmaxf(base_of<T>(fmaxf(both.a, both.b)), m);
       const float f = m == -INFINITY ? 0.f : exp2f(m - to);
