@@ -11,8 +11,8 @@ Operands are torch tensors on one HIP device, bfloat16 or float16 (``rope`` and
 ``paged_append`` float32 too); any strides whose heads are contiguous.  Kernels are enqueued on
 torch's current stream of that device and nothing waits for them.  Calls that the kernels
 cannot serve raise ``ValueError`` before anything is enqueued, ones that autograd would have to
-follow among them (``rope`` alone has a backward pass); HIP's own failures raise
-``TileGenHipError``.  The C ABI below is ``include/tilegen_attention.h`` (``libtgattn.so``); it
+follow among them (``rope`` and ``rope_backward`` alone have a backward pass); HIP's own failures
+raise ``TileGenHipError``.  The C ABI below is ``include/tilegen_attention.h`` (``libtgattn.so``); it
 allocates nothing, and may be captured into a graph like the calls here.
 
     frequency, magnitude = rope_frequencies(128, scaling="yarn", factor=32, trained=4096)
@@ -439,8 +439,8 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     right, only slower).  A row that sees no key (or scores of -inf alone), or belongs to no
     sequence, gives 0; what hidden keys and values hold does not matter.  With ``return_lse``
     also each row's logarithm of the sum of its exponentials, float32 [tokens, heads] (-inf for
-    such a row), by which results over disjoint keys can be joined.  ``out`` may be the query, and share no other memory with
-    the operands.
+    such a row), by which results over disjoint keys can be joined.  ``out`` may be the query,
+    and share no other memory with the operands.
 
     Scores, probabilities and sums are held in 32 bits; probabilities are rounded to the
     caches' type for the matrix instructions that weigh the values.  Results do not depend on

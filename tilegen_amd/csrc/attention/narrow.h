@@ -10,14 +10,15 @@
 //
 // The running maximum of a row follows the scores only when they pass it by 2^8: until then
 // probabilities are up to 256 times too large (in float16 another 128 times, base_of), sums and
-// products as well, and their quotient is the same.  So most tiles need neither the exchange between lanes nor the rescaling.
+// products as well, and their quotient is the same.  So most tiles need neither the exchange
+// between lanes nor the rescaling.
 //
 // Memory bounds it: 16 rows are half a matrix instruction's worth of work for the bytes read.
 // Keys go straight to registers (the A operand is 16 bytes of a key a lane), the next tile's
 // while this one's values go through LDS, and page numbers are asked for a tile earlier still.
-// 128 sequences of 1 to 2048 own keys, 8 kv heads of 128 (540 MB): 138 us, 3.9 TB/s with the
-// joining; a plain sum of as much reaches 5.7.  Tiles through an LDS ring with one wave a
-// workgroup took 145 to 155, loads that bypass the caches 161.
+// 128 sequences of 1 to 2048 own keys, 8 kv heads of 128 (540 MB): 135 us, 4.0 TB/s with the
+// joining; a plain sum of as much reaches 5.7.  When it took 138, tiles through an LDS ring with
+// one wave a workgroup took 145 to 155, loads that bypass the caches 161.
 #pragma once
 
 #include "parts.h"

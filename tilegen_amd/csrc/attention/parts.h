@@ -87,18 +87,18 @@ __device__ __forceinline__ float apart(float s, float scale, float base) {
 
 // What a row's probabilities are taken against: its largest score, 2^kLift down, so that the
 // largest probability is 2^kLift, and 2^(kLift + kSlack) before the maximum follows, 2^15 in
-// float16.  The factor is in sums and products alike.  It keeps probabilities down to 2^-32 of the
-// largest apart from 0 where float16 by itself ends at 2^-25: on long prefixes what is below counts
-// (131071 keys 18 nats under one have 0.2% of the weight).  Past kHuge differences are whole and the
-// lift would be rounded.
+// float16.  The factor is in sums and products alike.  It keeps probabilities down to 2^-32 of
+// the largest apart from 0 where float16 by itself ends at 2^-25: on long prefixes what is below
+// counts (131071 keys 18 nats under one have 0.2% of the weight).  Past kHuge differences are
+// whole and the lift would be rounded.
 template <typename T>
 __device__ __forceinline__ float base_of(float top) {
   return fabsf(top) > kHuge ? top : top - Matrix<T>::kLift;
 }
 // Whether the maximum has to follow `top`.  Past 2^27 neighbouring scores are 16 apart, and a sum
-// would round up to the next one and leave a probability of 2^16: bfloat16 holds it, float16 does not
-// and compares the difference, which is exact for neighbours (in bfloat16 that costs heads of 256
-// up to 4%, 262 us for 253: 2 prompts of up to 2048 tokens, 16 heads).
+// would round up to the next one and leave a probability of 2^16: bfloat16 holds it, float16 does
+// not and compares the difference, which is exact for neighbours (in bfloat16 that costs heads of
+// 256 up to 4%, 262 us for 253: 2 prompts of up to 2048 tokens, 16 heads).
 template <typename T>
 __device__ __forceinline__ bool passes(float top, float base) {
   if constexpr (Matrix<T>::kLift > 0.f) return top - base > kSlack + Matrix<T>::kLift;

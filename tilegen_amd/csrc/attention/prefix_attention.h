@@ -14,7 +14,7 @@ struct Attention {
   void* out;
   float* lse;
   float* part;        // [slots, tokens * heads, dim]: each part's sums, not yet divided
-  float2* part_ml;    // [slots, tokens * heads]: its largest score (times log2 e) and its sum
+  float2* part_ml;    // [slots, tokens * heads]: what its exponents are taken against, and its sum
   i64 q_token, q_head, o_token, o_head;
   i64 kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head;
   i64 pages, n_indices;

@@ -242,7 +242,9 @@ int plan(const tg_prefix_attention* r, Plan* p) {
     // ones are cut in any case, into three parts or more: 48 sequences, 8 kv heads, 4000 keys: 111
     // us, 161 without; 1800 keys: 60 and 80; but 1500 keys in two 62 to 85, 69 to 78 without.
     // More than run at once go in order of length instead, and cutting them costs: 128
-    // sequences, 8 kv heads, 2048 keys: 138 us, 149 in three.
+    // sequences, 8 kv heads, 2048 keys: 138 us, 149 in three.  The order is for at most 256
+    // sequences, one a thread (own_place): 128 of them 135 us, 152 as they come; 256 248 and 269;
+    // 257, which go as they come, 274.
     int64_t splits = (p->own_rows == 16 ? room / 2 : room) / units;
     if (p->own_rows == 16 && units <= room && length > 1536 && splits < (length + 767) / 768)
       splits = (length + 767) / 768;

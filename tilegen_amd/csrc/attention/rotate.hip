@@ -4,8 +4,8 @@
 // Memory bounds it: every value is read and written once, in 16-byte units, and the cosines and
 // sines are computed once a token for all its heads.  16384 tokens of 40 heads of 128 in
 // bfloat16 (336 MB) take 59 us, 5.7 TB/s; an append of 16384 tokens with their queries (403 MB)
-// 79, 5.1 TB/s; a plain copy of 1 GiB reaches 4.8.  8 tokens take 3.0 us, an append of 32 with its
-// page lookups 4.2: the latency of the loads that follow from one another.
+// 75 to 79, 5.1 to 5.4 TB/s; a plain copy of 1 GiB reaches 4.8.  8 tokens take 3.2 us, an append of
+// 32 with its page lookups 4.1: the latency of the loads that follow from one another.
 #include "attention.h"
 
 namespace tg {

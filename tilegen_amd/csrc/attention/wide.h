@@ -3,18 +3,20 @@
 //
 // As in the narrow kernel scores are computed transposed, here on 32x32x16 instructions: a lane
 // holds, for query row lane % 32, keys 8 i + 4 (lane / 32) + 0..3 of each 32, and the
-// probabilities of 16 keys are a B operand of O^T = V^T P^T when the sum over the keys runs in that
-// order.  Tiles are double-buffered: the next one's loads are in flight while this one is
-// multiplied, and one barrier a tile separates the buffers.
+// probabilities of 16 keys are a B operand of O^T = V^T P^T when the sum over the keys runs in
+// that order.  Tiles are double-buffered, and one barrier a tile separates the buffers.  Loads
+// run a tile ahead, but only while scores are taken: the transposing reads of values might read
+// what the loads write for all that the compiler knows, so it waits for every load before the
+// first of them and not at the barrier alone.
 //
-// A 32x32x16 product takes 32 cycles of a SIMD's matrix core and reads 1 KB of keys or values from
-// LDS, so four waves ask for LDS's 128 bytes a cycle and the softmax of a tile takes as
-// many vector cycles as its products take matrix cycles.  So the next tile's scores are computed
-// while this one's probabilities are, instruction by instruction (side_by_side), and two
-// workgroups share a CU.  1024 rows of each of 8 kv heads of 128 on 32768 keys (137 GFLOP):
-// 187 us, 735 TFLOP/s; a plain product of 8192^3 reaches 1330.  64 rows a wave (half the LDS
-// reads, one wave a SIMD) took 1.8 times as long; eight waves and 256 rows a workgroup as long
-// for the prefix and 8% longer beside own pages.
+// A 32x32x16 product takes 32 cycles of a SIMD's matrix core and reads 1 KB of keys or values
+// from LDS, so four waves ask for LDS's 128 bytes a cycle, the loads' writes for a quarter more,
+// and the softmax of a tile takes as many vector cycles as its products take matrix cycles.  So
+// the next tile's scores are computed while this one's probabilities are, instruction by
+// instruction (side_by_side), and two workgroups share a CU.  1024 rows of each of 8 kv heads of
+// 128 on 32768 keys (137 GFLOP): 187 to 200 us, 690 to 735 TFLOP/s; a plain product of 8192^3
+// reaches 1330.  64 rows a wave (half the LDS reads, one wave a SIMD) took 1.8 times as long;
+// eight waves and 256 rows a workgroup as long for the prefix and 8% longer beside own pages.
 #pragma once
 
 #include <type_traits>
