@@ -12,7 +12,7 @@
  *                            prefix's pages and each sequence's own
  *
  * Every pointer is a device pointer of the caller's; nothing is allocated.  Strides count
- * elements; the elements of a head are contiguous.  dtype is 0 (bfloat16), 1 (float16) or 2
+ * elements; the elements of a head are contiguous, and no two of an output share memory.  dtype is 0 (bfloat16), 1 (float16) or 2
  * (float32).  Structures hold 8-byte fields only, so that a binding packs them flat.
  *
  * Returns 0 on success, -1 for a bad argument, -2 for a size beyond one launch, or a hipError_t;

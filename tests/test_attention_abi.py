@@ -335,3 +335,33 @@ def test_kernels_that_spill(tmp_path):
     # for 2 types, in one wave and four; rotations by type, layout, whole chunks, append
     assert found == 4 * 8 + 12 + 24
     assert most == SPILLS       # a list that is out of date says so
+
+
+def test_outputs_whose_elements_share_memory():
+    """Refused whatever the strides are that make them; layouts that only interleave are not.
+    (Null arrays end the calls that pass.)"""
+    L = at._lib()
+
+    def append(**change):
+        assert L.launch_paged_append(_append_args(**change), None) == -1
+        return runtime.last_error()
+
+    def rope(token, head, tokens=5, heads=4, dim=64):
+        args = at._ROPE.pack(0, 1 << 20, 0, 0, 0, tokens, heads, dim, 0, 0, 0, 0, token, head, 1.0, 1)
+        assert L.launch_rope(args, None) == -1
+        return runtime.last_error()
+
+    for fine in (dict(), dict(out_token=64, out_head=320), dict(kc_page=64, kc_slot=18 * 64,
+                                                                kc_head=9 * 64)):
+        assert "null" in append(**fine), fine
+    for change, name in [(dict(out_head=32), "query_out"), (dict(out_head=0), "query_out"),
+                         (dict(out_token=192), "query_out"), (dict(out_head=63), "query_out"),
+                         (dict(out_token=-192), "query_out"), (dict(kc_page=0), "key_cache"),
+                         (dict(vc_slot=64), "value_cache"), (dict(vc_page=2047), "value_cache")]:
+        assert name + " is written" in append(**change), change
+    assert "null" in rope(256, 64) and "null" in rope(64, 320) and "null" in rope(0, 64, tokens=1)
+    # 2 heads 64 and 160 apart under 2 tokens; three tokens 4 apart are one step of heads 6 apart
+    # twice, but there have to be four tokens for it
+    assert "share" in rope(96, 64, tokens=2, heads=2) and "null" in rope(64, 160, tokens=2, heads=2)
+    assert "share" in rope(4, 6, tokens=4, heads=3, dim=2) and "null" in rope(
+        4, 6, tokens=3, heads=3, dim=2)

@@ -184,6 +184,66 @@ inline bool meet(const Operand& x, const Operand& y, int bytes) {
   return x0 < y1 && y0 < x1;
 }
 
+// Whether two elements of one operand stand in the same place: whether steps along its axes, not
+// all 0, lead back.  An axis that lies inside the next one's stride settles it for all before.
+class Repeating {
+ public:
+  explicit Repeating(const Operand& x) {
+    for (int i = 0; i < x.axes; ++i) {
+      if (x.size[i] < 1) empty_ = true;
+      if (x.size[i] < 2) continue;
+      const Wide stride = x.stride[i] < 0 ? -static_cast<Wide>(x.stride[i]) : x.stride[i];
+      int at = n_++;      // the shortest first
+      for (; at && stride_[at - 1] > stride; --at) {
+        stride_[at] = stride_[at - 1];
+        last_[at] = last_[at - 1];
+      }
+      stride_[at] = stride;
+      last_[at] = x.size[i] - 1;
+    }
+  }
+  bool operator()() {
+    if (empty_) return false;
+    Wide span = 0;      // of the axes below i
+    for (int i = 0; i < n_; ++i) {
+      if (stride_[i] <= span)
+        for (Wide k = 1; k <= last_[i] && k * stride_[i] <= span; ++k) {
+          if (++trials_ > 16384 || back(i - 1, span, k * stride_[i])) return true;
+        }
+      if (stride_[i] == 0) return true;
+      span += stride_[i] * last_[i];
+    }
+    return false;
+  }
+
+ private:
+  using Wide = __int128;
+  // whether steps along axes 0 .. i, which reach `span` to either side, make up `left`
+  bool back(int i, Wide span, Wide left) {
+    if (left == 0) return true;
+    if (i < 0 || left > span || -left > span) return false;
+    const Wide below = span - stride_[i] * last_[i];
+    for (Wide k = -last_[i]; k <= last_[i]; ++k) {
+      const Wide rest = left - k * stride_[i];
+      if (rest > below || -rest > below) continue;
+      if (++trials_ > 16384 || back(i - 1, below, rest)) return true;
+    }
+    return false;
+  }
+  Wide stride_[4], last_[4];
+  int n_ = 0, trials_ = 0;
+  bool empty_ = false;
+};
+
+// Refuses an output whose own elements share memory.
+inline int once(const char* what, const Operand& out) {
+  if (!Repeating(out)()) return 0;
+  char msg[256];
+  std::snprintf(msg, sizeof(msg), "%s: %s is written, but its elements share memory", what,
+                out.name);
+  return tg_fail(-1, msg);
+}
+
 // Refuses an output that shares memory with another operand.
 inline int apart(const char* what, const Operand& out, const Operand& x, int bytes) {
   if (!meet(out, x, bytes) || !Sharing(out, x, bytes)()) return 0;

@@ -352,6 +352,7 @@ extern "C" __attribute__((visibility("default"))) int launch_prefix_attention(
                       {r->kc_page, r->kc_slot, r->kc_head, 1}};
   const Operand vc = {"value_cache", r->value_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
                       {r->vc_page, r->vc_slot, r->vc_head, 1}};
+  if (const int rc = once(what, out)) return rc;
   if (!same(out, query))
     if (const int rc = apart(what, out, query, 2)) return rc;
   for (const Operand* x : {&kc, &vc})

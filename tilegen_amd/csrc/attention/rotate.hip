@@ -307,6 +307,7 @@ extern "C" __attribute__((visibility("default"))) int launch_rope(const tg_rope*
   if (r->tokens == 0 || r->heads == 0) return 0;
   const Operand x = {"x", r->x, 3, {r->tokens, r->heads, r->dim}, {r->x_token, r->x_head, 1}};
   const Operand y = {"out", r->y, 3, {r->tokens, r->heads, r->dim}, {r->y_token, r->y_head, 1}};
+  if (const int rc = once(what, y)) return rc;
   if (!same(y, x))
     if (const int rc = apart(what, y, x, r->dtype == TG_F32 ? 4 : 2)) return rc;
   if (!r->x || !r->y || !r->positions || (r->rotary && !r->frequency))
@@ -361,7 +362,10 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_append(const 
   const Operand vc = {"value_cache", r->value_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
                       {r->vc_page, r->vc_slot, r->vc_head, 1}};
   const int bytes = r->dtype == TG_F32 ? 4 : 2;
+  for (const Operand* x : {&kc, &vc})
+    if (const int rc = once(what, *x)) return rc;
   if (r->heads) {
+    if (const int rc = once(what, out)) return rc;
     if (!same(out, query))
       if (const int rc = apart(what, out, query, bytes)) return rc;
     for (const Operand* x : {&key, &value, &kc, &vc})
