@@ -1,5 +1,7 @@
-"""Attention over a paged cache whose page table is CSR: rotary positions, appending to the
-cache, and attention of a batch whose sequences share a prefix.
+"""Attention over a paged cache whose page table is CSR: rotary positions, with norms of the
+heads or without, appending to the cache, attention of a batch whose sequences share a prefix,
+and, for a cache of bounded length, the attention weight of its keys and the eviction of all but
+the heaviest.
 
 ``sddmm`` and ``spmm`` are the two products of attention over a CSR pattern; a served model's
 pattern is its page table.  Sequence b's pages are ``indices[indptr[b]:indptr[b + 1]]``, int64
@@ -11,9 +13,10 @@ Operands are torch tensors on one HIP device, bfloat16 or float16 (``rope`` and
 ``paged_append`` float32 too); any strides whose heads are contiguous.  Kernels are enqueued on
 torch's current stream of that device and nothing waits for them.  Calls that the kernels
 cannot serve raise ``ValueError`` before anything is enqueued, ones that autograd would have to
-follow among them (``rope`` and ``rope_backward`` alone have a backward pass); HIP's own failures
-raise ``TileGenHipError``.  The C ABI below is ``include/tilegen_attention.h`` (``libtgattn.so``); it
-allocates nothing, and may be captured into a graph like the calls here.
+follow among them (``rope``, ``rope_backward`` and ``norm_rope`` alone have a backward pass); HIP's
+own failures raise ``TileGenHipError``.  The C ABI below is ``include/tilegen_attention.h``
+(``libtgattn.so``) and ``include/tilegen_cache.h`` (``libtgcache.so``); it allocates nothing, and may
+be captured into a graph like the calls here.
 
     frequency, magnitude = rope_frequencies(128, scaling="yarn", factor=32, trained=4096)
     lengths += 1                              # of each sequence's own pages, new token included
@@ -21,6 +24,19 @@ allocates nothing, and may be captured into a graph like the calls here.
                      query=q, offset=prefix_length, magnitude=magnitude)
     o = prefix_attention(q, key_cache, value_cache, prefix, prefix_length, indptr, indices,
                          lengths, max_length=1024)
+
+A cache of bounded length: ``shift`` counts the tokens that each sequence has lost, ``weights``
+[pages, page, kv_heads] holds what each key has received.
+
+    q = paged_append(k, v, key_cache, value_cache, indptr, indices, lengths, frequency, query=q,
+                     query_weight=wq, key_weight=wk, epsilon=1e-6, shift=shift)
+    o, lse = prefix_attention(q, key_cache, value_cache, prefix, prefix_length, indptr, indices,
+                              lengths, max_length=1088, return_lse=True)
+    attention_weights(q, lse, key_cache, weights, indptr, indices, lengths, max_length=1088)
+    fewer, kept = paged_evict(weights, key_cache, value_cache, indptr, indices, lengths, keep=1024,
+                              recent=256, first=4, max_length=1088)     # every 64 steps, say
+    shift += lengths - fewer
+    lengths.copy_(fewer)
 """
 
 from __future__ import annotations
@@ -36,7 +52,8 @@ from torch.autograd import forward_ad as _forward
 
 from . import runtime as _rt
 
-__all__ = ["rope_frequencies", "rope", "rope_backward", "paged_append", "prefix_attention"]
+__all__ = ["rope_frequencies", "rope", "rope_backward", "norm_rope", "norm_rope_backward",
+           "paged_append", "prefix_attention", "attention_weights", "paged_evict"]
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -45,6 +62,12 @@ _LAYOUTS = {"half": 0, "interleaved": 1}
 _ROPE = struct.Struct("4P10qdq")
 _APPEND = struct.Struct("11P26qd")
 _ATTENTION = struct.Struct("11P24qd")
+# include/tilegen_cache.h: tg_norm_rope, .., tg_paged_evict
+_NORM = struct.Struct("8P18q2d")
+_NORM_BACKWARD = struct.Struct("13P23q2d")
+_APPEND_NORMED = struct.Struct("14P30q2d")
+_WEIGHTS = struct.Struct("9P22q2d")
+_EVICT = struct.Struct("8P21q")
 
 
 def _unfit(e: struct.error) -> ValueError:
@@ -52,25 +75,42 @@ def _unfit(e: struct.error) -> ValueError:
                       "no number: %s" % e)
 
 
-_LIB = None
+_LIB = _CACHE_LIB = None
+
+
+def _load(name, launches, workspaces):
+    _rt.lib()  # the runtime first, RTLD_GLOBAL
+    path = os.path.join(_rt.lib_dir(), name)
+    if not os.path.exists(path):
+        raise _rt.TileGenHipError("%s is not built (%s); run __graft_entry__.build()"
+                                  % (name, path))
+    L = ctypes.CDLL(path)
+    for entry in launches:
+        getattr(L, entry).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        getattr(L, entry).restype = ctypes.c_int
+    for entry in workspaces:
+        getattr(L, entry).argtypes = [ctypes.c_char_p]
+        getattr(L, entry).restype = ctypes.c_int64
+    return L
 
 
 def _lib():
     global _LIB
     if _LIB is None:
-        _rt.lib()  # the runtime first, RTLD_GLOBAL
-        path = os.path.join(_rt.lib_dir(), "libtgattn.so")
-        if not os.path.exists(path):
-            raise _rt.TileGenHipError("libtgattn.so is not built (%s); run "
-                                      "__graft_entry__.build()" % path)
-        L = ctypes.CDLL(path)
-        for name in ("launch_rope", "launch_paged_append", "launch_prefix_attention"):
-            getattr(L, name).argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-            getattr(L, name).restype = ctypes.c_int
-        L.prefix_attention_workspace.argtypes = [ctypes.c_char_p]
-        L.prefix_attention_workspace.restype = ctypes.c_int64
-        _LIB = L
+        _LIB = _load("libtgattn.so", ("launch_rope", "launch_paged_append",
+                                      "launch_prefix_attention"),
+                     ("prefix_attention_workspace",))
     return _LIB
+
+
+def _cache_lib():
+    global _CACHE_LIB
+    if _CACHE_LIB is None:
+        _CACHE_LIB = _load("libtgcache.so", (
+            "launch_norm_rope", "launch_norm_rope_backward", "launch_paged_append_normed",
+            "launch_attention_weights", "launch_paged_evict"),
+            ("norm_rope_backward_workspace", "attention_weights_workspace"))
+    return _CACHE_LIB
 
 
 # --------------------------------------------------------------------------- #
@@ -317,6 +357,220 @@ def rope_backward(grad: torch.Tensor, positions: torch.Tensor, frequency: torch.
 
 
 # --------------------------------------------------------------------------- #
+# norms that turn
+# --------------------------------------------------------------------------- #
+def _learned(name: str, w: Optional[torch.Tensor], heads: int, dim: int, device: int, dtype):
+    """(address, stride of a head, type) of a norm's weight: [dim], or [heads, dim]."""
+    if w is None:
+        return 0, 0, dtype
+    shape, strides = w.shape, w.stride()
+    if not (w.get_device() == device and w.dtype in (dtype, torch.float32)
+            and tuple(shape) in ((dim,), (heads, dim)) and (strides[-1] == 1 or dim == 1)):
+        raise ValueError("%s is %s %s with strides %s on %s, expected [%d] or [%d, %d] of %s or "
+                         "float32 on device %d" % (name, w.dtype, tuple(shape), strides, w.device,
+                                                   dim, heads, dim, dtype, device))
+    return w.data_ptr(), 0 if len(shape) == 1 else strides[0] if heads > 1 else dim, w.dtype
+
+
+def _norm_operands(query, key, positions, frequency, query_weight, key_weight):
+    """What both directions of a norm check: (device, type, tokens, heads, kv_heads, dim, packed
+    parts)."""
+    device, dtype = _operand("query", query, _DTYPES)
+    shape, qs = _heads("query", query, device, dtype, 3)
+    tokens, heads, dim = shape
+    kv_heads, ks = 0, (0, 0)
+    if key is not None:
+        kshape, ks = _heads("key", key, device, dtype, 3)
+        if kshape[0] != tokens or kshape[2] != dim:
+            raise ValueError("query is %s, key %s" % (tuple(shape), tuple(kshape)))
+        kv_heads = kshape[1]
+    elif key_weight is not None:
+        raise ValueError("key_weight without key")
+    wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
+    wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
+    if query_weight is None:
+        kind = other
+    elif key_weight is not None and other is not kind:
+        raise ValueError("query_weight is %s and key_weight %s" % (kind, other))
+    p_frequency = p_positions = rotary = 0
+    if frequency is not None:
+        p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
+        rotary = 2 * frequency.shape[0]
+    if positions is not None:
+        p_positions = _list("positions", positions, device, tokens)
+    elif rotary:
+        raise ValueError("frequency without positions")
+    return (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind,
+            p_positions, p_frequency, rotary)
+
+
+def _normed(query, key, positions, frequency, query_weight, key_weight, epsilon, layout,
+            magnitude, query_out, key_out):
+    (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind, p_positions,
+     p_frequency, rotary) = _norm_operands(query, key, positions, frequency, query_weight,
+                                           key_weight)
+    written = tuple(t for t in (query_out, key_out) if t is not None)
+    if query_out is None:
+        query_out = _like(query)
+    oshape, qos = _heads("query_out", query_out, device, dtype, 3, write=True)
+    if oshape != query.shape:
+        raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(query.shape)))
+    p_key = p_key_out = 0
+    kos = (0, 0)
+    if key is not None:
+        if key_out is None:
+            key_out = _like(key)
+        oshape, kos = _heads("key_out", key_out, device, dtype, 3, write=True)
+        if oshape != key.shape:
+            raise ValueError("key_out is %s, expected %s" % (tuple(oshape), tuple(key.shape)))
+        p_key, p_key_out = key.data_ptr(), key_out.data_ptr()
+    elif key_out is not None:
+        raise ValueError("key_out without key")
+    try:
+        packed = _NORM.pack(
+            query.data_ptr(), p_key, query_out.data_ptr(), p_key_out, wq, wk, p_positions,
+            p_frequency, _DTYPES[dtype], _DTYPES[kind], tokens, heads, kv_heads, dim, rotary,
+            _layout(layout), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], wqs, wks,
+            magnitude, epsilon)
+    except struct.error as e:
+        raise _unfit(e) from None
+    _call(_cache_lib().launch_norm_rope, packed, device, "norm_rope")
+    if written:
+        _written(written)
+    return query_out, key_out
+
+
+def _normed_backward(grad_query, grad_key, query, key, positions, frequency, query_weight,
+                     key_weight, epsilon, layout, magnitude, want_weights=(True, True)):
+    # an expanded weight's heads have gradients of their own
+    query_weight, key_weight = (
+        w.contiguous() if w is not None and w.dim() == 2 and w.stride(0) == 0 else w
+        for w in (query_weight, key_weight))
+    (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind, p_positions,
+     p_frequency, rotary) = _norm_operands(query, key, positions, frequency, query_weight,
+                                           key_weight)
+    gshape, gqs = _heads("grad_query", grad_query, device, dtype, 3)
+    if gshape != query.shape:
+        raise ValueError("grad_query is %s, expected %s" % (tuple(gshape), tuple(query.shape)))
+    query_out, key_out = _like(query), None
+    p_grad_key = p_key = p_key_out = 0
+    gks = kos = (0, 0)
+    if key is not None:
+        gshape, gks = _heads("grad_key", grad_key, device, dtype, 3)
+        if gshape != key.shape:
+            raise ValueError("grad_key is %s, expected %s" % (tuple(gshape), tuple(key.shape)))
+        key_out = _like(key)
+        kos = key_out.stride()
+        p_grad_key, p_key, p_key_out = grad_key.data_ptr(), key.data_ptr(), key_out.data_ptr()
+    elif grad_key is not None:
+        raise ValueError("grad_key without key")
+    qos = query_out.stride()
+    dqw, dkw = (None if w is None or not wanted else
+                torch.empty_like(w, memory_format=torch.contiguous_format)
+                for w, wanted in zip((query_weight, key_weight), want_weights))
+    fields = [grad_query.data_ptr(), p_grad_key, query.data_ptr(), p_key, query_out.data_ptr(),
+              p_key_out, 0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr(),
+              wq, wk, p_positions, p_frequency, 0, 0, _DTYPES[dtype], _DTYPES[kind], tokens, heads,
+              kv_heads, dim, rotary, _layout(layout), gqs[0], gqs[1], gks[0], gks[1], qs[0], qs[1],
+              ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], wqs, wks, magnitude, epsilon]
+    L = _cache_lib()
+    _run(query, fields, _NORM_BACKWARD, 12, L.norm_rope_backward_workspace,
+         L.launch_norm_rope_backward, device, "norm_rope_backward")
+    return query_out, key_out, dqw, dkw
+
+
+def _run(like, fields, packing, workspace_at, workspace, launch, device, what):
+    """A call that may need a workspace, from torch, with the operands' device current."""
+    def plan_and_launch():
+        packed = packing.pack(*fields)
+        n = workspace(packed)
+        if n < 0:
+            return n
+        if n:
+            space = like.new_empty(n, dtype=torch.uint8)
+            fields[workspace_at:workspace_at + 2] = space.data_ptr(), n
+            packed = packing.pack(*fields)
+        return launch(packed, _raw_stream(device))
+
+    try:
+        rc = _on(device, plan_and_launch)
+    except struct.error as e:
+        raise _unfit(e) from None
+    if rc:
+        _raise(rc, what)
+
+
+class _NormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, query, key, query_weight, key_weight, positions, frequency, how):
+        ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequency)
+        ctx.how = how
+        query, key = _normed(query, key, positions, frequency, query_weight, key_weight, *how,
+                             None, None)
+        return query if key is None else (query, key)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_query, grad_key=None):
+        query, key, query_weight, key_weight, positions, frequency = ctx.saved_tensors
+        grad_query, grad_key = (
+            g.contiguous() if g is not None and g.stride(-1) != 1 else g
+            for g in (grad_query, grad_key))
+        got = _normed_backward(grad_query, grad_key, query, key, positions, frequency,
+                               query_weight, key_weight, *ctx.how,
+                               want_weights=ctx.needs_input_grad[2:4])
+        return got + (None, None, None)
+
+
+def norm_rope(query: torch.Tensor, key: Optional[torch.Tensor],
+              positions: Optional[torch.Tensor], frequency: Optional[torch.Tensor],
+              query_weight: Optional[torch.Tensor] = None,
+              key_weight: Optional[torch.Tensor] = None, *, epsilon: float = 1e-6,
+              layout: str = "half", magnitude: float = 1.0,
+              query_out: Optional[torch.Tensor] = None, key_out: Optional[torch.Tensor] = None
+              ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """query [tokens, heads, dim] and key [tokens, kv_heads, dim] with every head divided by its
+    root mean square, x / sqrt(mean(x^2) + epsilon), multiplied by its weight and turned as ``rope``
+    does, in one pass and with one rounding.
+
+    A weight is [dim], one for all heads, or [heads, dim], of the heads' type or float32 (None:
+    ones).  ``frequency=None`` turns nothing, and ``key=None`` leaves the keys out.  Heads are up
+    to 256 elements, and may be those of a packed projection.  Outputs may be their inputs, and
+    share no other memory with the operands.  Sums of squares are held in 32 bits.  Differentiable
+    once, backward, in the heads and the weights; the gradients of weights are summed in 32 bits in
+    an order that the sizes alone decide."""
+    operands = (query, key, query_weight, key_weight)
+    if frequency is not None:
+        _no_gradient("norm_rope", frequency)
+    if _forward._current_level >= 0 and any(_tangent(t) for t in operands if t is not None):
+        raise ValueError("norm_rope has no forward derivative")
+    if torch.is_grad_enabled():
+        if any(t is not None and t.requires_grad for t in operands):
+            if query_out is not None or key_out is not None:
+                raise ValueError("outputs cannot be given where operands need gradients")
+            got = _NormRope.apply(query, key, query_weight, key_weight, positions, frequency,
+                                  (epsilon, layout, magnitude))
+            return (got, None) if key is None else got
+    _no_gradient("norm_rope", query_out, key_out)
+    return _normed(query, key, positions, frequency, query_weight, key_weight, epsilon, layout,
+                   magnitude, query_out, key_out)
+
+
+def norm_rope_backward(grad_query: torch.Tensor, grad_key: Optional[torch.Tensor],
+                       query: torch.Tensor, key: Optional[torch.Tensor],
+                       positions: Optional[torch.Tensor], frequency: Optional[torch.Tensor],
+                       query_weight: Optional[torch.Tensor] = None,
+                       key_weight: Optional[torch.Tensor] = None, *, epsilon: float = 1e-6,
+                       layout: str = "half", magnitude: float = 1.0):
+    """The gradients of ``norm_rope`` by (query, key, query_weight, key_weight) from those of its two
+    results; None for what it was not given."""
+    _no_gradient("norm_rope_backward", grad_query, grad_key, query, key, query_weight, key_weight,
+                 frequency)
+    return _normed_backward(grad_query, grad_key, query, key, positions, frequency, query_weight,
+                            key_weight, epsilon, layout, magnitude)
+
+
+# --------------------------------------------------------------------------- #
 # the cache
 # --------------------------------------------------------------------------- #
 def _caches(key_cache, value_cache, device, dtype, write):
@@ -345,7 +599,10 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
                  query: Optional[torch.Tensor] = None,
                  query_out: Optional[torch.Tensor] = None,
                  query_indptr: Optional[torch.Tensor] = None, offset: int = 0,
-                 layout: str = "half", magnitude: float = 1.0) -> Optional[torch.Tensor]:
+                 layout: str = "half", magnitude: float = 1.0,
+                 query_weight: Optional[torch.Tensor] = None,
+                 key_weight: Optional[torch.Tensor] = None, epsilon: Optional[float] = None,
+                 shift: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
     """Writes the new tokens' key and value [tokens, kv_heads, dim] into the caches, keys
     turned as ``rope`` does (``frequency=None``: as they are), and returns the same tokens'
     ``query`` [tokens, heads, dim] turned with them, in one launch.
@@ -357,9 +614,15 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     query_indptr[0] (slices of a larger batch's row pointers) and from query_indptr[-1] on (a
     batch padded for a graph) belong to no sequence: nothing is written for them and their
     queries come back zero.  ``query_out`` may be ``query`` itself, and share no other memory
-    with the operands."""
+    with the operands.
+
+    With ``epsilon`` keys and queries are first normed as by ``norm_rope``, by ``query_weight`` and
+    ``key_weight``.  ``shift`` [sequences] counts tokens that came before those in a sequence's
+    pages and left them (``paged_evict``): its tokens are turned at that many more.  Both are for
+    heads of up to 256 elements."""
     device, dtype = _operand("key", key, _DTYPES)
-    _no_gradient("paged_append", key, value, query, key_cache, value_cache, frequency, query_out)
+    _no_gradient("paged_append", key, value, query, key_cache, value_cache, frequency, query_out,
+                 query_weight, key_weight)
     shape, ks = _heads("key", key, device, dtype, 3)
     vshape, vs = _heads("value", value, device, dtype, 3)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, True)
@@ -389,6 +652,17 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     if frequency is not None:
         p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
         rotary = 2 * frequency.shape[0]
+    if epsilon is not None or shift is not None:
+        _append_normed(
+            key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(), value_cache.data_ptr(), out,
+            p_indptr, p_indices, p_lengths, p_ends, shift, p_frequency, query_weight, key_weight,
+            device, dtype, tokens, sequences, heads, kv_heads, dim, rotary, _layout(layout),
+            cache[0], cache[1], indices.shape[0], offset, ks, vs, qs, os_, kcs, vcs, magnitude,
+            epsilon)
+        _written(written)
+        return query_out
+    if query_weight is not None or key_weight is not None:
+        raise ValueError("weights of a norm without epsilon")
     try:
         packed = _APPEND.pack(
             key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(), value_cache.data_ptr(), out,
@@ -401,6 +675,33 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
     _call(_lib().launch_paged_append, packed, device, "paged_append")
     _written(written)
     return query_out
+
+
+def _append_normed(key, value, q, key_cache, value_cache, out, indptr, indices, lengths, ends,
+                   shift, frequency, query_weight, key_weight, device, dtype, tokens, sequences,
+                   heads, kv_heads, dim, rotary, layout, pages, page, n_indices, offset, ks, vs,
+                   qs, os_, kcs, vcs, magnitude, epsilon):
+    if epsilon is None and (query_weight is not None or key_weight is not None):
+        raise ValueError("weights of a norm without epsilon")
+    if query_weight is not None and not q:
+        raise ValueError("query_weight without query")
+    wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
+    wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
+    if query_weight is None:
+        kind = other
+    elif key_weight is not None and other is not kind:
+        raise ValueError("query_weight is %s and key_weight %s" % (kind, other))
+    p_shift = 0 if shift is None else _list("shift", shift, device, sequences)
+    try:
+        packed = _APPEND_NORMED.pack(
+            key, value, q, key_cache, value_cache, out, indptr, indices, lengths, ends, p_shift,
+            frequency, wq, wk, _DTYPES[dtype], _DTYPES[kind], tokens, sequences, heads, kv_heads,
+            dim, rotary, layout, pages, page, n_indices, offset, epsilon is not None, ks[0], ks[1],
+            vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1],
+            vcs[2], wqs, wks, magnitude, 0.0 if epsilon is None else epsilon)
+    except struct.error as e:
+        raise _unfit(e) from None
+    _call(_cache_lib().launch_paged_append_normed, packed, device, "paged_append")
 
 
 # --------------------------------------------------------------------------- #
@@ -478,3 +779,105 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
     if given:
         _written(out)
     return (out, lse) if return_lse else out
+
+
+# --------------------------------------------------------------------------- #
+# a cache of bounded length
+# --------------------------------------------------------------------------- #
+def _key_weights(weights, cache, device):
+    """Strides of the keys' weights, for a cache of this shape."""
+    shape, strides = weights.shape, weights.stride()
+    if not (weights.get_device() == device and weights.dtype is torch.float32
+            and tuple(shape) == tuple(cache[:3])):
+        raise ValueError("weights is %s %s on %s, expected float32 %s on device %d" % (
+            weights.dtype, tuple(shape), weights.device, tuple(cache[:3]), device))
+    if 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+        raise ValueError("weights is written, but its elements share memory (strides %s)"
+                         % (strides,))
+    return strides
+
+
+def attention_weights(query: torch.Tensor, lse: torch.Tensor, key_cache: torch.Tensor,
+                      weights: torch.Tensor, indptr: torch.Tensor, indices: torch.Tensor,
+                      lengths: torch.Tensor, *, max_length: int,
+                      query_indptr: Optional[torch.Tensor] = None, max_query: int = 1,
+                      scale: Optional[float] = None, decay: float = 1.0) -> torch.Tensor:
+    """Adds to ``weights`` [pages, page, kv_heads] (float32) the attention that each key of the
+    sequences' own pages receives from the new tokens: the sum of exp(scale q.k - lse) over those
+    that see it and the query heads that read it, ``lse`` being what ``prefix_attention`` returned
+    for the same ``query`` (a prefix's share is in it).  What a key had is multiplied by ``decay``
+    first; the new tokens' own keys start from nothing.  Returns ``weights``.
+
+    The other arguments are ``prefix_attention``'s.  Rows that see no key add nothing, and a
+    sequence without new tokens keeps its weights as they are.  ``weights`` may have any strides
+    and is fastest where a head's slots lie side by side: ``torch.zeros(pages, kv_heads,
+    page).transpose(1, 2)``.  Scores, exponentials and sums are held in 32 bits; sums are taken in
+    an order that the sizes alone decide."""
+    device, dtype = _operand("query", query, _CACHED)
+    _no_gradient("attention_weights", query, lse, key_cache, weights)
+    shape, qs = _heads("query", query, device, dtype, 3)
+    cache, kcs = _heads("key_cache", key_cache, device, dtype, 4)
+    tokens, heads, dim = shape
+    if cache[3] != dim or not cache[2] or heads % cache[2]:
+        raise ValueError("query is %s, the cache %s" % (tuple(shape), tuple(cache)))
+    ws = _key_weights(weights, cache, device)
+    if not (lse.get_device() == device and lse.dtype is torch.float32
+            and lse.shape == shape[:2]):
+        raise ValueError("lse is %s %s on %s, expected float32 %s on device %d" % (
+            lse.dtype, tuple(lse.shape), lse.device, tuple(shape[:2]), device))
+    ls = lse.stride()
+    (p_indptr, p_indices, p_lengths, p_ends), sequences = _table(
+        indptr, indices, lengths, query_indptr, tokens, device)
+    fields = [query.data_ptr(), lse.data_ptr(), key_cache.data_ptr(), weights.data_ptr(), p_indptr,
+              p_indices, p_lengths, p_ends, 0, 0, _DTYPES[dtype], tokens, sequences, heads,
+              cache[2], dim, cache[0], cache[1], indices.shape[0], max_query, max_length, qs[0],
+              qs[1], ls[0], ls[1], kcs[0], kcs[1], kcs[2], ws[0], ws[1], ws[2],
+              dim ** -0.5 if scale is None else scale, decay]
+    L = _cache_lib()
+    _run(query, fields, _WEIGHTS, 8, L.attention_weights_workspace, L.launch_attention_weights,
+         device, "attention_weights")
+    _written(weights)
+    return weights
+
+
+def paged_evict(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                indptr: torch.Tensor, indices: torch.Tensor, lengths: torch.Tensor, *, keep: int,
+                recent: int = 0, first: int = 0, max_length: int, move_weights: bool = True
+                ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cuts every sequence of more than ``keep`` tokens in its own pages to ``keep``, each kv head
+    by itself: its ``first`` and its last ``recent`` tokens stay, and of the others the heaviest by
+    ``weights`` [pages, page, kv_heads] (float32; of equal ones those that stand first, NaN counts
+    as the heaviest).  Returns (the new lengths, kept): kept[b, h, i], int32 [sequences, kv_heads,
+    keep], is the position that the token now at position i had, -1 past the end.
+
+    Keys and values move within their sequence's pages, in place and no more than needed: kept
+    tokens at positions below ``keep - recent`` stay where they are, later ones fill the gaps
+    there in order, and the last ``recent`` follow in order, so that the next call finds them last
+    again.  Slots past the new length hold anything.  Keys stay turned as they were: give what
+    sequences have lost to ``paged_append`` as ``shift``.  Weights move along unless
+    ``move_weights=False``.  ``max_length`` bounds ``lengths``, as in ``prefix_attention``.  A page
+    belongs to one sequence; slots whose page is not in the cache go first and nothing moves
+    there."""
+    device, dtype = _operand("key_cache", key_cache, _DTYPES)
+    _no_gradient("paged_evict", weights, key_cache, value_cache)
+    cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, True)
+    ws = _key_weights(weights, cache, device)
+    sequences = lengths.shape[0] if lengths.dim() == 1 else -1
+    p_indptr = _list("indptr", indptr, device, sequences + 1)
+    p_indices, p_lengths = _list("indices", indices, device), _list("lengths", lengths, device)
+    if not 0 <= keep <= 1 << 22 or not cache[2]:
+        raise ValueError("keep is %s for caches %s, expected 0 to 2^22" % (keep, tuple(cache)))
+    fewer = torch.empty_like(lengths)
+    kept = lengths.new_empty((sequences, cache[2], keep), dtype=torch.int32)
+    try:
+        packed = _EVICT.pack(
+            key_cache.data_ptr(), value_cache.data_ptr(), weights.data_ptr(), p_indptr, p_indices,
+            p_lengths, fewer.data_ptr(), kept.data_ptr(), _DTYPES[dtype], sequences, cache[2],
+            cache[3], cache[0], cache[1], indices.shape[0], max_length, keep, recent, first,
+            bool(move_weights), kcs[0], kcs[1], kcs[2], vcs[0], vcs[1], vcs[2], ws[0], ws[1],
+            ws[2])
+    except struct.error as e:
+        raise _unfit(e) from None
+    _call(_cache_lib().launch_paged_evict, packed, device, "paged_evict")
+    _written((key_cache, value_cache) + ((weights,) if move_weights else ()))
+    return fewer, kept

@@ -4,8 +4,9 @@
    C++ compiler against the ROCm HIP runtime and hipRTC;
 2. ``libtg_vendor.so``, the rocSPARSE comparison (when rocSPARSE is installed),
    ``tilegen_bench``, the native host harness (TGM1 matrix + variant library),
-   ``libtgna.so`` (hipcc), the SpMV entry point that allocates nothing, and
-   ``libtgattn.so`` (hipcc), attention over a paged cache;
+   ``libtgna.so`` (hipcc), the SpMV entry point that allocates nothing,
+   ``libtgattn.so`` (hipcc), attention over a paged cache, and ``libtgcache.so``
+   (hipcc), what bounds that cache;
 3. the test oracle (``oracle/Makefile``: the C restatement, and the
    reference's own ref.cpp where its sources are present);
 4. the hipRTC code objects and C launchers of every named schedule
@@ -139,13 +140,21 @@ def noalloc_code_object(out: str) -> str:
     return out
 
 
-def attention_sources() -> List[str]:
-    src = os.path.join(PKG, "csrc", "attention")
+def _sources(folder: str) -> List[str]:
+    src = os.path.join(PKG, "csrc", folder)
     return [os.path.join(src, f) for f in sorted(os.listdir(src)) if f.endswith(".hip")]
 
 
-def _attention_compile(source: str) -> List[str]:
-    """hipcc and the compile flags of one of libtgattn.so's sources."""
+def attention_sources() -> List[str]:
+    return _sources("attention")
+
+
+def cache_sources() -> List[str]:
+    return _sources("cache")
+
+
+def _operator_compile(source: str) -> List[str]:
+    """hipcc and the compile flags of one of libtgattn.so's or libtgcache.so's sources."""
     from .verify import hip_arch
     return [os.path.join(ROCM, "bin", "hipcc"), "--offload-arch=%s" % hip_arch(), "-O3",
             "-std=c++17", "-fPIC", "-fvisibility=hidden",
@@ -153,39 +162,59 @@ def _attention_compile(source: str) -> List[str]:
             "-I", os.path.join(REPO, "include"), "-c", source]
 
 
-def build_attention() -> str:
-    """libtgattn.so: attention over a paged cache (include/tilegen_attention.h), hipcc for
-    gfx950, its sources side by side."""
+def _build_operators(name: str, sources: List[str]) -> str:
+    """lib<name>.so from its sources, compiled side by side."""
     lib_dir = os.path.join(PKG, "_lib")
-    obj_dir = os.path.join(REPO, "build", "attention")
+    obj_dir = os.path.join(REPO, "build", name)
     os.makedirs(obj_dir, exist_ok=True)
-    out = os.path.join(lib_dir, "libtgattn.so")
+    out = os.path.join(lib_dir, "lib%s.so" % name)
     tmp = out + ".tmp%d" % os.getpid()
 
     def one(source: str) -> str:
         obj = os.path.join(obj_dir, os.path.basename(source)[:-len(".hip")] + ".o")
-        _run(_attention_compile(source) + ["-o", obj])
+        _run(_operator_compile(source) + ["-o", obj])
         return obj
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-        objects = list(pool.map(one, attention_sources()))
+        objects = list(pool.map(one, sources))
     _run([os.path.join(ROCM, "bin", "hipcc"), "-shared", "-o", tmp] + objects +
          ["-L", lib_dir, "-ltgrt", "-Wl,-rpath," + lib_dir])
     os.replace(tmp, out)
     return out
 
 
-def attention_code_objects(out_dir: str) -> List[str]:
-    """libtgattn's device code objects alone (the same sources and flags as the library, device
-    pass only), for checks of their kernels' registers and spills."""
+def build_attention() -> str:
+    """libtgattn.so: attention over a paged cache (include/tilegen_attention.h), hipcc for
+    gfx950."""
+    return _build_operators("tgattn", attention_sources())
+
+
+def build_cache() -> str:
+    """libtgcache.so: a paged cache of bounded length (include/tilegen_cache.h), hipcc for
+    gfx950."""
+    return _build_operators("tgcache", cache_sources())
+
+
+def _code_objects(sources: List[str], out_dir: str) -> List[str]:
     def one(source: str) -> str:
         out = os.path.join(out_dir, os.path.basename(source)[:-len(".hip")] + ".co")
-        _run(_attention_compile(source) +
+        _run(_operator_compile(source) +
              ["--offload-device-only", "--no-gpu-bundle-output", "-o", out])
         return out
 
     with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
-        return list(pool.map(one, attention_sources()))
+        return list(pool.map(one, sources))
+
+
+def attention_code_objects(out_dir: str) -> List[str]:
+    """libtgattn's device code objects alone (the same sources and flags as the library, device
+    pass only), for checks of their kernels' registers and spills."""
+    return _code_objects(attention_sources(), out_dir)
+
+
+def cache_code_objects(out_dir: str) -> List[str]:
+    """libtgcache's, likewise."""
+    return _code_objects(cache_sources(), out_dir)
 
 
 def build_oracle(force: bool = False) -> None:
@@ -262,6 +291,9 @@ def build_all(verbose: bool = True, force: bool = False) -> None:
     build_attention()
     if verbose:
         print("[build] attention library (%.1fs)" % (time.time() - t0))
+    build_cache()
+    if verbose:
+        print("[build] cache library (%.1fs)" % (time.time() - t0))
     build_oracle(force)
     if force:
         from .verify import cache_dir

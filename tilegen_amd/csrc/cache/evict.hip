@@ -1,0 +1,446 @@
+// Eviction by weight (launch_paged_evict): which tokens stay is decided for each sequence and kv
+// head by one workgroup, then workgroups for slices of each head move what has to.
+//
+// Of the C candidates between the first and the recent tokens the n heaviest stay.  Weights map to
+// whole numbers of the same order, and the n-th largest is found digit by digit from the top, by
+// counting.  Ties at it go to the lowest positions, by a scan over the positions' counts.  Moves:
+// tokens that stay below `front` are left alone; the others are as many as the holes there, and
+// both lists are taken in order.  No place is both a source and a target of those, so they go in
+// any order; then the recent tokens go down, chunk by chunk, each read whole before it is
+// written.
+#include "cache.h"
+
+namespace tg {
+namespace {
+
+struct Evict {
+  void *key_cache, *value_cache;
+  float* weights;
+  int64_t* lengths_out;
+  int32_t* kept;
+  Table table;
+  i64 kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head, w_page, w_slot, w_head;
+  int kv_heads, dim, keep, recent, first, move_weights;
+  int slices, slice;      // of a row of a cache: workgroups, units of 16 bytes of each
+  Div by_heads, by_slices, by_units, by_last;   // units of a slice, of the last one
+};
+
+// Sequence b's pages, as far as its tokens go.
+struct Held {
+  const int64_t* list;
+  int keys;
+};
+__device__ __forceinline__ Held held_of(const Evict& a, int b) {
+  const Table& t = a.table;
+  i64 begin = t.indptr[b], end = t.indptr[b + 1];
+  begin = begin < 0 ? 0 : begin > t.n_indices ? t.n_indices : begin;
+  end = end < begin ? begin : end > t.n_indices ? t.n_indices : end;
+  i64 length = t.lengths[b];
+  length = length < 0 ? 0 : length > kMostKeys ? kMostKeys : length;
+  const i64 room = (end - begin) * t.page;
+  return {t.indices + begin, static_cast<int>(length < room ? length : room)};
+}
+
+// A position's page (-1: outside the cache) and slot.
+struct Place {
+  i64 page;
+  int slot;
+};
+__device__ __forceinline__ Place place_of(const Evict& a, const int64_t* list, int p) {
+  const int nth = a.table.by_page(p);
+  const i64 page = list[nth];
+  return {page >= 0 && page < a.table.pages ? page : -1, p - nth * a.table.page};
+}
+
+// Whole numbers in the order of the weights: 0 for none, the largest for NaN; -0 is 0.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, w + 0.f);
+  if (w != w) return 0xFFFFFFFFu;
+  return x >> 31 ? ~x : x | 0x80000000u;
+}
+
+constexpr int kWindow = 2048;     // moves that are listed at a time
+
+// THREADS a workgroup; keys of the first CACHED candidates stay in LDS.
+template <int THREADS, int CACHED>
+__global__ __launch_bounds__(THREADS) void choose(Evict a) {
+  constexpr int kWaves = THREADS / 64;
+  constexpr int kBins = 2048, kCopies = 2;
+  __shared__ uint32_t s_keys[CACHED];
+  __shared__ uint32_t s_bins[kCopies][kBins];   // later the list of moves
+  __shared__ int s_wave[2][kWaves];
+  __shared__ uint32_t s_prefix;
+  __shared__ int s_left;
+  static_assert(kWindow <= kCopies * kBins, "");
+  int* s_list = reinterpret_cast<int*>(&s_bins[0][0]);
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
+  const Held s = held_of(a, b);
+  const int gone = s.keys > a.keep ? s.keys - a.keep : 0;
+  int32_t* kept = a.kept + static_cast<i64>(blockIdx.x) * a.keep;
+  if (h == 0 && tid == 0) a.lengths_out[b] = s.keys - gone;
+  if (gone == 0) {
+    for (int i = tid; i < a.keep; i += THREADS) kept[i] = i < s.keys ? i : -1;
+    return;
+  }
+  const int front = a.keep - a.recent;
+  for (int i = tid; i < a.keep; i += THREADS)
+    if (i < a.first || i >= front) kept[i] = i < front ? i : i + gone;
+  const int want = front - a.first;           // of the candidates
+  if (want == 0) return;
+  const int count = s.keys - a.recent - a.first;
+
+  auto fetch = [&](int c) {     // candidate c's key
+    const Place at = place_of(a, s.list, a.first + c);
+    return at.page < 0 ? 0u : order_of(a.weights[at.page * a.w_page + at.slot * a.w_slot +
+                                                 h * a.w_head]);
+  };
+  auto key = [&](int c) { return c < CACHED ? s_keys[c] : fetch(c); };
+#pragma unroll 4
+  for (int c = tid; c < min(count, CACHED); c += THREADS) s_keys[c] = fetch(c);
+
+  // the want-th largest, by digits of 11, 11 and 10 bits; `left` of those equal to it stay
+  uint32_t prefix = 0;
+  int left = want;
+#pragma unroll 1
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+    const int bins = digit == 2 ? 1024 : kBins;
+    for (int i = tid; i < kCopies * kBins; i += THREADS) (&s_bins[0][0])[i] = 0;
+    __syncthreads();
+    for (int c = tid; c < count; c += THREADS) {
+      const uint32_t k = key(c);
+      if (digit == 0 || k >> (shift + (digit == 1 ? 11 : 10)) == prefix)
+        atomicAdd(&s_bins[lane % kCopies][k >> shift & (bins - 1)], 1u);
+    }
+    __syncthreads();
+    // each thread takes a run of bins, from the largest down
+    const int run = bins / THREADS > 0 ? bins / THREADS : 1;
+    const int top = bins - 1 - tid * run;
+    int mine = 0;
+    for (int i = 0; i < run && top - i >= 0; ++i) {
+      int n = 0;
+#pragma unroll
+      for (int copy = 0; copy < kCopies; ++copy) n += s_bins[copy][top - i];
+      mine += n;
+    }
+    int before = mine;          // of the threads up to this one
+    for (int d = 1; d < 64; d *= 2) {
+      const int other = __shfl_up(before, d);
+      if (lane >= d) before += other;
+    }
+    if (lane == 63) s_wave[0][wave] = before;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) before += s_wave[0][w];
+    before -= mine;
+    if (before < left && before + mine >= left) {
+      for (int i = 0; i < run; ++i) {
+        int n = 0;
+#pragma unroll
+        for (int copy = 0; copy < kCopies; ++copy) n += s_bins[copy][top - i];
+        if (before + n >= left) {
+          s_prefix = prefix << (digit == 2 ? 10 : 11) | static_cast<uint32_t>(top - i);
+          s_left = left - before;
+          break;
+        }
+        before += n;
+      }
+    }
+    __syncthreads();
+    prefix = s_prefix;
+    left = s_left;
+    __syncthreads();
+  }
+
+  // each thread takes a run of candidates (an odd number: LDS banks); two exclusive sums at once
+  const int run = (count + THREADS - 1) / THREADS | 1;
+  const int c0 = min(static_cast<int64_t>(tid) * run, static_cast<int64_t>(count));
+  const int c1 = min(c0 + run, count);
+  auto scan = [&](int& x, int& y) {
+    int u = x, v = y;
+    for (int d = 1; d < 64; d *= 2) {
+      const int other_u = __shfl_up(u, d), other_v = __shfl_up(v, d);
+      if (lane >= d) {
+        u += other_u;
+        v += other_v;
+      }
+    }
+    if (lane == 63) {
+      s_wave[0][wave] = u;
+      s_wave[1][wave] = v;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+      u += s_wave[0][w];
+      v += s_wave[1][w];
+    }
+    x = u - x;
+    y = v - y;
+    __syncthreads();
+  };
+  int ties = 0, none = 0;
+  for (int c = c0; c < c1; ++c) ties += key(c) == prefix;
+  scan(ties, none);
+  // candidates below the front stay where they are, or leave a hole; those past it fill one
+  int holes = 0, fills = 0;
+  auto each = [&](auto&& visit) {
+    int tie = ties;
+    for (int c = c0; c < c1; ++c) {
+      const uint32_t k = key(c);
+      const bool stays = k > prefix || (k == prefix && tie < left);
+      tie += k == prefix;
+      visit(a.first + c, stays);
+    }
+  };
+  each([&](int p, bool stays) {
+    holes += p < front && !stays;
+    fills += p >= front && stays;
+  });
+  scan(holes, fills);
+  // (gone candidates less than all from the front on: as many holes as fills)
+  bool more = true;
+  for (int base = 0; more; base += kWindow) {
+    int nth = fills;
+    bool past = false;
+    each([&](int p, bool stays) {
+      if (p >= front && stays) {
+        if (nth >= base && nth < base + kWindow) s_list[nth - base] = p;
+        past |= nth >= base + kWindow;
+        ++nth;
+      }
+    });
+    more = __syncthreads_or(past);
+    nth = holes;
+    each([&](int p, bool stays) {
+      if (p < front) {
+        if (stays) {
+          if (base == 0) kept[p] = p;
+        } else {
+          if (nth >= base && nth < base + kWindow) kept[p] = s_list[nth - base];
+          ++nth;
+        }
+      }
+    });
+    __syncthreads();
+  }
+}
+
+constexpr int kMovers = 256;      // threads
+
+// Units of 16 bytes of a row; the last may be shorter.
+template <typename T>
+__device__ __forceinline__ typename Chunk<T>::Vec read_unit(const T* p, int n) {
+  typename Chunk<T>::Vec v = typename Chunk<T>::Vec(T(0));
+  if (n >= Chunk<T>::N) return Chunk<T>::load(p);
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; ++i)
+    if (i < n) v[i] = p[i];
+  return v;
+}
+template <typename T>
+__device__ __forceinline__ void write_unit(T* p, int n, typename Chunk<T>::Vec v) {
+  if (n >= Chunk<T>::N) {
+    Chunk<T>::store(p, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < Chunk<T>::N; ++i)
+    if (i < n) p[i] = v[i];
+}
+
+// Rows of one head of a cache move: `units` units of `dim` elements from `at` on.
+template <typename T>
+__device__ __forceinline__ void move_rows(const Evict& a, const Held& s, const int32_t* kept,
+                                          T* base, i64 by_page, i64 by_slot, int dim, int units,
+                                          Div by_units) {
+  constexpr int kList = 1024, kDeep = 8;
+  __shared__ int s_to[kList], s_from[kList];
+  __shared__ int s_count;
+  const int tid = threadIdx.x;
+  const int front = a.keep - a.recent, gone = s.keys - a.keep;
+  auto row = [&](int p) -> T* {
+    const Place at = place_of(a, s.list, p);
+    return at.page < 0 ? nullptr : base + at.page * by_page + at.slot * by_slot;
+  };
+  // the holes' fills, listed some at a time
+  for (int i0 = a.first; i0 < front; i0 += kList) {
+    if (tid == 0) s_count = 0;
+    __syncthreads();
+    for (int i = i0 + tid; i < min(i0 + kList, front); i += kMovers) {
+      const int from = kept[i];
+      if (from != i) {
+        const int n = atomicAdd(&s_count, 1);
+        s_to[n] = i;
+        s_from[n] = from;
+      }
+    }
+    __syncthreads();
+    const int work = s_count * units;
+#pragma unroll 4
+    for (int w = tid; w < work; w += kMovers) {
+      const int n = by_units(w), u = (w - n * units) * Chunk<T>::N;
+      const T* from = row(s_from[n]);
+      T* to = row(s_to[n]);
+      if (from && to) write_unit(to + u, dim - u, read_unit(from + u, dim - u));
+    }
+    __syncthreads();
+  }
+  // the recent tokens, each chunk read whole before any of it is written
+  const int64_t work = static_cast<int64_t>(a.recent) * units;
+  for (int64_t w0 = 0; w0 < work; w0 += kDeep * kMovers) {
+    typename Chunk<T>::Vec v[kDeep];
+    T* to[kDeep];
+    int left[kDeep];
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      const int64_t w = w0 + i * kMovers + tid;
+      to[i] = nullptr;
+      if (w < work) {
+        const int n = by_units(static_cast<uint32_t>(w));
+        const int u = (static_cast<int>(w) - n * units) * Chunk<T>::N;
+        const T* from = row(front + n + gone);
+        T* target = row(front + n);
+        left[i] = dim - u;
+        if (from && target) {
+          to[i] = target + u;
+          v[i] = read_unit(from + u, left[i]);
+        }
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i)
+      if (to[i]) write_unit(to[i], left[i], v[i]);
+  }
+}
+
+// One workgroup for a slice of a head's rows of one cache, or for its weights.
+template <typename T>
+__global__ __launch_bounds__(kMovers) void move(Evict a) {
+  const int per = 2 * a.slices + a.move_weights;
+  const int unit = a.by_slices(blockIdx.x), part = blockIdx.x - unit * per;
+  const int b = a.by_heads(unit), h = unit - b * a.kv_heads;
+  const Held s = held_of(a, b);
+  if (s.keys <= a.keep) return;
+  const int32_t* kept = a.kept + static_cast<i64>(unit) * a.keep;
+  if (part == 2 * a.slices) {
+    Div by_one;
+    by_one.mul = 1;
+    by_one.shift = 0;
+    move_rows<float>(a, s, kept, a.weights + h * a.w_head, a.w_page, a.w_slot, 1, 1, by_one);
+    return;
+  }
+  const bool value = part >= a.slices;
+  const int first = (value ? part - a.slices : part) * a.slice * Chunk<T>::N;
+  const int dim = min(a.dim - first, a.slice * Chunk<T>::N);
+  const int units = (dim + Chunk<T>::N - 1) / Chunk<T>::N;
+  T* base = static_cast<T*>(value ? a.value_cache : a.key_cache) + first +
+            h * (value ? a.vc_head : a.kc_head);
+  move_rows<T>(a, s, kept, base, value ? a.vc_page : a.kc_page, value ? a.vc_slot : a.kc_slot, dim,
+               units, units == a.slice ? a.by_units : a.by_last);
+}
+
+}  // namespace
+}  // namespace tg
+
+using namespace tg;
+
+extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const tg_paged_evict* r,
+                                                                         void* stream) {
+  const char* what = "launch_paged_evict";
+  if (!r) return refuse(-1, what, "null arguments", 0);
+  if (r->dtype < TG_BF16 || r->dtype > TG_F32) return refuse(-1, what, "unknown dtype", r->dtype);
+  if (const int rc =
+          check_table(what, r->sequences, r->pages, r->page, r->n_indices, r->max_length))
+    return rc;
+  if (r->kv_heads < 1 || r->kv_heads > 0x10000)
+    return refuse(-1, what, "kv_heads must be 1 to 65536", r->kv_heads);
+  if (r->dim < 1 || r->dim > 1024) return refuse(-1, what, "dim must be 1 to 1024", r->dim);
+  if (r->keep < 0 || r->recent < 0 || r->first < 0)
+    return refuse(-1, what, "negative size", r->keep < 0 ? r->keep : r->recent);
+  if (r->keep > (1 << 22)) return refuse(-2, what, "more than 2^22 tokens to keep", r->keep);
+  if (r->recent > r->keep || r->first > r->keep - r->recent)
+    return refuse(-1, what, "first and recent are more than keep", r->first);
+  if (r->move_weights != 0 && r->move_weights != 1)
+    return refuse(-1, what, "move_weights must be 0 or 1", r->move_weights);
+  const int64_t strides[] = {r->kc_page, r->kc_slot, r->kc_head, r->vc_page, r->vc_slot,
+                             r->vc_head, r->w_page,  r->w_slot,  r->w_head};
+  if (const int rc = check_strides(what, strides, 9)) return rc;
+  if (r->sequences == 0) return 0;
+  const Operand kc = {"key_cache", r->key_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->kc_page, r->kc_slot, r->kc_head, 1}};
+  const Operand vc = {"value_cache", r->value_cache, 4, {r->pages, r->page, r->kv_heads, r->dim},
+                      {r->vc_page, r->vc_slot, r->vc_head, 1}};
+  const Operand w = {"weights", r->weights, 3, {r->pages, r->page, r->kv_heads},
+                     {r->w_page, r->w_slot, r->w_head}};
+  const int bytes = r->dtype == TG_F32 ? 4 : 2;
+  const Operand weights = bytes == 4 ? w : in_halves(w);
+  for (const Operand* x : {&kc, &vc})
+    if (const int rc = once(what, *x)) return rc;
+  if (r->move_weights)
+    if (const int rc = once(what, w)) return rc;
+  if (const int rc = apart(what, vc, kc, bytes)) return rc;
+  for (const Operand* x : {&kc, &vc})
+    if (const int rc = apart(what, weights, *x, bytes)) return rc;
+  const Operand lengths = {"lengths", r->lengths, 1, {r->sequences}, {1}};
+  const Operand lengths_out = {"lengths_out", r->lengths_out, 1, {r->sequences}, {1}};
+  if (const int rc = apart(what, lengths_out, lengths, 8)) return rc;
+  if (!r->indptr || !r->lengths || !r->lengths_out || (r->keep && !r->kept) ||
+      (r->n_indices && !r->indices) ||
+      (r->pages && (!r->key_cache || !r->value_cache || !r->weights)))
+    return refuse(-1, what, "null array", r->sequences);
+  Evict a = {};
+  a.key_cache = r->key_cache;
+  a.value_cache = r->value_cache;
+  a.weights = r->weights;
+  a.lengths_out = r->lengths_out;
+  a.kept = r->kept;
+  a.table.indptr = r->indptr;
+  a.table.indices = r->indices;
+  a.table.lengths = r->lengths;
+  a.table.pages = r->pages;
+  a.table.n_indices = r->n_indices;
+  a.table.sequences = static_cast<int>(r->sequences);
+  a.table.page = static_cast<int>(r->page);
+  a.table.by_page = Div(a.table.page);
+  a.kc_page = r->kc_page;
+  a.kc_slot = r->kc_slot;
+  a.kc_head = r->kc_head;
+  a.vc_page = r->vc_page;
+  a.vc_slot = r->vc_slot;
+  a.vc_head = r->vc_head;
+  a.w_page = r->w_page;
+  a.w_slot = r->w_slot;
+  a.w_head = r->w_head;
+  a.kv_heads = static_cast<int>(r->kv_heads);
+  a.dim = static_cast<int>(r->dim);
+  a.keep = static_cast<int>(r->keep);
+  a.recent = static_cast<int>(r->recent);
+  a.first = static_cast<int>(r->first);
+  a.move_weights = static_cast<int>(r->move_weights);
+  a.by_heads = Div(a.kv_heads);
+  const int64_t heads = r->sequences * r->kv_heads;
+  const int units = (a.dim * bytes + 15) / 16;
+  // rows in slices of 64 bytes at least, while there are fewer workgroups than two a compute unit
+  int slices = 1;
+  while (heads * 2 * slices < 512 && units / (2 * slices) >= 4) slices *= 2;
+  a.slice = (units + slices - 1) / slices;
+  a.slices = (units + a.slice - 1) / a.slice;
+  a.by_units = Div(a.slice);
+  a.by_last = Div(units - (a.slices - 1) * a.slice);
+  const int per = 2 * a.slices + a.move_weights;
+  a.by_slices = Div(per);
+  if (heads * per > kMostGroups) return refuse(-2, what, "2^24 workgroups or more", heads * per);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  void* args[] = {&a};
+  const bool small = r->max_length <= 4096;
+  hipError_t e = launch(small ? reinterpret_cast<const void*>(&choose<256, 4096>)
+                              : reinterpret_cast<const void*>(&choose<1024, 32768>),
+                        heads, small ? 256 : 1024, args, s);
+  if (e != hipSuccess) return hip_failed(e, what);
+  if (r->keep == 0) return 0;
+  e = launch(bytes == 4 ? reinterpret_cast<const void*>(&move<uint32_t>)
+                        : reinterpret_cast<const void*>(&move<uint16_t>),
+             heads * per, kMovers, args, s);
+  return e == hipSuccess ? 0 : hip_failed(e, what);
+}
