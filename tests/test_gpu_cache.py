@@ -505,6 +505,13 @@ SHAPES = [
     (10, 2, 256, 5, [120, 31, 600], [5, 4, 300]),
     (6, 2, 128, 16, [1100, 513], [700, 513]),
     (4, 2, 64, 16, [2, 0, 9], [5, 3, 1]),       # fewer tokens than new ones
+    # workgroups of many rows, and rows in parts
+    (16, 1, 64, 16, [600, 300, 0, 257], [500, 20, 0, 2]),
+    (16, 2, 96, 24, [520, 700], [300, 300]),
+    (32, 1, 128, 64, [256, 900, 40], [70, 130, 40]),
+    (32, 2, 256, 7, [300, 129, 128], [160, 1, 128]),
+    (48, 1, 72, 16, [70, 33, 1], [1, 1, 1]),
+    (40, 1, 128, 16, [20, 1], [33, 2]),
 ]
 
 
@@ -522,6 +529,16 @@ def test_attention_weights(hip_ready, dtype, heads, kv_heads, dim, page, lengths
     assert torch.equal(b.w.nan_to_num(-7), got.nan_to_num(-7))
 
 
+@pytest.mark.parametrize("bounds", [dict(max_length=100), dict(max_query=40), dict(max_query=1),
+                                    dict(max_length=1, max_query=130), dict(max_length=5000)])
+def test_attention_weights_past_their_bounds(hip_ready, bounds):
+    """max_length and max_query size the launch: what is longer is right all the same."""
+    b = Batch(BF16, 32, 2, 128, 16, [900, 300, 77], [400, 5, 60]).fill()
+    lse, before = b.lse(), b.w.clone()
+    b.weigh(lse, **bounds)
+    b.check_weights(before, lse)
+
+
 def test_attention_weights_sum_to_one(hip_ready):
     """With prefix_attention's own logarithms, each row's weights sum to one."""
     b = Batch(BF16, 8, 2, 128, 16, [300, 77, 64], [9, 77, 1]).fill()
@@ -537,9 +554,10 @@ def test_attention_weights_sum_to_one(hip_ready):
         assert abs(total - n * 8) <= n * 8 * 2.0 ** -14
 
 
-def test_attention_weights_of_strange_rows_and_keys(hip_ready):
+@pytest.mark.parametrize("heads", [4, 40])
+def test_attention_weights_of_strange_rows_and_keys(hip_ready, heads):
     """Hidden keys may hold anything; rows without keys add nothing; a NaN that is seen is seen."""
-    b = Batch(BF16, 4, 2, 64, 16, [40, 20], [3, 2]).fill()
+    b = Batch(BF16, heads, 2, 64, 16, [40, 20], [3, 2]).fill()
     lse, before = b.lse(), b.w.clone()
     lse[1, 2] = -math.inf
     b.weigh(lse)
@@ -559,8 +577,9 @@ def test_attention_weights_of_strange_rows_and_keys(hip_ready):
     assert torch.equal(b.w.nan_to_num(-7), want.nan_to_num(-7))
 
 
-def test_attention_weights_of_lost_pages(hip_ready):
-    b = Batch(F16, 8, 2, 64, 8, [50, 40, 30], [3, 1, 30]).fill()
+@pytest.mark.parametrize("counts", [[3, 1, 4], [3, 1, 30]])
+def test_attention_weights_of_lost_pages(hip_ready, counts):
+    b = Batch(F16, 8, 2, 64, 8, [50, 40, 30], counts).fill()
     lse = b.lse()
     indices = b.indices.clone()
     indices[1], indices[int(b.indptr[1]) + 2] = -5, b.pages + 3
