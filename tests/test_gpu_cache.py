@@ -491,6 +491,8 @@ def test_append_leaves_out_what_has_no_place(hip_ready):
 # --------------------------------------------------------------------------- #
 # the weight of keys
 # --------------------------------------------------------------------------- #
+MANY = dict(max_query=10 ** 6, max_length=1100)     # bounds that make workgroups of many rows
+
 SHAPES = [
     # heads, kv_heads, dim, page, lengths, counts
     (4, 2, 64, 16, [70, 33, 1], [1, 1, 1]),
@@ -515,17 +517,18 @@ SHAPES = [
 ]
 
 
+@pytest.mark.parametrize("bounds", [dict(), MANY])
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("heads,kv_heads,dim,page,lengths,counts", SHAPES)
-def test_attention_weights(hip_ready, dtype, heads, kv_heads, dim, page, lengths, counts):
+def test_attention_weights(hip_ready, dtype, heads, kv_heads, dim, page, lengths, counts, bounds):
     b = Batch(dtype, heads, kv_heads, dim, page, lengths, counts, seed=dim,
               side_by_side=page != 16).fill()
     lse, before = b.lse(), b.w.clone()
-    assert b.weigh(lse, decay=0.75) is b.w
+    assert b.weigh(lse, decay=0.75, **bounds) is b.w
     b.check_weights(before, lse, decay=0.75)
-    # the same bits again, whatever bounds the launch was sized by
+    # the same bits again
     got, b.w = b.w, before.clone()
-    b.weigh(lse, decay=0.75)
+    b.weigh(lse, decay=0.75, **bounds)
     assert torch.equal(b.w.nan_to_num(-7), got.nan_to_num(-7))
 
 
@@ -557,23 +560,24 @@ def test_attention_weights_sum_to_one(hip_ready):
 @pytest.mark.parametrize("heads", [4, 40])
 def test_attention_weights_of_strange_rows_and_keys(hip_ready, heads):
     """Hidden keys may hold anything; rows without keys add nothing; a NaN that is seen is seen."""
-    b = Batch(BF16, heads, 2, 64, 16, [40, 20], [3, 2]).fill()
+    b = Batch(BF16, heads, 2, 64, 16, [40, 20], [3, 2] if heads == 4 else [7, 8]).fill()
+    bounds = dict(max_query=10 ** 6, max_length=5000) if heads > 4 else {}
     lse, before = b.lse(), b.w.clone()
     lse[1, 2] = -math.inf
-    b.weigh(lse)
+    b.weigh(lse, **bounds)
     b.check_weights(before, lse)
     # a later token's key is not seen by earlier rows, and stands for itself alone
     page, slot = b.places(0)
     b.kc[page[39], slot[39]] = math.nan
     want, b.w = b.w.clone(), before.clone()
-    b.weigh(lse)
+    b.weigh(lse, **bounds)
     assert b.w[page[39], slot[39]].isnan().all()
     want[page[39], slot[39]] = math.nan
     assert torch.equal(b.w.nan_to_num(-7), want.nan_to_num(-7))
     # rows of no sequence hold anything
     query, b.query = b.query, torch.cat([b.query, torch.full_like(b.query, math.nan)])
     b.w = before.clone()
-    b.weigh(torch.cat([lse, torch.full_like(lse, math.nan)]))
+    b.weigh(torch.cat([lse, torch.full_like(lse, math.nan)]), **bounds)
     assert torch.equal(b.w.nan_to_num(-7), want.nan_to_num(-7))
 
 
@@ -585,9 +589,9 @@ def test_attention_weights_of_lost_pages(hip_ready, counts):
     indices[1], indices[int(b.indptr[1]) + 2] = -5, b.pages + 3
     kept = b.indices
     before, b.indices = b.w.clone(), indices
-    b.weigh(lse)
+    b.weigh(lse, **(MANY if max(counts) > 4 else {}))
     got, b.w, b.indices = b.w.clone(), before.clone(), kept
-    b.weigh(lse)
+    b.weigh(lse, **(MANY if max(counts) > 4 else {}))
     same = torch.ones(b.pages, dtype=torch.bool, device="cuda")
     lost = kept[[1, int(b.indptr[1]) + 2]]
     same[lost] = False

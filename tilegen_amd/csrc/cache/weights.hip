@@ -24,9 +24,10 @@ struct Weights {
   i64 q_token, q_head, l_token, l_head, kc_page, kc_slot, kc_head, w_page, w_slot, w_head;
   float* part;            // [unit, part, keys of a workgroup]: sums of a part of the rows
   int heads, kv_heads, group, dim, chunk, splits;
-  int parts, part_rows;   // wide: a sequence's rows are cut into parts of so many
+  int parts, part_stages; // wide: a sequence's stages of rows are cut into parts of so many
+  int stage_rows;         // of 64: whole tokens' where a group fits
   float scale, decay;     // scale * log2 e
-  Div by_group, by_heads, by_splits, by_parts;
+  Div by_group, by_heads, by_splits, by_parts, by_stage;
 };
 
 
@@ -124,17 +125,22 @@ __global__ __launch_bounds__(64 * kWaves) void weigh_narrow(Weights a) {
   }
 }
 
-// Many rows.  A wave keeps KT tiles of 32 keys in registers, a workgroup reads the rows once for its
-// four: the next stage of 64 rows is in flight to registers while this one's scores are taken from
-// LDS.
+// Many rows.  A wave keeps KT tiles of 32 keys in registers, a workgroup reads the rows for its four:
+// a stage of up to 64 rows (of heads over 128 32), whole tokens', is taken from LDS while the next
+// one is in flight to registers.  A tile's exponentials and sums run between the products of the
+// next tile: 8 products of 32 cycles beside 16 times (fma, exponential, add) of 4, 8 and 4.
+constexpr int wide_rows(int dim) { return dim > 128 ? 32 : 64; }
+
 template <int DP>
 struct Wide {
   static constexpr int KT = DP > 128 ? 1 : 2;             // tiles of a wave
   static constexpr int kKeys = 32 * KT * kWaves;          // of a workgroup
-  static constexpr int kRows = 64;                        // of a stage
+  static constexpr int kRows = wide_rows(DP);             // of a stage, some of them empty
   static constexpr int kUnits = DP / 8;                   // of 16 bytes of a row
+  static constexpr int kLanes = DP == 96 ? 16 : kUnits;   // that read a row
   static constexpr int kRow = DP * 2 + 16;                // bytes of a row in LDS: an odd number of units
-  static constexpr int kEach = kRows * kUnits / (64 * kWaves);
+  static constexpr int kStep = 64 * kWaves / kLanes;      // rows that a workgroup reads at once
+  static constexpr int kEach = kRows / kStep;
 };
 
 template <typename T, int DP>
@@ -149,19 +155,31 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
   __shared__ int s_strange[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int col = lane & 31, half = lane >> 5;
-  // the kv heads side by side (each XCD has its own of 8), the parts of the same keys next
+  // the kv heads side by side (each XCD has its own of 8), then those that read the same rows
   const int unit = a.by_heads(blockIdx.x), kv_head = blockIdx.x - unit * a.kv_heads;
-  const int up = a.by_parts(unit), part = unit - up * a.parts;
-  const int b = a.by_splits(up), split = up - b * a.splits;
+  const int up = a.by_splits(unit), split = unit - up * a.splits;
+  const int b = a.by_parts(up), part = up - b * a.parts;
   const Own s = own_of(a.table, b);
   const int first_key = split * W::kKeys;
   if (s.count == 0 || first_key >= s.keys) return;
   const int rows = s.count * a.group;
+  const int stages = a.by_stage(rows + a.stage_rows - 1);
   const int key_blocks = split + 1 < a.splits ? 1 : (s.keys - first_key + W::kKeys - 1) / W::kKeys;
   const T* q_head = static_cast<const T*>(a.query) + s.first * a.q_token +
                     kv_head * a.group * a.q_head;
   const float* l_head = a.lse + s.first * a.l_token + kv_head * a.group * a.l_head;
   const T* kc = static_cast<const T*>(a.key_cache) + kv_head * a.kc_head;
+
+  // this thread's unit of the rows r0 + i kStep of a stage, and where they stand from the first
+  const int unit_at = (tid & (W::kLanes - 1)) * 8, r0 = tid / W::kLanes;
+  uint32_t off[W::kEach];   // bytes
+#pragma unroll
+  for (int i = 0; i < W::kEach; ++i) {
+    const int r = r0 + i * W::kStep, j = a.by_group(r);
+    off[i] = unit_at < a.dim ? static_cast<uint32_t>(2 * (j * a.q_token + (r - j * a.group) *
+                                                          a.q_head + unit_at))
+                             : 0x80000000u;
+  }
 
   // (keys past the bound that sized the launch: the last split takes them in turn, its first part
   // with all rows)
@@ -170,26 +188,42 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     const int key0 = first_key + block * W::kKeys + wave * 32 * KT;
     // from the first token that sees the first key on
     const int seen_from =
-        (max(first_key + block * W::kKeys - s.before, 0) * a.group) & -W::kRows;
-    const int row_begin = whole ? seen_from : max(seen_from, part * a.part_rows);
-    const int row_end =
-        whole || part + 1 == a.parts ? rows : min(rows, (part + 1) * a.part_rows);
-    if (!whole && row_begin >= row_end) continue;
+        a.by_stage(max(first_key + block * W::kKeys - s.before, 0) * a.group);
+    const int begin = whole ? seen_from : max(seen_from, part * a.part_stages);
+    const int end = whole || part + 1 == a.parts ? stages : min(stages, (part + 1) * a.part_stages);
+    if (!whole && begin >= end) continue;
     s16x8 k[KT][KS];
+    const T* k_at[KT];
+    bool bad[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       const int key = min(key0 + 32 * t + col, s.keys - 1);
       const int nth = a.table.by_page(key);
       const i64 page = s.list[nth];
-      const bool bad = page < 0 || page >= a.table.pages;
-      const T* from =
-          kc + (bad ? 0 : page * a.kc_page + (key - nth * a.table.page) * a.kc_slot) + 8 * half;
+      bad[t] = page < 0 || page >= a.table.pages;
+      k_at[t] = kc + (bad[t] ? 0 : page * a.kc_page + (key - nth * a.table.page) * a.kc_slot);
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {    // (elements past the head: any of it, zero below)
+        const int d = 16 * i + 8 * half;
+        k[t][i] = __builtin_bit_cast(s16x8, C::load(k_at[t] + (d < a.dim ? d : 0)));
+      }
+    }
+    bool odd = false;     // an infinity or NaN among the keys: rows that are 0 would be NaN
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
 #pragma unroll
       for (int i = 0; i < KS; ++i)
-        k[t][i] = !bad && 16 * i + 8 * half < a.dim
-                      ? __builtin_bit_cast(s16x8, C::load(from + 16 * i))
-                      : s16x8(0);
+        if (bad[t] || 16 * i + 8 * half >= a.dim) k[t][i] = s16x8(0);
+      f32x16 zero = f32x16(0.f);
+#pragma unroll
+      for (int i = 0; i < KS; ++i) zero = M::mul32(k[t][i], s16x8(0), zero);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) odd |= zero[e] != 0.f;
     }
+    odd = __any(odd);
     float sum[KT][16];
 #pragma unroll
     for (int t = 0; t < KT; ++t)
@@ -199,75 +233,144 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     s16x8 next[W::kEach];
     float next_lse = 0.f;
     int next_see = 0;
-    auto load = [&](int row0) {
+    auto load = [&](int stage) __attribute__((always_inline)) {
+      const int row0 = stage * a.stage_rows, left = min(rows - row0, a.stage_rows);
+      const T* from = q_head + static_cast<i64>(a.by_group(row0)) * a.q_token;
+      const auto memory = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, 0x7FFFFFFF,
+                                                            0x00027000);
 #pragma unroll
-      for (int i = 0; i < W::kEach; ++i) {
-        const int at = tid + i * 64 * kWaves, r = at / W::kUnits, d = (at - r * W::kUnits) * 8;
-        const int row = min(row0 + r, rows - 1), j = a.by_group(row);
-        next[i] = d < a.dim ? __builtin_bit_cast(s16x8, C::load(q_head + j * a.q_token +
-                                                                (row - j * a.group) * a.q_head + d))
-                            : s16x8(0);
-      }
+      for (int i = 0; i < W::kEach; ++i)    // (past the last row: out of range, zero)
+        next[i] = __builtin_bit_cast(
+            s16x8, __builtin_amdgcn_raw_buffer_load_b128(
+                       memory, r0 + i * W::kStep < left ? off[i] : 0x80000000u, 0, 0));
       if (wave == 0) {
         const int row = min(row0 + lane, rows - 1), j = a.by_group(row);
         next_lse = l_head[j * a.l_token + (row - j * a.group) * a.l_head];
-        next_see = row0 + lane < row_end && next_lse != -INFINITY ? s.before + j + 1 : 0;
+        next_see = lane < left ? s.before + j + 1 : INT32_MIN;
       }
     };
-    auto put = [&](int to) {
+    auto put = [&](int to) __attribute__((always_inline)) {
+      if (unit_at < DP) {
 #pragma unroll
-      for (int i = 0; i < W::kEach; ++i) {
-        const int at = tid + i * 64 * kWaves, r = at / W::kUnits, u = at - r * W::kUnits;
-        *reinterpret_cast<s16x8*>(&s_rows[to][r * W::kRow + u * 16]) = next[i];
+        for (int i = 0; i < W::kEach; ++i)
+          *reinterpret_cast<s16x8*>(&s_rows[to][(r0 + i * W::kStep) * W::kRow + 2 * unit_at]) =
+              next[i];
       }
       if (wave == 0) {
-        s_base[to][lane] = next_lse * kLog2e;
-        s_see[to][lane] = next_see;
-        const int strange = __any(next_see == 0);
+        const bool live = next_see != INT32_MIN;
+        if (lane < W::kRows) {
+          s_base[to][lane] = live ? next_lse * kLog2e : INFINITY;
+          s_see[to][lane] = live && next_lse != -INFINITY ? next_see : 0;
+        }
+        const int strange = __any(live && !(fabsf(next_lse) < INFINITY));
         if (lane == 0) s_strange[to] = strange;
       }
     };
-    if (row_begin < row_end) {
-      load(row_begin);
+
+    // q: rows 32 h .. of a stage; before: the scores of the tile before, which are added up between
+    // the products of this one; see: of the lane's keys, counted from its first
+    s16x8 q[KS];
+    float base = 0.f, base_before = 0.f;
+    int see = 0;
+    f32x16 before = f32x16(-INFINITY);
+    auto fetch = [&](int at, int h, int i) __attribute__((always_inline)) {
+      q[i] = *reinterpret_cast<const s16x8*>(
+          &s_rows[at][(32 * h + col) * W::kRow + 16 * half + 32 * i]);
+    };
+    auto fetch_row = [&](int at, int h) __attribute__((always_inline)) {
+      base = s_base[at][32 * h + col];
+      see = s_see[at][32 * h + col] - key0 - 4 * half;
+    };
+    // TILE's products; then, in the last tile of these rows, the rows 32 h of buffer `at` are read
+    auto step = [&](auto tile, bool masked, int at, int h) __attribute__((always_inline)) {
+      constexpr int TILE = decltype(tile)::value, LAST = TILE == KT - 1;
+      constexpr int BEFORE = TILE ? TILE - 1 : KT - 1;
+      f32x16 sc;
+      if (masked) {     // scores start from -inf where a row does not see a key
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          sc[e] = 32 * TILE + 8 * (e / 4) + e % 4 < see ? 0.f : -INFINITY;
+        sc = M::mul32(k[TILE][0], q[0], sc);
+      } else {
+        sc = M::mul32(k[TILE][0], q[0], f32x16(0.f));
+      }
+#pragma unroll
+      for (int i = 0; i < KS; ++i) {
+        if (i) sc = M::mul32(k[TILE][i], q[i], sc);
+        if (LAST) fetch(at, h, i);
+#pragma unroll
+        for (int e = 16 * i / KS; e < 16 * (i + 1) / KS; ++e)
+          sum[BEFORE][e] +=
+              __builtin_amdgcn_exp2f(__builtin_fmaf(before[e], a.scale, -base_before));
+      }
+      // (the sums stay here: they would be taken behind all products otherwise)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) asm volatile("" : "+v"(sum[BEFORE][e]));
+      before = sc;
+      base_before = base;
+      if (LAST) fetch_row(at, h);
+    };
+    auto rows32 = [&](bool masked, int at, int h) __attribute__((always_inline)) {
+      step(std::integral_constant<int, 0>{}, masked, at, h);
+      if constexpr (KT > 1) step(std::integral_constant<int, KT - 1>{}, masked, at, h);
+    };
+
+    bool strange = false;
+    if (begin < end) {
+      load(begin);
       put(0);
-    }
-    __syncthreads();
-    int at = 0;
-    for (int row0 = row_begin; row0 < row_end; row0 += W::kRows, at ^= 1) {
-      const bool more = row0 + W::kRows < row_end;
-      if (more) load(row0 + W::kRows);
-      // every row of the stage sees every key of the wave's, or some may not
-      const bool masked =
-          s_strange[at] || s.before + static_cast<int>(a.by_group(row0)) + 1 < key0 + 32 * KT;
+      if (begin + 1 < end) load(begin + 1);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < KS; ++i) fetch(0, 0, i);
+      fetch_row(0, 0);
+      int at = 0;
 #pragma unroll 1
-      for (int h = 0; h < 2; ++h) {
-        const char* from = &s_rows[at][(32 * h + col) * W::kRow + 16 * half];
-        s16x8 q[KS];
+      for (int stage = begin; stage < end; ++stage, at ^= 1) {
+        strange |= s_strange[at] != 0;
+        const int token = a.by_group(stage * a.stage_rows);
+        const bool masked = __builtin_amdgcn_readfirstlane(s.before + token + 1 < key0 + 32 * KT);
+        if constexpr (W::kRows == 64) rows32(masked, at, 1);
+        // this buffer's rows are all in registers, the next stage's go to the other
+        if (stage + 1 < end) put(at ^ 1);
+        __syncthreads();
+        if (stage + 2 < end) load(stage + 2);
+        rows32(masked, at ^ 1, 0);
+      }
 #pragma unroll
-        for (int i = 0; i < KS; ++i) q[i] = *reinterpret_cast<const s16x8*>(from + 32 * i);
-        const float base = s_base[at][32 * h + col];
-        const int see = s_see[at][32 * h + col];
+      for (int e = 0; e < 16; ++e)
+        sum[KT - 1][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(before[e], a.scale, -base_before));
+    }
+    if (__syncthreads_or(odd || strange)) {
+      // infinities or NaN among the keys or the logarithms: once more, adding what is seen alone
 #pragma unroll
-        for (int t = 0; t < KT; ++t) {
-          f32x16 sc = f32x16(0.f);
+      for (int t = 0; t < KT; ++t)
 #pragma unroll
-          for (int i = 0; i < KS; ++i) sc = M::mul32(k[t][i], q[i], sc);
-          if (!masked) {
+        for (int e = 0; e < 16; ++e) sum[t][e] = 0.f;
+#pragma unroll 1
+      for (int stage = begin; stage < end; ++stage) {
+        load(stage);
+        put(0);
+        __syncthreads();
+#pragma unroll 1
+        for (int h = 0; h < W::kRows / 32; ++h) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sum[t][i] += __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.scale, -base));
-          } else {
+          for (int i = 0; i < KS; ++i) fetch(0, h, i);
+          fetch_row(0, h);
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[i], a.scale, -base));
-              const int key = key0 + 32 * t + 8 * (i / 4) + 4 * half + i % 4;
-              sum[t][i] += key < see ? e : 0.f;
+          for (int t = 0; t < KT; ++t) {
+            f32x16 sc = f32x16(0.f);
+#pragma unroll
+            for (int i = 0; i < KS; ++i) sc = M::mul32(k[t][i], q[i], sc);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[e], a.scale, -base));
+              sum[t][e] += 32 * t + 8 * (e / 4) + e % 4 < see ? x : 0.f;
             }
           }
         }
+        __syncthreads();
       }
-      if (more) put(at ^ 1);
-      __syncthreads();
     }
 
     // over the 32 rows that lanes hold; lane (half, c) of 16 has key 8 (c / 4) + 4 half + c % 4
@@ -305,13 +408,13 @@ __global__ __launch_bounds__(256) void join_weights(Weights a, int keys) {
   const Own s = own_of(a.table, b);
   const int first_key = split * keys, key = first_key + threadIdx.x;
   if (s.count == 0 || static_cast<int>(threadIdx.x) >= keys || key >= s.keys) return;
-  const int rows = s.count * a.group;
-  const int seen_from = (max(first_key - s.before, 0) * a.group) & -64;
-  const int last = min(a.parts - 1, (rows - 1) / a.part_rows);
+  const int stages = a.by_stage(s.count * a.group + a.stage_rows - 1);
+  const int seen_from = a.by_stage(max(first_key - s.before, 0) * a.group);
+  const int last = min(a.parts - 1, (stages - 1) / a.part_stages);
   float sum = 0.f;
-  for (int part = min(seen_from / a.part_rows, a.parts - 1); part <= last; ++part)
-    sum += a.part[((static_cast<i64>(unit) * a.parts + part) * a.kv_heads + kv_head) * keys +
-                  threadIdx.x];
+  for (int part = min(seen_from / a.part_stages, a.parts - 1); part <= last; ++part)
+    sum += a.part[((static_cast<i64>(b * a.parts + part) * a.splits + split) * a.kv_heads + kv_head) *
+                      keys + threadIdx.x];
   const int nth = a.table.by_page(key);
   const i64 page = s.list[nth];
   if (page < 0 || page >= a.table.pages) return;
@@ -407,17 +510,28 @@ int plan(const tg_attention_weights* r, Plan* p) {
   const int64_t bound = r->max_query < r->tokens ? r->max_query : r->tokens;
   const int64_t rows = (r->query_indptr && bound > 0 ? bound : 1) * a.group;   // of a sequence
   a.parts = 1;
-  if (rows > 32) {
+  // Wide for many rows (whole tokens in a stage, within 32 bits of its first).  32 sequences of up to
+  // 2048 keys, 8 kv heads of 128: 64 rows 28 us narrow, 36 wide; 128 rows 40 both; 256 rows 63 and
+  // 47; 1024 rows 199 and 92.  One of 16384 keys, 128 rows: 14.2 and 13.0.  4 of up to 700 keys, 4
+  // kv heads of 64: 256 rows 10.4 and 12.6, 512 rows 16.7 and 17.2, 1024 rows 29 and 26.
+  const int64_t room = wide_rows(a.dim), tokens = room / a.group;
+  auto within = [](int64_t steps, int64_t stride) {
+    return steps == 0 || (stride >= 0 && stride <= (int64_t(1) << 28) / steps);
+  };
+  if (rows >= 128 && (length > 1024 || rows > 512) && tokens > 0 && within(tokens - 1, r->query_token) &&
+      within(a.group - 1, r->query_head)) {
     p->keys = a.dim > 128 ? 128 : 256;
     a.splits = static_cast<int>((length + p->keys - 1) / p->keys);
-    // Parts of the rows, at least 16 stages each, while there are few workgroups: earlier keys are
-    // seen by more rows, so that a round of workgroups with all rows ends with a few long ones.
-    const int64_t units = heads * a.splits, stages = (rows + 63) / 64;
-    int64_t parts = units ? 2048 / units : 1;
+    a.stage_rows = static_cast<int>(tokens * a.group);
+    a.by_stage = Div(a.stage_rows);
+    // Parts of the rows, at least so many stages each, while there are few workgroups: earlier keys
+    // are seen by more rows, so that a round of workgroups with all rows ends with a few long ones.
+    const int64_t units = heads * a.splits, stages = (rows + a.stage_rows - 1) / a.stage_rows;
+    int64_t parts = units ? 4096 / units : 1;
     if (parts > stages / 16) parts = stages / 16;
     if (parts > 1) {
-      a.part_rows = static_cast<int>((stages + parts - 1) / parts * 64);
-      a.parts = static_cast<int>((rows + a.part_rows - 1) / a.part_rows);
+      a.part_stages = static_cast<int>((stages + parts - 1) / parts);
+      a.parts = static_cast<int>((stages + a.part_stages - 1) / a.part_stages);
     }
     p->groups = units * a.parts;
     if (a.parts > 1) p->bytes = p->groups * p->keys * 4;
