@@ -2,8 +2,8 @@
 // head by one workgroup, then workgroups for slices of each head move what has to.
 //
 // Of the C candidates between the first and the recent tokens the n heaviest stay.  Weights map to
-// whole numbers of the same order, and the n-th largest is found digit by digit from the top, by
-// counting.  Ties at it go to the lowest positions, by a scan over the positions' counts.  Moves:
+// whole numbers of the same order, which threads hold in registers, and the n-th largest is found
+// digit by digit from the top, by counting.  Ties at it go to the lowest positions.  Moves:
 // tokens that stay below `front` are left alone; the others are as many as the holes there, and
 // both lists are taken in order.  No place is both a source and a target of those, so they go in
 // any order; then the recent tokens go down, chunk by chunk, each read whole before it is
@@ -59,153 +59,227 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return x >> 31 ? ~x : x | 0x80000000u;
 }
 
-constexpr int kWindow = 2048;     // moves that are listed at a time
+// The sum of a value over a wave's lanes up to each.
+__device__ __forceinline__ int upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below,
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // within 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last lane of each 16 to
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // the next, of 32 to the other
+  return v;
+}
 
-// THREADS a workgroup; keys of the first CACHED candidates stay in LDS.
-template <int THREADS, int CACHED>
-__global__ __launch_bounds__(THREADS) void choose(Evict a) {
-  constexpr int kWaves = THREADS / 64;
-  constexpr int kBins = 2048, kCopies = 2;
-  __shared__ uint32_t s_keys[CACHED];
-  __shared__ uint32_t s_bins[kCopies][kBins];   // later the list of moves
-  __shared__ int s_wave[2][kWaves];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
-  static_assert(kWindow <= kCopies * kBins, "");
-  int* s_list = reinterpret_cast<int*>(&s_bins[0][0]);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
-  const Held s = held_of(a, b);
-  const int gone = s.keys > a.keep ? s.keys - a.keep : 0;
-  int32_t* kept = a.kept + static_cast<i64>(blockIdx.x) * a.keep;
-  if (h == 0 && tid == 0) a.lengths_out[b] = s.keys - gone;
-  if (gone == 0) {
-    for (int i = tid; i < a.keep; i += THREADS) kept[i] = i < s.keys ? i : -1;
-    return;
+// What a workgroup that chooses shares.
+constexpr int kBins = 256, kCopies = 8, kCopy = kBins + 1;   // copies start in banks of their own
+template <int WAVES, int MOVES>
+struct Shared {
+  uint32_t bins[kCopies * kCopy];
+  int waves[2][WAVES];
+  uint32_t prefix;
+  int left, equal;
+  uint32_t moves[MOVES];
+};
+
+// After a digit's counts: in which bin the `left`-th largest is, how many of it are left, and how
+// many it holds.  Bins are counted from the largest down, one a thread.
+template <int THREADS, typename S>
+__device__ __forceinline__ void find_bin(S& s, uint32_t prefix, int left) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bin = kBins - 1 - tid;
+  int mine = 0;
+  if (tid < kBins) {
+#pragma unroll
+    for (int c = 0; c < kCopies; ++c) mine += s.bins[c * kCopy + bin];
   }
-  const int front = a.keep - a.recent;
-  for (int i = tid; i < a.keep; i += THREADS)
-    if (i < a.first || i >= front) kept[i] = i < front ? i : i + gone;
-  const int want = front - a.first;           // of the candidates
-  if (want == 0) return;
-  const int count = s.keys - a.recent - a.first;
+  int sum = upto(mine);
+  if (lane == 63) s.waves[0][wave] = sum;
+  __syncthreads();
+  if (tid < kBins) {
+    for (int w = 0; w < wave; ++w) sum += s.waves[0][w];
+    if (sum - mine < left && sum >= left) {
+      s.prefix = prefix << 8 | static_cast<uint32_t>(bin);
+      s.left = left - (sum - mine);
+      s.equal = mine;
+    }
+  }
+  __syncthreads();
+}
 
-  auto fetch = [&](int c) {     // candidate c's key
-    const Place at = place_of(a, s.list, a.first + c);
-    return at.page < 0 ? 0u : order_of(a.weights[at.page * a.w_page + at.slot * a.w_slot +
-                                                 h * a.w_head]);
-  };
-  auto key = [&](int c) { return c < CACHED ? s_keys[c] : fetch(c); };
-#pragma unroll 4
-  for (int c = tid; c < min(count, CACHED); c += THREADS) s_keys[c] = fetch(c);
+template <int THREADS, typename S>
+__device__ __forceinline__ void clear_bins(S& s) {
+#pragma unroll
+  for (int i = 0; i < (kCopies * kCopy + THREADS - 1) / THREADS; ++i)
+    if (threadIdx.x + i * THREADS < kCopies * kCopy) s.bins[threadIdx.x + i * THREADS] = 0;
+  __syncthreads();
+}
 
-  // the want-th largest, by digits of 11, 11 and 10 bits; `left` of those equal to it stay
+// Of a sequence and kv head that loses tokens: what stays, from keys that threads hold, EACH to a
+// thread (candidate tid + k THREADS).
+template <int THREADS, int EACH, typename S, typename F>
+__device__ __forceinline__ void choose_held(S& s, int count, int first, int front, int32_t* kept,
+                                            F&& place) {
+  constexpr int kWaves = THREADS / 64, kRuns = EACH * kWaves;   // of 64 candidates
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  uint32_t key[EACH];
+  constexpr int kAtOnce = EACH < 8 ? EACH : 8;
+#pragma unroll
+  for (int k0 = 0; k0 < EACH; k0 += kAtOnce) {
+    const float* at[kAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) {
+      const int c = tid + (k0 + k) * THREADS;
+      at[k] = c < count ? place(first + c) : nullptr;
+    }
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k) key[k0 + k] = at[k] ? order_of(*at[k]) : 0u;
+  }
+  // the (front - first)-th largest, by digits of 8 bits; done when all that a bin holds stay
   uint32_t prefix = 0;
-  int left = want;
-#pragma unroll 1
-  for (int digit = 0; digit < 3; ++digit) {
-    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
-    const int bins = digit == 2 ? 1024 : kBins;
-    for (int i = tid; i < kCopies * kBins; i += THREADS) (&s_bins[0][0])[i] = 0;
+  int left = front - first, equal = 0, shift = 32;
+  do {
+    shift -= 8;
+    clear_bins<THREADS>(s);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (tid + k * THREADS < count && (shift == 24 || key[k] >> (shift + 8) == prefix))
+        atomicAdd(&s.bins[(lane % kCopies) * kCopy + (key[k] >> shift & 255)], 1u);
     __syncthreads();
+    find_bin<THREADS>(s, prefix, left);
+    prefix = s.prefix;
+    left = s.left;
+    equal = s.equal;
+  } while (shift && left != equal);
+  const uint32_t least = prefix << shift;       // what is above stays, and of what is equal `left`
+  const bool ties = left != equal;
+
+  // Places among the flagged, run by run of 64 candidates.
+  int* runs = reinterpret_cast<int*>(s.bins);
+  static_assert(kRuns <= kCopies * kCopy && kRuns <= 16 * 64, "");
+  uint64_t mask[EACH];
+  auto rank = [&](auto&& flag) __attribute__((always_inline)) {
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) {
+      mask[k] = __ballot(flag(k, tid + k * THREADS));
+      if (lane == 0) runs[k * kWaves + wave] = __popcll(mask[k]);
+    }
+    __syncthreads();
+    if (wave == 0) {
+      int before = 0;
+      for (int r = lane; r < (kRuns + 63) / 64 * 64; r += 64) {
+        const int n = r < kRuns ? runs[r] : 0, sum = upto(n);
+        if (r < kRuns) runs[r] = before + sum - n;
+        before += __builtin_amdgcn_readlane(sum, 63);
+      }
+      if (lane == 0) s.left = before;
+    }
+    __syncthreads();
+  };
+  auto nth = [&](int k) __attribute__((always_inline)) {
+    return runs[k * kWaves + wave] + __popcll(mask[k] & ((1ull << lane) - 1));
+  };
+  uint32_t stays = 0;
+  if (ties) {
+    rank([&](int k, int c) { return c < count && key[k] == least; });
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (tid + k * THREADS < count &&
+          (key[k] > least || (key[k] == least && nth(k) < left)))
+        stays |= 1u << k;
+  } else {
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if (tid + k * THREADS < count && key[k] >= least) stays |= 1u << k;
+  }
+  // holes below the front, then as many that stay past it, which fill them
+  rank([&](int k, int c) {
+    return c < count && (first + c < front) != static_cast<bool>(stays >> k & 1);
+  });
+  const int holes = s.left / 2;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int p = first + tid + k * THREADS;
+    if (p >= front && (stays >> k & 1)) s.moves[nth(k) - holes] = p;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int p = first + tid + k * THREADS;
+    if (p < front && p - first < count)
+      kept[p] = stays >> k & 1 ? p : static_cast<int>(s.moves[nth(k)]);
+  }
+}
+
+// The same from memory, key by key, for any number of candidates.  Each thread has a run of them
+// for the places; moves are listed some at a time.
+template <int THREADS, int MOVES, typename S, typename F>
+__device__ __forceinline__ void choose_any(S& s, int count, int first, int front, int32_t* kept,
+                                        F place) {
+  constexpr int kWaves = THREADS / 64;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto key = [&](int c) {
+    const float* at = place(first + c);
+    return at ? order_of(*at) : 0u;
+  };
+  uint32_t prefix = 0;
+  int left = front - first;
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    clear_bins<THREADS>(s);
+#pragma unroll 8
     for (int c = tid; c < count; c += THREADS) {
       const uint32_t k = key(c);
-      if (digit == 0 || k >> (shift + (digit == 1 ? 11 : 10)) == prefix)
-        atomicAdd(&s_bins[lane % kCopies][k >> shift & (bins - 1)], 1u);
+      if (shift == 24 || k >> (shift + 8) == prefix)
+        atomicAdd(&s.bins[(lane % kCopies) * kCopy + (k >> shift & 255)], 1u);
     }
     __syncthreads();
-    // each thread takes a run of bins, from the largest down
-    const int run = bins / THREADS > 0 ? bins / THREADS : 1;
-    const int top = bins - 1 - tid * run;
-    int mine = 0;
-    for (int i = 0; i < run && top - i >= 0; ++i) {
-      int n = 0;
-#pragma unroll
-      for (int copy = 0; copy < kCopies; ++copy) n += s_bins[copy][top - i];
-      mine += n;
-    }
-    int before = mine;          // of the threads up to this one
-    for (int d = 1; d < 64; d *= 2) {
-      const int other = __shfl_up(before, d);
-      if (lane >= d) before += other;
-    }
-    if (lane == 63) s_wave[0][wave] = before;
-    __syncthreads();
-    for (int w = 0; w < wave; ++w) before += s_wave[0][w];
-    before -= mine;
-    if (before < left && before + mine >= left) {
-      for (int i = 0; i < run; ++i) {
-        int n = 0;
-#pragma unroll
-        for (int copy = 0; copy < kCopies; ++copy) n += s_bins[copy][top - i];
-        if (before + n >= left) {
-          s_prefix = prefix << (digit == 2 ? 10 : 11) | static_cast<uint32_t>(top - i);
-          s_left = left - before;
-          break;
-        }
-        before += n;
-      }
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    left = s_left;
-    __syncthreads();
+    find_bin<THREADS>(s, prefix, left);
+    prefix = s.prefix;
+    left = s.left;
   }
-
-  // each thread takes a run of candidates (an odd number: LDS banks); two exclusive sums at once
-  const int run = (count + THREADS - 1) / THREADS | 1;
+  const int run = (count + THREADS - 1) / THREADS;
   const int c0 = min(static_cast<int64_t>(tid) * run, static_cast<int64_t>(count));
   const int c1 = min(c0 + run, count);
-  auto scan = [&](int& x, int& y) {
-    int u = x, v = y;
-    for (int d = 1; d < 64; d *= 2) {
-      const int other_u = __shfl_up(u, d), other_v = __shfl_up(v, d);
-      if (lane >= d) {
-        u += other_u;
-        v += other_v;
-      }
-    }
+  auto scan = [&](int& x, int& y) {     // sums over the threads before
+    const int u = upto(x), v = upto(y);
     if (lane == 63) {
-      s_wave[0][wave] = u;
-      s_wave[1][wave] = v;
+      s.waves[0][wave] = u;
+      s.waves[1][wave] = v;
     }
     __syncthreads();
-    for (int w = 0; w < wave; ++w) {
-      u += s_wave[0][w];
-      v += s_wave[1][w];
-    }
     x = u - x;
     y = v - y;
+    for (int w = 0; w < wave; ++w) {
+      x += s.waves[0][w];
+      y += s.waves[1][w];
+    }
     __syncthreads();
   };
   int ties = 0, none = 0;
   for (int c = c0; c < c1; ++c) ties += key(c) == prefix;
   scan(ties, none);
-  // candidates below the front stay where they are, or leave a hole; those past it fill one
-  int holes = 0, fills = 0;
   auto each = [&](auto&& visit) {
     int tie = ties;
     for (int c = c0; c < c1; ++c) {
       const uint32_t k = key(c);
       const bool stays = k > prefix || (k == prefix && tie < left);
       tie += k == prefix;
-      visit(a.first + c, stays);
+      visit(first + c, stays);
     }
   };
+  int holes = 0, fills = 0;
   each([&](int p, bool stays) {
     holes += p < front && !stays;
     fills += p >= front && stays;
   });
   scan(holes, fills);
-  // (gone candidates less than all from the front on: as many holes as fills)
   bool more = true;
-  for (int base = 0; more; base += kWindow) {
+  for (int base = 0; more; base += MOVES) {
     int nth = fills;
     bool past = false;
     each([&](int p, bool stays) {
       if (p >= front && stays) {
-        if (nth >= base && nth < base + kWindow) s_list[nth - base] = p;
-        past |= nth >= base + kWindow;
+        if (nth >= base && nth < base + MOVES) s.moves[nth - base] = p;
+        past |= nth >= base + MOVES;
         ++nth;
       }
     });
@@ -216,13 +290,42 @@ __global__ __launch_bounds__(THREADS) void choose(Evict a) {
         if (stays) {
           if (base == 0) kept[p] = p;
         } else {
-          if (nth >= base && nth < base + kWindow) kept[p] = s_list[nth - base];
+          if (nth >= base && nth < base + MOVES) kept[p] = static_cast<int>(s.moves[nth - base]);
           ++nth;
         }
       }
     });
     __syncthreads();
   }
+}
+
+template <int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void choose(Evict a) {
+  constexpr int kMoves = THREADS * EACH / 2;    // at most: as many leave holes as fill them
+  __shared__ Shared<THREADS / 64, kMoves> shared;
+  const int tid = threadIdx.x;
+  const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
+  const Held s = held_of(a, b);
+  const int gone = s.keys > a.keep ? s.keys - a.keep : 0;
+  int32_t* kept = a.kept + static_cast<i64>(blockIdx.x) * a.keep;
+  if (h == 0 && tid == 0) a.lengths_out[b] = s.keys - gone;
+  if (gone == 0) {
+    for (int i = tid; i < a.keep; i += THREADS) kept[i] = i < s.keys ? i : -1;
+    return;
+  }
+  const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
+  auto place = [&, weights = a.weights + h * a.w_head](int p) -> const float* {
+    const Place at = place_of(a, s.list, p);
+    return at.page < 0 ? nullptr : weights + at.page * a.w_page + at.slot * a.w_slot;
+  };
+  if (front > a.first) {
+    if (count <= THREADS * EACH)
+      choose_held<THREADS, EACH>(shared, count, a.first, front, kept, place);
+    else
+      choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, place);
+  }
+  for (int i = tid; i < a.keep; i += THREADS)
+    if (i < a.first || i >= front) kept[i] = i < front ? i : i + gone;
 }
 
 constexpr int kMovers = 256;      // threads
@@ -433,10 +536,13 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   if (heads * per > kMostGroups) return refuse(-2, what, "2^24 workgroups or more", heads * per);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   void* args[] = {&a};
-  const bool small = r->max_length <= 4096;
-  hipError_t e = launch(small ? reinterpret_cast<const void*>(&choose<256, 4096>)
-                              : reinterpret_cast<const void*>(&choose<1024, 32768>),
-                        heads, small ? 256 : 1024, args, s);
+  const int64_t most = r->max_length - r->first - r->recent;    // candidates
+  const int threads = most <= 2048 ? 256 : 1024;
+  hipError_t e = launch(most <= 2048    ? reinterpret_cast<const void*>(&choose<256, 8>)
+                        : most <= 4096  ? reinterpret_cast<const void*>(&choose<1024, 4>)
+                        : most <= 16384 ? reinterpret_cast<const void*>(&choose<1024, 16>)
+                                        : reinterpret_cast<const void*>(&choose<1024, 32>),
+                        heads, threads, args, s);
   if (e != hipSuccess) return hip_failed(e, what);
   if (r->keep == 0) return 0;
   e = launch(bytes == 4 ? reinterpret_cast<const void*>(&move<uint32_t>)
