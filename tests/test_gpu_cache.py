@@ -655,6 +655,8 @@ def _evict(b, keep, recent, first, **more):
     (1, 200, 16, [1300, 900], 700, 650, 1), (5, 128, 64, [4500, 5000, 100], 4096, 100, 4),
     (2, 24, 16, [9000, 4097], 5000, 0, 0), (1, 16, 128, [40000, 33000], 11000, 3000, 10),
     (1, 256, 16, [130, 140], 128, 100, 4), (1, 1000, 16, [50], 30, 11, 2),
+    (2, 128, 16, [4000, 3500], 1500, 200, 4), (2, 128, 24, [700, 701, 3], 600, 590, 0),
+    (1, 128, 16, [17000], 16000, 15000, 1), (100, 16, 16, [90, 70, 33], 40, 9, 0),
 ])
 def test_paged_evict(hip_ready, dtype, kv_heads, dim, page, lengths, keep, recent, first):
     b = Batch(dtype, kv_heads, kv_heads, dim, page, lengths, seed=keep,
@@ -686,10 +688,13 @@ def test_evict_without_the_weights(hip_ready):
     assert kept.tolist() == [[list(range(100))] * 2] * 2
 
 
-def test_evict_past_its_bound(hip_ready):
+@pytest.mark.parametrize("lengths,keep,max_length", [([6000, 300], 128, 10), ([6000, 300], 5000, 10),
+                                                     ([20000], 9000, 10), ([40000], 12000, 12000),
+                                                     ([7000], 3000, 3300)])
+def test_evict_past_its_bound(hip_ready, lengths, keep, max_length):
     """max_length sizes the launch: longer sequences are cut all the same."""
-    b = Batch(BF16, 2, 2, 64, 16, [6000, 300]).fill()
-    _evict(b, 128, 30, 2, max_length=10)
+    b = Batch(BF16, 2, 2, 64, 16, lengths).fill()
+    _evict(b, keep, 30, 2, max_length=max_length)
 
 
 def test_evict_lost_pages(hip_ready):
@@ -712,6 +717,24 @@ def test_evict_lost_pages(hip_ready):
         if i // 8 not in (1, 4) and p // 8 not in (1, 4):
             assert torch.equal(b.kc[page[i], slot[i]], kc[page[p], slot[p]]), i
     assert torch.equal(b.kc[b.indices[[1, 4]]].nan_to_num(-7), kc[b.indices[[1, 4]]].nan_to_num(-7))
+
+
+def test_a_cache_without_pages(hip_ready):
+    """Nothing is read or written; what is kept are the first, the recent and the first between."""
+    b = Batch(BF16, 2, 2, 16, 8, [80, 5], [3, 1]).fill()
+    lse = b.lse()
+    kc, vc, w = b.kc[:0], b.vc[:0], b.w[:0]
+    at.attention_weights(b.query, lse, kc, w, b.indptr, b.indices, b.lengths, max_length=80,
+                         query_indptr=b.ends, max_query=3)
+    fewer, kept = at.paged_evict(w, kc, vc, b.indptr, b.indices, b.lengths, keep=20, recent=4,
+                                 first=2, max_length=80)
+    assert fewer.tolist() == [20, 5]
+    assert kept[0, 0].tolist() == list(range(16)) + [76, 77, 78, 79]
+    assert kept[1, 1].tolist() == list(range(5)) + [-1] * 15
+    frequency, _ = at.rope_frequencies(16)
+    q = at.paged_append(b.key, b.value, kc, vc, b.indptr, b.indices, b.lengths, frequency,
+                        query=b.query, query_indptr=b.ends, epsilon=EPSILON)
+    assert q.any()
 
 
 def test_strides_of_weights_and_caches(hip_ready):

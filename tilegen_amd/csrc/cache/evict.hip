@@ -21,8 +21,10 @@ struct Evict {
   Table table;
   i64 kc_page, kc_slot, kc_head, vc_page, vc_slot, vc_head, w_page, w_slot, w_head;
   int kv_heads, dim, keep, recent, first, move_weights;
-  int slices, slice;      // of a row of a cache: workgroups, units of 16 bytes of each
-  Div by_heads, by_slices, by_units, by_last;   // units of a slice, of the last one
+  int units;              // of 16 bytes, of a row of a cache
+  int slices, slice;      // how it is cut, units of each
+  int chunks;             // the kept tokens, for fills
+  Div by_heads, by_parts, by_row, by_slice, by_last;    // units of a row, of a slice, of the last
 };
 
 // Sequence b's pages, as far as its tokens go.
@@ -78,8 +80,22 @@ struct Shared {
   int waves[2][WAVES];
   uint32_t prefix;
   int left, equal;
-  uint32_t moves[MOVES];
+  uint32_t moves[MOVES];        // where the fills come from, in order
 };
+
+// Where a position's weight stands; none: nowhere, and `at` is something that may be read.
+struct Spot {
+  const float* at;
+  bool none;
+};
+__device__ __forceinline__ Spot spot_of(const Evict& a, const Held& s, const float* weights, int p) {
+  const int nth = a.table.by_page(p);
+  const i64 page = s.list[nth];
+  const bool none = page < 0 || page >= a.table.pages;
+  return {none ? reinterpret_cast<const float*>(s.list + nth)
+               : weights + page * a.w_page + (p - nth * a.table.page) * a.w_slot,
+          none};
+}
 
 // After a digit's counts: in which bin the `left`-th largest is, how many of it are left, and how
 // many it holds.  Bins are counted from the largest down, one a thread.
@@ -114,24 +130,25 @@ __device__ __forceinline__ void clear_bins(S& s) {
 }
 
 // Of a sequence and kv head that loses tokens: what stays, from keys that threads hold, EACH to a
-// thread (candidate tid + k THREADS).
+// thread (candidate tid + k THREADS).  Returns how many fill holes; `targets`, if any, are those.
 template <int THREADS, int EACH, typename S, typename F>
-__device__ __forceinline__ void choose_held(S& s, int count, int first, int front, int32_t* kept,
-                                            F&& place) {
+__device__ __forceinline__ int choose_held(S& s, int count, int first, int front, int32_t* kept,
+                                           F&& spot, uint32_t* targets) {
   constexpr int kWaves = THREADS / 64, kRuns = EACH * kWaves;   // of 64 candidates
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   uint32_t key[EACH];
-  constexpr int kAtOnce = EACH < 8 ? EACH : 8;
+  constexpr int kAtOnce = EACH < 16 ? EACH : 16;    // loads in flight; past the last: the last's
 #pragma unroll
   for (int k0 = 0; k0 < EACH; k0 += kAtOnce) {
-    const float* at[kAtOnce];
+    Spot at[kAtOnce];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int c = tid + (k0 + k) * THREADS;
-      at[k] = c < count ? place(first + c) : nullptr;
-    }
+    for (int k = 0; k < kAtOnce; ++k)
+      at[k] = spot(first + min(tid + (k0 + k) * THREADS, count - 1));
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) key[k0 + k] = at[k] ? order_of(*at[k]) : 0u;
+    for (int k = 0; k < kAtOnce; ++k) key[k0 + k] = order_of(*at[k].at);
+#pragma unroll
+    for (int k = 0; k < kAtOnce; ++k)
+      if (at[k].none) key[k0 + k] = 0u;
   }
   // the (front - first)-th largest, by digits of 8 bits; done when all that a bin holds stay
   uint32_t prefix = 0;
@@ -205,21 +222,26 @@ __device__ __forceinline__ void choose_held(S& s, int count, int first, int fron
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
     const int p = first + tid + k * THREADS;
-    if (p < front && p - first < count)
-      kept[p] = stays >> k & 1 ? p : static_cast<int>(s.moves[nth(k)]);
+    if (p < front && p - first < count) {
+      const bool stay = stays >> k & 1;
+      kept[p] = stay ? p : static_cast<int>(s.moves[nth(k)]);
+      if (targets && !stay) targets[nth(k)] = p;
+    }
   }
+  return holes;
 }
 
 // The same from memory, key by key, for any number of candidates.  Each thread has a run of them
 // for the places; moves are listed some at a time.
 template <int THREADS, int MOVES, typename S, typename F>
 __device__ __forceinline__ void choose_any(S& s, int count, int first, int front, int32_t* kept,
-                                        F place) {
+                                        F&& spot) {
   constexpr int kWaves = THREADS / 64;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   auto key = [&](int c) {
-    const float* at = place(first + c);
-    return at ? order_of(*at) : 0u;
+    const Spot x = spot(first + c);
+    const uint32_t k = order_of(*x.at);
+    return x.none ? 0u : k;
   };
   uint32_t prefix = 0;
   int left = front - first;
@@ -314,15 +336,12 @@ __global__ __launch_bounds__(THREADS) void choose(Evict a) {
     return;
   }
   const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
-  auto place = [&, weights = a.weights + h * a.w_head](int p) -> const float* {
-    const Place at = place_of(a, s.list, p);
-    return at.page < 0 ? nullptr : weights + at.page * a.w_page + at.slot * a.w_slot;
-  };
+  auto spot = [&](int p) { return spot_of(a, s, a.weights + h * a.w_head, p); };
   if (front > a.first) {
     if (count <= THREADS * EACH)
-      choose_held<THREADS, EACH>(shared, count, a.first, front, kept, place);
+      choose_held<THREADS, EACH>(shared, count, a.first, front, kept, spot, nullptr);
     else
-      choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, place);
+      choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
   }
   for (int i = tid; i < a.keep; i += THREADS)
     if (i < a.first || i >= front) kept[i] = i < front ? i : i + gone;
@@ -351,96 +370,322 @@ __device__ __forceinline__ void write_unit(T* p, int n, typename Chunk<T>::Vec v
     if (i < n) p[i] = v[i];
 }
 
-// Rows of one head of a cache move: `units` units of `dim` elements from `at` on.
+constexpr int kWindow = 4, kListed = kWindow * kMovers, kDeep = 8;
+
+// Where rows go and come from, in elements from the head's first.
+constexpr i64 kNowhere = INT64_MIN;
+struct Moves {
+  i64 from[kListed], to[kListed];
+  int count, past;
+};
+
+// A slice of a head's rows: `units` units of 16 bytes (the last may be shorter), `dim` elements.
 template <typename T>
-__device__ __forceinline__ void move_rows(const Evict& a, const Held& s, const int32_t* kept,
-                                          T* base, i64 by_page, i64 by_slot, int dim, int units,
-                                          Div by_units) {
-  constexpr int kList = 1024, kDeep = 8;
-  __shared__ int s_to[kList], s_from[kList];
-  __shared__ int s_count;
+struct Slice {
+  T* base;
+  i64 by_page, by_slot;
+  int dim, units;
+  Div by_units;
+  __device__ __forceinline__ i64 row(const Evict& a, const int64_t* list, int p) const {
+    const Place at = place_of(a, list, p);
+    return at.page < 0 ? kNowhere : at.page * by_page + at.slot * by_slot;
+  }
+};
+
+// Of the kept tokens i0 .. i1 those that come from `least` or past it, or (before) from below.  No
+// place is both a source and a target.  Returns whether one came from `least` on.
+template <typename T>
+__device__ __forceinline__ bool fill(const Evict& a, const Held& s, const int32_t* kept,
+                                     const Slice<T>& slice, Moves& m, int i0, int i1, int least,
+                                     bool before) {
   const int tid = threadIdx.x;
-  const int front = a.keep - a.recent, gone = s.keys - a.keep;
-  auto row = [&](int p) -> T* {
-    const Place at = place_of(a, s.list, p);
-    return at.page < 0 ? nullptr : base + at.page * by_page + at.slot * by_slot;
-  };
-  // the holes' fills, listed some at a time
-  for (int i0 = a.first; i0 < front; i0 += kList) {
-    if (tid == 0) s_count = 0;
-    __syncthreads();
-    for (int i = i0 + tid; i < min(i0 + kList, front); i += kMovers) {
-      const int from = kept[i];
-      if (from != i) {
-        const int n = atomicAdd(&s_count, 1);
-        s_to[n] = i;
-        s_from[n] = from;
+  if (tid == 0) m.count = m.past = 0;
+  __syncthreads();
+  int from[kWindow];
+#pragma unroll
+  for (int k = 0; k < kWindow; ++k) {
+    const int i = i0 + k * kMovers + tid;
+    from[k] = i < i1 ? kept[i] : i;
+  }
+#pragma unroll
+  for (int k = 0; k < kWindow; ++k) {
+    const int i = i0 + k * kMovers + tid;
+    if (from[k] == i) continue;
+    if (from[k] >= least) m.past = 1;
+    if ((from[k] < least) != before) continue;
+    const i64 x = slice.row(a, s.list, from[k]), y = slice.row(a, s.list, i);
+    if (x != kNowhere && y != kNowhere) {
+      const int n = atomicAdd(&m.count, 1);
+      m.from[n] = x;
+      m.to[n] = y;
+    }
+  }
+  __syncthreads();
+  const int work = m.count * slice.units;
+  const bool past = m.past;
+  for (int w0 = tid; w0 < work; w0 += kDeep * kMovers) {    // (some reads, then their writes)
+    typename Chunk<T>::Vec v[kDeep];
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int w = w0 + k * kMovers;
+      if (w < work) {
+        const int n = slice.by_units(w), u = (w - n * slice.units) * Chunk<T>::N;
+        v[k] = read_unit(slice.base + m.from[n] + u, slice.dim - u);
       }
     }
+#pragma unroll
+    for (int k = 0; k < kDeep; ++k) {
+      const int w = w0 + k * kMovers;
+      if (w < work) {
+        const int n = slice.by_units(w), u = (w - n * slice.units) * Chunk<T>::N;
+        write_unit(slice.base + m.to[n] + u, slice.dim - u, v[k]);
+      }
+    }
+  }
+  __syncthreads();
+  return past;
+}
+
+// The recent tokens go down, chunk by chunk, each read whole before any of it is written: what a
+// chunk writes is behind all that later ones read.  Below `keep`, where they go, stand sources of
+// fills: those fills come before the first chunk is written, while it is on its way.
+template <typename T>
+__device__ __forceinline__ void shift_down(const Evict& a, const Held& s, const int32_t* kept,
+                                           const Slice<T>& slice, Moves& m, Moves& fills) {
+  const int tid = threadIdx.x, front = a.keep - a.recent, gone = s.keys - a.keep;
+  const int most = kDeep * kMovers / slice.units;       // rows of a chunk
+  const int rows = most < kMovers ? most : kMovers;
+  typename Chunk<T>::Vec v[kDeep];
+  auto read = [&](int row0) __attribute__((always_inline)) {
+    const int n = min(rows, a.recent - row0);
     __syncthreads();
-    const int work = s_count * units;
-#pragma unroll 4
-    for (int w = tid; w < work; w += kMovers) {
-      const int n = by_units(w), u = (w - n * units) * Chunk<T>::N;
-      const T* from = row(s_from[n]);
-      T* to = row(s_to[n]);
-      if (from && to) write_unit(to + u, dim - u, read_unit(from + u, dim - u));
+    if (tid < n) {
+      const i64 x = slice.row(a, s.list, front + row0 + tid + gone);
+      const i64 y = slice.row(a, s.list, front + row0 + tid);
+      m.from[tid] = x;
+      m.to[tid] = x == kNowhere ? x : y;
     }
     __syncthreads();
-  }
-  // the recent tokens, each chunk read whole before any of it is written
-  const int64_t work = static_cast<int64_t>(a.recent) * units;
-  for (int64_t w0 = 0; w0 < work; w0 += kDeep * kMovers) {
-    typename Chunk<T>::Vec v[kDeep];
-    T* to[kDeep];
-    int left[kDeep];
 #pragma unroll
     for (int i = 0; i < kDeep; ++i) {
-      const int64_t w = w0 + i * kMovers + tid;
-      to[i] = nullptr;
-      if (w < work) {
-        const int n = by_units(static_cast<uint32_t>(w));
-        const int u = (static_cast<int>(w) - n * units) * Chunk<T>::N;
-        const T* from = row(front + n + gone);
-        T* target = row(front + n);
-        left[i] = dim - u;
-        if (from && target) {
-          to[i] = target + u;
-          v[i] = read_unit(from + u, left[i]);
-        }
+      const int w = i * kMovers + tid;
+      if (w < n * slice.units) {
+        const int r = slice.by_units(w), u = (w - r * slice.units) * Chunk<T>::N;
+        if (m.to[r] != kNowhere) v[i] = read_unit(slice.base + m.from[r] + u, slice.dim - u);
       }
     }
+  };
+  if (a.recent) read(0);
+  for (int i0 = a.first; i0 < front; i0 += kListed)
+    if (fill(a, s, kept, slice, fills, i0, min(i0 + kListed, front), a.keep, true)) break;
+  for (int row0 = 0; row0 < a.recent; row0 += rows) {
+    if (row0) read(row0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // every thread has what it read
     __syncthreads();
+    const int n = min(rows, a.recent - row0);
 #pragma unroll
-    for (int i = 0; i < kDeep; ++i)
-      if (to[i]) write_unit(to[i], left[i], v[i]);
+    for (int i = 0; i < kDeep; ++i) {
+      const int w = i * kMovers + tid;
+      if (w < n * slice.units) {
+        const int r = slice.by_units(w), u = (w - r * slice.units) * Chunk<T>::N;
+        if (m.to[r] != kNowhere) write_unit(slice.base + m.to[r] + u, slice.dim - u, v[i]);
+      }
+    }
   }
 }
 
-// One workgroup for a slice of a head's rows of one cache, or for its weights.
+// Fills are in the order of their sources, so that those from below `keep` come first.  A cache's
+// head has one workgroup for each slice of its rows, which moves those and then the recent tokens,
+// and `chunks` for the other fills, a range of the kept tokens each.
 template <typename T>
 __global__ __launch_bounds__(kMovers) void move(Evict a) {
-  const int per = 2 * a.slices + a.move_weights;
-  const int unit = a.by_slices(blockIdx.x), part = blockIdx.x - unit * per;
+  __shared__ Moves m, fills;
+  const int per = 2 * (a.slices + a.chunks) + a.move_weights * (1 + a.chunks);
+  const int unit = a.by_parts(blockIdx.x);
+  int part = blockIdx.x - unit * per;
   const int b = a.by_heads(unit), h = unit - b * a.kv_heads;
   const Held s = held_of(a, b);
   if (s.keys <= a.keep) return;
   const int32_t* kept = a.kept + static_cast<i64>(unit) * a.keep;
-  if (part == 2 * a.slices) {
-    Div by_one;
-    by_one.mul = 1;
-    by_one.shift = 0;
-    move_rows<float>(a, s, kept, a.weights + h * a.w_head, a.w_page, a.w_slot, 1, 1, by_one);
+  const int front = a.keep - a.recent;
+  auto run = [&](const auto& slice, int chunk) __attribute__((always_inline)) {
+    if (chunk < 0) {
+      shift_down(a, s, kept, slice, m, fills);
+      return;
+    }
+    const int each = ((front - a.first + a.chunks - 1) / a.chunks + kMovers - 1) & -kMovers;
+    const int end = min(front, a.first + (chunk + 1) * each);
+    for (int i0 = a.first + chunk * each; i0 < end; i0 += kListed)
+      fill(a, s, kept, slice, fills, i0, min(i0 + kListed, end), a.keep, false);
+  };
+  if (part >= 2 * (a.slices + a.chunks)) {
+    part -= 2 * (a.slices + a.chunks);
+    Slice<float> w = {a.weights + h * a.w_head, a.w_page, a.w_slot, 1, 1, {}};
+    w.by_units.mul = 1;
+    w.by_units.shift = 0;
+    run(w, part - 1);
     return;
   }
-  const bool value = part >= a.slices;
-  const int first = (value ? part - a.slices : part) * a.slice * Chunk<T>::N;
-  const int dim = min(a.dim - first, a.slice * Chunk<T>::N);
-  const int units = (dim + Chunk<T>::N - 1) / Chunk<T>::N;
-  T* base = static_cast<T*>(value ? a.value_cache : a.key_cache) + first +
-            h * (value ? a.vc_head : a.kc_head);
-  move_rows<T>(a, s, kept, base, value ? a.vc_page : a.kc_page, value ? a.vc_slot : a.kc_slot, dim,
-               units, units == a.slice ? a.by_units : a.by_last);
+  const bool value = part >= a.slices + a.chunks;
+  if (value) part -= a.slices + a.chunks;
+  const int chunk = part - a.slices;
+  const int first = chunk < 0 ? part * a.slice : 0;     // units
+  const int units = chunk < 0 ? min(a.units - first, a.slice) : a.units;
+  Slice<T> x;
+  x.base = static_cast<T*>(value ? a.value_cache : a.key_cache) +
+           h * (value ? a.vc_head : a.kc_head) + first * Chunk<T>::N;
+  x.by_page = value ? a.vc_page : a.kc_page;
+  x.by_slot = value ? a.vc_slot : a.kc_slot;
+  x.dim = min(a.dim - first * Chunk<T>::N, units * Chunk<T>::N);
+  x.units = units;
+  x.by_units = chunk >= 0 ? a.by_row : units == a.slice ? a.by_slice : a.by_last;
+  run(x, chunk);
+}
+
+// All of it in one launch, for many heads or few bytes: a workgroup chooses for a head and moves its
+// keys, values and weights, the recent tokens' on their way while it chooses.
+template <typename T, int THREADS, int EACH>
+__global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
+  constexpr int kMoves = THREADS * EACH / 2, kRows = 256, kFills = 4;
+  __shared__ Shared<THREADS / 64, kMoves> shared;
+  __shared__ uint32_t s_to[kMoves];
+  __shared__ i64 s_from[2][kRows], s_target[2][kRows];    // of keys and values
+  const int tid = threadIdx.x;
+  const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
+  const Held s = held_of(a, b);
+  const int gone = s.keys > a.keep ? s.keys - a.keep : 0;
+  int32_t* kept = a.kept + static_cast<i64>(blockIdx.x) * a.keep;
+  if (h == 0 && tid == 0) a.lengths_out[b] = s.keys - gone;
+  if (gone == 0) {
+    for (int i = tid; i < a.keep; i += THREADS) kept[i] = i < s.keys ? i : -1;
+    return;
+  }
+  const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
+  T* const keys = static_cast<T*>(a.key_cache) + h * a.kc_head;
+  T* const values = static_cast<T*>(a.value_cache) + h * a.vc_head;
+  float* const weights = a.weights + h * a.w_head;
+  auto put_row = [&](int n, int from, int to) {
+    const Place x = place_of(a, s.list, from), y = place_of(a, s.list, to);
+    const bool none = x.page < 0 || y.page < 0;
+    s_from[0][n] = none ? kNowhere : x.page * a.kc_page + x.slot * a.kc_slot;
+    s_target[0][n] = none ? kNowhere : y.page * a.kc_page + y.slot * a.kc_slot;
+    s_from[1][n] = x.page * a.vc_page + x.slot * a.vc_slot;
+    s_target[1][n] = y.page * a.vc_page + y.slot * a.vc_slot;
+  };
+  // units of the recent tokens' rows, of keys and then of values, some rows at a time
+  const int most = kDeep * THREADS / (2 * a.units), rows = most < kRows ? most : kRows;
+  typename Chunk<T>::Vec v[kDeep];
+  auto read = [&](int row0) __attribute__((always_inline)) {
+    const int n = min(rows, a.recent - row0);
+    __syncthreads();
+    if (tid < n) put_row(tid, front + row0 + tid + gone, front + row0 + tid);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      int w = i * THREADS + tid;
+      const bool value = w >= n * a.units;
+      if (value) w -= n * a.units;
+      if (w < n * a.units) {
+        const int r = a.by_row(w), u = (w - r * a.units) * Chunk<T>::N;
+        if (s_target[0][r] != kNowhere)
+          v[i] = read_unit((value ? values : keys) + s_from[value][r] + u, a.dim - u);
+      }
+    }
+  };
+  if (a.recent) read(0);
+  auto spot = [&](int p) { return spot_of(a, s, weights, p); };
+  // (the first chunk's targets, which the fills' places go over)
+  i64 target[2] = {kNowhere, 0};
+  if (tid < kRows && a.recent) {
+    target[0] = s_target[0][tid];
+    target[1] = s_target[1][tid];
+  }
+  int fills = 0;
+  bool listed = true;
+  if (front > a.first) {
+    if (count <= THREADS * EACH) {
+      fills = choose_held<THREADS, EACH>(shared, count, a.first, front, kept, spot, s_to);
+    } else {
+      choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
+      listed = false;
+      fills = front - a.first;      // any of them may be one
+    }
+  }
+  for (int i = tid; i < a.keep; i += THREADS)
+    if (i < a.first || i >= front) kept[i] = i < front ? i : i + gone;
+  __syncthreads();
+  for (int n0 = 0; n0 < fills; n0 += kRows) {
+    const int n = min(kRows, fills - n0);
+    if (tid < n) {
+      const int to = listed ? s_to[n0 + tid] : a.first + n0 + tid;
+      const int from = listed ? shared.moves[n0 + tid] : kept[to];
+      put_row(tid, from, to);
+      if (from == to) s_target[0][tid] = kNowhere;
+      if (a.move_weights && from != to) {
+        const Spot x = spot(from), y = spot(to);
+        if (!x.none && !y.none) *const_cast<float*>(y.at) = *x.at;
+      }
+    }
+    __syncthreads();
+    for (int w0 = tid; w0 < 2 * n * a.units; w0 += kFills * THREADS) {
+      typename Chunk<T>::Vec x[kFills];
+#pragma unroll
+      for (int i = 0; i < kFills; ++i) {
+        int w = w0 + i * THREADS;
+        const bool value = w >= n * a.units;
+        if (value) w -= n * a.units;
+        const int r = a.by_row(w), u = (w - r * a.units) * Chunk<T>::N;
+        if (w < n * a.units && s_target[0][r] != kNowhere)
+          x[i] = read_unit((value ? values : keys) + s_from[value][r] + u, a.dim - u);
+      }
+#pragma unroll
+      for (int i = 0; i < kFills; ++i) {
+        int w = w0 + i * THREADS;
+        const bool value = w >= n * a.units;
+        if (value) w -= n * a.units;
+        const int r = a.by_row(w), u = (w - r * a.units) * Chunk<T>::N;
+        if (w < n * a.units && s_target[0][r] != kNowhere)
+          write_unit((value ? values : keys) + s_target[value][r] + u, a.dim - u, x[i]);
+      }
+    }
+    __syncthreads();
+  }
+  if (tid < kRows && a.recent) {
+    s_target[0][tid] = target[0];
+    s_target[1][tid] = target[1];
+  }
+  for (int row0 = 0; row0 < a.recent; row0 += rows) {
+    if (row0) read(row0);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // every thread has what it read
+    __syncthreads();
+    const int n = min(rows, a.recent - row0);
+#pragma unroll
+    for (int i = 0; i < kDeep; ++i) {
+      int w = i * THREADS + tid;
+      const bool value = w >= n * a.units;
+      if (value) w -= n * a.units;
+      if (w < n * a.units) {
+        const int r = a.by_row(w), u = (w - r * a.units) * Chunk<T>::N;
+        if (s_target[0][r] != kNowhere)
+          write_unit((value ? values : keys) + s_target[value][r] + u, a.dim - u, v[i]);
+      }
+    }
+  }
+  if (!a.move_weights) return;
+  for (int row0 = 0; row0 < a.recent; row0 += THREADS) {
+    const int p = front + row0 + tid;
+    const Spot x = spot(min(p, a.keep - 1) + gone), y = spot(min(p, a.keep - 1));
+    const float w = *x.at;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (p < a.keep && !x.none && !y.none) *const_cast<float*>(y.at) = w;
+  }
+}
+
+template <typename T>
+const void* whole_of(int64_t candidates) {
+  return candidates <= 2048 ? reinterpret_cast<const void*>(&evict_whole<T, 1024, 2>)
+                            : reinterpret_cast<const void*>(&evict_whole<T, 1024, 4>);
 }
 
 }  // namespace
@@ -523,20 +768,35 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   a.move_weights = static_cast<int>(r->move_weights);
   a.by_heads = Div(a.kv_heads);
   const int64_t heads = r->sequences * r->kv_heads;
-  const int units = (a.dim * bytes + 15) / 16;
-  // rows in slices of 64 bytes at least, while there are fewer workgroups than two a compute unit
+  a.units = (a.dim * bytes + 15) / 16;
+  // rows in slices of 64 bytes at least, and kept tokens in chunks, while there are few workgroups
   int slices = 1;
-  while (heads * 2 * slices < 512 && units / (2 * slices) >= 4) slices *= 2;
-  a.slice = (units + slices - 1) / slices;
-  a.slices = (units + a.slice - 1) / a.slice;
-  a.by_units = Div(a.slice);
-  a.by_last = Div(units - (a.slices - 1) * a.slice);
-  const int per = 2 * a.slices + a.move_weights;
-  a.by_slices = Div(per);
+  while (heads * 2 * slices < 512 && a.units / (2 * slices) >= 4) slices *= 2;
+  a.slice = (a.units + slices - 1) / slices;
+  a.slices = (a.units + a.slice - 1) / a.slice;
+  const int64_t filled = r->max_length > r->keep ? r->keep - r->recent - r->first : 0;
+  int64_t chunks = (filled + kMovers - 1) / kMovers;
+  if (chunks * heads > 512) chunks = 512 / heads;
+  a.chunks = static_cast<int>(chunks > 1 ? chunks : 1);
+  a.by_row = Div(a.units);
+  a.by_slice = Div(a.slice);
+  a.by_last = Div(a.units - (a.slices - 1) * a.slice);
+  const int per = 2 * (a.slices + a.chunks) + a.move_weights * (1 + a.chunks);
+  a.by_parts = Div(per);
   if (heads * per > kMostGroups) return refuse(-2, what, "2^24 workgroups or more", heads * per);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   void* args[] = {&a};
   const int64_t most = r->max_length - r->first - r->recent;    // candidates
+  // One launch where a workgroup's threads hold a head's candidates, unless few heads have many
+  // recent tokens to move, which slices do side by side.  8 kv heads of 128, 1088 tokens cut to 1024
+  // with 256 recent: 1 sequence 12.9 us, 15.7 in two launches, 32 19.3 and 27.9, 128 87 and 109; 4000
+  // to 1024: 13.3 and 14.8, 16.6 and 22.8; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.4, 8
+  // 36.9 and 39.1, 64 144 and 188.
+  if (most <= 4096 && (heads >= 64 || r->recent * a.units <= 8192)) {
+    const hipError_t e = launch(bytes == 4 ? whole_of<uint32_t>(most) : whole_of<uint16_t>(most),
+                                heads, 1024, args, s);
+    return e == hipSuccess ? 0 : hip_failed(e, what);
+  }
   const int threads = most <= 2048 ? 256 : 1024;
   hipError_t e = launch(most <= 2048    ? reinterpret_cast<const void*>(&choose<256, 8>)
                         : most <= 4096  ? reinterpret_cast<const void*>(&choose<1024, 4>)

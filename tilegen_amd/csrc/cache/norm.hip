@@ -306,9 +306,9 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_append_normed
       if (const int rc = apart(what, out, *x, bytes)) return rc;
   }
   if (const int rc = apart(what, vc, kc, bytes)) return rc;
-  if (!r->key || !r->value || !r->key_cache || !r->value_cache || !r->indptr || !r->lengths ||
-      (r->n_indices && !r->indices) || (r->heads && (!r->query || !r->query_out)) ||
-      (r->rotary && !r->frequency))
+  if (!r->key || !r->value || (r->pages && (!r->key_cache || !r->value_cache)) || !r->indptr ||
+      !r->lengths || (r->n_indices && !r->indices) ||
+      (r->heads && (!r->query || !r->query_out)) || (r->rotary && !r->frequency))
     return refuse(-1, what, "null array", r->tokens);
   Normed a = {};
   a.query = r->query;
