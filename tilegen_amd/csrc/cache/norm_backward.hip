@@ -185,6 +185,7 @@ const void* kernel_of(int64_t layout, bool whole, int lanes) {
   return layout == TG_HALF                                                                      \
              ? reinterpret_cast<const void*>(&norm_rows_backward<T, Whole<T, TG_HALF, G>>)      \
              : reinterpret_cast<const void*>(&norm_rows_backward<T, Whole<T, TG_INTERLEAVED, G>>)
+  TG_LANES(4);
   TG_LANES(8);
   TG_LANES(16);
   TG_LANES(32);
@@ -227,9 +228,13 @@ int plan(const tg_norm_rope_backward* r, Plan* p) {
   a.eights = (a.rows + R - 1) / R;
   a.key_first = a.heads / R;
   a.by_eights = Div(a.eights ? a.eights : 1);
-  // Workgroups that share the tokens: about 1536 in all.
+  // Workgroups that share the tokens, as many in all as the chip holds of them at once: by their
+  // registers 768, or twice that where a lane has few pairs.  16384 tokens of 40 heads of 128 in
+  // bfloat16: 100 us by 768, 108 by 1536; 4095 of 25 heads of 96 in float32, interleaved: 29.2 and
+  // 25.9; 8192 of 128 elements with 62 turned: 210 and 145.
   const int64_t most = (r->tokens + kWavesOf - 1) / kWavesOf;
-  int64_t blocks = a.eights ? 1536 / a.eights : 1;
+  const bool many = !p->whole || (r->dtype == TG_F32 && a.layout == TG_INTERLEAVED);
+  int64_t blocks = a.eights ? (many ? 1536 : 768) / a.eights : 1;
   blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
   a.blocks = static_cast<int>(blocks);
   a.query_each = r->query_weight_head != 0;

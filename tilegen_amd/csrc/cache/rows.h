@@ -35,10 +35,10 @@ __device__ __forceinline__ float plus(float v) {
 // The sum over each G lanes, in all of them.
 template <int G>
 __device__ __forceinline__ float lanes_sum(float v) {
-  static_assert(G == 8 || G == 16 || G == 32 || G == 64, "");
+  static_assert(G == 4 || G == 8 || G == 16 || G == 32 || G == 64, "");
   v = plus<0xB1>(v);                    // neighbours: lanes 1 0 3 2
   v = plus<0x4E>(v);                    // pairs: lanes 2 3 0 1
-  v = plus<0x141>(v);                   // quads: the mirror of each 8
+  if (G >= 8) v = plus<0x141>(v);       // quads: the mirror of each 8
   if (G >= 16) v = plus<0x140>(v);      // the mirror of each 16
   if (G >= 32) {
     const Both q = quarters(v);
@@ -221,7 +221,9 @@ __device__ __forceinline__ void turns_of(Turns& t, i64 position, const double* f
 }
 
 // Lanes of a row for `units` units.
-inline int lanes_for(int units) { return units <= 8 ? 8 : units <= 16 ? 16 : units <= 32 ? 32 : 64; }
+inline int lanes_for(int units) {
+  return units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : units <= 32 ? 32 : 64;
+}
 
 inline bool whole_rows(int64_t dtype, int64_t dim, int64_t half, int64_t layout) {
   const int n = dtype == TG_F32 ? 4 : 8;
