@@ -140,7 +140,9 @@ NORMS = [
     (6, 7, 3, 256, 62, "one32"), (7, 5, 3, 256, 256, "each"), (1, 3, 1, 255, 100, "one"),
     (300, 2, 1, 96, 64, "one"), (70, 3, 2, 17, 16, "each"), (3, 150, 70, 24, 24, "one"),
     (2, 9, 9, 8, 8, "one32"), (515, 12, 4, 72, 24, "one"), (2100, 32, 8, 16, 16, "one32"),
-    (1, 64, 1, 160, 80, "each"), (11, 3, 2, 192, 192, "one")]
+    (1, 64, 1, 160, 80, "each"), (11, 3, 2, 192, 192, "one"), (2100, 8, 2, 66, 34, "each32"),
+    (33, 3, 1, 18, 0, "one"), (5, 2, 2, 12, 10, "one32"), (2, 1, 3, 254, 254, "one"),
+    (40, 2, 1, 9, 0, "each"), (7, 3, 3, 46, 20, "one")]
 
 
 def _operands(layout, dtype, tokens, heads, kv_heads, dim, rotary, kind):

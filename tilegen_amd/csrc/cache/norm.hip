@@ -104,8 +104,10 @@ __global__ __launch_bounds__(64 * kWavesOf) void norm_rows(Normed a) {
 #pragma unroll
       for (int i = 0; i < P::NP; ++i) {
         const float u = x.first(i), w = x.second(i);
-        sum = __builtin_fmaf(u, u, sum);
-        sum = __builtin_fmaf(w, w, sum);
+        if (place.counts(i)) {
+          sum = __builtin_fmaf(u, u, sum);
+          sum = __builtin_fmaf(w, w, sum);
+        }
       }
       r = rsqrtf(__builtin_fmaf(lanes_sum<P::G>(sum), a.inverse, a.epsilon));
     }
@@ -150,39 +152,37 @@ __global__ __launch_bounds__(64 * kWavesOf) void norm_rows(Normed a) {
   }
 }
 
-template <typename T, int LAYOUT>
+template <typename T, typename P>
+const void* kernel_of(bool append) {
+  return append ? reinterpret_cast<const void*>(&norm_rows<T, P, true>)
+                : reinterpret_cast<const void*>(&norm_rows<T, P, false>);
+}
+
+template <typename T, int LAYOUT, bool EDGE>
 const void* kernel_of(int lanes, bool append) {
   switch (lanes) {
-#define TG_LANES(G)                                                                      \
-  case G:                                                                                \
-    return append ? reinterpret_cast<const void*>(&norm_rows<T, Whole<T, LAYOUT, G>, true>) \
-                  : reinterpret_cast<const void*>(&norm_rows<T, Whole<T, LAYOUT, G>, false>)
-    TG_LANES(4);
-    TG_LANES(8);
-    TG_LANES(16);
-    TG_LANES(32);
-    TG_LANES(64);
-#undef TG_LANES
+    case 4: return kernel_of<T, Whole<T, LAYOUT, 4, EDGE>>(append);
+    case 8: return kernel_of<T, Whole<T, LAYOUT, 8, EDGE>>(append);
+    case 16: return kernel_of<T, Whole<T, LAYOUT, 16, EDGE>>(append);
+    case 32: return kernel_of<T, Whole<T, LAYOUT, 32, EDGE>>(append);
+    default: return kernel_of<T, Whole<T, LAYOUT, 64, EDGE>>(append);
   }
-  return nullptr;
 }
 
 template <typename T>
-const void* kernel_of(int64_t layout, bool whole, int lanes, bool append) {
-  if (!whole)
-    return append ? reinterpret_cast<const void*>(&norm_rows<T, Ragged<T>, true>)
-                  : reinterpret_cast<const void*>(&norm_rows<T, Ragged<T>, false>);
-  return layout == TG_HALF ? kernel_of<T, TG_HALF>(lanes, append)
-                           : kernel_of<T, TG_INTERLEAVED>(lanes, append);
+const void* kernel_of(int64_t layout, Lanes l, bool append) {
+  if (l.cut == kRagged) return kernel_of<T, Ragged<T>>(append);
+  if (layout == TG_HALF)
+    return l.cut == kEdge ? kernel_of<T, TG_HALF, true>(l.lanes, append)
+                          : kernel_of<T, TG_HALF, false>(l.lanes, append);
+  return l.cut == kEdge ? kernel_of<T, TG_INTERLEAVED, true>(l.lanes, append)
+                        : kernel_of<T, TG_INTERLEAVED, false>(l.lanes, append);
 }
 
 int enqueue(Normed& a, int64_t dtype, bool append, const char* what, hipStream_t stream) {
-  const bool whole = whole_rows(dtype, a.dim, a.half, a.layout);
-  const int n = dtype == TG_F32 ? 4 : 8;
-  int units = a.layout == TG_HALF ? a.half / n + (a.dim - 2 * a.half) / n : a.dim / n;
-  const int lanes = whole ? lanes_for(units) : 64;
+  const Lanes l = lanes_of(dtype, a.dim, a.half, a.layout);
   a.rows = a.heads + (append ? 2 : 1) * a.kv_heads;
-  a.eights = (a.rows + 64 / lanes - 1) / (64 / lanes);
+  a.eights = (a.rows + 64 / l.lanes - 1) / (64 / l.lanes);
   // Tasks of one group of rows while there are few, else of two or more: waves start with the
   // token's lookups and angles, and long ones end in an uneven round.  16384 tokens of 40 heads of 128
   // in bfloat16: 73.6 us by 5 groups, 66.3 by 2 or 1; interleaved, 10 groups, 73.1 by 5, 94.9 by 1.
@@ -193,9 +193,9 @@ int enqueue(Normed& a, int64_t dtype, bool append, const char* what, hipStream_t
   a.splits = (a.eights + a.each - 1) / a.each;
   a.by_splits = Div(a.splits);
   const int64_t tasks = static_cast<int64_t>(a.tokens) * a.splits;
-  const void* k = dtype == TG_F32   ? kernel_of<float>(a.layout, whole, lanes, append)
-                  : dtype == TG_F16 ? kernel_of<_Float16>(a.layout, whole, lanes, append)
-                                    : kernel_of<__bf16>(a.layout, whole, lanes, append);
+  const void* k = dtype == TG_F32   ? kernel_of<float>(a.layout, l, append)
+                  : dtype == TG_F16 ? kernel_of<_Float16>(a.layout, l, append)
+                                    : kernel_of<__bf16>(a.layout, l, append);
   void* args[] = {&a};
   const hipError_t e = launch(k, (tasks + kWavesOf - 1) / kWavesOf, 64 * kWavesOf, args, stream);
   return e == hipSuccess ? 0 : hip_failed(e, what);

@@ -90,10 +90,12 @@ __global__ __launch_bounds__(64 * kWavesOf) void norm_rows_backward(Back a) {
         ua[i] = p * c + q * s;
         ub[i] = q * c - p * s;
       }
-      square = __builtin_fmaf(y, y, square);
-      square = __builtin_fmaf(z, z, square);
-      dot = __builtin_fmaf(ua[i] * w.a[i], y, dot);
-      dot = __builtin_fmaf(ub[i] * w.b[i], z, dot);
+      if (place.counts(i)) {
+        square = __builtin_fmaf(y, y, square);
+        square = __builtin_fmaf(z, z, square);
+        dot = __builtin_fmaf(ua[i] * w.a[i], y, dot);
+        dot = __builtin_fmaf(ub[i] * w.b[i], z, dot);
+      }
     }
     const float r = rsqrtf(__builtin_fmaf(lanes_sum<P::G>(square), a.inverse, a.epsilon));
     const float back = lanes_sum<P::G>(dot) * a.inverse * r * r;
@@ -177,28 +179,36 @@ __global__ __launch_bounds__(kColumns* kSlices) void sum_parts(Sums a) {
         static_cast<W>(s_sum[0][threadIdx.x % kColumns]);
 }
 
+template <typename T, typename P>
+const void* kernel_of() {
+  return reinterpret_cast<const void*>(&norm_rows_backward<T, P>);
+}
+
+template <typename T, int LAYOUT, bool EDGE>
+const void* kernel_of(int lanes) {
+  switch (lanes) {
+    case 4: return kernel_of<T, Whole<T, LAYOUT, 4, EDGE>>();
+    case 8: return kernel_of<T, Whole<T, LAYOUT, 8, EDGE>>();
+    case 16: return kernel_of<T, Whole<T, LAYOUT, 16, EDGE>>();
+    case 32: return kernel_of<T, Whole<T, LAYOUT, 32, EDGE>>();
+    default: return kernel_of<T, Whole<T, LAYOUT, 64, EDGE>>();
+  }
+}
+
 template <typename T>
-const void* kernel_of(int64_t layout, bool whole, int lanes) {
-  if (!whole) return reinterpret_cast<const void*>(&norm_rows_backward<T, Ragged<T>>);
-#define TG_LANES(G)                                                                             \
-  if (lanes == G)                                                                               \
-  return layout == TG_HALF                                                                      \
-             ? reinterpret_cast<const void*>(&norm_rows_backward<T, Whole<T, TG_HALF, G>>)      \
-             : reinterpret_cast<const void*>(&norm_rows_backward<T, Whole<T, TG_INTERLEAVED, G>>)
-  TG_LANES(4);
-  TG_LANES(8);
-  TG_LANES(16);
-  TG_LANES(32);
-  TG_LANES(64);
-#undef TG_LANES
-  return nullptr;
+const void* kernel_of(int64_t layout, Lanes l) {
+  if (l.cut == kRagged) return kernel_of<T, Ragged<T>>();
+  if (layout == TG_HALF)
+    return l.cut == kEdge ? kernel_of<T, TG_HALF, true>(l.lanes)
+                          : kernel_of<T, TG_HALF, false>(l.lanes);
+  return l.cut == kEdge ? kernel_of<T, TG_INTERLEAVED, true>(l.lanes)
+                        : kernel_of<T, TG_INTERLEAVED, false>(l.lanes);
 }
 
 struct Plan {
   Back a;
   Sums sums;
-  bool whole, weights;
-  int lanes;
+  Lanes lanes;
   int64_t query_floats, key_floats;
 };
 
@@ -219,12 +229,8 @@ int plan(const tg_norm_rope_backward* r, Plan* p) {
   a.half = static_cast<int>(r->rotary / 2);
   a.layout = static_cast<int>(r->layout);
   a.rows = a.heads + a.kv_heads;
-  p->whole = whole_rows(r->dtype, a.dim, a.half, a.layout);
-  const int n = r->dtype == TG_F32 ? 4 : 8;
-  p->lanes = !p->whole ? 64
-                       : lanes_for(a.layout == TG_HALF ? a.half / n + (a.dim - 2 * a.half) / n
-                                                       : a.dim / n);
-  const int R = 64 / p->lanes;
+  p->lanes = lanes_of(r->dtype, a.dim, a.half, a.layout);
+  const int R = 64 / p->lanes.lanes;
   a.eights = (a.rows + R - 1) / R;
   a.key_first = a.heads / R;
   a.by_eights = Div(a.eights ? a.eights : 1);
@@ -233,7 +239,7 @@ int plan(const tg_norm_rope_backward* r, Plan* p) {
   // bfloat16: 100 us by 768, 108 by 1536; 4095 of 25 heads of 96 in float32, interleaved: 29.2 and
   // 25.9; 8192 of 128 elements with 62 turned: 210 and 145.
   const int64_t most = (r->tokens + kWavesOf - 1) / kWavesOf;
-  const bool many = !p->whole || (r->dtype == TG_F32 && a.layout == TG_INTERLEAVED);
+  const bool many = p->lanes.cut == kRagged || (r->dtype == TG_F32 && a.layout == TG_INTERLEAVED);
   int64_t blocks = a.eights ? (many ? 1536 : 768) / a.eights : 1;
   blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
   a.blocks = static_cast<int>(blocks);
@@ -335,9 +341,9 @@ extern "C" __attribute__((visibility("default"))) int launch_norm_rope_backward(
   a.key_part = p.key_floats ? space + p.query_floats : nullptr;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const int64_t groups = static_cast<int64_t>(a.blocks) * a.eights;
-  const void* k = r->dtype == TG_F32   ? kernel_of<float>(a.layout, p.whole, p.lanes)
-                  : r->dtype == TG_F16 ? kernel_of<_Float16>(a.layout, p.whole, p.lanes)
-                                       : kernel_of<__bf16>(a.layout, p.whole, p.lanes);
+  const void* k = r->dtype == TG_F32   ? kernel_of<float>(a.layout, p.lanes)
+                  : r->dtype == TG_F16 ? kernel_of<_Float16>(a.layout, p.lanes)
+                                       : kernel_of<__bf16>(a.layout, p.lanes);
   if (a.tokens) {
     void* args[] = {&a};
     const hipError_t e = launch(k, groups, 64 * kWavesOf, args, s);

@@ -51,25 +51,36 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// Rows of whole 16-byte chunks (dim, and for halves rotary/2, are multiples of a chunk).  Halves: a
-// lane's unit is a chunk of the first half with its partners, or a chunk of what is not turned.
-// Interleaved: a chunk, whose pairs are neighbours.
-template <typename T, int LAYOUT, int LANES>
+// Rows in 16-byte chunks.  Halves: a lane's unit is a chunk of the first half with its partners, or
+// a chunk of what is not turned.  Interleaved: a chunk, whose pairs are neighbours.  EDGE: a part of
+// the row that does not end with a chunk has a last one that reaches back over the one before; the
+// pairs that both have count once (and are written twice, the same).
+template <typename T, int LAYOUT, int LANES, bool EDGE>
 struct Whole {
   static constexpr int G = LANES, N = Chunk<T>::N, NP = LAYOUT == TG_HALF ? N : N / 2;
   int at, partner, pair;    // elements; the first pair's number; partner -1: none
+  int again;                // pairs that the unit before has
   bool active;
+  static __host__ __device__ __forceinline__ int chunks(int n) {
+    return EDGE ? (n + N - 1) / N : n / N;
+  }
   __device__ __forceinline__ Whole(int unit, int dim, int half, int)
-      : Whole(unit, unit - half / N, dim, half, true) {}
+      : Whole(unit, unit - chunks(half), dim, half, true) {}
   // past: the units of pairs of halves, negative for those
   __device__ __forceinline__ Whole(int unit, int past, int dim, int half, bool)
-      : at(LAYOUT != TG_HALF || past < 0 ? unit * N : 2 * half + past * N),
-        partner(LAYOUT != TG_HALF ? 0 : past < 0 ? half + unit * N : -1),
-        pair(LAYOUT != TG_HALF ? unit * N / 2 : past < 0 ? unit * N : half),
-        active(LAYOUT != TG_HALF ? unit < dim / N : past < (dim - 2 * half) / N) {}
-  static int units(int dim, int half, int) {
-    return LAYOUT == TG_HALF ? half / N + (dim - 2 * half) / N : dim / N;
+      : Whole(LAYOUT != TG_HALF || past < 0 ? unit * N : 2 * half + past * N,
+              LAYOUT != TG_HALF || past >= 0 ? dim : half, LAYOUT == TG_HALF && past < 0, half,
+              LAYOUT != TG_HALF ? unit < chunks(dim) : past < chunks(dim - 2 * half)) {}
+  __device__ __forceinline__ Whole(int from, int end, bool two, int half, bool active)
+      : at(EDGE && from + N > end ? end - N : from),
+        partner(LAYOUT != TG_HALF ? 0 : two ? half + at : -1),
+        pair(LAYOUT != TG_HALF ? at / 2 : two ? at : half),
+        again(LAYOUT != TG_HALF ? (from - at) / 2 : from - at),
+        active(active) {}
+  static int units(int dim, int half) {
+    return LAYOUT == TG_HALF ? chunks(half) + chunks(dim - 2 * half) : chunks(dim);
   }
+  __device__ __forceinline__ bool counts(int i) const { return !EDGE || i >= again; }
   template <typename S>
   struct Raw {
     typename Loose<S, N>::Vec a, b;
@@ -105,7 +116,7 @@ struct Whole {
   __device__ __forceinline__ int turn(int i) const { return pair + i; }
   // where element (first or second) of pair i of `unit` stands in its row, or -1
   __device__ __forceinline__ int element(int i, bool second) const {
-    if (!active || (LAYOUT == TG_HALF && second && partner < 0)) return -1;
+    if (!active || !counts(i) || (LAYOUT == TG_HALF && second && partner < 0)) return -1;
     return LAYOUT == TG_HALF ? (second ? partner : at) + i : at + 2 * i + second;
   }
 };
@@ -118,7 +129,7 @@ struct Ragged {
   int lane, dim, half, layout;
   __device__ __forceinline__ Ragged(int unit, int dim, int half, int layout)
       : lane(unit), dim(dim), half(half), layout(layout) {}
-  static int units(int, int, int) { return 64; }
+  __device__ __forceinline__ bool counts(int) const { return true; }
   template <typename S>
   struct Raw {
     typedef S Vec __attribute__((ext_vector_type(NP)));
@@ -220,14 +231,25 @@ __device__ __forceinline__ void turns_of(Turns& t, i64 position, const double* f
   __builtin_amdgcn_wave_barrier();
 }
 
-// Lanes of a row for `units` units.
-inline int lanes_for(int units) {
-  return units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : units <= 32 ? 32 : 64;
-}
-
-inline bool whole_rows(int64_t dtype, int64_t dim, int64_t half, int64_t layout) {
-  const int n = dtype == TG_F32 ? 4 : 8;
-  return dim % n == 0 && (layout != TG_HALF || half % n == 0);
+// How rows are cut: whole chunks, chunks that reach back, or single elements; and lanes of a row.
+enum Cut { kWhole, kEdge, kRagged };
+struct Lanes {
+  Cut cut;
+  int lanes;
+};
+inline Lanes lanes_of(int64_t dtype, int dim, int half, int64_t layout) {
+  const int n = dtype == TG_F32 ? 4 : 8, rest = dim - 2 * half;
+  const auto up = [n](int x) { return (x + n - 1) / n; };
+  int units = up(dim);
+  Cut cut = dim % n == 0 ? kWhole : dim % 2 == 0 && dim >= n ? kEdge : kRagged;
+  if (layout == TG_HALF) {
+    units = up(half) + up(rest);
+    cut = half % n == 0 && rest % n == 0 ? kWhole
+          : (half == 0 || half >= n) && (rest == 0 || rest >= n) ? kEdge
+                                                                 : kRagged;
+  }
+  if (cut == kRagged) return {cut, 64};
+  return {cut, units <= 4 ? 4 : units <= 8 ? 8 : units <= 16 ? 16 : units <= 32 ? 32 : 64};
 }
 
 // The checks that the norms share; 0 or a status.
