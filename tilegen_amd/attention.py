@@ -362,76 +362,81 @@ def rope_backward(grad: torch.Tensor, positions: torch.Tensor, frequency: torch.
 def _learned(name: str, w: Optional[torch.Tensor], heads: int, dim: int, device: int, dtype):
     """(address, stride of a head, type) of a norm's weight: [dim], or [heads, dim]."""
     if w is None:
-        return 0, 0, dtype
-    shape, strides = w.shape, w.stride()
-    if not (w.get_device() == device and w.dtype in (dtype, torch.float32)
-            and tuple(shape) in ((dim,), (heads, dim)) and (strides[-1] == 1 or dim == 1)):
-        raise ValueError("%s is %s %s with strides %s on %s, expected [%d] or [%d, %d] of %s or "
-                         "float32 on device %d" % (name, w.dtype, tuple(shape), strides, w.device,
-                                                   dim, heads, dim, dtype, device))
-    return w.data_ptr(), 0 if len(shape) == 1 else strides[0] if heads > 1 else dim, w.dtype
+        return 0, 0, None
+    shape, strides, kind = w.shape, w.stride(), w.dtype
+    if (w.get_device() == device and (kind is dtype or kind is torch.float32)
+            and shape and shape[-1] == dim and (strides[-1] == 1 or dim == 1)):
+        if len(shape) == 1:
+            return w.data_ptr(), 0, kind
+        if len(shape) == 2 and shape[0] == heads:
+            return w.data_ptr(), strides[0] if heads > 1 else dim, kind
+    raise ValueError("%s is %s %s with strides %s on %s, expected [%d] or [%d, %d] of %s or "
+                     "float32 on device %d" % (name, kind, tuple(shape), strides, w.device, dim,
+                                               heads, dim, dtype, device))
 
 
-def _norm_operands(query, key, positions, frequency, query_weight, key_weight):
-    """What both directions of a norm check: (device, type, tokens, heads, kv_heads, dim, packed
-    parts)."""
-    device, dtype = _operand("query", query, _DTYPES)
-    shape, qs = _heads("query", query, device, dtype, 3)
-    tokens, heads, dim = shape
-    kv_heads, ks = 0, (0, 0)
-    if key is not None:
-        kshape, ks = _heads("key", key, device, dtype, 3)
-        if kshape[0] != tokens or kshape[2] != dim:
-            raise ValueError("query is %s, key %s" % (tuple(shape), tuple(kshape)))
-        kv_heads = kshape[1]
-    elif key_weight is not None:
-        raise ValueError("key_weight without key")
-    wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
-    wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
-    if query_weight is None:
-        kind = other
-    elif key_weight is not None and other is not kind:
-        raise ValueError("query_weight is %s and key_weight %s" % (kind, other))
-    p_frequency = p_positions = rotary = 0
-    if frequency is not None:
-        p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
-        rotary = 2 * frequency.shape[0]
-    if positions is not None:
-        p_positions = _list("positions", positions, device, tokens)
-    elif rotary:
+def _kind(query_kind, key_kind, dtype):
+    """The type of both weights."""
+    if query_kind is None or key_kind is None:
+        return query_kind or key_kind or dtype
+    if query_kind is not key_kind:
+        raise ValueError("query_weight is %s and key_weight %s" % (query_kind, key_kind))
+    return query_kind
+
+
+def _turns(positions, frequency, tokens, device):
+    """(addresses of positions and frequency, elements turned)"""
+    if frequency is None:
+        return 0 if positions is None else _list("positions", positions, device, tokens), 0, 0
+    if positions is None:
         raise ValueError("frequency without positions")
-    return (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind,
-            p_positions, p_frequency, rotary)
+    return (_list("positions", positions, device, tokens),
+            _list("frequency", frequency, device, dtype=torch.float64), 2 * frequency.shape[0])
+
+
+def _unlike(name, x, shape):
+    raise ValueError("%s is %s, expected %s" % (name, tuple(x.shape), tuple(shape)))
 
 
 def _normed(query, key, positions, frequency, query_weight, key_weight, epsilon, layout,
             magnitude, query_out, key_out):
-    (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind, p_positions,
-     p_frequency, rotary) = _norm_operands(query, key, positions, frequency, query_weight,
-                                           key_weight)
-    written = tuple(t for t in (query_out, key_out) if t is not None)
+    device, dtype = _operand("query", query, _DTYPES)
+    shape, qs = _heads("query", query, device, dtype, 3)
+    tokens, heads, dim = shape
+    written = ()
     if query_out is None:
-        query_out = _like(query)
-    oshape, qos = _heads("query_out", query_out, device, dtype, 3, write=True)
-    if oshape != query.shape:
-        raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(query.shape)))
-    p_key = p_key_out = 0
-    kos = (0, 0)
+        query_out, qos = _like(query), (heads * dim, dim)
+    else:
+        oshape, qos = _heads("query_out", query_out, device, dtype, 3, write=True)
+        if oshape != shape:
+            _unlike("query_out", query_out, shape)
+        written = (query_out,)
+    kv_heads, p_key, p_key_out, ks, kos = 0, 0, 0, (0, 0), (0, 0)
     if key is not None:
+        shape, ks = _heads("key", key, device, dtype, 3)
+        kv_heads = shape[1]
+        if shape[0] != tokens or shape[2] != dim:
+            raise ValueError("query is %s, key %s" % (tuple(query.shape), tuple(shape)))
         if key_out is None:
-            key_out = _like(key)
-        oshape, kos = _heads("key_out", key_out, device, dtype, 3, write=True)
-        if oshape != key.shape:
-            raise ValueError("key_out is %s, expected %s" % (tuple(oshape), tuple(key.shape)))
+            key_out, kos = _like(key), (kv_heads * dim, dim)
+        else:
+            oshape, kos = _heads("key_out", key_out, device, dtype, 3, write=True)
+            if oshape != shape:
+                _unlike("key_out", key_out, shape)
+            written += (key_out,)
         p_key, p_key_out = key.data_ptr(), key_out.data_ptr()
-    elif key_out is not None:
-        raise ValueError("key_out without key")
+    elif key_weight is not None or key_out is not None:
+        raise ValueError("key_weight or key_out without key")
+    wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
+    wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
+    kind = kind if kind is other else _kind(kind, other, dtype)
+    p_positions, p_frequency, rotary = _turns(positions, frequency, tokens, device)
     try:
         packed = _NORM.pack(
             query.data_ptr(), p_key, query_out.data_ptr(), p_key_out, wq, wk, p_positions,
-            p_frequency, _DTYPES[dtype], _DTYPES[kind], tokens, heads, kv_heads, dim, rotary,
-            _layout(layout), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], wqs, wks,
-            magnitude, epsilon)
+            p_frequency, _DTYPES[dtype], _DTYPES[kind or dtype], tokens, heads, kv_heads, dim,
+            rotary, _layout(layout), qs[0], qs[1], ks[0], ks[1], qos[0], qos[1], kos[0], kos[1],
+            wqs, wks, magnitude, epsilon)
     except struct.error as e:
         raise _unfit(e) from None
     _call(_cache_lib().launch_norm_rope, packed, device, "norm_rope")
@@ -442,58 +447,69 @@ def _normed(query, key, positions, frequency, query_weight, key_weight, epsilon,
 
 def _normed_backward(grad_query, grad_key, query, key, positions, frequency, query_weight,
                      key_weight, epsilon, layout, magnitude, want_weights=(True, True)):
-    # an expanded weight's heads have gradients of their own
-    query_weight, key_weight = (
-        w.contiguous() if w is not None and w.dim() == 2 and w.stride(0) == 0 else w
-        for w in (query_weight, key_weight))
-    (device, dtype, tokens, heads, kv_heads, dim, qs, ks, wq, wqs, wk, wks, kind, p_positions,
-     p_frequency, rotary) = _norm_operands(query, key, positions, frequency, query_weight,
-                                           key_weight)
+    device, dtype = _operand("query", query, _DTYPES)
+    shape, qs = _heads("query", query, device, dtype, 3)
+    tokens, heads, dim = shape
     gshape, gqs = _heads("grad_query", grad_query, device, dtype, 3)
-    if gshape != query.shape:
-        raise ValueError("grad_query is %s, expected %s" % (tuple(gshape), tuple(query.shape)))
-    query_out, key_out = _like(query), None
-    p_grad_key = p_key = p_key_out = 0
-    gks = kos = (0, 0)
+    if gshape != shape:
+        _unlike("grad_query", grad_query, shape)
+    kv_heads, p_grad_key, p_key, p_key_out, gks, ks = 0, 0, 0, 0, (0, 0), (0, 0)
+    key_out = None
     if key is not None:
+        shape, ks = _heads("key", key, device, dtype, 3)
+        kv_heads = shape[1]
+        if shape[0] != tokens or shape[2] != dim:
+            raise ValueError("query is %s, key %s" % (tuple(query.shape), tuple(shape)))
         gshape, gks = _heads("grad_key", grad_key, device, dtype, 3)
-        if gshape != key.shape:
-            raise ValueError("grad_key is %s, expected %s" % (tuple(gshape), tuple(key.shape)))
+        if gshape != shape:
+            _unlike("grad_key", grad_key, shape)
         key_out = _like(key)
-        kos = key_out.stride()
         p_grad_key, p_key, p_key_out = grad_key.data_ptr(), key.data_ptr(), key_out.data_ptr()
-    elif grad_key is not None:
-        raise ValueError("grad_key without key")
-    qos = query_out.stride()
-    dqw, dkw = (None if w is None or not wanted else
-                torch.empty_like(w, memory_format=torch.contiguous_format)
-                for w, wanted in zip((query_weight, key_weight), want_weights))
+    elif grad_key is not None or key_weight is not None:
+        raise ValueError("grad_key or key_weight without key")
+    # an expanded weight's heads have gradients of their own
+    if query_weight is not None and query_weight.dim() == 2 and query_weight.stride(0) == 0:
+        query_weight = query_weight.contiguous()
+    if key_weight is not None and key_weight.dim() == 2 and key_weight.stride(0) == 0:
+        key_weight = key_weight.contiguous()
+    wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
+    wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
+    kind = kind if kind is other else _kind(kind, other, dtype)
+    p_positions, p_frequency, rotary = _turns(positions, frequency, tokens, device)
+    query_out, dqw, dkw = _like(query), None, None
+    if wq and want_weights[0]:
+        dqw = _like(query_weight)
+    if wk and want_weights[1]:
+        dkw = _like(key_weight)
     fields = [grad_query.data_ptr(), p_grad_key, query.data_ptr(), p_key, query_out.data_ptr(),
               p_key_out, 0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr(),
-              wq, wk, p_positions, p_frequency, 0, 0, _DTYPES[dtype], _DTYPES[kind], tokens, heads,
-              kv_heads, dim, rotary, _layout(layout), gqs[0], gqs[1], gks[0], gks[1], qs[0], qs[1],
-              ks[0], ks[1], qos[0], qos[1], kos[0], kos[1], wqs, wks, magnitude, epsilon]
+              wq, wk, p_positions, p_frequency, 0, 0, _DTYPES[dtype], _DTYPES[kind or dtype],
+              tokens, heads, kv_heads, dim, rotary, _layout(layout), gqs[0], gqs[1], gks[0],
+              gks[1], qs[0], qs[1], ks[0], ks[1], heads * dim, dim, kv_heads * dim, dim, wqs, wks,
+              magnitude, epsilon]
     L = _cache_lib()
     _run(query, fields, _NORM_BACKWARD, 12, L.norm_rope_backward_workspace,
          L.launch_norm_rope_backward, device, "norm_rope_backward")
     return query_out, key_out, dqw, dkw
 
 
-def _run(like, fields, packing, workspace_at, workspace, launch, device, what):
-    """A call that may need a workspace, from torch, with the operands' device current."""
-    def plan_and_launch():
+def _plan_and_launch(like, fields, packing, at, workspace, launch, device):
+    packed = packing.pack(*fields)
+    n = workspace(packed)
+    if n < 0:
+        return n
+    if n:
+        space = like.new_empty(n, dtype=torch.uint8)
+        fields[at], fields[at + 1] = space.data_ptr(), n
         packed = packing.pack(*fields)
-        n = workspace(packed)
-        if n < 0:
-            return n
-        if n:
-            space = like.new_empty(n, dtype=torch.uint8)
-            fields[workspace_at:workspace_at + 2] = space.data_ptr(), n
-            packed = packing.pack(*fields)
-        return launch(packed, _raw_stream(device))
+    return launch(packed, _raw_stream(device))
 
+
+def _run(like, fields, packing, at, workspace, launch, device, what):
+    """A call that may need a workspace (fields `at` and on), from torch, with the operands' device
+    current."""
     try:
-        rc = _on(device, plan_and_launch)
+        rc = _on(device, _plan_and_launch, like, fields, packing, at, workspace, launch, device)
     except struct.error as e:
         raise _unfit(e) from None
     if rc:
@@ -539,19 +555,23 @@ def norm_rope(query: torch.Tensor, key: Optional[torch.Tensor],
     share no other memory with the operands.  Sums of squares are held in 32 bits.  Differentiable
     once, backward, in the heads and the weights; the gradients of weights are summed in 32 bits in
     an order that the sizes alone decide."""
-    operands = (query, key, query_weight, key_weight)
-    if frequency is not None:
-        _no_gradient("norm_rope", frequency)
-    if _forward._current_level >= 0 and any(_tangent(t) for t in operands if t is not None):
-        raise ValueError("norm_rope has no forward derivative")
+    if _forward._current_level >= 0:
+        if any(t is not None and _tangent(t) for t in (query, key, query_weight, key_weight)):
+            raise ValueError("norm_rope has no forward derivative")
+        _no_gradient("norm_rope", frequency, query_out, key_out)
     if torch.is_grad_enabled():
-        if any(t is not None and t.requires_grad for t in operands):
+        if (query.requires_grad or (key is not None and key.requires_grad)
+                or (query_weight is not None and query_weight.requires_grad)
+                or (key_weight is not None and key_weight.requires_grad)):
             if query_out is not None or key_out is not None:
                 raise ValueError("outputs cannot be given where operands need gradients")
+            _no_gradient("norm_rope", frequency)
             got = _NormRope.apply(query, key, query_weight, key_weight, positions, frequency,
                                   (epsilon, layout, magnitude))
             return (got, None) if key is None else got
-    _no_gradient("norm_rope", query_out, key_out)
+        if query_out is not None or key_out is not None or (frequency is not None
+                                                            and frequency.requires_grad):
+            _no_gradient("norm_rope", frequency, query_out, key_out)
     return _normed(query, key, positions, frequency, query_weight, key_weight, epsilon, layout,
                    magnitude, query_out, key_out)
 
@@ -687,15 +707,12 @@ def _append_normed(key, value, q, key_cache, value_cache, out, indptr, indices, 
         raise ValueError("query_weight without query")
     wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
     wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
-    if query_weight is None:
-        kind = other
-    elif key_weight is not None and other is not kind:
-        raise ValueError("query_weight is %s and key_weight %s" % (kind, other))
+    kind = kind if kind is other else _kind(kind, other, dtype)
     p_shift = 0 if shift is None else _list("shift", shift, device, sequences)
     try:
         packed = _APPEND_NORMED.pack(
             key, value, q, key_cache, value_cache, out, indptr, indices, lengths, ends, p_shift,
-            frequency, wq, wk, _DTYPES[dtype], _DTYPES[kind], tokens, sequences, heads, kv_heads,
+            frequency, wq, wk, _DTYPES[dtype], _DTYPES[kind or dtype], tokens, sequences, heads, kv_heads,
             dim, rotary, layout, pages, page, n_indices, offset, epsilon is not None, ks[0], ks[1],
             vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1],
             vcs[2], wqs, wks, magnitude, 0.0 if epsilon is None else epsilon)
