@@ -561,25 +561,32 @@ int plan(const tg_attention_weights* r, Plan* p) {
   const int64_t bound = r->max_query < r->tokens ? r->max_query : r->tokens;
   const int64_t rows = (r->query_indptr && bound > 0 ? bound : 1) * a.group;   // of a sequence
   a.parts = 1;
-  // Wide for many rows (whole tokens in a stage, within 32 bits of its first).  32 sequences of up to
-  // 2048 keys, 8 kv heads of 128: 64 rows 28 us narrow, 36 wide; 128 rows 40 both; 256 rows 63 and
-  // 47; 1024 rows 199 and 92.  One of 16384 keys, 128 rows: 14.2 and 13.0.  4 of up to 700 keys, 4
-  // kv heads of 64: 256 rows 10.4 and 12.6, 512 rows 16.7 and 17.2, 1024 rows 29 and 26.
+  // Wide for many rows, or not so few with much work for all (whole tokens in a stage, within 32 bits
+  // of its first).  32 sequences of up to 2048 keys, 8 kv heads of 128: 64 rows 29 us narrow, 36 wide;
+  // 128 rows 40 and 39; 512 rows 109 and 60.  8 of up to 1000 keys: 256 rows 19 and 14, 512 rows 32
+  // and 22.  One of 16384 keys, 4 kv heads: 64 rows 10.0 and 11.4, 256 rows 21 and 16.  4 of up to 700
+  // keys, 4 kv heads of 64: 256 rows 9.5 and 12.5, 512 rows 15.5 and 15.2, 1024 rows 27 and 16.  2 of
+  // up to 1500, 16 kv heads of 128: 128 rows 9.7 and 10.5.
   const int64_t room = wide_rows(a.dim), tokens = room / a.group;
   auto within = [](int64_t steps, int64_t stride) {
     return steps == 0 || (stride >= 0 && stride <= (int64_t(1) << 28) / steps);
   };
-  if (rows >= 128 && (length > 1024 || rows > 512) && tokens > 0 && within(tokens - 1, r->query_token) &&
+  const bool many = rows > 512 || (rows >= 128 && rows * heads >= (1 << 22) / length);
+  if (many && tokens > 0 && within(tokens - 1, r->query_token) &&
       within(a.group - 1, r->query_head)) {
     p->keys = a.dim > 128 ? 128 : 256;
     a.splits = static_cast<int>((length + p->keys - 1) / p->keys);
     a.stage_rows = static_cast<int>(tokens * a.group);
     a.by_stage = Div(a.stage_rows);
-    // Parts of the rows, at least so many stages each, while there are few workgroups: earlier keys
-    // are seen by more rows, so that a round of workgroups with all rows ends with a few long ones.
+    // Parts of the rows, of 16 stages at least: earlier keys are seen by more rows, so that a round of
+    // workgroups with all rows ends with a few long ones.  Of 4 stages while two workgroups a compute
+    // unit are not there yet: 1 sequence of 2048 keys, 8 kv heads of 128, 2048 rows 35 us by 16 and
+    // 22 by 4; of 512 keys of 64, 2048 rows 31 and 16; with work for all, by 8, 188 instead of 165.
     const int64_t units = heads * a.splits, stages = (rows + a.stage_rows - 1) / a.stage_rows;
     int64_t parts = units ? 4096 / units : 1;
-    if (parts > stages / 16) parts = stages / 16;
+    const int64_t few = units ? 512 / units : 1;
+    const int64_t fine = few < stages / 4 ? few : stages / 4;
+    if (parts > stages / 16) parts = stages / 16 > fine ? stages / 16 : fine;
     if (parts > 1) {
       a.part_stages = static_cast<int>((stages + parts - 1) / parts);
       a.parts = static_cast<int>((stages + a.part_stages - 1) / a.part_stages);
