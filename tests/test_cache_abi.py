@@ -235,3 +235,12 @@ def test_kernels_do_not_spill(tmp_path):
             assert used == (0, 0), (name.group(1), used)
             found += 1
     assert found >= 80      # norms by type, layout and lanes, forward, append and backward, ...
+
+
+def test_paged_decode_refuses_bounds_it_cannot_keep():
+    """Before it asks for a device."""
+    from tilegen_amd import paged_decode
+    for sizes in (dict(bound=-1), dict(every=0), dict(first=-1), dict(recent=9, bound=8),
+                  dict(recent=-1, bound=8), dict(recent=6, first=3, bound=8)):
+        with pytest.raises(ValueError, match=list(sizes)[0]):
+            paged_decode.run(**sizes)

@@ -893,6 +893,98 @@ def test_a_bounded_cache_in_a_graph(hip_ready):
     assert torch.equal(b.kc, eager.kc)
 
 
+@pytest.mark.parametrize("norm,bound,recent,first", [(True, 0, None, 0), (False, 12, 4, 1),
+                                                     (True, 10, None, 2)])
+def test_paged_decode_with_norms_and_a_bound(hip_ready, norm, bound, recent, first):
+    """The decode loop of tilegen_amd.paged_decode, against attention over what each kv head has kept
+    of its unrotated inputs in 64 bits.  Keys and queries are rounded once, to bfloat16 (and off by
+    the norm's and the rotation's errors): a score is off by at most S = scale sum (dk |q| + |k| dq +
+    dk dq) + dim 2^-23 scale sum |k q|, an output, with probabilities and itself rounded, by 2 u + exp
+    2 S - 1 of its sum of magnitudes.  A key's weight is off by exp(2 S + 2^-16) - 1 of itself: its at
+    most 60 terms, the exponents' size below 64 and the exponential come to less than 2^-16."""
+    from tilegen_amd import paged_decode
+    heads, kv_heads, dim, prompt, every, steps = 4, 2, 64, 50, 5, 21
+    r = paged_decode.run(sequences=3, prompt=prompt, steps=steps, heads=heads, kv_heads=kv_heads,
+                         dim=dim, page=16, start=20, seed=5, keep=True, norm=norm, bound=bound,
+                         recent=recent, first=first, every=every)
+    f, magnitude, counts, u = r["frequency"], r["magnitude"], r["counts"], U[BF16]
+    learned = r["norm"] or {}
+    recent = bound // 4 if recent is None else recent
+    assert (r["norm"] is not None) == norm and len(r["calls"]) == steps + 1
+    assert [call for call, _ in r["stayed"]] == ([0, 5, 10, 15, 20] if bound else [])
+
+    def made(x, which, positions):
+        """(normed and turned in 64 bits, by how much the calls' may be off)"""
+        z, N = _cpu(x), 0.0
+        if norm:
+            z, N = _normed(x, learned[which], learned["epsilon"]), (dim / 2 + 8) * E
+        y, size = _turned(z, torch.tensor(positions), f, "half", magnitude)
+        return y, u * y.abs() + (2.0 ** -21 + N) * size
+
+    shared, eshared = made(r["prompt"][0], "key_weight", list(range(prompt)))
+    vshared = _cpu(r["prompt"][1])
+    own = [[(torch.empty(0, dim, dtype=torch.float64),) * 3] * kv_heads for _ in range(3)]
+    weight = [[torch.zeros(2, 0, dtype=torch.float64)] * kv_heads for _ in range(3)]  # and bounds
+    seen, stayed = [0, 0, 0], dict(r["stayed"])
+    for call, (q, k, v, out) in enumerate(r["calls"]):
+        n = counts if call == 0 else [1, 1, 1]
+        row = 0
+        for b in range(3):
+            mine = slice(row, row + n[b])
+            at_ = [prompt + seen[b] + j for j in range(n[b])]
+            (ks, eks), (qs, eqs) = made(k[mine], "key_weight", at_), made(q[mine], "query_weight", at_)
+            vs = _cpu(v[mine])
+            for h in range(kv_heads):
+                key, ekey, value = (torch.cat([a, x[:, h]])
+                                    for a, x in zip(own[b][h], (ks, eks, vs)))
+                own[b][h] = key, ekey, value
+                weight[b][h] = torch.cat([weight[b][h], torch.zeros(2, n[b])], 1)
+                for j in range(n[b]):
+                    see = key.shape[0] - n[b] + j + 1
+                    kh = torch.cat([shared[:, h], key[:see]])
+                    ek = torch.cat([eshared[:, h], ekey[:see]])
+                    vh = torch.cat([vshared[:, h], value[:see]])
+                    for g in range(2 * h, 2 * h + 2):
+                        qh, eq = qs[j, g], eqs[j, g]
+                        p = torch.softmax(kh @ qh / 8, 0)
+                        S = float((ek @ qh.abs() + kh.abs() @ eq + ek @ eq
+                                   + dim * 2.0 ** -23 * (kh.abs() @ qh.abs())).max()) / 8
+                        size = p @ vh.abs()
+                        bound_ = (2 * u + math.exp(2 * S) - 1) * size
+                        off = (_cpu(out[row + j, g]) - p @ vh).abs()
+                        assert (off <= bound_ * (1 + 2.0 ** -6)).all(), (call, b, j, g)
+                        weight[b][h][0, :see] += p[prompt:]
+                        weight[b][h][1, :see] += p[prompt:] * (math.exp(2 * S + 2.0 ** -16) - 1)
+            row += n[b]
+            seen[b] += n[b]
+            length = own[b][0][0].shape[0]
+            if call not in stayed:
+                continue
+            for h in range(kv_heads):
+                where = stayed[call][b, h].tolist()
+                there = [p for p in where if p >= 0]
+                assert len(there) == min(length, bound) and where[len(there):] == [-1] * (
+                    bound - len(there))
+                kept = set(there)
+                assert len(kept) == len(there) and max(there) < length
+                if length > bound:
+                    always = set(range(first)) | set(range(length - recent, length))
+                    w, e = weight[b][h]
+                    left = [p for p in range(length) if p not in kept]
+                    chosen = [p for p in there if p not in always]
+                    assert always <= kept and chosen
+                    assert float((w + e)[chosen].min()) >= float((w - e)[left].max())
+                own[b][h] = tuple(x[there] for x in own[b][h])
+                weight[b][h] = weight[b][h][:, there]
+    cache = r["cache"]
+    assert seen == [n + steps for n in counts]
+    if bound:
+        assert cache.capacity == 20 and cache.lengths.tolist() == [bound + steps % every] * 3
+        assert (cache.lengths + cache.shift).tolist() == seen
+    else:
+        assert cache.lengths.tolist() == seen and cache.shift is None
+
+
 def test_norms_in_a_graph_and_on_streams(hip_ready):
     """Forward and backward calls captured, replayed, and two streams at once."""
     g = _gen(3)

@@ -13,8 +13,9 @@ Modules keep the reference's names and entry points:
 
 Attention over a paged cache with a CSR page table, on torch tensors (no counterpart in the
 reference):
-    attention         rotary positions, paged append, attention behind a shared prefix
-    paged_decode      a decode loop that runs the three together
+    attention         rotary positions, norms of heads, paged append, attention behind a shared
+                      prefix; the attention weight of cached keys, eviction to a bound
+    paged_decode      a decode loop that runs them together
 
 Around them (the reference's scripts/ and harness, rebuilt for this backend):
     variant           one compiled variant: launch, geometry, timing handles
@@ -25,8 +26,8 @@ Around them (the reference's scripts/ and harness, rebuilt for this backend):
     vendor            rocSPARSE SpMV timing beside the tuned kernel
     profiling         rocprofv3 summaries for profiles/
     cpu_tuned         CPU-tuned OpenMP schedules for the CPU baseline
-    build             in-tree native build (libtgrt, harness, attention, oracle, kernel
-                      cache)
+    build             in-tree native build (libtgrt, harness, attention and its cache, oracle,
+                      kernel cache)
 """
 
 __version__ = "0.1.0"
