@@ -40,25 +40,36 @@ __global__ __launch_bounds__(64 * kWavesOf) void norm_rows(Normed a) {
   const int last = min(first + a.each, a.eights);
   const P place(lane & (P::G - 1), a.dim, a.half, a.layout);
 
-  // the token's position, and (append) its slots in the caches, if it has any
+  using Raw = typename P::template Raw<T>;
+  // row `row` of the token: where it is read, whether it is at all
+  auto from = [&](int row) -> const T* {
+    if (row < a.heads)
+      return static_cast<const T*>(a.query) + token * a.q_token + row * a.q_head;
+    row -= a.heads;
+    if (!APPEND || row < a.kv_heads)
+      return static_cast<const T*>(a.key) + token * a.k_token + row * a.k_head;
+    return static_cast<const T*>(a.value) + token * a.v_token + (row - a.kv_heads) * a.v_head;
+  };
+  auto live = [&](int row) { return row < a.rows; };
+  Raw next;
+  int row = first * R + lane / P::G;
+  place.load(from(live(row) ? row : 0), live(row), next);
+
+  // the token's position, and (append) its slots in the caches, if it has any: two rounds of
+  // lookups, which the rows' loads do not wait for
   i64 position = 0, key_at = 0, value_at = 0;
   bool lost = false, placed = false;
   if (APPEND) {
     const Table& t = a.table;
     int b = token;
-    i64 start = token, n = 1;
-    if (t.ends) {
-      b = sequence_of(t.ends, t.sequences, token);
-      if (b < t.sequences) {
-        start = t.ends[b];
-        n = t.ends[b + 1] - start;
-      }
-    }
+    if (t.ends) b = sequence_of(t.ends, t.sequences, token);
     lost = b >= t.sequences;
     if (!lost) {
-      const i64 p = t.lengths[b] - n + (token - start);
-      position = a.offset + p + (a.shift ? a.shift[b] : 0);
+      const i64 start = t.ends ? t.ends[b] : token, stop = t.ends ? t.ends[b + 1] : token + 1;
+      const i64 length = t.lengths[b], shift = a.shift ? a.shift[b] : 0;
       const i64 begin = t.indptr[b], end = min(static_cast<i64>(t.indptr[b + 1]), t.n_indices);
+      const i64 p = length - (stop - start) + (token - start);
+      position = a.offset + p + shift;
       if (p >= 0 && p <= INT32_MAX && begin >= 0 && begin < end) {
         const uint32_t nth = t.by_page(static_cast<uint32_t>(p));
         if (begin + nth < end) {
@@ -74,29 +85,12 @@ __global__ __launch_bounds__(64 * kWavesOf) void norm_rows(Normed a) {
   } else if (a.half) {
     position = a.positions[token];
   }
-
-  using Raw = typename P::template Raw<T>;
-  // row `row` of the token: where it is read, whether it is at all
-  auto from = [&](int row) -> const T* {
-    if (row < a.heads)
-      return static_cast<const T*>(a.query) + token * a.q_token + row * a.q_head;
-    row -= a.heads;
-    if (!APPEND || row < a.kv_heads)
-      return static_cast<const T*>(a.key) + token * a.k_token + row * a.k_head;
-    return static_cast<const T*>(a.value) + token * a.v_token + (row - a.kv_heads) * a.v_head;
-  };
-  auto live = [&](int row) {
-    return row < a.rows && (!APPEND || (row < a.heads ? !lost : placed));
-  };
-  Raw next;
-  int row = first * R + lane / P::G;
-  place.load(from(row < a.rows ? row : 0), live(row), next);
   Turns& turns = s_turns[wave];
   turns_of(turns, position, a.frequency, a.half, a.magnitude);
 
   for (int group = first; group < last; ++group, row += R) {
     Raw x = next;
-    if (group + 1 < last) place.load(from(row + R < a.rows ? row + R : 0), live(row + R), next);
+    if (group + 1 < last) place.load(from(live(row + R) ? row + R : 0), live(row + R), next);
     const bool is_query = row < a.heads, is_value = APPEND && row >= a.heads + a.kv_heads;
     float r = 1.f;
     if (a.normed) {
@@ -183,14 +177,17 @@ int enqueue(Normed& a, int64_t dtype, bool append, const char* what, hipStream_t
   const Lanes l = lanes_of(dtype, a.dim, a.half, a.layout);
   a.rows = a.heads + (append ? 2 : 1) * a.kv_heads;
   a.eights = (a.rows + 64 / l.lanes - 1) / (64 / l.lanes);
-  // Tasks of one group of rows while there are few, else of two or more: waves start with the
-  // token's lookups and angles, and long ones end in an uneven round.  16384 tokens of 40 heads of 128
-  // in bfloat16: 73.6 us by 5 groups, 66.3 by 2 or 1; interleaved, 10 groups, 73.1 by 5, 94.9 by 1.
+  // Tasks of one group of rows while there are few, else of three (of pairs of halves, 32 bytes a lane;
+  // five of 16 bytes): waves start with the token's lookups and angles, and long ones end in an uneven
+  // last turn.  16384 tokens of 40 heads of 128 in bfloat16: 73.6 us by 5 groups, 66.0 by 3, 66.5 by 1;
+  // interleaved 73.2 by 5, 77.0 by 3, 94.9 by 1.  Appending up to 16384 tokens of 48 rows: 53.0 by 1,
+  // 43.9 by 3, 46.9 by 5; interleaved 56.9 by 3, 55.2 by 4.  3000 tokens of 40 heads: 14.5 by 1, 12.7
+  // by 3.
   const int64_t groups = static_cast<int64_t>(a.tokens) * a.eights;
-  int64_t each = groups / 32768;
-  each = each < 1 ? 1 : each < a.eights ? each : a.eights;
-  a.each = static_cast<int>(each);
-  a.splits = (a.eights + a.each - 1) / a.each;
+  int64_t each = groups / 4096, most = a.layout == TG_HALF ? 3 : 5;
+  each = each < 1 ? 1 : each < most ? each : most;
+  a.splits = static_cast<int>((a.eights + each - 1) / each);
+  a.each = (a.eights + a.splits - 1) / a.splits;
   a.by_splits = Div(a.splits);
   const int64_t tasks = static_cast<int64_t>(a.tokens) * a.splits;
   const void* k = dtype == TG_F32   ? kernel_of<float>(a.layout, l, append)
