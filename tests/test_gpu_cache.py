@@ -659,6 +659,9 @@ def _evict(b, keep, recent, first, **more):
     (1, 256, 16, [130, 140], 128, 100, 4), (1, 1000, 16, [50], 30, 11, 2),
     (2, 128, 16, [4000, 3500], 1500, 200, 4), (2, 128, 24, [700, 701, 3], 600, 590, 0),
     (1, 128, 16, [17000], 16000, 15000, 1), (100, 16, 16, [90, 70, 33], 40, 9, 0),
+    # fours of positions that start before the candidates, and as many as threads hold
+    (2, 64, 4, [33, 47, 64], 20, 6, 5), (1, 32, 16, [4161, 4160], 1000, 64, 1),
+    (1, 8, 16, [16394, 16395], 3000, 8, 3), (1, 8, 64, [32780], 3000, 10, 2),
 ])
 def test_paged_evict(hip_ready, dtype, kv_heads, dim, page, lengths, keep, recent, first):
     b = Batch(dtype, kv_heads, kv_heads, dim, page, lengths, seed=keep,

@@ -45,6 +45,21 @@ __device__ __forceinline__ Own own_of(const Table& t, int b) {
   return s;
 }
 
+// N elements that stand anywhere.
+template <typename S, int N>
+struct Loose {
+  typedef S Vec __attribute__((ext_vector_type(N)));
+  struct __attribute__((packed, aligned(sizeof(S)))) Held {
+    Vec v;
+  };
+  static __device__ __forceinline__ Vec load(const S* p) {
+    return reinterpret_cast<const Held*>(p)->v;
+  }
+  static __device__ __forceinline__ void store(S* p, Vec v) {
+    reinterpret_cast<Held*>(p)->v = v;
+  }
+};
+
 constexpr int64_t kMostKeys = INT32_MAX / 2;
 constexpr int64_t kMostStride = int64_t(1) << 60;
 constexpr int64_t kMostGroups = 0xFFFFFF;   // workgroups of a launch

@@ -73,11 +73,20 @@ __device__ __forceinline__ int upto(int v) {
 }
 
 // What a workgroup that chooses shares.
-constexpr int kBins = 256, kCopies = 8, kCopy = kBins + 1;   // copies start in banks of their own
-template <int WAVES, int MOVES>
+// Digits of 11 bits for a large workgroup: two passes mostly, three of 8 bits, and weights of one
+// magnitude spread over four bins (4 x 8 heads of up to 16384 tokens cut to 2048: 29.0 us, 30.4 by 8
+// bits in 8 copies).
+template <int THREADS>
+struct Digit {
+  static constexpr int kBits = THREADS >= 1024 ? 11 : 8, kBins = 1 << kBits;
+  static constexpr int kCopies = THREADS >= 1024 ? 2 : 8;
+  static constexpr int kCopy = kBins + 1;       // copies start in banks of their own
+  static constexpr int kEach = (kBins + THREADS - 1) / THREADS;   // bins of a thread
+};
+template <int THREADS, int MOVES>
 struct Shared {
-  uint32_t bins[kCopies * kCopy];
-  int waves[2][WAVES];
+  uint32_t bins[Digit<THREADS>::kCopies * Digit<THREADS>::kCopy];
+  int waves[2][THREADS / 64];
   uint32_t prefix;
   int left, equal;
   uint32_t moves[MOVES];        // where the fills come from, in order
@@ -88,34 +97,56 @@ struct Spot {
   const float* at;
   bool none;
 };
+__device__ __forceinline__ Spot spot_at(const Evict& a, const int64_t* entry, const float* weights,
+                                        uint32_t slot) {
+  const i64 page = *entry;
+  const bool none = static_cast<uint64_t>(page) >= static_cast<uint64_t>(a.table.pages);
+  // (32 bits each, by strides of 64)
+  return {none ? reinterpret_cast<const float*>(entry)
+               : weights + static_cast<i64>(static_cast<uint32_t>(page)) * a.w_page +
+                     static_cast<i64>(slot) * a.w_slot,
+          none};
+}
 __device__ __forceinline__ Spot spot_of(const Evict& a, const Held& s, const float* weights, int p) {
   const int nth = a.table.by_page(p);
-  const i64 page = s.list[nth];
-  const bool none = page < 0 || page >= a.table.pages;
-  return {none ? reinterpret_cast<const float*>(s.list + nth)
-               : weights + page * a.w_page + (p - nth * a.table.page) * a.w_slot,
-          none};
+  return spot_at(a, s.list + nth, weights, p - nth * a.table.page);
 }
 
 // After a digit's counts: in which bin the `left`-th largest is, how many of it are left, and how
-// many it holds.  Bins are counted from the largest down, one a thread.
+// many it holds.  Bins are counted from the largest down, neighbours by one thread.
 template <int THREADS, typename S>
-__device__ __forceinline__ void find_bin(S& s, uint32_t prefix, int left) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, bin = kBins - 1 - tid;
-  int mine = 0;
-  if (tid < kBins) {
+__device__ __forceinline__ void find_bin(S& s, uint32_t prefix, int bits, int left) {
+  using D = Digit<THREADS>;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int top = D::kBins - 1 - tid * D::kEach;
+  int n[D::kEach], mine = 0;
 #pragma unroll
-    for (int c = 0; c < kCopies; ++c) mine += s.bins[c * kCopy + bin];
+  for (int i = 0; i < D::kEach; ++i) {
+    n[i] = 0;
+    if (top >= i) {
+#pragma unroll
+      for (int c = 0; c < D::kCopies; ++c) n[i] += s.bins[c * D::kCopy + top - i];
+    }
+    mine += n[i];
   }
   int sum = upto(mine);
   if (lane == 63) s.waves[0][wave] = sum;
   __syncthreads();
-  if (tid < kBins) {
-    for (int w = 0; w < wave; ++w) sum += s.waves[0][w];
-    if (sum - mine < left && sum >= left) {
-      s.prefix = prefix << 8 | static_cast<uint32_t>(bin);
-      s.left = left - (sum - mine);
-      s.equal = mine;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int other = s.waves[0][w];
+    sum += w < wave ? other : 0;
+  }
+  if (sum >= left && sum - mine < left) {
+    sum -= mine;
+#pragma unroll
+    for (int i = 0; i < D::kEach; ++i) {
+      if (sum < left && sum + n[i] >= left) {
+        s.prefix = prefix << bits | static_cast<uint32_t>(top - i);
+        s.left = left - sum;
+        s.equal = n[i];
+      }
+      sum += n[i];
     }
   }
   __syncthreads();
@@ -123,109 +154,193 @@ __device__ __forceinline__ void find_bin(S& s, uint32_t prefix, int left) {
 
 template <int THREADS, typename S>
 __device__ __forceinline__ void clear_bins(S& s) {
+  constexpr int kAll = Digit<THREADS>::kCopies * Digit<THREADS>::kCopy;
 #pragma unroll
-  for (int i = 0; i < (kCopies * kCopy + THREADS - 1) / THREADS; ++i)
-    if (threadIdx.x + i * THREADS < kCopies * kCopy) s.bins[threadIdx.x + i * THREADS] = 0;
+  for (int i = 0; i < (kAll + THREADS - 1) / THREADS; ++i)
+    if (threadIdx.x + i * THREADS < kAll) s.bins[threadIdx.x + i * THREADS] = 0;
   __syncthreads();
 }
+// Counts a key: the digit of `bits` from `shift` on.
+template <int THREADS, typename S>
+__device__ __forceinline__ void count_key(S& s, uint32_t key, int shift, int bits) {
+  using D = Digit<THREADS>;
+  atomicAdd(&s.bins[(threadIdx.x % D::kCopies) * D::kCopy + (key >> shift & ((1u << bits) - 1))], 1u);
+}
+
+// Of positions, from the four of the first one on, those that threads have to hold.
+__device__ __forceinline__ int span_of(int count, int first) { return count + (first & 3); }
 
 // Of a sequence and kv head that loses tokens: what stays, from keys that threads hold, EACH to a
-// thread (candidate tid + k THREADS).  Returns how many fill holes; `targets`, if any, are those.
-template <int THREADS, int EACH, typename S, typename F>
-__device__ __forceinline__ int choose_held(S& s, int count, int first, int front, int32_t* kept,
-                                           F&& spot, uint32_t* targets) {
-  constexpr int kWaves = THREADS / 64, kRuns = EACH * kWaves;   // of 64 candidates
+// thread, by fours of neighbouring positions, which start at a multiple of four: one lookup and one
+// load for a four where pages hold whole ones.  The workgroup's instructions bound it, some 100 for a
+// key before and 60 so (14.4 us of 29.0 in the case above, 19 of 34 key by key).  Returns how many
+// fill holes; `targets`, if any, are those.
+template <int THREADS, int EACH, typename S>
+__device__ __forceinline__ int choose_held(const Evict& a, const Held& held, const float* weights,
+                                           S& s, int count, int first, int front, int32_t* kept,
+                                           uint32_t* targets) {
+  constexpr int kWaves = THREADS / 64, kFours = EACH / 4, kRuns = kFours * kWaves;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int last = first + count - 1, base = (first & ~3) + 4 * tid;
+  auto at = [&](int q) { return base + 4 * THREADS * q; };
+  // The keys; 0: none of the candidates, below all of them.
   uint32_t key[EACH];
-  constexpr int kAtOnce = EACH < 16 ? EACH : 16;    // loads in flight; past the last: the last's
+  auto put = [&](int q, int j, float w, bool none) __attribute__((always_inline)) {
+    const uint32_t k = none ? 1u : order_of(w);
+    key[4 * q + j] = static_cast<uint32_t>(at(q) + j - first) < static_cast<uint32_t>(count) ? k : 0u;
+  };
+  constexpr int kAtOnce = kFours < 4 ? kFours : 4;      // loads in flight
+  if (a.table.page % 4 == 0) {
+    // fours lie within a page; past the last candidate: the last's
+    const int page = a.table.page, nth0 = a.table.by_page(first);
+    const int pages = a.table.by_page(4 * THREADS), slots = 4 * THREADS - pages * page;
+    const int64_t* const list = held.list + nth0;
+    const uint32_t last_nth = a.table.by_page(last), last_slot = (last & ~3) - last_nth * page;
+    uint32_t nth = a.table.by_page(base), slot = base - nth * page;
 #pragma unroll
-  for (int k0 = 0; k0 < EACH; k0 += kAtOnce) {
-    Spot at[kAtOnce];
+    for (int q0 = 0; q0 < kFours; q0 += kAtOnce) {
+      Spot x[kAtOnce];
+      float w[kAtOnce][4];
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k)
-      at[k] = spot(first + min(tid + (k0 + k) * THREADS, count - 1));
+      for (int q = 0; q < kAtOnce; ++q) {
+        const bool past = at(q0 + q) > last;
+        x[q] = spot_at(a, list + ((past ? last_nth : nth) - nth0), weights, past ? last_slot : slot);
+        nth += pages;
+        slot += slots;
+        const bool turn = slot >= static_cast<uint32_t>(page);
+        nth += turn;
+        slot -= turn ? page : 0;
+      }
+      if (a.w_slot == 1) {
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) key[k0 + k] = order_of(*at[k].at);
+        for (int q = 0; q < kAtOnce; ++q) {
+          if (!x[q].none) {
+            const auto v = Loose<float, 4>::load(x[q].at);
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k)
-      if (at[k].none) key[k0 + k] = 0u;
+            for (int j = 0; j < 4; ++j) w[q][j] = v[j];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < kAtOnce; ++q) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[q][j] = x[q].at[x[q].none ? 0 : j * a.w_slot];
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kAtOnce; ++q) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put(q0 + q, j, w[q][j], x[q].none);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < kFours; ++q) {
+      Spot x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        x[j] = spot_of(a, held, weights, min(max(at(q) + j, first), last));
+#pragma unroll
+      for (int j = 0; j < 4; ++j) put(q, j, *x[j].at, x[j].none);
+    }
   }
-  // the (front - first)-th largest, by digits of 8 bits; done when all that a bin holds stay
+  // the (front - first)-th largest, digit by digit; done when all that a bin holds stay
   uint32_t prefix = 0;
   int left = front - first, equal = 0, shift = 32;
   do {
-    shift -= 8;
+    const int above = shift, bits = min(Digit<THREADS>::kBits, shift);
+    shift -= bits;
     clear_bins<THREADS>(s);
 #pragma unroll
     for (int k = 0; k < EACH; ++k)
-      if (tid + k * THREADS < count && (shift == 24 || key[k] >> (shift + 8) == prefix))
-        atomicAdd(&s.bins[(lane % kCopies) * kCopy + (key[k] >> shift & 255)], 1u);
+      if (key[k] && (above == 32 || key[k] >> above == prefix))
+        count_key<THREADS>(s, key[k], shift, bits);
     __syncthreads();
-    find_bin<THREADS>(s, prefix, left);
+    find_bin<THREADS>(s, prefix, bits, left);
     prefix = s.prefix;
     left = s.left;
     equal = s.equal;
   } while (shift && left != equal);
   const uint32_t least = prefix << shift;       // what is above stays, and of what is equal `left`
-  const bool ties = left != equal;
 
-  // Places among the flagged, run by run of 64 candidates.
+  // Places among the flagged, run by run: a wave's lanes' fours.
   int* runs = reinterpret_cast<int*>(s.bins);
-  static_assert(kRuns <= kCopies * kCopy && kRuns <= 16 * 64, "");
-  uint64_t mask[EACH];
-  auto rank = [&](auto&& flag) __attribute__((always_inline)) {
-    __syncthreads();
+  static_assert(kRuns <= Digit<THREADS>::kCopies * Digit<THREADS>::kCopy && kFours <= 64, "");
+  int before[kFours];     // flagged, before a lane's own four
+  auto rank = [&](uint32_t flags) __attribute__((always_inline)) {
+    int mine = 0;
 #pragma unroll
-    for (int k = 0; k < EACH; ++k) {
-      mask[k] = __ballot(flag(k, tid + k * THREADS));
-      if (lane == 0) runs[k * kWaves + wave] = __popcll(mask[k]);
+    for (int q = 0; q < kFours; ++q) {
+      int n = 0, all = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t mask = __ballot(flags >> (4 * q + j) & 1);
+        n = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(mask >> 32),
+                                      __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(mask), n));
+        all += __popcll(mask);
+      }
+      before[q] = n;
+      if (lane == q) mine = all;
     }
+    __syncthreads();
+    if (lane < kFours) runs[lane * kWaves + wave] = mine;
     __syncthreads();
     if (wave == 0) {
-      int before = 0;
+      int sums = 0;
+#pragma unroll
       for (int r = lane; r < (kRuns + 63) / 64 * 64; r += 64) {
         const int n = r < kRuns ? runs[r] : 0, sum = upto(n);
-        if (r < kRuns) runs[r] = before + sum - n;
-        before += __builtin_amdgcn_readlane(sum, 63);
+        if (r < kRuns) runs[r] = sums + sum - n;
+        sums += __builtin_amdgcn_readlane(sum, 63);
       }
-      if (lane == 0) s.left = before;
+      if (lane == 0) s.left = sums;
     }
     __syncthreads();
-  };
-  auto nth = [&](int k) __attribute__((always_inline)) {
-    return runs[k * kWaves + wave] + __popcll(mask[k] & ((1ull << lane) - 1));
-  };
-  uint32_t stays = 0;
-  if (ties) {
-    rank([&](int k, int c) { return c < count && key[k] == least; });
+    const int starts = runs[min(lane, kFours - 1) * kWaves + wave];
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (tid + k * THREADS < count &&
-          (key[k] > least || (key[k] == least && nth(k) < left)))
-        stays |= 1u << k;
-  } else {
-#pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (tid + k * THREADS < count && key[k] >= least) stays |= 1u << k;
-  }
-  // holes below the front, then as many that stay past it, which fill them
-  rank([&](int k, int c) {
-    return c < count && (first + c < front) != static_cast<bool>(stays >> k & 1);
-  });
-  const int holes = s.left / 2;
+    for (int q = 0; q < kFours; ++q) before[q] += __builtin_amdgcn_readlane(starts, q);
+  };
+  auto nth_of = [&](uint32_t flags, int q, int j) __attribute__((always_inline)) {
+    return before[q] + __popc(flags >> (4 * q) & ((1u << j) - 1));
+  };
+  uint32_t stays = 0, real = 0;
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
-    const int p = first + tid + k * THREADS;
-    if (p >= front && (stays >> k & 1)) s.moves[nth(k) - holes] = p;
+    stays |= key[k] >= least ? 1u << k : 0u;
+    real |= key[k] ? 1u << k : 0u;
   }
+  if (left != equal) {
+    uint32_t ties = 0;
+#pragma unroll
+    for (int k = 0; k < EACH; ++k) ties |= key[k] == least ? 1u << k : 0u;
+    rank(ties);
+#pragma unroll
+    for (int k = 0; k < EACH; ++k)
+      if ((ties >> k & 1) && nth_of(ties, k / 4, k % 4) >= left) stays &= ~(1u << k);
+  }
+  // holes below the front, then as many that stay past it, which fill them
+  uint32_t below = 0;
+#pragma unroll
+  for (int q = 0; q < kFours; ++q) {
+    const int n = min(max(front - at(q), 0), 4);
+    below |= ((1u << n) - 1) << (4 * q);
+  }
+  const uint32_t flags = (below & real) ^ stays;
+  rank(flags);
+  const int holes = s.left / 2;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k)
+    if ((flags & ~below) >> k & 1)
+      s.moves[nth_of(flags, k / 4, k % 4) - holes] = at(k / 4) + k % 4;
   __syncthreads();
 #pragma unroll
   for (int k = 0; k < EACH; ++k) {
-    const int p = first + tid + k * THREADS;
-    if (p < front && p - first < count) {
+    if ((below & real) >> k & 1) {
+      const int p = at(k / 4) + k % 4;
       const bool stay = stays >> k & 1;
-      kept[p] = stay ? p : static_cast<int>(s.moves[nth(k)]);
-      if (targets && !stay) targets[nth(k)] = p;
+      const int n = nth_of(flags, k / 4, k % 4);
+      kept[p] = stay ? p : static_cast<int>(s.moves[n]);
+      if (targets && !stay) targets[n] = p;
     }
   }
   return holes;
@@ -245,16 +360,17 @@ __device__ __forceinline__ void choose_any(S& s, int count, int first, int front
   };
   uint32_t prefix = 0;
   int left = front - first;
-  for (int shift = 24; shift >= 0; shift -= 8) {
+  for (int shift = 32; shift > 0;) {
+    const int above = shift, bits = min(Digit<THREADS>::kBits, shift);
+    shift -= bits;
     clear_bins<THREADS>(s);
 #pragma unroll 8
     for (int c = tid; c < count; c += THREADS) {
       const uint32_t k = key(c);
-      if (shift == 24 || k >> (shift + 8) == prefix)
-        atomicAdd(&s.bins[(lane % kCopies) * kCopy + (k >> shift & 255)], 1u);
+      if (above == 32 || k >> above == prefix) count_key<THREADS>(s, k, shift, bits);
     }
     __syncthreads();
-    find_bin<THREADS>(s, prefix, left);
+    find_bin<THREADS>(s, prefix, bits, left);
     prefix = s.prefix;
     left = s.left;
   }
@@ -324,7 +440,7 @@ __device__ __forceinline__ void choose_any(S& s, int count, int first, int front
 template <int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void choose(Evict a) {
   constexpr int kMoves = THREADS * EACH / 2;    // at most: as many leave holes as fill them
-  __shared__ Shared<THREADS / 64, kMoves> shared;
+  __shared__ Shared<THREADS, kMoves> shared;
   const int tid = threadIdx.x;
   const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
   const Held s = held_of(a, b);
@@ -338,8 +454,9 @@ __global__ __launch_bounds__(THREADS) void choose(Evict a) {
   const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
   auto spot = [&](int p) { return spot_of(a, s, a.weights + h * a.w_head, p); };
   if (front > a.first) {
-    if (count <= THREADS * EACH)
-      choose_held<THREADS, EACH>(shared, count, a.first, front, kept, spot, nullptr);
+    if (span_of(count, a.first) <= THREADS * EACH)
+      choose_held<THREADS, EACH>(a, s, a.weights + h * a.w_head, shared, count, a.first, front, kept,
+                                 nullptr);
     else
       choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
   }
@@ -547,7 +664,7 @@ __global__ __launch_bounds__(kMovers) void move(Evict a) {
 template <typename T, int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
   constexpr int kMoves = THREADS * EACH / 2, kRows = 256, kFills = 4;
-  __shared__ Shared<THREADS / 64, kMoves> shared;
+  __shared__ Shared<THREADS, kMoves> shared;
   __shared__ uint32_t s_to[kMoves];
   __shared__ i64 s_from[2][kRows], s_target[2][kRows];    // of keys and values
   const int tid = threadIdx.x;
@@ -603,8 +720,8 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
   int fills = 0;
   bool listed = true;
   if (front > a.first) {
-    if (count <= THREADS * EACH) {
-      fills = choose_held<THREADS, EACH>(shared, count, a.first, front, kept, spot, s_to);
+    if (span_of(count, a.first) <= THREADS * EACH) {
+      fills = choose_held<THREADS, EACH>(a, s, weights, shared, count, a.first, front, kept, s_to);
     } else {
       choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
       listed = false;
@@ -680,12 +797,6 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
     __syncthreads();
     if (p < a.keep && !x.none && !y.none) *const_cast<float*>(y.at) = w;
   }
-}
-
-template <typename T>
-const void* whole_of(int64_t candidates) {
-  return candidates <= 2048 ? reinterpret_cast<const void*>(&evict_whole<T, 1024, 2>)
-                            : reinterpret_cast<const void*>(&evict_whole<T, 1024, 4>);
 }
 
 }  // namespace
@@ -786,15 +897,16 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   if (heads * per > kMostGroups) return refuse(-2, what, "2^24 workgroups or more", heads * per);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   void* args[] = {&a};
-  const int64_t most = r->max_length - r->first - r->recent;    // candidates
+  const int64_t most = r->max_length - r->recent - (r->first & ~int64_t(3));    // candidates, in fours
   // One launch where a workgroup's threads hold a head's candidates, unless few heads have many
   // recent tokens to move, which slices do side by side.  8 kv heads of 128, 1088 tokens cut to 1024
   // with 256 recent: 1 sequence 12.9 us, 15.7 in two launches, 32 19.3 and 27.9, 128 87 and 109; 4000
   // to 1024: 13.3 and 14.8, 16.6 and 22.8; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.4, 8
   // 36.9 and 39.1, 64 144 and 188.
   if (most <= 4096 && (heads >= 64 || r->recent * a.units <= 8192)) {
-    const hipError_t e = launch(bytes == 4 ? whole_of<uint32_t>(most) : whole_of<uint16_t>(most),
-                                heads, 1024, args, s);
+    const void* k = bytes == 4 ? reinterpret_cast<const void*>(&evict_whole<uint32_t, 1024, 4>)
+                               : reinterpret_cast<const void*>(&evict_whole<uint16_t, 1024, 4>);
+    const hipError_t e = launch(k, heads, 1024, args, s);
     return e == hipSuccess ? 0 : hip_failed(e, what);
   }
   const int threads = most <= 2048 ? 256 : 1024;

@@ -11,20 +11,6 @@ namespace tg {
 
 constexpr int kMostDim = 256;
 
-template <typename S, int N>
-struct Loose {
-  typedef S Vec __attribute__((ext_vector_type(N)));
-  struct __attribute__((packed, aligned(sizeof(S)))) Held {
-    Vec v;
-  };
-  static __device__ __forceinline__ Vec load(const S* p) {
-    return reinterpret_cast<const Held*>(p)->v;
-  }
-  static __device__ __forceinline__ void store(S* p, Vec v) {
-    reinterpret_cast<Held*>(p)->v = v;
-  }
-};
-
 // v + the same lane's value in another order of its 16 lanes
 template <int ORDER>
 __device__ __forceinline__ float plus(float v) {
