@@ -660,11 +660,12 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
             raise ValueError("query is %s, key %s" % (tuple(qshape), tuple(shape)))
         if query_out is None:
             query_out = _like(query)
+            os_ = query_out.stride()
         else:
             written += (query_out,)
-        oshape, os_ = _heads("query_out", query_out, device, dtype, 3, write=True)
-        if oshape != qshape:
-            raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(qshape)))
+            oshape, os_ = _heads("query_out", query_out, device, dtype, 3, write=True)
+            if oshape != qshape:
+                raise ValueError("query_out is %s, expected %s" % (tuple(oshape), tuple(qshape)))
         heads, q, out = qshape[1], query.data_ptr(), query_out.data_ptr()
     elif query_out is not None:
         raise ValueError("query_out without query")
