@@ -178,8 +178,13 @@ __global__ __launch_bounds__(64 * kWaves) void weigh_narrow(Weights a) {
 
 // Many rows.  A wave keeps KT tiles of 32 keys in registers, a workgroup reads the rows for its four:
 // a stage of up to 64 rows (of heads over 128 32), whole tokens', is taken from LDS while the next
-// one is in flight to registers.  A tile's exponentials and sums run between the products of the
-// next tile: 8 products of 32 cycles beside 16 times (fma, exponential, add) of 4, 8 and 4.
+// one comes, straight to LDS (4 x 4096 tokens on 8192 older keys 399 us, 413 through registers).  A
+// tile's exponentials and sums run between the products of the next tile: 8 products of 32 cycles
+// beside 16 times (fma, exponential, add) of 4, 8 and 4, which by themselves take 256 and 268
+// cycles of a SIMD and together, from registers alone, 412.  Here a tile takes about 570: one sequence
+// of 4096 tokens on 8192 older keys, 32/8 heads of 128, 363 us, 947 TFLOP/s; prompts of up to 4096,
+// where half of what a workgroup's last stages see is masked, 165 us, 712 TFLOP/s.  Neither the loads
+// (15% with none) nor the order of the workgroups (8% slower, all long ones first) is most of it.
 constexpr int wide_rows(int dim) { return dim > 128 ? 32 : 64; }
 
 template <int DP>
@@ -188,11 +193,20 @@ struct Wide {
   static constexpr int kKeys = 32 * KT * kWaves;          // of a workgroup
   static constexpr int kRows = wide_rows(DP);             // of a stage, some of them empty
   static constexpr int kUnits = DP / 8;                   // of 16 bytes of a row
-  static constexpr int kLanes = DP == 96 ? 16 : kUnits;   // that read a row
-  static constexpr int kRow = DP * 2 + 16;                // bytes of a row in LDS: an odd number of units
-  static constexpr int kStep = 64 * kWaves / kLanes;      // rows that a workgroup reads at once
-  static constexpr int kEach = kRows / kStep;
+  static constexpr int kEach = kRows * kUnits / (64 * kWaves);    // units that a lane brings
+  // Rows come straight to LDS, 16 bytes a lane side by side, so they cannot be padded: a row's units
+  // change places instead, and a lane brings the unit that belongs to its place.  8 rows' units of one
+  // number then lie in all banks (16 rows' where a row has 256 bytes).
+  static __device__ __forceinline__ int place(int row) {
+    return DP == 64 ? row >> 1 & 7 : DP == 96 ? row >> 1 & 3 : row & 15;
+  }
 };
+
+// 16 bytes of every lane to LDS at `to` + 16 * lane, without a register between.
+__device__ __forceinline__ void units_to_lds(__amdgpu_buffer_rsrc_t memory, uint32_t at, char* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(memory, (__attribute__((address_space(3))) void*)to, 16,
+                                           at, 0, 0, 0);
+}
 
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
@@ -200,11 +214,12 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
   using M = Matrix<T>;
   using C = Chunk<T>;
   constexpr int KS = DP / 16, KT = W::KT;
-  __shared__ __align__(16) char s_rows[2][W::kRows * W::kRow];
+  // (two arrays: reads of one need not wait for what comes to the other)
+  __shared__ __align__(16) char s_even[W::kRows * 2 * DP], s_odd[W::kRows * 2 * DP];
   __shared__ float s_base[2][W::kRows];
   __shared__ int s_see[2][W::kRows];
   __shared__ int s_strange[2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   // the kv heads side by side (each XCD has its own of 8), then those that read the same rows
   const int unit = a.by_heads(blockIdx.x), kv_head = blockIdx.x - unit * a.kv_heads;
@@ -221,16 +236,19 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
   const float* l_head = a.lse + s.first * a.l_token + kv_head * a.group * a.l_head;
   const T* kc = static_cast<const T*>(a.key_cache) + kv_head * a.kc_head;
 
-  // this thread's unit of the rows r0 + i kStep of a stage, and where they stand from the first
-  const int unit_at = (tid & (W::kLanes - 1)) * 8, r0 = tid / W::kLanes;
-  uint32_t off[W::kEach];   // bytes
+  // where this lane's units of a stage stand from its first row, in bytes; past the last of `left`
+  // rows the last, past the head its first unit (and zero in the keys)
+  auto units_of = [&](int left, uint32_t (&off)[W::kEach]) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < W::kEach; ++i) {
-    const int r = r0 + i * W::kStep, j = a.by_group(r);
-    off[i] = unit_at < a.dim ? static_cast<uint32_t>(2 * (j * a.q_token + (r - j * a.group) *
-                                                          a.q_head + unit_at))
-                             : 0x80000000u;
-  }
+    for (int i = 0; i < W::kEach; ++i) {
+      const int at = (i * kWaves + wave) * 64 + lane, nth = at / W::kUnits;
+      const int r = min(nth, left - 1), j = a.by_group(r), unit = at % W::kUnits ^ W::place(nth);
+      off[i] = static_cast<uint32_t>(2 * (j * a.q_token + (r - j * a.group) * a.q_head +
+                                          (unit * 8 < a.dim ? unit * 8 : 0)));
+    }
+  };
+  uint32_t all[W::kEach];
+  units_of(a.stage_rows, all);
 
   // (keys past the bound that sized the launch: the last split takes them in turn, its first part
   // with all rows)
@@ -243,6 +261,43 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     const int begin = whole ? seen_from : max(seen_from, part * a.part_stages);
     const int end = whole || part + 1 == a.parts ? stages : min(stages, (part + 1) * a.part_stages);
     if (!whole && begin >= end) continue;
+    float next_lse = 0.f;
+    int next_see = 0;
+    auto load = [&](int stage, auto odd) __attribute__((always_inline)) {
+      const int row0 = stage * a.stage_rows, left = min(rows - row0, a.stage_rows);
+      const T* from = q_head + static_cast<i64>(a.by_group(row0)) * a.q_token;
+      const auto memory = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, 0x7FFFFFFF,
+                                                            0x00027000);
+      char* to = (decltype(odd)::value ? s_odd : s_even) + wave * 1024;
+      if (wave == 0) {
+        const int row = min(row0 + lane, rows - 1), j = a.by_group(row);
+        next_lse = l_head[j * a.l_token + (row - j * a.group) * a.l_head];
+        next_see = lane < left ? s.before + j + 1 : INT32_MIN;
+      }
+      uint32_t off[W::kEach];
+#pragma unroll
+      for (int i = 0; i < W::kEach; ++i) off[i] = all[i];
+      if (left < a.stage_rows) units_of(left, off);
+#pragma unroll
+      for (int i = 0; i < W::kEach; ++i)
+        units_to_lds(memory, off[i], to + i * kWaves * 1024);
+    };
+    auto put = [&](int to) __attribute__((always_inline)) {
+      if (wave == 0) {
+        const bool live = next_see != INT32_MIN;
+        if (lane < W::kRows) {
+          s_base[to][lane] = live ? next_lse * kLog2e : INFINITY;
+          s_see[to][lane] = live && next_lse != -INFINITY ? next_see : 0;
+        }
+        const int strange = __any(live && !(fabsf(next_lse) < INFINITY));
+        if (lane == 0) s_strange[to] = strange;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");    // what this wave brings is there
+    };
+    const std::integral_constant<int, 0> even;
+    const std::integral_constant<int, 1> uneven;
+    if (begin < end) load(begin, even);     // under way while the keys' pages are looked up
+
     s16x8 k[KT][KS];
     const T* k_at[KT];
     bool bad[KT];
@@ -281,59 +336,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) sum[t][i] = 0.f;
 
-    s16x8 next[W::kEach];
-    float next_lse = 0.f;
-    int next_see = 0;
-    auto load = [&](int stage) __attribute__((always_inline)) {
-      const int row0 = stage * a.stage_rows, left = min(rows - row0, a.stage_rows);
-      const T* from = q_head + static_cast<i64>(a.by_group(row0)) * a.q_token;
-      const auto memory = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(from), 0, 0x7FFFFFFF,
-                                                            0x00027000);
-#pragma unroll
-      for (int i = 0; i < W::kEach; ++i)    // (past the last row: out of range, zero)
-        next[i] = __builtin_bit_cast(
-            s16x8, __builtin_amdgcn_raw_buffer_load_b128(
-                       memory, r0 + i * W::kStep < left ? off[i] : 0x80000000u, 0, 0));
-      if (wave == 0) {
-        const int row = min(row0 + lane, rows - 1), j = a.by_group(row);
-        next_lse = l_head[j * a.l_token + (row - j * a.group) * a.l_head];
-        next_see = lane < left ? s.before + j + 1 : INT32_MIN;
-      }
-    };
-    auto put = [&](int to) __attribute__((always_inline)) {
-      if (unit_at < DP) {
-#pragma unroll
-        for (int i = 0; i < W::kEach; ++i)
-          *reinterpret_cast<s16x8*>(&s_rows[to][(r0 + i * W::kStep) * W::kRow + 2 * unit_at]) =
-              next[i];
-      }
-      if (wave == 0) {
-        const bool live = next_see != INT32_MIN;
-        if (lane < W::kRows) {
-          s_base[to][lane] = live ? next_lse * kLog2e : INFINITY;
-          s_see[to][lane] = live && next_lse != -INFINITY ? next_see : 0;
-        }
-        const int strange = __any(live && !(fabsf(next_lse) < INFINITY));
-        if (lane == 0) s_strange[to] = strange;
-      }
-    };
-
     // q: rows 32 h .. of a stage; before: the scores of the tile before, which are added up between
     // the products of this one; see: of the lane's keys, counted from its first
     s16x8 q[KS];
     float base = 0.f, base_before = 0.f;
     int see = 0;
     f32x16 before = f32x16(-INFINITY);
-    auto fetch = [&](int at, int h, int i) __attribute__((always_inline)) {
-      q[i] = *reinterpret_cast<const s16x8*>(
-          &s_rows[at][(32 * h + col) * W::kRow + 16 * half + 32 * i]);
+    int in_row = (half ^ W::place(col)) * 16;     // (the same in both halves of 32 rows)
+    auto fetch = [&](auto odd, int h, int i) __attribute__((always_inline)) {
+      q[i] = *reinterpret_cast<const s16x8*>(&(decltype(odd)::value ? s_odd : s_even)[
+          (32 * h + col) * 2 * DP + (2 * i * 16 ^ in_row)]);
     };
-    auto fetch_row = [&](int at, int h) __attribute__((always_inline)) {
-      base = s_base[at][32 * h + col];
-      see = s_see[at][32 * h + col] - key0 - 4 * half;
+    auto fetch_row = [&](auto odd, int h) __attribute__((always_inline)) {
+      base = s_base[odd][32 * h + col];
+      see = s_see[odd][32 * h + col] - key0 - 4 * half;
     };
-    // TILE's products; then, in the last tile of these rows, the rows 32 h of buffer `at` are read
-    auto step = [&](auto tile, bool masked, int at, int h) __attribute__((always_inline)) {
+    // TILE's products; then, in the last tile of these rows, the rows 32 h of a buffer are read
+    auto step = [&](auto tile, bool masked, auto at, int h) __attribute__((always_inline)) {
       constexpr int TILE = decltype(tile)::value, LAST = TILE == KT - 1;
       constexpr int BEFORE = TILE ? TILE - 1 : KT - 1;
       f32x16 sc;
@@ -361,32 +380,36 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
       base_before = base;
       if (LAST) fetch_row(at, h);
     };
-    auto rows32 = [&](bool masked, int at, int h) __attribute__((always_inline)) {
+    auto rows32 = [&](bool masked, auto at, int h) __attribute__((always_inline)) {
+      if (DP > 128) asm volatile("" : "+v"(in_row));    // (16 addresses would not fit beside the rest)
       step(std::integral_constant<int, 0>{}, masked, at, h);
       if constexpr (KT > 1) step(std::integral_constant<int, KT - 1>{}, masked, at, h);
     };
 
     bool strange = false;
+    // the rest of a stage's rows, then the first of the next one's
+    auto stage_of = [&](int stage, auto at, auto other) __attribute__((always_inline)) {
+      strange |= s_strange[at] != 0;
+      const int token = a.by_group(stage * a.stage_rows);
+      const bool masked = __builtin_amdgcn_readfirstlane(s.before + token + 1 < key0 + 32 * KT);
+      if constexpr (W::kRows == 64) rows32(masked, at, 1);
+      // this buffer's rows are all in registers, the next stage's are in the other
+      if (stage + 1 < end) put(other);
+      __syncthreads();
+      if (stage + 2 < end) load(stage + 2, at);
+      rows32(masked, other, 0);
+    };
     if (begin < end) {
-      load(begin);
       put(0);
-      if (begin + 1 < end) load(begin + 1);
+      if (begin + 1 < end) load(begin + 1, uneven);
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < KS; ++i) fetch(0, 0, i);
-      fetch_row(0, 0);
-      int at = 0;
+      for (int i = 0; i < KS; ++i) fetch(even, 0, i);
+      fetch_row(even, 0);
 #pragma unroll 1
-      for (int stage = begin; stage < end; ++stage, at ^= 1) {
-        strange |= s_strange[at] != 0;
-        const int token = a.by_group(stage * a.stage_rows);
-        const bool masked = __builtin_amdgcn_readfirstlane(s.before + token + 1 < key0 + 32 * KT);
-        if constexpr (W::kRows == 64) rows32(masked, at, 1);
-        // this buffer's rows are all in registers, the next stage's go to the other
-        if (stage + 1 < end) put(at ^ 1);
-        __syncthreads();
-        if (stage + 2 < end) load(stage + 2);
-        rows32(masked, at ^ 1, 0);
+      for (int stage = begin; stage < end; stage += 2) {
+        stage_of(stage, even, uneven);
+        if (stage + 1 < end) stage_of(stage + 1, uneven, even);
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e)
@@ -400,14 +423,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
         for (int e = 0; e < 16; ++e) sum[t][e] = 0.f;
 #pragma unroll 1
       for (int stage = begin; stage < end; ++stage) {
-        load(stage);
+        load(stage, even);
         put(0);
         __syncthreads();
 #pragma unroll 1
         for (int h = 0; h < W::kRows / 32; ++h) {
 #pragma unroll
-          for (int i = 0; i < KS; ++i) fetch(0, h, i);
-          fetch_row(0, h);
+          for (int i = 0; i < KS; ++i) {
+            fetch(even, h, i);
+            if (16 * i + 8 * half >= a.dim) q[i] = s16x8(0);
+          }
+          fetch_row(even, h);
 #pragma unroll
           for (int t = 0; t < KT; ++t) {
             f32x16 sc = f32x16(0.f);
@@ -436,7 +462,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
       const int c = lane & 15, key = key0 + 32 * t + 8 * (c / 4) + 4 * half + c % 4;
       if (!(lane & 16) && key < s.keys) {
         if (!whole) {
-          a.part[(static_cast<i64>(unit) * a.kv_heads + kv_head) * W::kKeys + key - first_key] = mine;
+          a.part[((static_cast<i64>(b * a.parts + part) * a.splits + split) * a.kv_heads + kv_head) *
+                     W::kKeys + key - first_key] = mine;
         } else {
           const int nth = a.table.by_page(key);
           const i64 page = s.list[nth];
