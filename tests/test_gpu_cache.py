@@ -279,6 +279,48 @@ def test_norm_rope_gradient(hip_ready, layout):
     assert not packed.grad[:, 3:].any()
 
 
+def test_norm_rope_of_many_heads(hip_ready):
+    """More groups of rows than a launch has waves: heads of one element, which norm to their sign."""
+    x = torch.ones(1 << 20, 200, 1, device="cuda", dtype=BF16)
+    x[::3], x[5, 7], x[-1, -1] = -2, 0, 3
+    y, _ = at.norm_rope(x, None, None, None, epsilon=EPSILON)
+    # 1 and 2 are off by epsilon / 2 and less of themselves, under the type's half step
+    assert torch.equal(y, x.sign())
+
+
+def test_norm_rope_gradient_in_a_graph(hip_ready):
+    """A forward and backward pass captured and replayed, against eager ones."""
+    g = _gen(8)
+    frequency, _ = at.rope_frequencies(64)
+    q, k = (_normal(g, 70, n, 64, dtype=BF16).requires_grad_() for n in (6, 2))
+    wq, wk = (_weights(g, "one", 1, 64, F32).requires_grad_() for _ in range(2))
+    positions = torch.arange(70, device="cuda")
+    gq, gk = torch.ones_like(q), torch.ones_like(k)
+
+    def step():
+        y, z = at.norm_rope(q, k, positions, frequency, wq, wk)
+        return torch.autograd.grad([y, z], [q, k, wq, wk], [gq, gk])
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for i in range(3):
+        with torch.no_grad():
+            q.copy_(_normal(g, *q.shape, dtype=BF16))
+            wk.mul_(1.25)
+        gk.copy_(_normal(g, *gk.shape, dtype=BF16))
+        graph.replay()
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want)), i
+
+
 def test_norm_rope_at_the_ends(hip_ready):
     """Heads of zeros, of infinities and NaN; no tokens; sums past 32 bits' range."""
     frequency, _ = at.rope_frequencies(64)
@@ -516,6 +558,11 @@ SHAPES = [
     (32, 2, 256, 7, [300, 129, 128], [160, 1, 128]),
     (48, 1, 72, 16, [70, 33, 1], [1, 1, 1]),
     (40, 1, 128, 16, [20, 1], [33, 2]),
+    # and heads that do not fill their tiles
+    (16, 1, 40, 16, [200, 100], [60, 3]),
+    (48, 1, 72, 16, [70, 33, 1], [9, 8, 1]),
+    (20, 1, 104, 8, [150, 60], [30, 9]),
+    (32, 1, 200, 8, [133, 70], [20, 2]),
 ]
 
 

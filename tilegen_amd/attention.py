@@ -826,8 +826,9 @@ def attention_weights(query: torch.Tensor, lse: torch.Tensor, key_cache: torch.T
     for the same ``query`` (a prefix's share is in it).  What a key had is multiplied by ``decay``
     first; the new tokens' own keys start from nothing.  Returns ``weights``.
 
-    The other arguments are ``prefix_attention``'s.  Rows that see no key add nothing, and a
-    sequence without new tokens keeps its weights as they are.  ``weights`` may have any strides
+    The other arguments are ``prefix_attention``'s, but a page belongs to one sequence and stands on
+    its list once.  Rows that see no key add nothing, and a sequence without new tokens keeps its
+    weights as they are.  ``weights`` may have any strides
     and is fastest where a head's slots lie side by side: ``torch.zeros(pages, kv_heads,
     page).transpose(1, 2)``.  Scores, exponentials and sums are held in 32 bits; sums are taken in
     an order that the sizes alone decide."""

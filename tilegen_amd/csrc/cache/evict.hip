@@ -8,6 +8,11 @@
 // both lists are taken in order.  No place is both a source and a target of those, so they go in
 // any order; then the recent tokens go down, chunk by chunk, each read whole before it is
 // written.
+//
+// 256 heads of up to 1088 tokens of 128 cut to 1024 (78 MB): 19.8 us, 3.9 TB/s.  32 heads of up to
+// 16384 cut to 2048: 14.4 us to choose, which as many compute units' instructions bound, and 14.7 to
+// move 60 MB, 4.1 TB/s.  9 heads of 210: 11 us, the chain of lookups, two counts, two rankings
+// and the moves' own lookups.
 #include "cache.h"
 
 namespace tg {

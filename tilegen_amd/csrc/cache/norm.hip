@@ -3,6 +3,11 @@
 //
 // z = x r w, r = (mean of x^2 + epsilon)^-1/2, then the pairs (a, b) of z become
 // (a cos - b sin, b cos + a sin).  All in 32 bits, rounded once.
+//
+// Every head is read and written once and memory bounds it: 16384 tokens of 40 heads of 128 in
+// bfloat16 (336 MB) take 66 us, 5.1 TB/s, a large copy's rate; float32 likewise.  A head's sum is 2
+// to 6 exchanges between the lanes that hold it.  The append of up to 16384 tokens of 48 rows
+// takes 43.8 us; of small calls (4.5 to 5 us) launch and lookups are all.
 #include "rows.h"
 
 namespace tg {
@@ -186,7 +191,8 @@ int enqueue(Normed& a, int64_t dtype, bool append, const char* what, hipStream_t
   const int64_t groups = static_cast<int64_t>(a.tokens) * a.eights;
   int64_t each = groups / 4096, most = a.layout == TG_HALF ? 3 : 5;
   each = each < 1 ? 1 : each < most ? each : most;
-  a.splits = static_cast<int>((a.eights + each - 1) / each);
+  const int64_t room = kWavesOf * kMostGroups / a.tokens, splits = (a.eights + each - 1) / each;
+  a.splits = static_cast<int>(splits < room ? splits : room);     // (one launch: at least 8 fit)
   a.each = (a.eights + a.splits - 1) / a.splits;
   a.by_splits = Div(a.splits);
   const int64_t tasks = static_cast<int64_t>(a.tokens) * a.splits;
