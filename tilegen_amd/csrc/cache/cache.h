@@ -45,6 +45,18 @@ __device__ __forceinline__ Own own_of(const Table& t, int b) {
   return s;
 }
 
+// The sum of a value over a wave's lanes up to each.
+__device__ __forceinline__ int upto(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below,
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // within 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last lane of each 16 to
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // the next, of 32 to the other
+  return v;
+}
+
+// What a workgroup that chooses shares.
 // N elements that stand anywhere.
 template <typename S, int N>
 struct Loose {

@@ -66,18 +66,6 @@ __device__ __forceinline__ uint32_t order_of(float w) {
   return x >> 31 ? ~x : x | 0x80000000u;
 }
 
-// The sum of a value over a wave's lanes up to each.
-__device__ __forceinline__ int upto(int v) {
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);   // from 1, 2, 4, 8 lanes below,
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);   // within 16
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);   // the last lane of each 16 to
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);   // the next, of 32 to the other
-  return v;
-}
-
-// What a workgroup that chooses shares.
 // Digits of 11 bits for a large workgroup: two passes mostly, three of 8 bits, and weights of one
 // magnitude spread over four bins (4 x 8 heads of up to 16384 tokens cut to 2048: 29.0 us, 30.4 by 8
 // bits in 8 copies).

@@ -11,6 +11,10 @@
 #include "cache.h"
 
 #include <type_traits>
+#ifndef TG_PARTS
+#define TG_PARTS 4096
+#define TG_STAGES 16
+#endif
 
 namespace tg {
 namespace {
@@ -26,8 +30,9 @@ struct Weights {
   int heads, kv_heads, group, dim, chunk, splits;
   int parts, part_stages; // wide: a sequence's stages of rows are cut into parts of so many
   int stage_rows;         // of 64: whole tokens' where a group fits
+  int packed;             // wide: workgroups take the pieces that there are, those without come last
   float scale, decay;     // scale * log2 e
-  Div by_group, by_heads, by_splits, by_parts, by_stage;
+  Div by_group, by_heads, by_splits, by_parts, by_stage, by_sequences;
 };
 
 
@@ -202,6 +207,19 @@ struct Wide {
   }
 };
 
+// Splits of a sequence's keys that a part of its rows sees; all, if there are more keys than the bound
+// that sized the launch and the part is the one that takes them.
+constexpr int kPairs = 1024;      // of parts and sequences
+template <int KEYS>
+__device__ __forceinline__ int pieces_of(const Weights& a, const Own& s, int part) {
+  const int stages = a.by_stage(s.count * a.group + a.stage_rows - 1);
+  if (part * a.part_stages >= stages) return 0;
+  if (part == 0 && s.keys > a.splits * KEYS) return a.splits;
+  const int end = part + 1 < a.parts ? min(stages, (part + 1) * a.part_stages) : stages;
+  const int tokens = min(s.count, end * a.by_group(a.stage_rows));
+  return min((max(0, min(s.before + tokens, s.keys)) + KEYS - 1) / KEYS, a.splits);
+}
+
 // 16 bytes of every lane to LDS at `to` + 16 * lane, without a register between.
 __device__ __forceinline__ void units_to_lds(__amdgpu_buffer_rsrc_t memory, uint32_t at, char* to) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(memory, (__attribute__((address_space(3))) void*)to, 16,
@@ -223,9 +241,51 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
   const int col = lane & 31, half = lane >> 5;
   // the kv heads side by side (each XCD has its own of 8), then those that read the same rows
   const int unit = a.by_heads(blockIdx.x), kv_head = blockIdx.x - unit * a.kv_heads;
-  const int up = a.by_splits(unit), split = unit - up * a.splits;
-  const int b = a.by_parts(up), part = up - b * a.parts;
-  const Own s = own_of(a.table, b);
+  int b, part, split;
+  Own s;
+  if (!a.packed) {
+    const int up = a.by_splits(unit);
+    split = unit - up * a.splits;
+    b = a.by_parts(up);
+    part = up - b * a.parts;
+    s = own_of(a.table, b);
+  } else {
+    // the unit-th piece of those that there are: a part's splits follow one another
+    __shared__ int s_sum[kWaves];
+    __shared__ struct {
+      Own s;
+      int b, part, split;
+    } s_piece;
+    const int pairs = a.parts * a.table.sequences;
+    if (tid == 0) s_piece.part = -1;
+    int before = 0;
+    for (int pair0 = 0; pair0 < pairs && before <= unit; pair0 += 64 * kWaves) {
+      const int pair = pair0 + tid, nth = a.by_sequences(pair);
+      const Own own = own_of(a.table, pair < pairs ? pair - nth * a.table.sequences : 0);
+      const int n = pair < pairs ? pieces_of<W::kKeys>(a, own, nth) : 0;
+      int sum = upto(n);
+      if (lane == 63) s_sum[wave] = sum;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        if (w == wave) sum += before;
+        before += s_sum[w];
+      }
+      // (before: all so far; sum: those up to this thread's)
+      if (unit < sum && unit >= sum - n) {
+        s_piece.s = own;
+        s_piece.b = pair - nth * a.table.sequences;
+        s_piece.part = nth;
+        s_piece.split = unit - (sum - n);
+      }
+      __syncthreads();
+    }
+    if (s_piece.part < 0) return;
+    b = __builtin_amdgcn_readfirstlane(s_piece.b);
+    part = __builtin_amdgcn_readfirstlane(s_piece.part);
+    split = __builtin_amdgcn_readfirstlane(s_piece.split);
+    s = s_piece.s;
+  }
   const int first_key = split * W::kKeys;
   if (s.count == 0 || first_key >= s.keys) return;
   const int rows = s.count * a.group;
@@ -372,6 +432,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
         for (int e = 16 * i / KS; e < 16 * (i + 1) / KS; ++e)
           sum[BEFORE][e] +=
               __builtin_amdgcn_exp2f(__builtin_fmaf(before[e], a.scale, -base_before));
+        if (LAST) __builtin_amdgcn_sched_barrier(0);    // (the reads would all come behind the products)
       }
       // (the sums stay here: they would be taken behind all products otherwise)
 #pragma unroll
@@ -387,27 +448,41 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     };
 
     bool strange = false;
+    // the other buffer's rows are there, this one's are in registers and the next go over them
+    auto turn = [&](int stage, auto at, int other) __attribute__((always_inline)) {
+      if (stage + 1 < end) put(other);
+      __syncthreads();
+      if (stage + 2 < end) load(stage + 2, at);
+    };
     // the rest of a stage's rows, then the first of the next one's
     auto stage_of = [&](int stage, auto at, auto other) __attribute__((always_inline)) {
       strange |= s_strange[at] != 0;
       const int token = a.by_group(stage * a.stage_rows);
       const bool masked = __builtin_amdgcn_readfirstlane(s.before + token + 1 < key0 + 32 * KT);
       if constexpr (W::kRows == 64) rows32(masked, at, 1);
-      // this buffer's rows are all in registers, the next stage's are in the other
-      if (stage + 1 < end) put(other);
-      __syncthreads();
-      if (stage + 2 < end) load(stage + 2, at);
+      turn(stage, at, other);
       rows32(masked, other, 0);
     };
     if (begin < end) {
       put(0);
       if (begin + 1 < end) load(begin + 1, uneven);
       __syncthreads();
-#pragma unroll
-      for (int i = 0; i < KS; ++i) fetch(even, 0, i);
-      fetch_row(even, 0);
+      // (a wave without a key, or whose keys come later than the workgroup's first, waits for them)
+      const int from = key0 < s.keys ? a.by_stage(max(key0 - s.before, 0) * a.group) - begin : end;
+      const int mine = begin + (max(__builtin_amdgcn_readfirstlane(from), 0) + (key0 >= s.keys) & ~1);
+      int stage = begin;
 #pragma unroll 1
-      for (int stage = begin; stage < end; stage += 2) {
+      for (; stage < mine && stage < end; stage += 2) {
+        turn(stage, even, 1);
+        if (stage + 1 < end) turn(stage + 1, uneven, 0);
+      }
+      if (stage < end) {
+#pragma unroll
+        for (int i = 0; i < KS; ++i) fetch(even, 0, i);
+        fetch_row(even, 0);
+      }
+#pragma unroll 1
+      for (; stage < end; stage += 2) {
         stage_of(stage, even, uneven);
         if (stage + 1 < end) stage_of(stage + 1, uneven, even);
       }
@@ -519,7 +594,7 @@ const void* narrow_of(int dim) {
 
 struct Plan {
   Weights a;
-  int64_t groups, bytes;
+  int64_t groups, pieces, bytes;
   int keys;     // of a wide workgroup; 0: narrow
 };
 
@@ -610,16 +685,27 @@ int plan(const tg_attention_weights* r, Plan* p) {
     // unit are not there yet: 1 sequence of 2048 keys, 8 kv heads of 128, 2048 rows 35 us by 16 and
     // 22 by 4; of 512 keys of 64, 2048 rows 31 and 16; with work for all, by 8, 188 instead of 165.
     const int64_t units = heads * a.splits, stages = (rows + a.stage_rows - 1) / a.stage_rows;
-    int64_t parts = units ? 4096 / units : 1;
+    int64_t parts = units ? TG_PARTS / units : 1;
     const int64_t few = units ? 512 / units : 1;
     const int64_t fine = few < stages / 4 ? few : stages / 4;
-    if (parts > stages / 16) parts = stages / 16 > fine ? stages / 16 : fine;
+    if (parts > stages / TG_STAGES) parts = stages / TG_STAGES > fine ? stages / TG_STAGES : fine;
+    a.part_stages = static_cast<int>(stages);
     if (parts > 1) {
       a.part_stages = static_cast<int>((stages + parts - 1) / parts);
       a.parts = static_cast<int>((stages + a.part_stages - 1) / a.part_stages);
     }
-    p->groups = units * a.parts;
-    if (a.parts > 1) p->bytes = p->groups * p->keys * 4;
+    p->groups = p->pieces = units * a.parts;
+    if (a.parts > 1) p->bytes = p->pieces * p->keys * 4;
+    // Which pieces there are is for the lengths to say, and costs every workgroup a look at all of them:
+    // 158 us without, 149 with for 4 prompts of up to 4096 tokens, 26.1 and 22.1 for 4 of 1024
+    // tokens with 8 heads of their own, 27.5 and 30.6 for 1 of 1024 (512 pieces).
+    const int64_t pairs = static_cast<int64_t>(a.parts) * a.table.sequences;
+    if (p->pieces > (a.table.sequences > 1 ? 256 : 512) && pairs <= kPairs) {
+      a.packed = 1;
+      // all the tokens' stages, and a part of each sequence's that is not whole
+      const int64_t some = (r->tokens / tokens + a.table.sequences) / a.part_stages + a.table.sequences;
+      if (some < pairs) p->groups = some * a.splits * a.kv_heads;
+    }
   } else {
     // Two tiles a wave where there are many: one sequence of 131072 keys, 8 kv heads 55.2 us, 58.2
     // by one; 32 of 2048 19.4 and 18.0.
@@ -630,6 +716,7 @@ int plan(const tg_attention_weights* r, Plan* p) {
   }
   a.by_splits = Div(a.splits);
   a.by_parts = Div(a.parts);
+  a.by_sequences = Div(a.table.sequences > 0 ? a.table.sequences : 1);
   if (p->groups > kMostGroups) return refuse(-2, what, "2^24 workgroups or more", p->groups);
   return 0;
 }
@@ -681,7 +768,7 @@ extern "C" __attribute__((visibility("default"))) int launch_attention_weights(
   hipError_t e = launch(k, p.groups, 64 * kWaves, args, st);
   if (e == hipSuccess && a.parts > 1) {
     void* more[] = {&a, &p.keys};
-    e = launch(reinterpret_cast<const void*>(&join_weights), p.groups / a.parts, 256, more, st);
+    e = launch(reinterpret_cast<const void*>(&join_weights), p.pieces / a.parts, 256, more, st);
   }
   return e == hipSuccess ? 0 : hip_failed(e, what);
 }
