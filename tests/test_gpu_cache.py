@@ -591,6 +591,26 @@ def test_attention_weights_past_their_bounds(hip_ready, bounds):
     b.check_weights(before, lse)
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,lengths,counts,max_length", [
+    # parts of two sizes, most of what there might be absent
+    (64, 1, 64, [900, 50, 40, 10, 300, 17], [520, 40, 3, 0, 20, 17], 8000),
+    (128, 2, 128, [90, 600], [90, 510], 12000),
+    # the same with more keys, and with more new tokens, than the bounds
+    (64, 1, 64, [900, 50, 40, 10, 300, 17], [520, 40, 3, 0, 20, 17], 700),
+    # more sequences than are looked over
+    (1, 1, 64, [3 + i % 50 for i in range(1100)], [i % 3 for i in range(1100)], 1100),
+])
+def test_attention_weights_of_many_pieces(hip_ready, heads, kv_heads, dim, lengths, counts,
+                                          max_length):
+    b = Batch(BF16, heads, kv_heads, dim, 16, lengths, counts).fill()
+    lse, before = b.lse(), b.w.clone()
+    b.weigh(lse, max_query=10 ** 6, max_length=max_length, decay=0.5)
+    b.check_weights(before, lse, decay=0.5)
+    b.w = before.clone()
+    b.weigh(lse, max_query=400, max_length=max_length, decay=0.5)
+    b.check_weights(before, lse, decay=0.5)
+
+
 def test_attention_weights_sum_to_one(hip_ready):
     """With prefix_attention's own logarithms, each row's weights sum to one."""
     b = Batch(BF16, 8, 2, 128, 16, [300, 77, 64], [9, 77, 1]).fill()

@@ -11,10 +11,6 @@
 #include "cache.h"
 
 #include <type_traits>
-#ifndef TG_PARTS
-#define TG_PARTS 4096
-#define TG_STAGES 16
-#endif
 
 namespace tg {
 namespace {
@@ -28,7 +24,8 @@ struct Weights {
   i64 q_token, q_head, l_token, l_head, kc_page, kc_slot, kc_head, w_page, w_slot, w_head;
   float* part;            // [unit, part, keys of a workgroup]: sums of a part of the rows
   int heads, kv_heads, group, dim, chunk, splits;
-  int parts, part_stages; // wide: a sequence's stages of rows are cut into parts of so many
+  int parts, part_stages; // wide: a sequence's stages of rows are cut into parts of so many,
+  int large, last_stages; // the first `large` of them, the others of these
   int stage_rows;         // of 64: whole tokens' where a group fits
   int packed;             // wide: workgroups take the pieces that there are, those without come last
   float scale, decay;     // scale * log2 e
@@ -187,9 +184,9 @@ __global__ __launch_bounds__(64 * kWaves) void weigh_narrow(Weights a) {
 // tile's exponentials and sums run between the products of the next tile: 8 products of 32 cycles
 // beside 16 times (fma, exponential, add) of 4, 8 and 4, which by themselves take 256 and 268
 // cycles of a SIMD and together, from registers alone, 412.  Here a tile takes about 570: one sequence
-// of 4096 tokens on 8192 older keys, 32/8 heads of 128, 363 us, 947 TFLOP/s; prompts of up to 4096,
-// where half of what a workgroup's last stages see is masked, 165 us, 712 TFLOP/s.  Neither the loads
-// (15% with none) nor the order of the workgroups (8% slower, all long ones first) is most of it.
+// of 4096 tokens on 8192 older keys, 32/8 heads of 128, 363 us, 947 TFLOP/s (323 us with zeros for
+// operands: power is part of it).  4 prompts of up to 4096 tokens take 146 us, 805 TFLOP/s: the
+// start of a workgroup, masked halves and the last workgroups' end are the rest.
 constexpr int wide_rows(int dim) { return dim > 128 ? 32 : 64; }
 
 template <int DP>
@@ -207,15 +204,24 @@ struct Wide {
   }
 };
 
+// Where a part begins (the last ends with the rows), and whose a stage is.
+__device__ __forceinline__ int part_begin(const Weights& a, int part) {
+  return min(part, a.large) * a.part_stages + max(part - a.large, 0) * a.last_stages;
+}
+__device__ __forceinline__ int part_of(const Weights& a, int stage) {
+  const int past = stage - a.large * a.part_stages;
+  return min(past < 0 ? stage / a.part_stages : a.large + past / a.last_stages, a.parts - 1);
+}
+
 // Splits of a sequence's keys that a part of its rows sees; all, if there are more keys than the bound
 // that sized the launch and the part is the one that takes them.
 constexpr int kPairs = 1024;      // of parts and sequences
 template <int KEYS>
 __device__ __forceinline__ int pieces_of(const Weights& a, const Own& s, int part) {
   const int stages = a.by_stage(s.count * a.group + a.stage_rows - 1);
-  if (part * a.part_stages >= stages) return 0;
+  if (part_begin(a, part) >= stages) return 0;
   if (part == 0 && s.keys > a.splits * KEYS) return a.splits;
-  const int end = part + 1 < a.parts ? min(stages, (part + 1) * a.part_stages) : stages;
+  const int end = part + 1 < a.parts ? min(stages, part_begin(a, part + 1)) : stages;
   const int tokens = min(s.count, end * a.by_group(a.stage_rows));
   return min((max(0, min(s.before + tokens, s.keys)) + KEYS - 1) / KEYS, a.splits);
 }
@@ -318,8 +324,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     // from the first token that sees the first key on
     const int seen_from =
         a.by_stage(max(first_key + block * W::kKeys - s.before, 0) * a.group);
-    const int begin = whole ? seen_from : max(seen_from, part * a.part_stages);
-    const int end = whole || part + 1 == a.parts ? stages : min(stages, (part + 1) * a.part_stages);
+    const int begin = whole ? seen_from : max(seen_from, part_begin(a, part));
+    const int end = whole || part + 1 == a.parts ? stages : min(stages, part_begin(a, part + 1));
     if (!whole && begin >= end) continue;
     float next_lse = 0.f;
     int next_see = 0;
@@ -563,9 +569,9 @@ __global__ __launch_bounds__(256) void join_weights(Weights a, int keys) {
   if (s.count == 0 || static_cast<int>(threadIdx.x) >= keys || key >= s.keys) return;
   const int stages = a.by_stage(s.count * a.group + a.stage_rows - 1);
   const int seen_from = a.by_stage(max(first_key - s.before, 0) * a.group);
-  const int last = min(a.parts - 1, (stages - 1) / a.part_stages);
+  const int last = part_of(a, stages - 1);
   float sum = 0.f;
-  for (int part = min(seen_from / a.part_stages, a.parts - 1); part <= last; ++part)
+  for (int part = part_of(a, seen_from); part <= last; ++part)
     sum += a.part[((static_cast<i64>(b * a.parts + part) * a.splits + split) * a.kv_heads + kv_head) *
                       keys + threadIdx.x];
   const int nth = a.table.by_page(key);
@@ -683,16 +689,28 @@ int plan(const tg_attention_weights* r, Plan* p) {
     // Parts of the rows, of 16 stages at least: earlier keys are seen by more rows, so that a round of
     // workgroups with all rows ends with a few long ones.  Of 4 stages while two workgroups a compute
     // unit are not there yet: 1 sequence of 2048 keys, 8 kv heads of 128, 2048 rows 35 us by 16 and
-    // 22 by 4; of 512 keys of 64, 2048 rows 31 and 16; with work for all, by 8, 188 instead of 165.
+    // 22 by 4; of 512 keys of 64, 2048 rows 31 and 16; with work for all, by 8, 188 instead of 165,
+    // since a workgroup spends 9 us on lookups and keys before its first product.
     const int64_t units = heads * a.splits, stages = (rows + a.stage_rows - 1) / a.stage_rows;
-    int64_t parts = units ? TG_PARTS / units : 1;
+    int64_t parts = units ? 4096 / units : 1;
     const int64_t few = units ? 512 / units : 1;
     const int64_t fine = few < stages / 4 ? few : stages / 4;
-    if (parts > stages / TG_STAGES) parts = stages / TG_STAGES > fine ? stages / TG_STAGES : fine;
-    a.part_stages = static_cast<int>(stages);
+    if (parts > stages / 16) parts = stages / 16 > fine ? stages / 16 : fine;
+    a.part_stages = a.last_stages = static_cast<int>(stages);
+    a.large = 1;
     if (parts > 1) {
-      a.part_stages = static_cast<int>((stages + parts - 1) / parts);
+      a.part_stages = a.last_stages = static_cast<int>((stages + parts - 1) / parts);
       a.parts = static_cast<int>((stages + a.part_stages - 1) / a.part_stages);
+      a.large = a.parts;
+      // The last quarter in halves where there are some rounds of workgroups: what starts last ends
+      // sooner (4 prompts of up to 4096 tokens 146 us, 152 in equal parts; on 8192 older keys 363 and 404;
+      // one such prompt 372 and 364).
+      if (units * a.parts > 1024 && a.part_stages >= 16) {
+        a.large = a.parts * 3 / 4;
+        a.last_stages = (a.part_stages + 1) / 2;
+        const int rest = static_cast<int>(stages) - a.large * a.part_stages;
+        a.parts = a.large + (rest + a.last_stages - 1) / a.last_stages;
+      }
     }
     p->groups = p->pieces = units * a.parts;
     if (a.parts > 1) p->bytes = p->pieces * p->keys * 4;
@@ -703,7 +721,7 @@ int plan(const tg_attention_weights* r, Plan* p) {
     if (p->pieces > (a.table.sequences > 1 ? 256 : 512) && pairs <= kPairs) {
       a.packed = 1;
       // all the tokens' stages, and a part of each sequence's that is not whole
-      const int64_t some = (r->tokens / tokens + a.table.sequences) / a.part_stages + a.table.sequences;
+      const int64_t some = (r->tokens / tokens + a.table.sequences) / a.last_stages + a.table.sequences;
       if (some < pairs) p->groups = some * a.splits * a.kv_heads;
     }
   } else {
