@@ -362,18 +362,23 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
     };
     const std::integral_constant<int, 0> even;
     const std::integral_constant<int, 1> uneven;
-    if (begin < end) load(begin, even);     // under way while the keys' pages are looked up
 
     s16x8 k[KT][KS];
     const T* k_at[KT];
     bool bad[KT];
+    i64 page[KT];
+    int slot[KT];
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      const int key = min(key0 + 32 * t + col, s.keys - 1);
-      const int nth = a.table.by_page(key);
-      const i64 page = s.list[nth];
-      bad[t] = page < 0 || page >= a.table.pages;
-      k_at[t] = kc + (bad[t] ? 0 : page * a.kc_page + (key - nth * a.table.page) * a.kc_slot);
+      const int key = min(key0 + 32 * t + col, s.keys - 1), nth = a.table.by_page(key);
+      page[t] = s.list[nth];
+      slot[t] = key - nth * a.table.page;
+    }
+    if (begin < end) load(begin, even);     // (on its way beside the keys, behind their pages)
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      bad[t] = page[t] < 0 || page[t] >= a.table.pages;
+      k_at[t] = kc + (bad[t] ? 0 : page[t] * a.kc_page + slot[t] * a.kc_slot);
     }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
