@@ -726,6 +726,9 @@ def _evict(b, keep, recent, first, **more):
     (1, 256, 16, [130, 140], 128, 100, 4), (1, 1000, 16, [50], 30, 11, 2),
     (2, 128, 16, [4000, 3500], 1500, 200, 4), (2, 128, 24, [700, 701, 3], 600, 590, 0),
     (1, 128, 16, [17000], 16000, 15000, 1), (100, 16, 16, [90, 70, 33], 40, 9, 0),
+    # workgroups of 512 and of 256 threads
+    (128, 24, 16, [90, 700, 33], 60, 9, 1), (350, 40, 8, [300, 41], 40, 17, 3),
+    (170, 128, 16, [1100, 90, 1200, 1030], 1000, 260, 2), (130, 8, 4, [4000, 20], 1500, 300, 0),
     # fours of positions that start before the candidates, and as many as threads hold
     (2, 64, 4, [33, 47, 64], 20, 6, 5), (1, 32, 16, [4161, 4160], 1000, 64, 1),
     (1, 8, 16, [16394, 16395], 3000, 8, 3), (1, 8, 64, [32780], 3000, 10, 2),
@@ -767,6 +770,12 @@ def test_evict_past_its_bound(hip_ready, lengths, keep, max_length):
     """max_length sizes the launch: longer sequences are cut all the same."""
     b = Batch(BF16, 2, 2, 64, 16, lengths).fill()
     _evict(b, keep, 30, 2, max_length=max_length)
+
+
+@pytest.mark.parametrize("kv_heads", [140, 350])
+def test_evict_many_heads_past_the_bound(hip_ready, kv_heads):
+    b = Batch(BF16, kv_heads, kv_heads, 8, 16, [4700, 50]).fill()
+    _evict(b, 3000, 30, 1, max_length=3300)
 
 
 def test_evict_lost_pages(hip_ready):

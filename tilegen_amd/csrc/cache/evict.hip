@@ -792,6 +792,13 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
   }
 }
 
+template <typename T>
+const void* whole_of(int threads) {
+  return threads == 256   ? reinterpret_cast<const void*>(&evict_whole<T, 256, 16>)
+         : threads == 512 ? reinterpret_cast<const void*>(&evict_whole<T, 512, 8>)
+                          : reinterpret_cast<const void*>(&evict_whole<T, 1024, 4>);
+}
+
 }  // namespace
 }  // namespace tg
 
@@ -897,9 +904,13 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   // to 1024: 13.3 and 14.8, 16.6 and 22.8; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.4, 8
   // 36.9 and 39.1, 64 144 and 188.
   if (most <= 4096 && (heads >= 64 || r->recent * a.units <= 8192)) {
-    const void* k = bytes == 4 ? reinterpret_cast<const void*>(&evict_whole<uint32_t, 1024, 4>)
-                               : reinterpret_cast<const void*>(&evict_whole<uint16_t, 1024, 4>);
-    const hipError_t e = launch(k, heads, 1024, args, s);
+    // Workgroups that fill a compute unit by themselves while there is one for each, smaller ones side by
+    // side for more heads.  By 1024, 512 and 256 threads, up to 949 tokens of 80 cut to 166: 384 heads
+    // 24.9, 18.1 and 20.6 us, 848 heads 50, 36 and 33; up to 1088 of 128 cut to 1024: 256 heads 20.4,
+    // 22.9 and 28.1, 512 heads 40.9, 38.9 and 41.3, 1024 heads 90, 79 and 73.
+    const int threads = heads <= 256 ? 1024 : heads <= 640 ? 512 : 256;
+    const void* k = bytes == 4 ? whole_of<uint32_t>(threads) : whole_of<uint16_t>(threads);
+    const hipError_t e = launch(k, heads, threads, args, s);
     return e == hipSuccess ? 0 : hip_failed(e, what);
   }
   const int threads = most <= 2048 ? 256 : 1024;
