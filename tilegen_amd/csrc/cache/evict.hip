@@ -900,9 +900,9 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   const int64_t most = r->max_length - r->recent - (r->first & ~int64_t(3));    // candidates, in fours
   // One launch where a workgroup's threads hold a head's candidates, unless few heads have many
   // recent tokens to move, which slices do side by side.  8 kv heads of 128, 1088 tokens cut to 1024
-  // with 256 recent: 1 sequence 12.9 us, 15.7 in two launches, 32 19.3 and 27.9, 128 87 and 109; 4000
-  // to 1024: 13.3 and 14.8, 16.6 and 22.8; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.4, 8
-  // 36.9 and 39.1, 64 144 and 188.
+  // with 256 recent: 1 sequence 14.2 us, 15.2 in two launches, 32 20.2 and 29.4, 128 74 and 134; 4000
+  // to 1024: 12.6 and 14.2, 15.5 and 23.9; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.3, 8
+  // 35.3 and 38.8, 64 138 and 214.
   if (most <= 4096 && (heads >= 64 || r->recent * a.units <= 8192)) {
     // Workgroups that fill a compute unit by themselves while there is one for each, smaller ones side by
     // side for more heads.  By 1024, 512 and 256 threads, up to 949 tokens of 80 cut to 166: 384 heads

@@ -675,11 +675,11 @@ int plan(const tg_attention_weights* r, Plan* p) {
   const int64_t rows = (r->query_indptr && bound > 0 ? bound : 1) * a.group;   // of a sequence
   a.parts = 1;
   // Wide for many rows, or not so few with much work for all (whole tokens in a stage, within 32 bits
-  // of its first).  32 sequences of up to 2048 keys, 8 kv heads of 128: 64 rows 29 us narrow, 36 wide;
-  // 128 rows 40 and 39; 512 rows 109 and 60.  8 of up to 1000 keys: 256 rows 19 and 14, 512 rows 32
-  // and 22.  One of 16384 keys, 4 kv heads: 64 rows 10.0 and 11.4, 256 rows 21 and 16.  4 of up to 700
-  // keys, 4 kv heads of 64: 256 rows 9.5 and 12.5, 512 rows 15.5 and 15.2, 1024 rows 27 and 16.  2 of
-  // up to 1500, 16 kv heads of 128: 128 rows 9.7 and 10.5.
+  // of its first).  32 sequences of up to 2048 keys, 8 kv heads of 128: 64 rows 29 us narrow, 33 wide;
+  // 128 rows 40 and 36; 512 rows 108 and 56.  8 of up to 1000 keys: 256 rows 19 and 14, 512 rows 32
+  // and 18.  One of 16384 keys, 4 kv heads: 64 rows 10 and 12, 256 rows 21 and 16.  4 of up to 700
+  // keys, 4 kv heads of 64: 256 rows 9.6 and 13.0, 512 rows 15.5 and 15.9, 1024 rows 27 and 16.  2 of
+  // up to 1500, 16 kv heads of 128: 128 rows 9.7 and 10.7.
   const int64_t room = wide_rows(a.dim), tokens = room / a.group;
   auto within = [](int64_t steps, int64_t stride) {
     return steps == 0 || (stride >= 0 && stride <= (int64_t(1) << 28) / steps);
