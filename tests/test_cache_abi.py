@@ -218,6 +218,54 @@ def test_operands_on_the_host_are_refused():
             call()
 
 
+def test_calls_go_by_the_operands_device(monkeypatch):
+    """Workspaces' sizes and launches are asked for with the operands' device current, on its stream
+    (a stand-in library; host tensors count as device -1)."""
+    current, seen = [0], []
+
+    class Device:
+        def __init__(self, device):
+            self.device = device
+
+        def __enter__(self):
+            self.before, current[0] = current[0], self.device
+
+        def __exit__(self, *_):
+            current[0] = self.before
+
+    class Library:
+        def __getattr__(self, name):
+            def entry(packed, *stream):
+                seen.append((name, current[0]) + stream)
+                return 0 if stream else 64
+            return entry
+
+    monkeypatch.setattr(at, "_cache_lib", Library)
+    monkeypatch.setattr(at, "_operand", lambda name, t, dtypes: (t.get_device(), t.dtype))
+    monkeypatch.setattr(at, "_raw_stream", lambda device: 1000 + device)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: current[0])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    n, f = torch.zeros(3, dtype=torch.int64), torch.zeros(32, dtype=torch.float64)
+    cache, w = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16), torch.zeros(2, 16, 2)
+    calls = [
+        (lambda: at.norm_rope(x, x, n[:2], f), ["launch_norm_rope"]),
+        (lambda: at.norm_rope_backward(x, x, x, x, n[:2], f),
+         ["norm_rope_backward_workspace", "launch_norm_rope_backward"]),
+        (lambda: at.paged_append(x, x, cache, cache, n, n, n[:2], f, shift=n[:2]),
+         ["launch_paged_append_normed"]),
+        (lambda: at.attention_weights(x, w[:, 0], cache, w, n, n, n[:2], max_length=1),
+         ["attention_weights_workspace", "launch_attention_weights"]),
+        (lambda: at.paged_evict(w, cache, cache, n, n, n[:2], keep=1, max_length=1),
+         ["launch_paged_evict"])]
+    for call, entries in calls:
+        for current[0] in (0, -1):
+            seen.clear()
+            call()
+            assert [(e[0], e[1]) for e in seen] == [(name, -1) for name in entries]
+            assert seen[-1][2] == 999
+
+
 def test_kernels_do_not_spill(tmp_path):
     readelf = "/opt/rocm/llvm/bin/llvm-readelf"
     if not os.path.exists(readelf):
