@@ -611,6 +611,32 @@ def test_attention_weights_of_many_pieces(hip_ready, heads, kv_heads, dim, lengt
     b.check_weights(before, lse, decay=0.5)
 
 
+def test_attention_weights_of_prompts_in_a_graph(hip_ready):
+    """Parts joined through a workspace, captured twice and replayed in turn, beside eager calls."""
+    b = Batch(BF16, 32, 2, 64, 16, [700, 90, 400], [600, 40, 300]).fill()
+    other = Batch(BF16, 32, 2, 64, 16, [500, 300], [420, 300], seed=5).fill()
+    sides = [(x, x.lse(), x.w.clone()) for x in (b, other)]
+    graphs = []
+    for x, lse, before in sides:
+        x.weigh(lse)
+    torch.cuda.synchronize()
+    for x, lse, before in sides:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            x.weigh(lse)
+    for i in range(3):
+        for (x, lse, before), graph in zip(sides, graphs):
+            x.query.copy_(_normal(_gen(i), *x.query.shape, dtype=BF16))
+            x.w.copy_(before)
+            x.weigh(lse)
+            want = x.w.clone()
+            x.w.copy_(before)
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(x.w.nan_to_num(-7), want.nan_to_num(-7)), i
+
+
 def test_attention_weights_sum_to_one(hip_ready):
     """With prefix_attention's own logarithms, each row's weights sum to one."""
     b = Batch(BF16, 8, 2, 128, 16, [300, 77, 64], [9, 77, 1]).fill()
