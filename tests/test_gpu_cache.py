@@ -637,6 +637,20 @@ def test_attention_weights_of_prompts_in_a_graph(hip_ready):
             assert torch.equal(x.w.nan_to_num(-7), want.nan_to_num(-7)), i
 
 
+@pytest.mark.parametrize("sequences", [2, 64, 65, 200, 256, 257])
+@pytest.mark.parametrize("several", [False, True])
+def test_attention_weights_of_many_sequences(hip_ready, sequences, several):
+    lengths = [(37 * i) % 150 + 1 for i in range(sequences)]
+    counts = [i % 3 if several else 1 for i in range(sequences)]
+    b = Batch(F16, 4, 2, 64, 8, lengths, counts).fill()
+    lse, before = b.lse(), b.w.clone()
+    b.weigh(lse)
+    b.check_weights(before, lse)
+    b.w = before.clone()
+    b.weigh(lse, max_length=40)     # the last piece of a sequence takes what is past the bound
+    b.check_weights(before, lse)
+
+
 def test_attention_weights_sum_to_one(hip_ready):
     """With prefix_attention's own logarithms, each row's weights sum to one."""
     b = Batch(BF16, 8, 2, 128, 16, [300, 77, 64], [9, 77, 1]).fill()
