@@ -48,15 +48,35 @@ __device__ __forceinline__ Held held_of(const Evict& a, int b) {
   return {t.indices + begin, static_cast<int>(length < room ? length : room)};
 }
 
-// A position's page (-1: outside the cache) and slot.
+// A sequence's pages, -1 for those outside the cache: from its list, or the first of them from LDS,
+// where a lookup does not wait for memory (1024 heads of 1088 tokens 69 us, 73 by the list; 3 to 8%
+// with many heads, nothing with few).
+struct Far {
+  const int64_t* list;
+  i64 pages;
+  __device__ __forceinline__ i64 operator()(int nth) const {
+    const i64 page = list[nth];
+    return page >= 0 && page < pages ? page : -1;
+  }
+};
+struct Near {
+  const int32_t* near;
+  int count;
+  Far far;
+  __device__ __forceinline__ i64 operator()(int nth) const {
+    return nth < count ? near[nth] : far(nth);
+  }
+};
+
+// A position's page and slot.
 struct Place {
   i64 page;
   int slot;
 };
-__device__ __forceinline__ Place place_of(const Evict& a, const int64_t* list, int p) {
+template <typename P>
+__device__ __forceinline__ Place place_of(const Evict& a, const P& page_of, int p) {
   const int nth = a.table.by_page(p);
-  const i64 page = list[nth];
-  return {page >= 0 && page < a.table.pages ? page : -1, p - nth * a.table.page};
+  return {page_of(nth), p - nth * a.table.page};
 }
 
 // Whole numbers in the order of the weights: 0 for none, the largest for NaN; -0 is 0.
@@ -90,19 +110,19 @@ struct Spot {
   const float* at;
   bool none;
 };
-__device__ __forceinline__ Spot spot_at(const Evict& a, const int64_t* entry, const float* weights,
+__device__ __forceinline__ Spot spot_at(const Evict& a, i64 page, const float* weights,
                                         uint32_t slot) {
-  const i64 page = *entry;
-  const bool none = static_cast<uint64_t>(page) >= static_cast<uint64_t>(a.table.pages);
   // (32 bits each, by strides of 64)
-  return {none ? reinterpret_cast<const float*>(entry)
-               : weights + static_cast<i64>(static_cast<uint32_t>(page)) * a.w_page +
-                     static_cast<i64>(slot) * a.w_slot,
-          none};
+  return {page < 0 ? reinterpret_cast<const float*>(a.table.indptr)
+                   : weights + static_cast<i64>(static_cast<uint32_t>(page)) * a.w_page +
+                         static_cast<i64>(slot) * a.w_slot,
+          page < 0};
 }
-__device__ __forceinline__ Spot spot_of(const Evict& a, const Held& s, const float* weights, int p) {
-  const int nth = a.table.by_page(p);
-  return spot_at(a, s.list + nth, weights, p - nth * a.table.page);
+template <typename P>
+__device__ __forceinline__ Spot spot_of(const Evict& a, const P& page_of, const float* weights,
+                                        int p) {
+  const Place at = place_of(a, page_of, p);
+  return spot_at(a, at.page, weights, at.slot);
 }
 
 // After a digit's counts: in which bin the `left`-th largest is, how many of it are left, and how
@@ -168,8 +188,8 @@ __device__ __forceinline__ int span_of(int count, int first) { return count + (f
 // load for a four where pages hold whole ones.  The workgroup's instructions bound it, some 100 for a
 // key before and 60 so (14.4 us of 29.0 in the case above, 19 of 34 key by key).  Returns how many
 // fill holes; `targets`, if any, are those.
-template <int THREADS, int EACH, typename S>
-__device__ __forceinline__ int choose_held(const Evict& a, const Held& held, const float* weights,
+template <int THREADS, int EACH, typename S, typename P>
+__device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, const float* weights,
                                            S& s, int count, int first, int front, int32_t* kept,
                                            uint32_t* targets) {
   constexpr int kWaves = THREADS / 64, kFours = EACH / 4, kRuns = kFours * kWaves;
@@ -185,9 +205,8 @@ __device__ __forceinline__ int choose_held(const Evict& a, const Held& held, con
   constexpr int kAtOnce = kFours < 4 ? kFours : 4;      // loads in flight
   if (a.table.page % 4 == 0) {
     // fours lie within a page; past the last candidate: the last's
-    const int page = a.table.page, nth0 = a.table.by_page(first);
+    const int page = a.table.page;
     const int pages = a.table.by_page(4 * THREADS), slots = 4 * THREADS - pages * page;
-    const int64_t* const list = held.list + nth0;
     const uint32_t last_nth = a.table.by_page(last), last_slot = (last & ~3) - last_nth * page;
     uint32_t nth = a.table.by_page(base), slot = base - nth * page;
 #pragma unroll
@@ -197,7 +216,7 @@ __device__ __forceinline__ int choose_held(const Evict& a, const Held& held, con
 #pragma unroll
       for (int q = 0; q < kAtOnce; ++q) {
         const bool past = at(q0 + q) > last;
-        x[q] = spot_at(a, list + ((past ? last_nth : nth) - nth0), weights, past ? last_slot : slot);
+        x[q] = spot_at(a, page_of(past ? last_nth : nth), weights, past ? last_slot : slot);
         nth += pages;
         slot += slots;
         const bool turn = slot >= static_cast<uint32_t>(page);
@@ -232,7 +251,7 @@ __device__ __forceinline__ int choose_held(const Evict& a, const Held& held, con
       Spot x[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        x[j] = spot_of(a, held, weights, min(max(at(q) + j, first), last));
+        x[j] = spot_of(a, page_of, weights, min(max(at(q) + j, first), last));
 #pragma unroll
       for (int j = 0; j < 4; ++j) put(q, j, *x[j].at, x[j].none);
     }
@@ -445,10 +464,11 @@ __global__ __launch_bounds__(THREADS) void choose(Evict a) {
     return;
   }
   const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
-  auto spot = [&](int p) { return spot_of(a, s, a.weights + h * a.w_head, p); };
+  const Far page_of = {s.list, a.table.pages};
+  auto spot = [&](int p) { return spot_of(a, page_of, a.weights + h * a.w_head, p); };
   if (front > a.first) {
     if (span_of(count, a.first) <= THREADS * EACH)
-      choose_held<THREADS, EACH>(a, s, a.weights + h * a.w_head, shared, count, a.first, front, kept,
+      choose_held<THREADS, EACH>(a, page_of, a.weights + h * a.w_head, shared, count, a.first, front, kept,
                                  nullptr);
     else
       choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
@@ -497,7 +517,7 @@ struct Slice {
   int dim, units;
   Div by_units;
   __device__ __forceinline__ i64 row(const Evict& a, const int64_t* list, int p) const {
-    const Place at = place_of(a, list, p);
+    const Place at = place_of(a, Far{list, a.table.pages}, p);
     return at.page < 0 ? kNowhere : at.page * by_page + at.slot * by_slot;
   }
 };
@@ -656,10 +676,11 @@ __global__ __launch_bounds__(kMovers) void move(Evict a) {
 // keys, values and weights, the recent tokens' on their way while it chooses.
 template <typename T, int THREADS, int EACH>
 __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
-  constexpr int kMoves = THREADS * EACH / 2, kRows = 256, kFills = 4;
+  constexpr int kMoves = THREADS * EACH / 2, kRows = 256, kFills = 4, kNear = 512;
   __shared__ Shared<THREADS, kMoves> shared;
   __shared__ uint32_t s_to[kMoves];
   __shared__ i64 s_from[2][kRows], s_target[2][kRows];    // of keys and values
+  __shared__ int32_t s_pages[kNear];
   const int tid = threadIdx.x;
   const int b = a.by_heads(blockIdx.x), h = blockIdx.x - b * a.kv_heads;
   const Held s = held_of(a, b);
@@ -671,11 +692,15 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
     return;
   }
   const int front = a.keep - a.recent, count = s.keys - a.recent - a.first;
+  const Far far = {s.list, a.table.pages};
+  const Near page_of = {s_pages, min(static_cast<int>(a.table.by_page(s.keys - 1)) + 1, kNear), far};
+  for (int i = tid; i < page_of.count; i += THREADS) s_pages[i] = static_cast<int32_t>(far(i));
+  __syncthreads();
   T* const keys = static_cast<T*>(a.key_cache) + h * a.kc_head;
   T* const values = static_cast<T*>(a.value_cache) + h * a.vc_head;
   float* const weights = a.weights + h * a.w_head;
   auto put_row = [&](int n, int from, int to) {
-    const Place x = place_of(a, s.list, from), y = place_of(a, s.list, to);
+    const Place x = place_of(a, page_of, from), y = place_of(a, page_of, to);
     const bool none = x.page < 0 || y.page < 0;
     s_from[0][n] = none ? kNowhere : x.page * a.kc_page + x.slot * a.kc_slot;
     s_target[0][n] = none ? kNowhere : y.page * a.kc_page + y.slot * a.kc_slot;
@@ -703,7 +728,7 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
     }
   };
   if (a.recent) read(0);
-  auto spot = [&](int p) { return spot_of(a, s, weights, p); };
+  auto spot = [&](int p) { return spot_of(a, page_of, weights, p); };
   // (the first chunk's targets, which the fills' places go over)
   i64 target[2] = {kNowhere, 0};
   if (tid < kRows && a.recent) {
@@ -714,7 +739,7 @@ __global__ __launch_bounds__(THREADS) void evict_whole(Evict a) {
   bool listed = true;
   if (front > a.first) {
     if (span_of(count, a.first) <= THREADS * EACH) {
-      fills = choose_held<THREADS, EACH>(a, s, weights, shared, count, a.first, front, kept, s_to);
+      fills = choose_held<THREADS, EACH>(a, page_of, weights, shared, count, a.first, front, kept, s_to);
     } else {
       choose_any<THREADS, kMoves>(shared, count, a.first, front, kept, spot);
       listed = false;
