@@ -651,6 +651,19 @@ def test_attention_weights_of_many_sequences(hip_ready, sequences, several):
     b.check_weights(before, lse)
 
 
+@pytest.mark.parametrize("extra,at_", [(1, 0), (2, 1), (2, 2), (6, 4), (8, 0)])
+def test_attention_weights_of_queries_anywhere(hip_ready, extra, at_):
+    """Many rows whose heads start at any element."""
+    b = Batch(BF16, 24, 2, 80, 16, [700, 90], [600, 40]).fill()
+    loose = torch.full((642, 25, 80 + extra), math.nan, device="cuda", dtype=BF16)
+    lse, before = b.lse(), b.w.clone()
+    query = loose[1:641, :24, at_:at_ + 80]
+    query.copy_(b.query)
+    b.query = query
+    b.weigh(lse)
+    b.check_weights(before, lse)
+
+
 def test_attention_weights_sum_to_one(hip_ready):
     """With prefix_attention's own logarithms, each row's weights sum to one."""
     b = Batch(BF16, 8, 2, 128, 16, [300, 77, 64], [9, 77, 1]).fill()

@@ -830,8 +830,9 @@ def attention_weights(query: torch.Tensor, lse: torch.Tensor, key_cache: torch.T
     its list once.  Rows that see no key add nothing, and a sequence without new tokens keeps its
     weights as they are.  ``weights`` may have any strides
     and is fastest where a head's slots lie side by side: ``torch.zeros(pages, kv_heads,
-    page).transpose(1, 2)``.  Scores, exponentials and sums are held in 32 bits; sums are taken in
-    an order that the sizes alone decide."""
+    page).transpose(1, 2)``; prompts, where the queries' heads start at multiples of 4 bytes.
+    Scores, exponentials and sums are held in 32 bits; sums are taken in an order that sizes, strides
+    and bounds alone decide."""
     device, dtype = _operand("query", query, _CACHED)
     _no_gradient("attention_weights", query, lse, key_cache, weights)
     shape, qs = _heads("query", query, device, dtype, 3)

@@ -717,7 +717,10 @@ int plan(const tg_attention_weights* r, Plan* p) {
     return steps == 0 || (stride >= 0 && stride <= (int64_t(1) << 28) / steps);
   };
   const bool many = rows > 512 || (rows >= 128 && rows * heads >= (1 << 22) / length);
-  if (many && tokens > 0 && within(tokens - 1, r->query_token) &&
+  // (what goes straight to LDS starts at a multiple of 4 bytes)
+  const bool fours = reinterpret_cast<uintptr_t>(r->query) % 4 == 0 && r->query_token % 2 == 0 &&
+                     r->query_head % 2 == 0;
+  if (many && tokens > 0 && fours && within(tokens - 1, r->query_token) &&
       within(a.group - 1, r->query_head)) {
     p->keys = a.dim > 128 ? 128 : 256;
     a.splits = static_cast<int>((length + p->keys - 1) / p->keys);
