@@ -196,6 +196,9 @@ __device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, con
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int last = first + count - 1, base = (first & ~3) + 4 * tid;
   auto at = [&](int q) { return base + 4 * THREADS * q; };
+  // the first position of a wave's fours: what none of them needs is passed over together
+  const int wave_base = (first & ~3) + 256 * __builtin_amdgcn_readfirstlane(wave);
+  auto wave_at = [&](int q) { return wave_base + 4 * THREADS * q; };
   // The keys; 0: none of the candidates, below all of them.
   uint32_t key[EACH];
   auto put = [&](int q, int j, float w, bool none) __attribute__((always_inline)) {
@@ -263,10 +266,14 @@ __device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, con
     const int above = shift, bits = min(Digit<THREADS>::kBits, shift);
     shift -= bits;
     clear_bins<THREADS>(s);
+    // (what is no candidate counts too, below all of them)
 #pragma unroll
-    for (int k = 0; k < EACH; ++k)
-      if (key[k] && (above == 32 || key[k] >> above == prefix))
-        count_key<THREADS>(s, key[k], shift, bits);
+    for (int q = 0; q < kFours; ++q) {
+      if (wave_at(q) > last) continue;
+#pragma unroll
+      for (int k = 4 * q; k < 4 * q + 4; ++k)
+        if (above == 32 || key[k] >> above == prefix) count_key<THREADS>(s, key[k], shift, bits);
+    }
     __syncthreads();
     find_bin<THREADS>(s, prefix, bits, left);
     prefix = s.prefix;
@@ -341,18 +348,24 @@ __device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, con
   rank(flags);
   const int holes = s.left / 2;
 #pragma unroll
-  for (int k = 0; k < EACH; ++k)
-    if ((flags & ~below) >> k & 1)
-      s.moves[nth_of(flags, k / 4, k % 4) - holes] = at(k / 4) + k % 4;
+  for (int q = 0; q < kFours; ++q) {
+    if (wave_at(q) + 256 <= front) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if ((flags & ~below) >> (4 * q + j) & 1) s.moves[nth_of(flags, q, j) - holes] = at(q) + j;
+  }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < EACH; ++k) {
-    if ((below & real) >> k & 1) {
-      const int p = at(k / 4) + k % 4;
-      const bool stay = stays >> k & 1;
-      const int n = nth_of(flags, k / 4, k % 4);
-      kept[p] = stay ? p : static_cast<int>(s.moves[n]);
-      if (targets && !stay) targets[n] = p;
+  for (int q = 0; q < kFours; ++q) {
+    if (wave_at(q) >= front) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if ((below & real) >> (4 * q + j) & 1) {
+        const int p = at(q) + j, n = nth_of(flags, q, j);
+        const bool stay = stays >> (4 * q + j) & 1;
+        kept[p] = stay ? p : static_cast<int>(s.moves[n]);
+        if (targets && !stay) targets[n] = p;
+      }
     }
   }
   return holes;
