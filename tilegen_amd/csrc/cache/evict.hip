@@ -9,8 +9,8 @@
 // any order; then the recent tokens go down, chunk by chunk, each read whole before it is
 // written.
 //
-// 256 heads of up to 1088 tokens of 128 cut to 1024 (78 MB): 19.8 us, 3.9 TB/s.  32 heads of up to
-// 16384 cut to 2048: 14.4 us to choose, which as many compute units' instructions bound, and 14.7 to
+// 256 heads of up to 1088 tokens of 128 cut to 1024 (78 MB): 19.6 us, 4 TB/s.  32 heads of up to
+// 16384 cut to 2048: 14.3 us to choose, which as many compute units' instructions bound, and 14.7 to
 // move 60 MB, 4.1 TB/s.  9 heads of 210: 11 us, the chain of lookups, two counts, two rankings
 // and the moves' own lookups.
 #include "cache.h"
@@ -87,7 +87,7 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 }
 
 // Digits of 11 bits for a large workgroup: two passes mostly, three of 8 bits, and weights of one
-// magnitude spread over four bins (4 x 8 heads of up to 16384 tokens cut to 2048: 29.0 us, 30.4 by 8
+// magnitude spread over four bins (4 x 8 heads of up to 16384 tokens cut to 2048: 5% faster than by 8
 // bits in 8 copies).
 template <int THREADS>
 struct Digit {
@@ -186,7 +186,7 @@ __device__ __forceinline__ int span_of(int count, int first) { return count + (f
 // Of a sequence and kv head that loses tokens: what stays, from keys that threads hold, EACH to a
 // thread, by fours of neighbouring positions, which start at a multiple of four: one lookup and one
 // load for a four where pages hold whole ones.  The workgroup's instructions bound it, some 100 for a
-// key before and 60 so (14.4 us of 29.0 in the case above, 19 of 34 key by key).  Returns how many
+// key before and 60 so (14.3 us of 28.2 in the case above, 19 of 34 key by key).  Returns how many
 // fill holes; `targets`, if any, are those.
 template <int THREADS, int EACH, typename S, typename P>
 __device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, const float* weights,
@@ -944,8 +944,8 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   if (most <= 4096 && (heads >= 64 || r->recent * a.units <= 8192)) {
     // Workgroups that fill a compute unit by themselves while there is one for each, smaller ones side by
     // side for more heads.  By 1024, 512 and 256 threads, up to 949 tokens of 80 cut to 166: 384 heads
-    // 24.9, 18.1 and 20.6 us, 848 heads 50, 36 and 33; up to 1088 of 128 cut to 1024: 256 heads 20.4,
-    // 22.9 and 28.1, 512 heads 40.9, 38.9 and 41.3, 1024 heads 90, 79 and 73.
+    // 24.9, 18.1 and 20.6 us, 848 heads 50, 36 and 30; up to 1088 of 128 cut to 1024: 256 heads 20,
+    // 23 and 28, 512 heads 41, 38 and 41, 1024 heads 90, 79 and 69.
     const int threads = heads <= 256 ? 1024 : heads <= 640 ? 512 : 256;
     const void* k = bytes == 4 ? whole_of<uint32_t>(threads) : whole_of<uint16_t>(threads);
     const hipError_t e = launch(k, heads, threads, args, s);
