@@ -713,8 +713,9 @@ def _append_normed(key, value, q, key_cache, value_cache, out, indptr, indices, 
     try:
         packed = _APPEND_NORMED.pack(
             key, value, q, key_cache, value_cache, out, indptr, indices, lengths, ends, p_shift,
-            frequency, wq, wk, _DTYPES[dtype], _DTYPES[kind or dtype], tokens, sequences, heads, kv_heads,
-            dim, rotary, layout, pages, page, n_indices, offset, epsilon is not None, ks[0], ks[1],
+            frequency, wq, wk, _DTYPES[dtype], _DTYPES[kind or dtype], tokens, sequences, heads,
+            kv_heads, dim, rotary, layout, pages, page, n_indices, offset, epsilon is not None,
+            ks[0], ks[1],
             vs[0], vs[1], qs[0], qs[1], os_[0], os_[1], kcs[0], kcs[1], kcs[2], vcs[0], vcs[1],
             vcs[2], wqs, wks, magnitude, 0.0 if epsilon is None else epsilon)
     except struct.error as e:
