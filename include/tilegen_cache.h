@@ -57,10 +57,10 @@ int launch_norm_rope(const tg_norm_rope* a, void* stream);
 /* The gradients of launch_norm_rope from those of its outputs, grad_query and grad_key: of query
  * and key into query_out and key_out, of the weights into query_weight_out and key_weight_out
  * (contiguous, of weight_dtype: [dim], or [heads, dim] where the stride is not 0; NULL: not
- * wanted), each summed in 32 bits in an order that the sizes alone decide.  query_out may be
- * grad_query or query (the same strides), and key_out likewise.  workspace holds
- * norm_rope_backward_workspace(a) bytes, 16-byte aligned, until the kernels have run; calls that
- * overlap need one each. */
+ * wanted), each summed in 32 bits in an order that the sizes alone decide; zeros where there are no
+ * tokens or no heads.  query_out may be grad_query or query (the same strides), and key_out
+ * likewise.  workspace holds norm_rope_backward_workspace(a) bytes, 16-byte aligned, until the
+ * kernels have run; calls that overlap need one each. */
 typedef struct {
   const void *grad_query, *grad_key, *query, *key;
   void *query_out, *key_out, *query_weight_out, *key_weight_out;

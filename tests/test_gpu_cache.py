@@ -341,6 +341,29 @@ def test_norm_rope_at_the_ends(hip_ready):
     assert not got[2].any() and not got[3].any() and got[0].shape == none.shape
 
 
+@pytest.mark.parametrize("tokens", [0, 1, 70])
+@pytest.mark.parametrize("kind", ["one", "each32"])
+@pytest.mark.parametrize("heads,kv_heads", [(3, 0), (40, 0), (0, 2), (0, 0)])
+def test_norm_rope_backward_without_heads(hip_ready, monkeypatch, heads, kv_heads, kind, tokens):
+    """A weight that no head reads has a gradient of zeros, whatever its memory held."""
+    monkeypatch.setattr(at, "_like", lambda x: torch.full(x.shape, math.nan, dtype=x.dtype,
+                                                          device=x.device))
+    _, q, k, wq, wk, positions, frequency, magnitude = _operands("half", BF16, tokens, heads,
+                                                                 kv_heads, 64, 64, kind)
+    if k is None:
+        k = torch.empty(tokens, 0, 64, device="cuda", dtype=BF16)
+        wk = _weights(_gen(1), kind, 0, 64, BF16)
+    g = _gen(2)
+    gq, gk = (_normal(g, *x.shape, dtype=BF16) for x in (q, k))
+    args, how = (q, k, positions, frequency, wq, wk), dict(epsilon=EPSILON, magnitude=magnitude)
+    dq, dk, dwq, dwk = at.norm_rope_backward(gq, gk, *args, **how)
+    _check_gradient(dq, dwq, gq, q, wq, positions, frequency, "half", magnitude)
+    _check_gradient(dk, dwk, gk, k, wk, positions, frequency, "half", magnitude)
+    y = at.norm_rope(q, k, positions, frequency, wq.requires_grad_(), wk.requires_grad_(), **how)
+    again = torch.autograd.grad(y, [wq, wk], [gq, gk])
+    assert torch.equal(again[0], dwq) and torch.equal(again[1], dwk)
+
+
 # --------------------------------------------------------------------------- #
 # a batch with its cache
 # --------------------------------------------------------------------------- #

@@ -477,9 +477,9 @@ def _normed_backward(grad_query, grad_key, query, key, positions, frequency, que
     kind = kind if kind is other else _kind(kind, other, dtype)
     p_positions, p_frequency, rotary = _turns(positions, frequency, tokens, device)
     query_out, dqw, dkw = _like(query), None, None
-    if wq and want_weights[0]:
+    if query_weight is not None and want_weights[0]:
         dqw = _like(query_weight)
-    if wk and want_weights[1]:
+    if key_weight is not None and want_weights[1]:
         dkw = _like(key_weight)
     fields = [grad_query.data_ptr(), p_grad_key, query.data_ptr(), p_key, query_out.data_ptr(),
               p_key_out, 0 if dqw is None else dqw.data_ptr(), 0 if dkw is None else dkw.data_ptr(),

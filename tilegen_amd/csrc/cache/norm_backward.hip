@@ -254,9 +254,11 @@ int plan(const tg_norm_rope_backward* r, Plan* p) {
   s.key_columns = a.key_each ? a.kv_heads * a.dim : a.dim;
   s.query_parts = a.blocks * (a.query_each ? 1 : (a.heads + R - 1) / R);
   s.key_parts = a.blocks * (a.key_each ? 1 : a.eights - a.key_first);
-  if (r->query_weight_out && r->heads)
+  if (!a.heads) s.query_parts = 0;
+  if (!a.kv_heads) s.key_parts = 0;
+  if (r->query_weight_out)
     p->query_floats = static_cast<int64_t>(s.query_columns) * s.query_parts;
-  if (r->key_weight_out && r->kv_heads)
+  if (r->key_weight_out)
     p->key_floats = static_cast<int64_t>(s.key_columns) * s.key_parts;
   return 0;
 }
@@ -279,7 +281,6 @@ extern "C" __attribute__((visibility("default"))) int launch_norm_rope_backward(
   Plan p;
   if (const int rc = plan(r, &p)) return rc;
   Back& a = p.a;
-  if (a.rows == 0) return 0;
   const Operand query = {"query", r->query, 3, {r->tokens, r->heads, r->dim},
                          {r->query_token, r->query_head, 1}};
   const Operand key = {"key", r->key, 3, {r->tokens, r->kv_heads, r->dim},
@@ -302,7 +303,7 @@ extern "C" __attribute__((visibility("default"))) int launch_norm_rope_backward(
     if (x == &query || x == &grad_query || !same(key_out, *x))
       if (const int rc = apart(what, key_out, *x, bytes)) return rc;
   }
-  if (a.tokens &&
+  if (a.tokens && a.rows &&
       ((r->heads && (!r->query || !r->grad_query || !r->query_out)) ||
        (r->kv_heads && (!r->key || !r->grad_key || !r->key_out)) ||
        (r->rotary && (!r->frequency || !r->positions))))
@@ -348,14 +349,14 @@ extern "C" __attribute__((visibility("default"))) int launch_norm_rope_backward(
   const void* k = r->dtype == TG_F32   ? kernel_of<float>(a.layout, p.lanes)
                   : r->dtype == TG_F16 ? kernel_of<_Float16>(a.layout, p.lanes)
                                        : kernel_of<__bf16>(a.layout, p.lanes);
-  if (a.tokens) {
+  if (a.tokens && a.rows) {
     void* args[] = {&a};
     const hipError_t e = launch(k, groups, 64 * kWavesOf, args, s);
     if (e != hipSuccess) return hip_failed(e, what);
   }
-  // (without tokens the sums have no parts and come out as 0)
+  // (without tokens or heads the sums have no parts and come out as 0)
   Sums& u = p.sums;
-  const bool q = r->query_weight_out && r->heads, w = r->key_weight_out && r->kv_heads;
+  const bool q = r->query_weight_out && u.query_columns, w = r->key_weight_out && u.key_columns;
   if (!q && !w) return 0;
   u.query = a.query_part;
   u.key = a.key_part;
