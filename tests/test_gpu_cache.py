@@ -726,6 +726,24 @@ def test_attention_weights_of_strange_rows_and_keys(hip_ready, heads):
     assert torch.equal(b.w.nan_to_num(-7), want.nan_to_num(-7))
 
 
+@pytest.mark.parametrize("large", [1e38, -1e38])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("bounds", [dict(), dict(max_query=10 ** 6, max_length=5000)])
+def test_attention_weights_of_hidden_scores_past_32_bits(hip_ready, bounds, dim, large):
+    """A finite key whose scores with rows that do not see it pass 32 bits: what they are does not
+    matter."""
+    b = Batch(BF16, 40, 2, dim, 16, [40, 300], [7, 8]).fill()
+    page, slot = b.places(0)
+    b.kc[page[38], slot[38], :, 0] = large
+    b.query[:5, :, 0] = 8.0          # positions 33 .. 37
+    b.query[5:7, :, 0] = 0.0         # 38 and 39, which see it
+    lse, before = b.lse(), b.w.clone()
+    assert lse.isfinite().all()
+    b.weigh(lse, **bounds)
+    b.check_weights(before, lse)
+    assert b.w[page, slot].isfinite().all()
+
+
 @pytest.mark.parametrize("counts", [[3, 1, 4], [3, 1, 30]])
 def test_attention_weights_of_lost_pages(hip_ready, counts):
     b = Batch(F16, 8, 2, 64, 8, [50, 40, 30], counts).fill()

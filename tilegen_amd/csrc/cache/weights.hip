@@ -533,8 +533,17 @@ __global__ __launch_bounds__(64 * kWaves, 2) void weigh_wide(Weights a) {
       for (int e = 0; e < 16; ++e)
         sum[KT - 1][e] += __builtin_amdgcn_exp2f(__builtin_fmaf(before[e], a.scale, -base_before));
     }
+    // (a finite key that is hidden from a row: -inf and a score past 32 bits are NaN; sums are not
+    // negative, so one of all is NaN where one of them is)
+    float all_sums = 0.f;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) all_sums += sum[t][e];
+    strange |= all_sums != all_sums;
     if (__syncthreads_or(odd || strange)) {
-      // infinities or NaN among the keys or the logarithms: once more, adding what is seen alone
+      // infinities or NaN among the keys, the logarithms or the sums: once more, adding what is seen
+      // alone
 #pragma unroll
       for (int t = 0; t < KT; ++t)
 #pragma unroll
