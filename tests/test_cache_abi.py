@@ -266,6 +266,34 @@ def test_calls_go_by_the_operands_device(monkeypatch):
             assert seen[-1][2] == 999
 
 
+def test_append_of_nothing_with_norms(monkeypatch):
+    """Whether there is a query is not for its address to say: a batch without tokens, or without
+    query heads, has none (a stand-in library; host tensors count as device -1)."""
+    seen = []
+
+    class Library:
+        def launch_paged_append_normed(self, packed, stream):
+            seen.append(dict(zip((f for f, _ in _fields("tg_paged_append_normed")),
+                                 at._APPEND_NORMED.unpack(packed))))
+            return 0
+
+    monkeypatch.setattr(at, "_cache_lib", Library)
+    monkeypatch.setattr(at, "_operand", lambda name, t, dtypes: (t.get_device(), t.dtype))
+    monkeypatch.setattr(at, "_raw_stream", lambda device: 0)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: -1)
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    n, f = torch.zeros(3, dtype=torch.int64), torch.zeros(32, dtype=torch.float64)
+    cache, w = torch.zeros(2, 16, 2, 64, dtype=torch.bfloat16), torch.ones(64)
+    how = dict(query_weight=w, key_weight=w, epsilon=1e-6)
+    for key, query, table in ((x[:0], x[:0], (n[:1], n[:0], n[:0])), (x, x[:, :0], (n, n, n[:2]))):
+        got = at.paged_append(key, key, cache, cache, *table, f, query=query, **how)
+        assert got.shape == query.shape
+        assert (seen[-1]["tokens"], seen[-1]["heads"]) == query.shape[:2]
+        assert seen[-1]["query_weight"] == seen[-1]["key_weight"] == w.data_ptr()
+    with pytest.raises(ValueError, match="query_weight without query"):
+        at.paged_append(x, x, cache, cache, n, n, n[:2], f, **how)
+
+
 def test_kernels_do_not_spill(tmp_path):
     readelf = "/opt/rocm/llvm/bin/llvm-readelf"
     if not os.path.exists(readelf):

@@ -538,6 +538,31 @@ def test_append_with_a_shift_alone(hip_ready):
         assert (off <= 2 * U[BF16] * keys[s].float().abs() + 2.0 ** -19).all()
 
 
+def test_append_of_nothing_with_norms(hip_ready):
+    """A batch without tokens, and one without query heads: presence goes by the operand."""
+    b = Batch(BF16, 4, 2, 64, 16, [20, 33], [0, 0]).fill()
+    frequency, _ = at.rope_frequencies(64)
+    wq, wk = (_weights(b.g, "one", 1, 64, BF16) for _ in range(2))
+    how = dict(query_weight=wq, key_weight=wk, epsilon=EPSILON)
+    before = b.kc.clone(), b.vc.clone()
+    table = (b.kc, b.vc, b.indptr, b.indices, b.lengths, frequency)
+    q = at.paged_append(b.key, b.value, *table, query=b.query, query_indptr=b.ends, **how)
+    assert q.shape == (0, 4, 64)
+    none = b.ends[:1], b.indices[:0], b.lengths[:0]
+    q = at.paged_append(b.key, b.value, b.kc, b.vc, *none, frequency, query=b.query, **how)
+    assert q.shape == (0, 4, 64)
+    for old, new in zip(before, (b.kc, b.vc)):
+        assert torch.equal(old.nan_to_num(-7), new.nan_to_num(-7))
+    key, value = (_normal(b.g, 2, 2, 64, dtype=BF16) for _ in range(2))
+    q = at.paged_append(key, value, *table, query=key[:, :0], **how)
+    assert q.shape == (2, 0, 64)
+    got = b.kc.clone(), b.vc.clone()
+    at.paged_append(key, value, *table, key_weight=wk, epsilon=EPSILON)
+    for old, new in zip(got, (b.kc, b.vc)):
+        assert torch.equal(old.nan_to_num(-7), new.nan_to_num(-7))
+    assert not torch.equal(b.kc.nan_to_num(-7), before[0].nan_to_num(-7))
+
+
 def test_append_leaves_out_what_has_no_place(hip_ready):
     """Rows of no sequence, positions past a sequence's pages, pages outside the cache."""
     b = Batch(F16, 4, 2, 64, 8, [9, 40, 8, 8], [2, 3, 1, 1])

@@ -674,6 +674,8 @@ def paged_append(key: torch.Tensor, value: torch.Tensor, key_cache: torch.Tensor
         p_frequency = _list("frequency", frequency, device, dtype=torch.float64)
         rotary = 2 * frequency.shape[0]
     if epsilon is not None or shift is not None:
+        if query_weight is not None and query is None:
+            raise ValueError("query_weight without query")
         _append_normed(
             key.data_ptr(), value.data_ptr(), q, key_cache.data_ptr(), value_cache.data_ptr(), out,
             p_indptr, p_indices, p_lengths, p_ends, shift, p_frequency, query_weight, key_weight,
@@ -704,8 +706,6 @@ def _append_normed(key, value, q, key_cache, value_cache, out, indptr, indices, 
                    qs, os_, kcs, vcs, magnitude, epsilon):
     if epsilon is None and (query_weight is not None or key_weight is not None):
         raise ValueError("weights of a norm without epsilon")
-    if query_weight is not None and not q:
-        raise ValueError("query_weight without query")
     wq, wqs, kind = _learned("query_weight", query_weight, heads, dim, device, dtype)
     wk, wks, other = _learned("key_weight", key_weight, kv_heads, dim, device, dtype)
     kind = kind if kind is other else _kind(kind, other, dtype)
