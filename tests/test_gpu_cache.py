@@ -882,6 +882,21 @@ def test_evict_without_the_weights(hip_ready):
     assert kept.tolist() == [[list(range(100))] * 2] * 2
 
 
+@pytest.mark.parametrize("kv_heads,lengths,keep", [(2, [300, 170], 100), (100, [90, 33], 40),
+                                                   (2, [5000, 4097, 20], 1500)])
+def test_evict_by_weights_that_heads_share(hip_ready, kv_heads, lengths, keep):
+    """Weights that are only read may share memory: one for all kv heads, one for all of a page."""
+    b = Batch(BF16, kv_heads, kv_heads, 24, 16, lengths).fill()
+    w, kc, vc = b.w, b.kc.clone(), b.vc.clone()
+    for shared in (w[:, :, :1], w[:, :1]):
+        b.kc.copy_(kc), b.vc.copy_(vc)
+        b.w = shared.expand(w.shape)
+        _evict(b, keep, 20, 4, move_weights=False)
+        with pytest.raises(ValueError, match="share memory"):
+            at.paged_evict(b.w, b.kc, b.vc, b.indptr, b.indices, b.lengths, keep=keep,
+                           max_length=5000)
+
+
 @pytest.mark.parametrize("lengths,keep,max_length", [([6000, 300], 128, 10), ([6000, 300], 5000, 10),
                                                      ([20000], 9000, 10), ([40000], 12000, 12000),
                                                      ([7000], 3000, 3300)])

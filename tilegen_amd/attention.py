@@ -803,14 +803,14 @@ def prefix_attention(query: torch.Tensor, key_cache: torch.Tensor, value_cache: 
 # --------------------------------------------------------------------------- #
 # a cache of bounded length
 # --------------------------------------------------------------------------- #
-def _key_weights(weights, cache, device):
+def _key_weights(weights, cache, device, write=True):
     """Strides of the keys' weights, for a cache of this shape."""
     shape, strides = weights.shape, weights.stride()
     if not (weights.get_device() == device and weights.dtype is torch.float32
             and tuple(shape) == tuple(cache[:3])):
         raise ValueError("weights is %s %s on %s, expected float32 %s on device %d" % (
             weights.dtype, tuple(shape), weights.device, tuple(cache[:3]), device))
-    if 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
+    if write and 0 in strides and any(s == 0 and n > 1 for s, n in zip(strides, shape)):
         raise ValueError("weights is written, but its elements share memory (strides %s)"
                          % (strides,))
     return strides
@@ -876,13 +876,13 @@ def paged_evict(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: tor
     there in order, and the last ``recent`` follow in order, so that the next call finds them last
     again.  Slots past the new length hold anything.  Keys stay turned as they were: give what
     sequences have lost to ``paged_append`` as ``shift``.  Weights move along unless
-    ``move_weights=False``.  ``max_length`` bounds ``lengths``, as in ``prefix_attention``.  A page
-    belongs to one sequence; slots whose page is not in the cache go first and nothing moves
-    there."""
+    ``move_weights=False``, with which they are only read and may be ones that heads share.
+    ``max_length`` bounds ``lengths``, as in ``prefix_attention``.  A page belongs to one sequence;
+    slots whose page is not in the cache go first and nothing moves there."""
     device, dtype = _operand("key_cache", key_cache, _DTYPES)
     _no_gradient("paged_evict", weights, key_cache, value_cache)
     cache, kcs, vcs = _caches(key_cache, value_cache, device, dtype, True)
-    ws = _key_weights(weights, cache, device)
+    ws = _key_weights(weights, cache, device, move_weights)
     sequences = lengths.shape[0] if lengths.dim() == 1 else -1
     p_indptr = _list("indptr", indptr, device, sequences + 1)
     p_indices, p_lengths = _list("indices", indices, device), _list("lengths", lengths, device)
