@@ -294,6 +294,14 @@ def test_append_of_nothing_with_norms(monkeypatch):
         at.paged_append(x, x, cache, cache, n, n, n[:2], f, **how)
 
 
+def test_backward_needs_both_gradients(monkeypatch):
+    monkeypatch.setattr(at, "_operand", lambda name, t, dtypes: (t.get_device(), t.dtype))
+    x = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    for gq, gk, key in ((None, x, x), (x, None, x), (None, None, None)):
+        with pytest.raises(ValueError, match="grad_query" if gq is None else "grad_key"):
+            at.norm_rope_backward(gq, gk, x, key, None, None)
+
+
 def test_kernels_do_not_spill(tmp_path):
     readelf = "/opt/rocm/llvm/bin/llvm-readelf"
     if not os.path.exists(readelf):

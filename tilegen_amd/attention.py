@@ -450,6 +450,8 @@ def _normed_backward(grad_query, grad_key, query, key, positions, frequency, que
     device, dtype = _operand("query", query, _DTYPES)
     shape, qs = _heads("query", query, device, dtype, 3)
     tokens, heads, dim = shape
+    if grad_query is None or (grad_key is None and key is not None):
+        raise ValueError("%s is not given" % ("grad_query" if grad_query is None else "grad_key"))
     gshape, gqs = _heads("grad_query", grad_query, device, dtype, 3)
     if gshape != shape:
         _unlike("grad_query", grad_query, shape)
@@ -583,7 +585,7 @@ def norm_rope_backward(grad_query: torch.Tensor, grad_key: Optional[torch.Tensor
                        key_weight: Optional[torch.Tensor] = None, *, epsilon: float = 1e-6,
                        layout: str = "half", magnitude: float = 1.0):
     """The gradients of ``norm_rope`` by (query, key, query_weight, key_weight) from those of its two
-    results; None for what it was not given."""
+    results, both of them; None for operands that it was not given."""
     _no_gradient("norm_rope_backward", grad_query, grad_key, query, key, query_weight, key_weight,
                  frequency)
     return _normed_backward(grad_query, grad_key, query, key, positions, frequency, query_weight,
