@@ -128,16 +128,17 @@ typedef struct {
 int64_t attention_weights_workspace(const tg_attention_weights* a);
 int launch_attention_weights(const tg_attention_weights* a, void* stream);
 
-/* Each sequence of L = lengths[b] > keep tokens loses all but `keep`, by kv head: the first `first`
- * and the last `recent` stay, and of those between the heaviest by `weights` (of equal ones the
- * first; NaN counts as the heaviest).  Kept tokens at positions below front = keep - recent do not
- * move; the others but the last `recent` go, in order, to the positions below front that became
- * free, in order; the last `recent` go to front and on, in order.  kept[b,h,i] is where the token
- * at position i was, -1 where there is none; lengths_out[b] = min(L, keep).  Slots from there on
- * hold anything.  With move_weights the weights move with their tokens.  A slot whose page is
- * outside the cache counts as one of the least weight, and what would come from it or go there
- * does not move.  The caches and weights may not overlap one another; kept and lengths_out are
- * contiguous and overlap nothing. */
+/* Each sequence of L > keep tokens loses all but `keep`, by kv head; L = lengths[b], or what its
+ * pages hold where that is less: the first `first` and the last `recent` stay, and of those between
+ * the heaviest by `weights` (of equal ones the first; NaN counts as the heaviest).  Kept tokens at
+ * positions below front = keep - recent do not move; the others but the last `recent` go, in order,
+ * to the positions below front that became free, in order; the last `recent` go to front and on, in
+ * order.  kept[b,h,i] is where the token at position i was, -1 where there is none; lengths_out[b] =
+ * min(L, keep).  Slots from there on hold anything.  With move_weights the weights move with their
+ * tokens; without they are only read, and may share memory.  A slot whose page is outside the cache
+ * counts as one of the least weight, and what would come from it or go there does not move.  The
+ * caches and weights may not overlap one another; kept and lengths_out are contiguous and overlap
+ * nothing. */
 typedef struct {
   void *key_cache, *value_cache;
   float* weights;

@@ -912,6 +912,18 @@ def test_evict_many_heads_past_the_bound(hip_ready, kv_heads):
     _evict(b, 3000, 30, 1, max_length=3300)
 
 
+def test_evict_lengths_past_the_pages(hip_ready):
+    """Tokens that a sequence's pages do not hold are not among those that it has: lengths end with
+    the pages, whether or not that is past `keep`."""
+    b = Batch(BF16, 2, 2, 64, 16, [70, 90, 33], seed=3).fill()
+    b.lengths_host = [1000, 91, 33]         # 5, 7 and 3 pages
+    b.lengths.copy_(torch.tensor(b.lengths_host, device="cuda"))
+    fewer, _ = _evict(b, 85, 9, 2)
+    assert fewer.tolist() == [80, 85, 33]
+    fewer, _ = _evict(b, 40, 9, 2, max_length=5000)
+    assert fewer.tolist() == [40, 40, 33]
+
+
 def test_evict_lost_pages(hip_ready):
     """Slots of pages outside the cache weigh least, and nothing is read or written there."""
     b = Batch(BF16, 1, 1, 16, 8, [80, 64]).fill()

@@ -871,7 +871,8 @@ def paged_evict(weights: torch.Tensor, key_cache: torch.Tensor, value_cache: tor
     by itself: its ``first`` and its last ``recent`` tokens stay, and of the others the heaviest by
     ``weights`` [pages, page, kv_heads] (float32; of equal ones those that stand first, NaN counts
     as the heaviest).  Returns (the new lengths, kept): kept[b, h, i], int32 [sequences, kv_heads,
-    keep], is the position that the token now at position i had, -1 past the end.
+    keep], is the position that the token now at position i had, -1 past the end.  Lengths past a
+    sequence's pages end with them, and so do the new ones.
 
     Keys and values move within their sequence's pages, in place and no more than needed: kept
     tokens at positions below ``keep - recent`` stay where they are, later ones fill the gaps
