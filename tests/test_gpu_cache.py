@@ -1027,6 +1027,93 @@ def test_cache_past_32_bits(hip_ready):
     assert torch.equal(vc[last].nan_to_num(-7), b.vc.nan_to_num(-7))
 
 
+def _far(near, pages, stride):
+    """The same values with pages `stride` elements apart, in memory that nothing else needs."""
+    far = torch.empty((pages - 1) * stride + near[0].numel(), dtype=near.dtype, device="cuda")
+    far = far.as_strided(near.shape, (stride,) + near[0].contiguous().stride())
+    far.copy_(near)
+    return far
+
+
+@pytest.mark.parametrize("bounds,group", [(dict(max_query=1), 20), (dict(), 20),
+                                          (dict(max_query=1, max_length=10), 1)])
+def test_cache_past_2_to_the_32_elements(hip_ready, bounds, group):
+    """Keys, values and weights past 2^32 elements: few rows and many, rows in parts, eviction in two
+    launches and in one, the append."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough memory")
+    b = Batch(BF16, 2 * group, 2, 64, 512, [5000, 4300, 600], [40, 30, 1], side_by_side=False)
+    b.fill()
+    stride = (1 << 28) + 1024
+    assert (b.pages - 1) * stride > 1 << 32
+    lse = b.lse()
+    kc, vc, w = (_far(x, b.pages, stride) for x in (b.kc, b.vc, b.w))
+    frequency, _ = at.rope_frequencies(64)
+
+    def both(call):
+        table = (b.indptr, b.indices, b.lengths)
+        return call(kc, vc, w, *table), call(b.kc, b.vc, b.w, *table)
+
+    def same():
+        for x, y in ((kc, b.kc), (vc, b.vc), (w, b.w)):
+            assert torch.equal(x.nan_to_num(-7), y.nan_to_num(-7))
+
+    how = dict(dict(max_query=40, max_length=5000), **bounds)
+    both(lambda kc, vc, w, *table: at.attention_weights(b.query, lse, kc, w, *table,
+                                                        query_indptr=b.ends, **how))
+    same()
+    both(lambda kc, vc, w, *table: at.paged_append(b.key, b.value, kc, vc, *table, frequency,
+                                                   query_indptr=b.ends, epsilon=EPSILON))
+    same()
+    for keep in (4200, 1500, 700):
+        (fewer, kept), (want, moved) = both(lambda kc, vc, w, *table: at.paged_evict(
+            w, kc, vc, *table, keep=keep, recent=100, first=3, max_length=int(b.lengths.max())))
+        assert torch.equal(fewer, want) and torch.equal(kept, moved)
+        same()
+        b.lengths.copy_(fewer)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("rotary", [64, 22])
+def test_norm_rope_past_2_to_the_32_elements(hip_ready, rotary, layout):
+    """Rows of tokens, and of heads, that far apart: forward into such rows, backward, the append."""
+    if torch.cuda.mem_get_info()[0] < 80 << 30:
+        pytest.skip("not enough memory")
+    far, g = (1 << 30) + 512, _gen(5)
+    frequency, _ = at.rope_frequencies(rotary)
+    positions = torch.arange(6, device="cuda")
+    q, k, gq, gk = (_normal(g, 6, 6, 64, dtype=BF16) for _ in range(4))
+    wq, wk = (_weights(g, "one", 1, 64, F32) for _ in range(2))
+    how = dict(layout=layout, epsilon=EPSILON)
+    # (one array for all, so that each starts elsewhere in it)
+    space = torch.empty(5 * far + (1 << 17), device="cuda", dtype=BF16)
+
+    def apart(x, tokens, start):
+        strides = (far, 64, 1) if tokens else (64, far, 1)
+        y = space[start << 14:].as_strided(x.shape, strides)
+        return y.copy_(x)
+
+    for tokens in (True, False):
+        want = at.norm_rope(q, k, positions, frequency, wq, wk, **how)
+        out = tuple(apart(torch.zeros_like(x), tokens, i) for i, x in enumerate((q, k)))
+        x, y = apart(q, tokens, 2), apart(k, tokens, 3)
+        at.norm_rope(x, y, positions, frequency, wq, wk, query_out=out[0], key_out=out[1], **how)
+        assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+        gx, gy = apart(gq, tokens, 4), apart(gk, tokens, 5)
+        want = at.norm_rope_backward(gq, gk, q, k, positions, frequency, wq, wk, **how)
+        got = at.norm_rope_backward(gx, gy, x, y, positions, frequency, wq, wk, **how)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        b = Batch(BF16, 6, 6, 64, 16, [9, 5, 1, 40, 2, 17], [1] * 6).fill()
+        table = (b.indptr, b.indices, b.lengths, frequency)
+        kc, vc = b.kc.clone(), b.vc.clone()
+        append = dict(how, query_weight=wq, key_weight=wk)
+        got = at.paged_append(y, gy, kc, vc, *table, query=x, query_out=out[0], **append)
+        want = at.paged_append(k, gk, b.kc, b.vc, *table, query=q, **append)
+        assert torch.equal(got, want)
+        for u, v in ((kc, b.kc), (vc, b.vc)):
+            assert torch.equal(u.nan_to_num(-7), v.nan_to_num(-7))
+
+
 # --------------------------------------------------------------------------- #
 # together
 # --------------------------------------------------------------------------- #
