@@ -834,8 +834,8 @@ def attention_weights(query: torch.Tensor, lse: torch.Tensor, key_cache: torch.T
     weights as they are.  ``weights`` may have any strides
     and is fastest where a head's slots lie side by side: ``torch.zeros(pages, kv_heads,
     page).transpose(1, 2)``; prompts, where the queries' heads start at multiples of 4 bytes.
-    Scores, exponentials and sums are held in 32 bits; sums are taken in an order that sizes, strides
-    and bounds alone decide."""
+    Scores, exponentials and sums are held in 32 bits; sums are taken in an order that sizes, strides,
+    bounds, lengths and whether the queries start at a multiple of 4 bytes alone decide."""
     device, dtype = _operand("query", query, _CACHED)
     _no_gradient("attention_weights", query, lse, key_cache, weights)
     shape, qs = _heads("query", query, device, dtype, 3)

@@ -56,7 +56,6 @@ __device__ __forceinline__ int upto(int v) {
   return v;
 }
 
-// What a workgroup that chooses shares.
 // N elements that stand anywhere.
 template <typename S, int N>
 struct Loose {

@@ -10,9 +10,11 @@
 // written.
 //
 // 256 heads of up to 1088 tokens of 128 cut to 1024 (78 MB): 19.6 us, 4 TB/s.  32 heads of up to
-// 16384 cut to 2048: 14.3 us to choose, which as many compute units' instructions bound, and 14.7 to
-// move 60 MB, 4.1 TB/s.  9 heads of 210: 11 us, the chain of lookups, two counts, two rankings
-// and the moves' own lookups.
+// 16384 cut to 2048: 14.1 us to choose, on as many compute units, and 14.6 to move 60 MB, 4.1 TB/s.  Of
+// the 14.1 some 60 instructions a key are 6.4 by their issue alone (256 waves of keys on 4 SIMDs at
+// 2.4 GHz); lookups, counts in LDS and the waits between the steps of one workgroup are the rest.  9
+// heads of up to 210: 11 us, the chain of lookups, two counts, two rankings and the moves' own
+// lookups.
 #include "cache.h"
 
 namespace tg {
@@ -185,9 +187,9 @@ __device__ __forceinline__ int span_of(int count, int first) { return count + (f
 
 // Of a sequence and kv head that loses tokens: what stays, from keys that threads hold, EACH to a
 // thread, by fours of neighbouring positions, which start at a multiple of four: one lookup and one
-// load for a four where pages hold whole ones.  The workgroup's instructions bound it, some 100 for a
-// key before and 60 so (14.3 us of 28.2 in the case above, 19 of 34 key by key).  Returns how many
-// fill holes; `targets`, if any, are those.
+// load for a four where pages hold whole ones: some 60 instructions for a key, 100 key by key (14.1 us
+// of 28.3 in the case above, 19 of 34 key by key).  Returns how many fill holes; `targets`, if any,
+// are those.
 template <int THREADS, int EACH, typename S, typename P>
 __device__ __forceinline__ int choose_held(const Evict& a, const P& page_of, const float* weights,
                                            S& s, int count, int first, int front, int32_t* kept,
@@ -937,7 +939,7 @@ extern "C" __attribute__((visibility("default"))) int launch_paged_evict(const t
   void* args[] = {&a};
   const int64_t most = r->max_length - r->recent - (r->first & ~int64_t(3));    // candidates, in fours
   // One launch where a workgroup's threads hold a head's candidates, unless few heads have many
-  // recent tokens to move, which slices do side by side.  8 kv heads of 128, 1088 tokens cut to 1024
+  // recent tokens to move, which slices do side by side.  8 kv heads of 128, up to 1088 tokens cut to 1024
   // with 256 recent: 1 sequence 14.2 us, 15.2 in two launches, 32 20.2 and 29.4, 128 74 and 134; 4000
   // to 1024: 12.6 and 14.2, 15.5 and 23.9; 4128 to 4096 with 1024 recent: 1 sequence 28.8 and 26.3, 8
   // 35.3 and 38.8, 64 138 and 214.

@@ -5,9 +5,9 @@
 // (a cos - b sin, b cos + a sin).  All in 32 bits, rounded once.
 //
 // Every head is read and written once and memory bounds it: 16384 tokens of 40 heads of 128 in
-// bfloat16 (336 MB) take 66 us, 5.1 TB/s, a large copy's rate; float32 likewise.  A head's sum is 2
-// to 6 exchanges between the lanes that hold it.  The append of up to 16384 tokens of 48 rows
-// takes 43.8 us; of small calls (4.5 to 5 us) launch and lookups are all.
+// bfloat16 (336 MB) take 67 us, 5.0 TB/s, a large copy's rate; float32 likewise.  A head's sum is 2
+// to 6 exchanges between the lanes that hold it.  The append of 4 prompts of up to 4096 tokens, 8194
+// in all, of 48 rows (201 MB) takes 44 us; of small calls (4.5 to 5 us) launch and lookups are all.
 #include "rows.h"
 
 namespace tg {
@@ -185,7 +185,7 @@ int enqueue(Normed& a, int64_t dtype, bool append, const char* what, hipStream_t
   // Tasks of one group of rows while there are few, else of three (of pairs of halves, 32 bytes a lane;
   // five of 16 bytes): waves start with the token's lookups and angles, and long ones end in an uneven
   // last turn.  16384 tokens of 40 heads of 128 in bfloat16: 73.6 us by 5 groups, 66.0 by 3, 66.5 by 1;
-  // interleaved 73.2 by 5, 77.0 by 3, 94.9 by 1.  Appending up to 16384 tokens of 48 rows: 53.0 by 1,
+  // interleaved 73.2 by 5, 77.0 by 3, 94.9 by 1.  Appending 8194 tokens of 48 rows: 53.0 by 1,
   // 43.9 by 3, 46.9 by 5; interleaved 56.9 by 3, 55.2 by 4.  3000 tokens of 40 heads: 14.5 by 1, 12.7
   // by 3.
   const int64_t groups = static_cast<int64_t>(a.tokens) * a.eights;

@@ -10,9 +10,10 @@
 // that all heads share, as one row; a second kernel adds them up.  All in 32 bits, in an order
 // that the sizes alone decide.
 //
-// Memory bounds it: 16384 tokens of 40 heads of 128 in bfloat16 (503 MB) take 95 us, 5.3 TB/s, and
-// adding up the sums of 5 x 153 workgroups 4.7; 4095 of 25 heads of 96 in float32 (118 MB) 23.3 and
-// 3.9.  Sums over tokens in registers cost no traffic; atomics would cost the order.
+// Memory bounds it: 16384 tokens of 40 heads of 128 in bfloat16 (503 MB) take 96 us, 5.2 TB/s, and
+// adding up the sums of 5 x 153 workgroups 4.8; 4095 of 25 heads of 96 in float32 (118 MB) 23.6 and
+// 4.0.  Sums over tokens in registers cost no traffic; atomics would cost the order.  Of 8 or 64
+// tokens it takes 8.3 and 2.6 us, behind a call that costs the host 19.
 #include "rows.h"
 
 namespace tg {

@@ -32,8 +32,6 @@ struct Weights {
   Div by_group, by_heads, by_splits, by_parts, by_stage, by_sequences;
 };
 
-
-
 __device__ __forceinline__ float sum16(float v) {
   auto add = [](float x, auto order) {
     const int i = __builtin_bit_cast(int, x);
@@ -212,13 +210,15 @@ __global__ __launch_bounds__(64 * kWaves) void weigh_narrow(Weights a) {
 
 // Many rows.  A wave keeps KT tiles of 32 keys in registers, a workgroup reads the rows for its four:
 // a stage of up to 64 rows (of heads over 128 32), whole tokens', is taken from LDS while the next
-// one comes, straight to LDS (4 x 4096 tokens on 8192 older keys 399 us, 413 through registers).  A
-// tile's exponentials and sums run between the products of the next tile: 8 products of 32 cycles
-// beside 16 times (fma, exponential, add) of 4, 8 and 4, which by themselves take 256 and 268
-// cycles of a SIMD and together, from registers alone, 412.  Here a tile takes about 570: one sequence
-// of 4096 tokens on 8192 older keys, 32/8 heads of 128, 363 us, 947 TFLOP/s (323 us with zeros for
-// operands: power is part of it).  4 prompts of up to 4096 tokens take 146 us, 805 TFLOP/s: the
-// start of a workgroup, masked halves and the last workgroups' end are the rest.
+// one comes, straight to LDS (4 prompts of up to 4096 tokens on up to 8192 older keys, 325 GFLOP, took
+// 399 us so and 413 through registers).  A tile's exponentials and sums run between the products of
+// the next tile: 8 products of 32 cycles beside 16 times (fma, exponential, add) of 4, 8 and 4, which
+// by themselves take 256 and 268 cycles of a SIMD and together, from registers alone, 412.  Here a
+// tile takes about 570: one sequence of 4096 tokens on 8192 older keys, 32/8 heads of 128, 348 GFLOP,
+// 363 us, 958 TFLOP/s (with zeros for operands it took 323 of 376 us: power is part of it).  4
+// prompts of up to 4096 tokens take 144 us, 825 TFLOP/s: the start of a workgroup, masked halves and
+// the last workgroups' end are the rest.  The same prompts with heads of 64, 80 and 96 take 126 us,
+// where exponentials are most of it, and with heads of 256 296 us, 799 TFLOP/s.
 constexpr int wide_rows(int dim) { return dim > 128 ? 32 : 64; }
 
 template <int DP>
@@ -716,7 +716,8 @@ int plan(const tg_attention_weights* r, Plan* p) {
   const int64_t rows = (r->query_indptr && bound > 0 ? bound : 1) * a.group;   // of a sequence
   a.parts = 1;
   // Wide for many rows, or not so few with much work for all (whole tokens in a stage, within 32 bits
-  // of its first).  32 sequences of up to 2048 keys, 8 kv heads of 128: 64 rows 29 us narrow, 33 wide;
+  // of its first).  Rows are the most that a sequence has, spread evenly down to one token's.  32
+  // sequences of up to 2048 keys, 8 kv heads of 128: 64 rows 29 us narrow, 33 wide;
   // 128 rows 40 and 36; 512 rows 108 and 56.  8 of up to 1000 keys: 256 rows 19 and 14, 512 rows 32
   // and 18.  One of 16384 keys, 4 kv heads: 64 rows 10 and 12, 256 rows 21 and 16.  4 of up to 700
   // keys, 4 kv heads of 64: 256 rows 9.6 and 13.0, 512 rows 15.5 and 15.9, 1024 rows 27 and 16.  2 of
@@ -752,8 +753,8 @@ int plan(const tg_attention_weights* r, Plan* p) {
       a.parts = static_cast<int>((stages + a.part_stages - 1) / a.part_stages);
       a.large = a.parts;
       // The last quarter in halves where there are some rounds of workgroups: what starts last ends
-      // sooner (4 prompts of up to 4096 tokens 146 us, 152 in equal parts; on 8192 older keys 363 and 404;
-      // one such prompt 372 and 364).
+      // sooner (4 prompts of up to 4096 tokens 144 us, 150 in equal parts, on up to 8192 older keys 355
+      // and 399; one of 4096 on 8192 363 and 357).
       if (units * a.parts > 1024 && a.part_stages >= 16) {
         a.large = a.parts * 3 / 4;
         a.last_stages = (a.part_stages + 1) / 2;
@@ -764,7 +765,7 @@ int plan(const tg_attention_weights* r, Plan* p) {
     p->groups = p->pieces = units * a.parts;
     if (a.parts > 1) p->bytes = p->pieces * p->keys * 4;
     // Which pieces there are is for the lengths to say, and costs every workgroup a look at all of them:
-    // 158 us without, 149 with for 4 prompts of up to 4096 tokens, 26.1 and 22.1 for 4 of 1024
+    // 158 us without, 149 with for 4 prompts of up to 4096 tokens, 26.1 and 22.1 for 4 of up to 1024
     // tokens with 8 heads of their own, 27.5 and 30.6 for 1 of 1024 (512 pieces).
     const int64_t pairs = static_cast<int64_t>(a.parts) * a.table.sequences;
     if (p->pieces > (a.table.sequences > 1 ? 256 : 512) && pairs <= kPairs) {
